@@ -987,6 +987,31 @@ int ntlb_swiglu_backward(const uint16_t* dh, int64_t lddh, const uint16_t* gu, i
 int ntlb_moe_token_grad(const void* dx, int64_t lddx, int dtype, const int32_t* pos, const void* topk_idx,
                         int idx_dtype, int64_t T, int64_t K, int64_t H, void* out, int64_t ldo, void* stream);
 
+/*
+ * Layer norm of the rows of x [T, H] (H <= 16384), in fp32:
+ *   m = mean(x), r = 1 / sqrt(mean((x - m)^2) + eps), y = (x - m) r w + b.
+ * y has x's dtype; w and b (w_dtype, H entries) may be NULL (ones, zeros).
+ * Pitches in elements; x's may be 0 (one row repeated).  Rows need only the
+ * element's alignment.  mean and rstd, fp32 [T], or both NULL, receive m and
+ * r for the backward.  NaN and infinity spread over their row.
+ */
+int ntlb_layer_norm_forward(const void* x, int x_dtype, int64_t T, int64_t H, int64_t ldx, const void* w,
+                            const void* b, int w_dtype, float eps, void* y, int64_t ldy, float* mean, float* rstd,
+                            void* stream);
+
+/*
+ * Its backward, with xh = (x - m) r and t = dy w:
+ *   dx = r (t - mean(t) - xh mean(t xh))        (x's dtype; NULL: not wanted)
+ *   dw = sum over rows of dy xh, db = of dy     (w_dtype; NULL: not wanted)
+ * summed in fp32 in an order that depends on the sizes only; T = 0 gives zero
+ * dw and db.  workspace: ntlb_layer_norm_workspace_bytes(x_dtype, T, H) bytes,
+ * needed where dw or db is wanted; it need not be cleared.
+ */
+int ntlb_layer_norm_backward(const void* x, int x_dtype, int64_t T, int64_t H, int64_t ldx, const void* dy,
+                             int64_t lddy, const float* mean, const float* rstd, const void* w, int w_dtype, void* dx,
+                             int64_t lddx, void* dw, void* db, void* workspace, int64_t ws_bytes, void* stream);
+int64_t ntlb_layer_norm_workspace_bytes(int x_dtype, int64_t T, int64_t H);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,533 @@
+// Layer norm of the rows of x [T, H], forward and backward:
+//   m = mean(x), r = 1 / sqrt(mean((x - m)^2) + eps), xh = (x - m) r
+//   y = xh w + b
+//   t = dy w,  dx = r (t - mean(t) - xh mean(t xh))
+//   dw = sum over rows of dy xh,  db = sum over rows of dy
+// All sums and statistics are fp32; y and dx are rounded once to x's type, dw
+// and db once to the weights'.
+//
+// HBM-bound: x in, y out; x and dy in, dx out.  A row is read once and stays in
+// registers: RT threads (one wave to eight) hold VPT 16-byte vectors each, and a
+// workgroup walks rows with the weights, and in the backward the column sums
+// dw and db, in registers, the next row's loads in flight while this one is
+// reduced.  The variance is the mean of (x - m)^2 over the registers, a second
+// reduction, because E[x^2] - m^2 cancels for rows far off centre.  The
+// backward takes m and r from the forward (8 bytes a row) and so needs one
+// reduction, of two sums.  Each workgroup writes one row of partial dw and db,
+// which a second kernel sums in a fixed order: the result does not depend on
+// how the workgroups are scheduled.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+
+#include "ntlb_device.h"
+#include "ntlb_host.h"
+#include "ntlb_splitk.h"
+
+namespace ntlb {
+namespace norm {
+
+typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
+// rows of an odd pitch start at any element: the vector accesses carry the
+// element's alignment, not 16 bytes
+typedef uint32_t u32x4_2 __attribute__((ext_vector_type(4), aligned(2)));
+
+template <int DT>
+struct El {
+  static constexpr int bytes = DT == DT_F32 ? 4 : 2;
+  static constexpr int n = 16 / bytes;  // elements of a vector
+};
+
+struct Raw {
+  uint32_t w[4];
+};
+
+// Unpacked values are not kept across a reduction (their registers cost more
+// than unpacking again): the raw vector is a new value once `sum` is there
+__device__ __forceinline__ void renew(Raw& r, float sum) {
+  asm("" : "+v"(r.w[0]), "+v"(r.w[1]), "+v"(r.w[2]), "+v"(r.w[3]) : "v"(sum));
+}
+
+// elements [c, c + n) of a row of H elements, zero past it
+template <int DT>
+__device__ __forceinline__ Raw load_vec(const void* row, int c, int H) {
+  constexpr int N = El<DT>::n;
+  Raw r = {{0, 0, 0, 0}};
+  if (c + N <= H) {
+    const u32x4_2 v = *reinterpret_cast<const u32x4_2*>((const uint8_t*)row + (size_t)c * El<DT>::bytes);
+    r.w[0] = v[0]; r.w[1] = v[1]; r.w[2] = v[2]; r.w[3] = v[3];
+  } else if (c < H) {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (c + i < H) {
+        if constexpr (DT == DT_F32)
+          r.w[i] = ((const uint32_t*)row)[c + i];
+        else
+          r.w[i >> 1] |= (uint32_t)((const uint16_t*)row)[c + i] << (16 * (i & 1));
+      }
+  }
+  return r;
+}
+
+template <int DT>
+__device__ __forceinline__ void unpack(const Raw& r, float (&f)[El<DT>::n]) {
+#pragma unroll
+  for (int i = 0; i < El<DT>::n; ++i) {
+    if constexpr (DT == DT_F32)
+      f[i] = __uint_as_float(r.w[i]);
+    else if constexpr (DT == DT_BF16)
+      f[i] = (i & 1) ? __uint_as_float(r.w[i >> 1] & 0xFFFF0000u) : __uint_as_float(r.w[i >> 1] << 16);
+    else
+      f[i] = __half2float(__ushort_as_half((uint16_t)(r.w[i >> 1] >> (16 * (i & 1)))));
+  }
+}
+
+template <int DT>
+__device__ __forceinline__ void store_vec(void* row, int c, int H, const float (&f)[El<DT>::n]) {
+  constexpr int N = El<DT>::n;
+  uint32_t w[4];
+  if constexpr (DT == DT_F32) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = __float_as_uint(f[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (DT == DT_BF16) {
+        const v2bf p = {(__bf16)f[2 * i], (__bf16)f[2 * i + 1]};
+        w[i] = __builtin_bit_cast(uint32_t, p);
+      } else {
+        w[i] = (uint32_t)__half_as_ushort(f32_to_f16(f[2 * i])) |
+               ((uint32_t)__half_as_ushort(f32_to_f16(f[2 * i + 1])) << 16);
+      }
+    }
+  }
+  if (c + N <= H) {
+    const u32x4_2 v = {w[0], w[1], w[2], w[3]};
+    *reinterpret_cast<u32x4_2*>((uint8_t*)row + (size_t)c * El<DT>::bytes) = v;
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (c + i < H) {
+        if constexpr (DT == DT_F32)
+          ((uint32_t*)row)[c + i] = w[i];
+        else
+          ((uint16_t*)row)[c + i] = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
+      }
+  }
+}
+
+// sum over the 64 lanes, in every lane
+__device__ __forceinline__ float wave_sum(float v) {
+  v += __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), 0xB1, 0xF, 0xF, false));
+  v += __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), 0x4E, 0xF, 0xF, false));
+  v += __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), 0x141, 0xF, 0xF, false));
+  v += __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), 0x140, 0xF, 0xF, false));
+  v += __shfl_xor(v, 16);
+  v += __shfl_xor(v, 32);
+  return v;
+}
+
+// N sums over the RT threads of a row; slot: LDS for RT / 64 waves, not the one
+// of the reduction before (its reads may still run on)
+template <int RT, int N>
+__device__ __forceinline__ void row_sum(float (&v)[N], float* slot) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = wave_sum(v[i]);
+  if constexpr (RT > 64) {
+    constexpr int NW = RT / 64;
+    if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) slot[(threadIdx.x >> 6) * N + i] = v[i];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      float s = slot[i];
+#pragma unroll
+      for (int w = 1; w < NW; ++w) s += slot[w * N + i];
+      v[i] = s;
+    }
+  }
+}
+
+struct Args {
+  const void* x;
+  int64_t ldx;  // in bytes, as the others
+  const void* w;
+  const void* b;
+  int w_dtype;
+  int64_t T;
+  int H;
+  float eps;
+  void* y;  // y, or dx
+  int64_t ldy;
+  float* mean;
+  float* rstd;
+  const void* dy;
+  int64_t lddy;
+  float* part;  // [2][workgroups][H]: dw, db
+};
+
+// a column vector of the weights as floats (w NULL: `none`)
+template <int N>
+__device__ __forceinline__ void load_weights(const void* w, int dt, int c, int H, float none, float (&f)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) f[i] = w && c + i < H ? load_elem(w, dt, c + i) : none;
+}
+
+template <int RT>
+constexpr int block_threads() { return RT < 256 ? 256 : RT; }
+
+template <int DT, int RT, int VPT>
+__global__ void __launch_bounds__(block_threads<RT>()) forward_kernel(Args g) {
+  constexpr int N = El<DT>::n, ROWS = block_threads<RT>() / RT;
+  __shared__ float red[2][RT / 64];
+  const int t = threadIdx.x % RT, H = g.H;
+  const int64_t stride = (int64_t)gridDim.x * ROWS;
+  // one row per wave or more waves: scalar, so that row addresses are
+  int64_t row = (int64_t)blockIdx.x * ROWS + __builtin_amdgcn_readfirstlane(threadIdx.x / RT);
+  const float inv = 1.0f / (float)H;
+  float w[VPT][N], b[VPT][N];
+#pragma unroll
+  for (int v = 0; v < VPT; ++v) {
+    load_weights(g.w, g.w_dtype, (t + v * RT) * N, H, 1.0f, w[v]);
+    load_weights(g.b, g.w_dtype, (t + v * RT) * N, H, 0.0f, b[v]);
+  }
+  Raw nx[VPT];
+  auto fetch = [&](int64_t r) {
+    const uint8_t* p = (const uint8_t*)g.x + r * g.ldx;
+#pragma unroll
+    for (int v = 0; v < VPT; ++v) nx[v] = load_vec<DT>(p, (t + v * RT) * N, H);
+  };
+  if (row < g.T) fetch(row);
+  for (; row < g.T; row += stride) {
+    Raw x[VPT];
+#pragma unroll
+    for (int v = 0; v < VPT; ++v) x[v] = nx[v];
+    if (row + stride < g.T) fetch(row + stride);
+    float s[1] = {0.f};
+#pragma unroll
+    for (int v = 0; v < VPT; ++v) {
+      float f[N];
+      unpack<DT>(x[v], f);
+#pragma unroll
+      for (int i = 0; i < N; ++i) s[0] += f[i];
+    }
+    row_sum<RT, 1>(s, red[0]);
+    const float m = s[0] * inv;
+    float q[1] = {0.f};
+#pragma unroll
+    for (int v = 0; v < VPT; ++v) {
+      float f[N];
+      renew(x[v], m);
+      unpack<DT>(x[v], f);
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const float d = (t + v * RT) * N + i < H ? f[i] - m : 0.f;
+        q[0] += d * d;
+      }
+    }
+    row_sum<RT, 1>(q, red[1]);
+    const float r = 1.0f / sqrtf(q[0] * inv + g.eps);
+    uint8_t* yp = (uint8_t*)g.y + row * g.ldy;
+#pragma unroll
+    for (int v = 0; v < VPT; ++v) {
+      const int c = (t + v * RT) * N;
+      float f[N];
+      renew(x[v], r);
+      unpack<DT>(x[v], f);
+#pragma unroll
+      for (int i = 0; i < N; ++i) f[i] = (f[i] - m) * r * w[v][i] + b[v][i];
+      if (c < H) store_vec<DT>(yp, c, H, f);
+    }
+    if (g.mean && t == 0) {
+      g.mean[row] = m;
+      g.rstd[row] = r;
+    }
+  }
+}
+
+// DX: dx is wanted; DW: the partial sums of dw and db are
+template <int DT, int RT, int VPT, bool DX, bool DW>
+__global__ void __launch_bounds__(block_threads<RT>()) backward_kernel(Args g) {
+  constexpr int N = El<DT>::n, BT = block_threads<RT>(), ROWS = BT / RT;
+  __shared__ float red[2][RT / 64 * 2];
+  const int t = threadIdx.x % RT, H = g.H;
+  const int64_t stride = (int64_t)gridDim.x * ROWS;
+  // one row per wave or more waves: scalar, so that row addresses are
+  int64_t row = (int64_t)blockIdx.x * ROWS + __builtin_amdgcn_readfirstlane(threadIdx.x / RT);
+  const float inv = 1.0f / (float)H;
+  float w[VPT][N], aw[VPT][N], ab[VPT][N];
+#pragma unroll
+  for (int v = 0; v < VPT; ++v) {
+    if constexpr (DX) load_weights(g.w, g.w_dtype, (t + v * RT) * N, H, 1.0f, w[v]);
+#pragma unroll
+    for (int i = 0; i < N; ++i) aw[v][i] = ab[v][i] = 0.f;
+  }
+  Raw nx[VPT], nd[VPT];
+  float nm = 0.f, nr = 0.f;
+  auto fetch = [&](int64_t r) {
+    const uint8_t* p = (const uint8_t*)g.x + r * g.ldx;
+    const uint8_t* d = (const uint8_t*)g.dy + r * g.lddy;
+#pragma unroll
+    for (int v = 0; v < VPT; ++v) {
+      nx[v] = load_vec<DT>(p, (t + v * RT) * N, H);
+      nd[v] = load_vec<DT>(d, (t + v * RT) * N, H);
+    }
+    nm = g.mean[r];
+    nr = g.rstd[r];
+  };
+  // eight vectors a thread leave no registers for a row in flight beside this one
+  constexpr bool AHEAD = VPT < 8;
+  if (AHEAD && row < g.T) fetch(row);
+  for (int buf = 0; row < g.T; row += stride, buf ^= 1) {
+    if (!AHEAD) fetch(row);
+    Raw x[VPT], d[VPT];
+    const float m = nm, r = nr;
+#pragma unroll
+    for (int v = 0; v < VPT; ++v) {
+      x[v] = nx[v];
+      d[v] = nd[v];
+    }
+    if (AHEAD && row + stride < g.T) fetch(row + stride);
+    float s[2] = {0.f, 0.f};
+#pragma unroll
+    for (int v = 0; v < VPT; ++v) {
+      float f[N], e[N];
+      unpack<DT>(x[v], f);
+      unpack<DT>(d[v], e);  // zero past H: nothing is added there
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const float xh = (f[i] - m) * r;
+        if constexpr (DW) {
+          aw[v][i] += e[i] * xh;
+          ab[v][i] += e[i];
+        }
+        if constexpr (DX) {
+          const float u = e[i] * w[v][i];
+          s[0] += u;
+          s[1] += u * xh;
+        }
+      }
+    }
+    if constexpr (DX) {
+      row_sum<RT, 2>(s, red[buf]);
+      const float s0 = s[0] * inv, s1 = s[1] * inv;
+      uint8_t* dp = (uint8_t*)g.y + row * g.ldy;
+#pragma unroll
+      for (int v = 0; v < VPT; ++v) {
+        const int c = (t + v * RT) * N;
+        float f[N], e[N];
+        renew(x[v], s0);
+        renew(d[v], s0);
+        unpack<DT>(x[v], f);
+        unpack<DT>(d[v], e);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const float xh = (f[i] - m) * r;
+          f[i] = r * (e[i] * w[v][i] - s0 - xh * s1);
+        }
+        if (c < H) store_vec<DT>(dp, c, H, f);
+      }
+    }
+  }
+  if constexpr (DW) {
+    float* pw = g.part + (int64_t)blockIdx.x * H;
+    float* pb = pw + (int64_t)gridDim.x * H;
+    if constexpr (ROWS == 1) {
+#pragma unroll
+      for (int v = 0; v < VPT; ++v)
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const int c = (t + v * RT) * N + i;
+          if (c < H) {
+            pw[c] = aw[v][i];
+            pb[c] = ab[v][i];
+          }
+        }
+    } else {
+      // the workgroup's row walkers, summed in their order
+      constexpr int W = RT * VPT * N;
+      __shared__ float sum[ROWS][W];
+      for (int k = 0; k < 2; ++k) {
+        __syncthreads();
+#pragma unroll
+        for (int v = 0; v < VPT; ++v)
+#pragma unroll
+          for (int i = 0; i < N; ++i) sum[threadIdx.x / RT][(t + v * RT) * N + i] = k ? ab[v][i] : aw[v][i];
+        __syncthreads();
+        for (int c = threadIdx.x; c < H; c += BT) {
+          float a = sum[0][c];
+#pragma unroll
+          for (int q = 1; q < ROWS; ++q) a += sum[q][c];
+          (k ? pb : pw)[c] = a;
+        }
+      }
+    }
+  }
+}
+
+// dw / db (blockIdx.y) of 32 columns: eight walkers down the P partial rows,
+// their sums added in order
+constexpr int FIN_COLS = 32, FIN_WALK = 8;
+__global__ void __launch_bounds__(FIN_COLS* FIN_WALK) finish_kernel(const float* part, int P, int H, void* dw, void* db,
+                                                                     int w_dtype) {
+  __shared__ float sum[FIN_WALK][FIN_COLS];
+  const int c = blockIdx.x * FIN_COLS + threadIdx.x % FIN_COLS, q = threadIdx.x / FIN_COLS;
+  const float* p = part + (int64_t)blockIdx.y * P * H;
+  float a = 0.f;
+  if (c < H)
+    for (int r = q; r < P; r += FIN_WALK) a += p[(int64_t)r * H + c];
+  sum[q][threadIdx.x % FIN_COLS] = a;
+  __syncthreads();
+  void* out = blockIdx.y ? db : dw;
+  if (q == 0 && c < H && out) {
+#pragma unroll
+    for (int k = 1; k < FIN_WALK; ++k) a += sum[k][threadIdx.x];
+    store_elem(out, w_dtype, c, a);
+  }
+}
+
+constexpr int MAX_H = 16384;
+
+// threads and vectors of a row, by its vectors of 16 bytes
+struct Shape {
+  int rt, vpt;
+};
+static Shape shape_for(int dt, int64_t H) {
+  const int64_t nv = cdiv(H * dtype_size(dt), 16);
+  if (nv <= 64) return {64, 1};
+  if (nv <= 128) return {64, 2};
+  if (nv <= 256) return {64, 4};
+  if (nv <= 512) return {256, 2};
+  if (nv <= 1024) return {512, 2};
+  if (nv <= 2048) return {512, 4};
+  return {512, 8};
+}
+
+// workgroups: as many as run at once, or fewer
+static int64_t groups_for(const Shape& s, int64_t T, int64_t per_cu) {
+  const int64_t rows = s.rt < 256 ? 256 / s.rt : 1;
+  return std::max<int64_t>(1, std::min(cdiv(T, rows), split_device_cus() * per_cu));
+}
+static int64_t forward_groups(const Shape& s, int64_t T) { return groups_for(s, T, s.rt <= 256 ? 8 : 4); }
+static int64_t backward_groups(const Shape& s, int64_t T) { return groups_for(s, T, s.rt <= 256 ? 2 : 1); }
+
+template <int DT, int RT, int VPT>
+static void launch_forward(const Args& g, int64_t n, hipStream_t st) {
+  forward_kernel<DT, RT, VPT><<<(unsigned)n, block_threads<RT>(), 0, st>>>(g);
+}
+template <int DT, int RT, int VPT>
+static void launch_backward(const Args& g, int64_t n, bool dx, bool dw, hipStream_t st) {
+  const dim3 grd((unsigned)n), blk(block_threads<RT>());
+  if (dx && dw)
+    backward_kernel<DT, RT, VPT, true, true><<<grd, blk, 0, st>>>(g);
+  else if (dx)
+    backward_kernel<DT, RT, VPT, true, false><<<grd, blk, 0, st>>>(g);
+  else
+    backward_kernel<DT, RT, VPT, false, true><<<grd, blk, 0, st>>>(g);
+}
+
+// f(RT, VPT) as constants for the shape
+#define NTLB_NORM_SHAPES(X) X(64, 1) X(64, 2) X(64, 4) X(256, 2) X(512, 2) X(512, 4)
+template <int DT>
+static bool forward(const Shape& s, const Args& g, int64_t n, hipStream_t st) {
+#define NTLB_CASE(RT, VPT) \
+  if (s.rt == RT && s.vpt == VPT) return launch_forward<DT, RT, VPT>(g, n, st), true;
+  NTLB_NORM_SHAPES(NTLB_CASE)
+#undef NTLB_CASE
+  if constexpr (DT == DT_F32)
+    if (s.rt == 512 && s.vpt == 8) return launch_forward<DT, 512, 8>(g, n, st), true;
+  return false;
+}
+template <int DT>
+static bool backward(const Shape& s, const Args& g, int64_t n, bool dx, bool dw, hipStream_t st) {
+#define NTLB_CASE(RT, VPT) \
+  if (s.rt == RT && s.vpt == VPT) return launch_backward<DT, RT, VPT>(g, n, dx, dw, st), true;
+  NTLB_NORM_SHAPES(NTLB_CASE)
+#undef NTLB_CASE
+  if constexpr (DT == DT_F32)
+    if (s.rt == 512 && s.vpt == 8) return launch_backward<DT, 512, 8>(g, n, dx, dw, st), true;
+  return false;
+}
+
+static int check(const char* fn, const void* x, int dt, int64_t T, int64_t H, int64_t ldx, int wdt) {
+  if (!valid_dtype(dt) || !valid_dtype(wdt)) return fail(NTLB_EINVAL, "%s: bad dtype %d / %d", fn, dt, wdt);
+  if (T < 0 || H < 1) return fail(NTLB_EINVAL, "%s: bad shape %lld x %lld", fn, (long long)T, (long long)H);
+  if (H > MAX_H) return fail(NTLB_EUNSUPPORTED, "%s: rows of %lld elements (at most %d)", fn, (long long)H, MAX_H);
+  if (T > 0 && !x) return fail(NTLB_EINVAL, "%s: NULL x", fn);
+  // rows may repeat (pitch 0) in an input, not overlap in part
+  if (ldx != 0 && ldx < H) return fail(NTLB_EINVAL, "%s: row pitch %lld below %lld", fn, (long long)ldx, (long long)H);
+  return NTLB_OK;
+}
+
+}  // namespace norm
+}  // namespace ntlb
+
+using namespace ntlb;
+
+extern "C" int ntlb_layer_norm_forward(const void* x, int x_dtype, int64_t T, int64_t H, int64_t ldx, const void* w,
+                                       const void* b, int w_dtype, float eps, void* y, int64_t ldy, float* mean,
+                                       float* rstd, void* stream) {
+  const char* fn = "ntlb_layer_norm_forward";
+  clear_error();
+  if (int rc = norm::check(fn, x, x_dtype, T, H, ldx, w_dtype)) return rc;
+  if (!(eps >= 0.0f)) return fail(NTLB_EINVAL, "%s: eps must not be negative", fn);
+  if ((mean == nullptr) != (rstd == nullptr)) return fail(NTLB_EINVAL, "%s: mean and rstd go together", fn);
+  if (T == 0) return NTLB_OK;
+  if (!y || ldy < H) return fail(NTLB_EINVAL, "%s: bad y", fn);
+  const int64_t e = dtype_size(x_dtype);
+  norm::Args g{};
+  g.x = x; g.ldx = ldx * e; g.w = w; g.b = b; g.w_dtype = w_dtype; g.T = T; g.H = (int)H; g.eps = eps;
+  g.y = y; g.ldy = ldy * e; g.mean = mean; g.rstd = rstd;
+  const norm::Shape s = norm::shape_for(x_dtype, H);
+  const int64_t n = norm::forward_groups(s, T);
+  hipStream_t st = as_stream(stream);
+  const bool ok = x_dtype == NTLB_F32    ? norm::forward<DT_F32>(s, g, n, st)
+                  : x_dtype == NTLB_BF16 ? norm::forward<DT_BF16>(s, g, n, st)
+                                         : norm::forward<DT_F16>(s, g, n, st);
+  if (!ok) return fail(NTLB_EUNSUPPORTED, "%s: no kernel for %lld columns", fn, (long long)H);
+  return check_launch(fn);
+}
+
+extern "C" int64_t ntlb_layer_norm_workspace_bytes(int x_dtype, int64_t T, int64_t H) {
+  if (!valid_dtype(x_dtype) || T < 1 || H < 1 || H > norm::MAX_H) return 0;
+  return norm::backward_groups(norm::shape_for(x_dtype, H), T) * H * 8;
+}
+
+extern "C" int ntlb_layer_norm_backward(const void* x, int x_dtype, int64_t T, int64_t H, int64_t ldx, const void* dy,
+                                        int64_t lddy, const float* mean, const float* rstd, const void* w, int w_dtype,
+                                        void* dx, int64_t lddx, void* dw, void* db, void* workspace, int64_t ws_bytes,
+                                        void* stream) {
+  const char* fn = "ntlb_layer_norm_backward";
+  clear_error();
+  if (int rc = norm::check(fn, x, x_dtype, T, H, ldx, w_dtype)) return rc;
+  if (T > 0 && (!dy || !mean || !rstd)) return fail(NTLB_EINVAL, "%s: NULL pointer", fn);
+  if (lddy != 0 && lddy < H) return fail(NTLB_EINVAL, "%s: dy's row pitch %lld below %lld", fn, (long long)lddy, (long long)H);
+  if (dx && lddx < H) return fail(NTLB_EINVAL, "%s: dx's row pitch %lld below %lld", fn, (long long)lddx, (long long)H);
+  const bool sums = dw || db;
+  if (!dx && !sums) return NTLB_OK;
+  const norm::Shape s = norm::shape_for(x_dtype, H);
+  const int64_t n = T > 0 ? norm::backward_groups(s, T) : 0;
+  if (sums && n * H * 8 > ws_bytes) return fail(NTLB_EINVAL, "%s: workspace of %lld bytes, %lld needed", fn, (long long)ws_bytes, (long long)(n * H * 8));
+  if (sums && n && (!workspace || !aligned(workspace, 4))) return fail(NTLB_EINVAL, "%s: bad workspace", fn);
+  const int64_t e = dtype_size(x_dtype);
+  norm::Args g{};
+  g.x = x; g.ldx = ldx * e; g.w = w; g.w_dtype = w_dtype; g.T = T; g.H = (int)H;
+  g.y = dx; g.ldy = lddx * e; g.mean = const_cast<float*>(mean); g.rstd = const_cast<float*>(rstd);
+  g.dy = dy; g.lddy = lddy * e; g.part = (float*)workspace;
+  hipStream_t st = as_stream(stream);
+  if (T > 0) {
+    const bool ok = x_dtype == NTLB_F32    ? norm::backward<DT_F32>(s, g, n, dx != nullptr, sums, st)
+                    : x_dtype == NTLB_BF16 ? norm::backward<DT_BF16>(s, g, n, dx != nullptr, sums, st)
+                                           : norm::backward<DT_F16>(s, g, n, dx != nullptr, sums, st);
+    if (!ok) return fail(NTLB_EUNSUPPORTED, "%s: no kernel for %lld columns", fn, (long long)H);
+    if (int rc = check_launch(fn)) return rc;
+  }
+  if (sums) {
+    const dim3 grd((unsigned)cdiv(H, norm::FIN_COLS), 2), blk(norm::FIN_COLS * norm::FIN_WALK);
+    norm::finish_kernel<<<grd, blk, 0, st>>>((const float*)workspace, (int)n, (int)H, dw, db, w_dtype);
+    return check_launch(fn);
+  }
+  return NTLB_OK;
+}

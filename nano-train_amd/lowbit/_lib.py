@@ -138,6 +138,9 @@ SIGNATURES = {
                                    _U64, _U64, _P, _P],
     "ntlb_ep_unpack_values": [_P, _I64, _I64, _I32, _P, _I64, _P, _I32, _P, _I64, _P, _P, _P, _P, _P],
     "ntlb_ep_combine_values": [_P, _I64, _I64, _I32, _P, _I32, _P, _I32, _I64, _I64, _P, _I32, _I64, _P, _P],
+    "ntlb_layer_norm_forward": [_P, _I32, _I64, _I64, _I64, _P, _P, _I32, _F32, _P, _I64, _P, _P, _P],
+    "ntlb_layer_norm_backward": [_P, _I32, _I64, _I64, _I64, _P, _I64, _P, _P, _P, _I32, _P, _I64, _P, _P, _P, _I64, _P],
+    "ntlb_layer_norm_workspace_bytes": [_I32, _I64, _I64],
 }
 
 
@@ -154,7 +157,8 @@ class LinearPlan(ctypes.Structure):
 # entry points that return a value instead of a status
 RESTYPES = {"ntlb_gemm_workspace_bytes": _I64, "ntlb_ep_record_bytes": _I64, "ntlb_colsum_workspace_bytes": _I64,
             "ntlb_ep_value_record_bytes": _I64, "ntlb_persistent_quant_ws_words": _I64,
-            "ntlb_gemm_lowbit_workspace_bytes": _I64, "ntlb_gemm_dq_workspace_bytes": _I64}
+            "ntlb_gemm_lowbit_workspace_bytes": _I64, "ntlb_gemm_dq_workspace_bytes": _I64,
+            "ntlb_layer_norm_workspace_bytes": _I64}
 
 _lib = None
 _lock = threading.Lock()
