@@ -1012,6 +1012,36 @@ int ntlb_layer_norm_backward(const void* x, int x_dtype, int64_t T, int64_t H, i
                              int64_t lddx, void* dw, void* db, void* workspace, int64_t ws_bytes, void* stream);
 int64_t ntlb_layer_norm_workspace_bytes(int x_dtype, int64_t T, int64_t H);
 
+/*
+ * Routing of T tokens to experts from the router's logits [T, E] (dtype, row
+ * pitch ld in elements, 0 for one row repeated; E <= 1024), in fp32:
+ *   p = softmax(z) or sigmoid(z); c = p + bias (bias fp32 [E] or NULL);
+ *   with topk_groups < n_groups (n_groups equal runs of experts, at most 16):
+ *     a group's score is the sum of its two highest c (its one c in groups of
+ *     one), and only the topk_groups highest groups' experts remain;
+ *   ids int32 [T, top_k] = the experts of the top_k highest c, highest first,
+ *     equal ones (and equal groups) lowest index first;
+ *   weights fp32 [T, top_k] = scale * p_i / (sum of the chosen p + 1e-20) if
+ *     renormalize, else scale * p_i.
+ * NaN orders above everything, and the ids are distinct and in range whatever
+ * the logits hold; a softmax row of -infinities has p = 0.  top_k <= 16.
+ */
+int ntlb_route_topk(const void* logits, int dtype, int64_t T, int64_t E, int64_t ld, int64_t top_k, int sigmoid,
+                    const float* bias, int64_t n_groups, int64_t topk_groups, int renormalize, float scale,
+                    int32_t* ids, float* weights, void* stream);
+
+/*
+ * The gradient of the logits (dlogits [T, E], dtype, pitch ldd) from dw fp32
+ * [T, top_k], the gradient of the weights, with the ids of the forward:
+ *   d_i = scale dw_i; if renormalize, (d_i - sum(d p) / S) / S;
+ *   softmax: dz = p (dp - sum(dp p)); sigmoid: dz = dp p (1 - p),
+ * dp being d_i at the chosen experts and 0 elsewhere.  The choice has no
+ * gradient, nor has the bias.
+ */
+int ntlb_route_topk_backward(const void* logits, int dtype, int64_t T, int64_t E, int64_t ld, int64_t top_k,
+                             int sigmoid, int renormalize, float scale, const int32_t* ids, const float* dw,
+                             void* dlogits, int64_t ldd, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -141,6 +141,8 @@ SIGNATURES = {
     "ntlb_layer_norm_forward": [_P, _I32, _I64, _I64, _I64, _P, _P, _I32, _F32, _P, _I64, _P, _P, _P],
     "ntlb_layer_norm_backward": [_P, _I32, _I64, _I64, _I64, _P, _I64, _P, _P, _P, _I32, _P, _I64, _P, _P, _P, _I64, _P],
     "ntlb_layer_norm_workspace_bytes": [_I32, _I64, _I64],
+    "ntlb_route_topk": [_P, _I32, _I64, _I64, _I64, _I64, _I32, _P, _I64, _I64, _I32, _F32, _P, _P, _P],
+    "ntlb_route_topk_backward": [_P, _I32, _I64, _I64, _I64, _I64, _I32, _I32, _F32, _P, _P, _P, _I64, _P],
 }
 
 
