@@ -1042,6 +1042,38 @@ int ntlb_route_topk_backward(const void* logits, int dtype, int64_t T, int64_t E
                              int sigmoid, int renormalize, float scale, const int32_t* ids, const float* dw,
                              void* dlogits, int64_t ldd, void* stream);
 
+/*
+ * Softmax cross entropy of a linear head without its logits: with z = X W^T
+ * (x bf16 [T, H], pitch ldx, 0 for one row repeated; w bf16 [V, H], 16-byte
+ * aligned with ldw % 8 == 0, its columns from H to the next multiple of 8
+ * zero) and targets int32 or int64 (targets64) [T],
+ *   loss_t = logsumexp(z_t) - z_t[targets_t]; 0 where targets_t == ignore_index.
+ * reduction 0: loss fp32 [T]; 1: loss[0] = the sum; 2: loss[0] = the mean over
+ * the rows that are not ignored (0 if there are none).  A target that is
+ * neither a word nor ignore_index makes its row's loss and gradients NaN.
+ * Ignored rows of x are not read.  state (ntlb_linear_xent_state_bytes, 256-byte
+ * aligned) holds what the backward needs: the live rows of x among it, not w.
+ * workspace: ntlb_linear_xent_workspace_bytes(T, H, V, 0), 16-byte aligned,
+ * contents free.
+ */
+int ntlb_linear_xent_forward(const uint16_t* x, int64_t ldx, const uint16_t* w, int64_t ldw, const void* targets,
+                             int targets64, int64_t T, int64_t H, int64_t V, int64_t ignore_index, int reduction,
+                             float* loss, void* state, void* workspace, int64_t ws_bytes, void* stream);
+
+/*
+ * Its gradients: with u_t = dloss[t] (reduction 0), dloss[0] (1) or dloss[0] /
+ * the number of live rows (2), dz_t = u_t (softmax(z_t) - onehot(targets_t)),
+ *   dx = dz W (bf16 [T, H], zero in ignored rows), dw = dz^T X (bf16 [V, H]),
+ * either NULL if not wanted.  The logits are formed again piece by piece of the
+ * vocabulary; dz, without the rows' common factor, is rounded to bf16 as the
+ * operand of the two products.  w must be as in the forward.  workspace: ntlb_linear_xent_workspace_bytes(T, H, V, 1).
+ */
+int ntlb_linear_xent_backward(const void* state, const uint16_t* w, int64_t ldw, int64_t T, int64_t H, int64_t V,
+                              int reduction, const float* dloss, uint16_t* dx, int64_t lddx, uint16_t* dw,
+                              int64_t lddw, void* workspace, int64_t ws_bytes, void* stream);
+int64_t ntlb_linear_xent_state_bytes(int64_t T, int64_t H);
+int64_t ntlb_linear_xent_workspace_bytes(int64_t T, int64_t H, int64_t V, int backward);
+
 #ifdef __cplusplus
 }
 #endif

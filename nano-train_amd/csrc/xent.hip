@@ -1,0 +1,695 @@
+// Softmax cross entropy of a linear head, without keeping the logits:
+//   z = X W^T [T, V],  loss_t = logsumexp(z_t) - z_t[y_t]
+//   dz_t = u_t (softmax(z_t) - onehot(y_t)),  dX = dz W,  dW = dz^T X
+// (u_t: the gradient that comes in for loss_t)
+// X bf16 [T, H], W bf16 [V, H]; products of bf16 values are exact in fp32 and
+// summed in fp32 on the matrix cores; statistics, exponentials and losses are
+// fp32.
+//
+// Matrix-core bound: 2 T V H operations forward, 4 T V H for the gradients and
+// 2 T V H more to form the logits again, which costs less than it would to write
+// and read T x V values of 32 bits.  Positions that are ignored are left out
+// before the products: X's live rows are gathered (and padded to whole 64-column
+// steps) into X', so masked positions cost nothing, hold no part in any sum and
+// cannot pass on a NaN.  How many are live is known to the device only: tiles
+// past them exit, and the contraction of dW ends there.
+//
+// Forward: 256x256 tiles of z; the epilogue reduces a tile's row to (max,
+// sum of exp(z - max)) and picks the label's logit, and a second kernel joins
+// the V / 256 pairs of a row.  Backward, per piece of the vocabulary (the piece's
+// dz, bf16, is the only matrix of logits' size that exists): dz from the logits
+// formed again, dX += dz W (fp32, in `slices` ranges of the piece where the tiles
+// alone would leave compute units idle), dW = dz^T X'.  dz is rounded to bf16
+// once, as the operand of its two products, which costs about what the
+// rounding of the outputs does as long as the roundings are independent.  The
+// large values, p - 1 at the labels, would not be if they held the factor 1 / n of
+// a mean: every one of them would be off by the same part, and so the whole
+// gradient.  So dz is formed without the rows' common factor (for u of its own
+// for each row, their largest magnitude), which the outputs take in fp32.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <type_traits>
+
+#include "ntlb_device.h"
+#include "ntlb_gemm_bf16.h"
+#include "ntlb_host.h"
+#include "ntlb_splitk.h"
+
+namespace ntlb {
+namespace xent {
+
+typedef int v8i __attribute__((ext_vector_type(8)));
+typedef int v4i __attribute__((ext_vector_type(4)));
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef short v4s __attribute__((ext_vector_type(4)));
+typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
+typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
+typedef __attribute__((address_space(3))) void* lds_ptr_t;
+typedef __attribute__((address_space(3))) v4s* lds_v4s_ptr;
+
+constexpr int TM = 256, TN = 256, ROWB = 128, KSTEP = 64, TILE = 256 * ROWB, NT = 512;
+constexpr float LOG2E = 1.44269502e+00f, LN2 = 6.93147182e-01f;
+
+// LDS stages and fragments as in gemm_dq.hip: row-major [256][128 bytes] with
+// 16-byte chunks XOR-swizzled by row, or [64 contraction rows][256] as stored,
+// read transposed
+__device__ __forceinline__ int sw_perm(int r) { return (r & 7) ^ ((r >> 3) & 1); }
+__device__ __forceinline__ int sw(int r, int c) { return r * ROWB + ((c ^ sw_perm(r)) << 4); }
+__device__ __forceinline__ int tr_perm(int k) { return (2 * (k & 3)) ^ (8 * ((k >> 4) & 1)); }
+
+template <bool TR>
+__device__ __forceinline__ v8i frag(const uint8_t* tile, int row0, int lane) {
+  const int g = lane >> 4;
+  v8i f;
+  if constexpr (!TR) {
+    const int r = row0 + (lane & 15);
+    const uint4 lo = *reinterpret_cast<const uint4*>(tile + sw(r, 2 * g));
+    const uint4 hi = *reinterpret_cast<const uint4*>(tile + sw(r, 2 * g + 1));
+    f[0] = (int)lo.x; f[1] = (int)lo.y; f[2] = (int)lo.z; f[3] = (int)lo.w;
+    f[4] = (int)hi.x; f[5] = (int)hi.y; f[6] = (int)hi.z; f[7] = (int)hi.w;
+  } else {
+    const int j = (lane >> 2) & 3, q = lane & 3, c = (row0 >> 3) + (q >> 1);
+#pragma unroll
+    for (int h = 0; h < 4; ++h) {
+      const int k = 16 * g + 4 * h + j;
+      const v4s v = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+          (lds_v4s_ptr)(tile + k * 512 + ((c ^ tr_perm(k)) << 4) + (q & 1) * 8));
+      f[2 * h] = (int)(((uint32_t)(uint16_t)v[1] << 16) | (uint16_t)v[0]);
+      f[2 * h + 1] = (int)(((uint32_t)(uint16_t)v[3] << 16) | (uint16_t)v[2]);
+    }
+  }
+  return f;
+}
+
+__device__ __forceinline__ v4f mma(const v8i& p, const v8i& q, v4f acc) {
+  const v4i pl = {p[0], p[1], p[2], p[3]}, ph = {p[4], p[5], p[6], p[7]};
+  const v4i ql = {q[0], q[1], q[2], q[3]}, qh = {q[4], q[5], q[6], q[7]};
+  acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, pl), __builtin_bit_cast(v8bf, ql), acc, 0, 0, 0);
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, ph), __builtin_bit_cast(v8bf, qh), acc, 0, 0, 0);
+}
+
+__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
+  const v2bf p = {(__bf16)a, (__bf16)b};
+  return __builtin_bit_cast(uint32_t, p);
+}
+
+// One operand: bf16, 16-byte aligned with whole 16-byte rows.
+//   stored by rows: [rows, cols], the contraction along cols; columns at or past
+//     cols read zero, rows past rows too
+//   transposed: [k, rows], the contraction down the rows; stored rows at or past
+//     k read zero
+struct Mat {
+  const uint8_t* p;
+  int64_t pitch;  // bytes
+  int64_t rows;   // of the operand
+  int64_t k;      // contraction
+};
+
+// Copies of one K step, global -> LDS: wave w takes copies w + 8j, j = 0..3, of
+// 1 KiB.  Resources begin at the tile (rows) or at the K step (transposed), so
+// offsets stay small whatever the matrix's size.
+struct RowCopy {
+  __amdgpu_buffer_rsrc_t rs;
+  uint32_t off, grp;
+  int64_t k;
+  int col;  // first column of the lane's chunk in a step
+  __device__ __forceinline__ void init(const Mat& o, int64_t r0, int wave, int lane) {
+    const int xr = wave * 8 + (lane >> 3), c = (lane & 7) ^ sw_perm(xr);
+    const int64_t rows = max<int64_t>(0, min<int64_t>(o.rows - r0, 256));
+    const int64_t last = min<int64_t>(o.pitch, (o.k * 2 + 15) / 16 * 16);
+    const int64_t bytes = rows > 0 ? (rows - 1) * o.pitch + last : 0;
+    rs = __builtin_amdgcn_make_buffer_rsrc((void*)uniform64(o.p + r0 * o.pitch), (short)0, (int)uniform64(bytes), 0x00020000);
+    off = (uint32_t)(xr * o.pitch + c * 16);
+    grp = (uint32_t)(64 * o.pitch);
+    col = c * 8;
+    k = o.k;
+  }
+  __device__ __forceinline__ void issue(uint8_t* stage, int kt, int wave, int j) const {
+    const uint32_t o = (int64_t)kt * KSTEP + col < k ? off : 0x80000000u;
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr_t)(stage + (wave + 8 * j) * 1024), 16, o,
+                                             (uint32_t)kt * ROWB + j * grp, 0, 0);
+  }
+};
+
+struct TrCopy {
+  const uint8_t* p;
+  int64_t pitch, k, last;
+  uint32_t off;
+  __device__ static int row0(int wave, int j) { return 2 * (wave & 3) + 16 * (wave >> 2) + 8 * (j & 1) + 32 * (j >> 1); }
+  __device__ __forceinline__ void init(const Mat& o, int64_t r0, int wave, int lane) {
+    const int R = row0(wave, 0) + (lane >> 5), c = (lane & 31) ^ tr_perm(R);
+    p = uniform64(o.p);
+    pitch = uniform64(o.pitch);
+    k = uniform64(o.k);
+    last = min<int64_t>(o.pitch, (o.rows * 2 + 15) / 16 * 16);
+    off = (uint32_t)(R * o.pitch + (r0 + 8 * c) * 2);
+  }
+  __device__ __forceinline__ void issue(uint8_t* stage, int kt, int wave, int j) const {
+    // a tile that overhangs its rows reads into the next stored row, where there is one
+    const int64_t rem = k - (int64_t)kt * KSTEP;
+    const int64_t bytes = rem <= 0 ? 0 : (min<int64_t>(rem, KSTEP + 1) - 1) * pitch + (rem > KSTEP + 1 ? pitch : last);
+    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)(p + (int64_t)kt * KSTEP * pitch), (short)0,
+                                                                        (int)bytes, 0x00020000);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr_t)(stage + row0(wave, j) * 512), 16, off,
+                                             (uint32_t)((8 * (j & 1) + 32 * (j >> 1)) * pitch), 0, 0);
+  }
+};
+
+constexpr int EPI_LSE = 0, EPI_DZ = 1, EPI_ACC = 2, EPI_STORE = 3;
+
+// The gradient that comes in: du[0] for all rows, over the number of live rows
+// if mean; or, `most` given, du[t] for row t, their common factor most[0]
+struct Up {
+  const float* du;
+  const float* most;
+  int mean;
+  __device__ float common(int live) const { return most ? most[0] : du[0] * (mean ? 1.0f / (float)max(live, 1) : 1.0f); }
+  __device__ float rest(int row, float c) const { return !most ? 1.0f : c == 0.f ? 0.f : du[row] / c; }
+};
+
+struct Args {
+  Mat a, b;
+  int64_t M, N;
+  const int32_t* live;  // device: the number of live rows (rows of A for LSE / DZ / ACC, the contraction for STORE)
+  int slices;           // ACC: ranges of the contraction, one after another in the grid
+  int group_m;          // raster: row tiles side by side
+  // LSE
+  float2* part;         // [column tiles][ldp] (max, sum)
+  int64_t ldp;
+  float* zl;            // [M] the label's logit
+  const int32_t* y;     // labels of the live rows, < 0: none
+  int64_t v0;           // first column's place in the vocabulary
+  // DZ
+  const float* lse;
+  const int32_t* rows;
+  Up up;
+  // outputs
+  void* out;            // DZ: bf16, ACC: fp32 [slices][..], STORE: bf16
+  int64_t ldo;          // elements
+  int64_t slice;        // elements of a slice
+  int add;              // ACC: add to what is there
+  int vec_out;
+};
+
+template <bool TA, bool TB, int EPI>
+__global__ void __launch_bounds__(NT, 1) head_kernel(Args g) {
+  __shared__ __attribute__((aligned(16))) uint8_t la0[TILE];
+  __shared__ __attribute__((aligned(16))) uint8_t lb0[TILE];
+  __shared__ __attribute__((aligned(16))) uint8_t la1[TILE];
+  __shared__ __attribute__((aligned(16))) uint8_t lb1[TILE];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave >> 2, wn = wave & 3;
+  const int live = g.live[0];
+  // tiles: each XCD walks a contiguous range of a raster of group_m row tiles
+  const int num_n = (int)((g.N + TN - 1) / TN);
+  const int num_m_all = (int)((g.M + TM - 1) / TM);
+  const int num_m = EPI == EPI_STORE ? num_m_all : (live + TM - 1) / TM;
+  int pid = (int)blockIdx.x;
+  int sl = 0;
+  if constexpr (EPI == EPI_ACC) {
+    const int tiles = num_m * num_n;
+    if (pid >= tiles * g.slices) return;
+    // the ranges of a tile lie on different XCDs' shares, side by side in k
+    const int nwg = tiles * g.slices, xcd = pid & 7, per = nwg >> 3, extra = nwg & 7;
+    const int q = xcd * per + min(xcd, extra) + (pid >> 3);
+    sl = q / tiles;
+    pid = q - sl * tiles;
+  } else {
+    const int nwg = num_m * num_n;
+    if (pid >= nwg) return;
+    const int xcd = pid & 7, per = nwg >> 3, extra = nwg & 7;
+    pid = xcd * per + min(xcd, extra) + (pid >> 3);
+  }
+  const int group = pid / (g.group_m * num_n), first_m = group * g.group_m;
+  const int gsize = min(num_m - first_m, g.group_m), in_group = pid - group * g.group_m * num_n;
+  const int64_t m0 = (int64_t)(first_m + in_group % gsize) * TM, n0 = (int64_t)(in_group / gsize) * TN;
+  if constexpr (EPI == EPI_STORE) {
+    g.a.k = live;
+    g.b.k = live;
+  } else {
+    g.M = live;
+    g.a.rows = live;
+  }
+  const int nk = max(1, (int)((g.a.k + KSTEP - 1) / KSTEP));
+  const int kb0 = EPI == EPI_ACC ? (int)((int64_t)sl * nk / g.slices) : 0;
+  const int kb1 = EPI == EPI_ACC ? (int)((int64_t)(sl + 1) * nk / g.slices) : nk;
+
+  typename std::conditional<TA, TrCopy, RowCopy>::type ca;
+  typename std::conditional<TB, TrCopy, RowCopy>::type cb;
+  ca.init(g.a, m0, wave, lane);
+  cb.init(g.b, n0, wave, lane);
+  v4f acc[8][4];
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[i][j] = (v4f){0.f, 0.f, 0.f, 0.f};
+  if (kb0 < kb1) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      ca.issue(la0, kb0, wave, j);
+      cb.issue(lb0, kb0, wave, j);
+    }
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    auto step = [&](auto bufc, int kt) {
+      constexpr int BUF = decltype(bufc)::value;
+      const uint8_t* ta = BUF ? la1 : la0;
+      const uint8_t* tb = BUF ? lb1 : lb0;
+      uint8_t* na = BUF ? la0 : la1;
+      uint8_t* nb = BUF ? lb0 : lb1;
+      const int kn = min(kt + 1, kb1 - 1);  // the last step copies itself into the idle stage
+      v8i bf[4];
+#pragma unroll
+      for (int tn = 0; tn < 4; ++tn) bf[tn] = frag<TB>(tb, wn * 64 + tn * 16, lane);
+      v8i af = frag<TA>(ta, wm * 128, lane);
+#pragma unroll
+      for (int tm = 0; tm < 8; ++tm) {
+        v8i af_next;
+        if (tm + 1 < 8) af_next = frag<TA>(ta, wm * 128 + (tm + 1) * 16, lane);
+        if (tm < 4) {
+          ca.issue(na, kn, wave, tm);
+          cb.issue(nb, kn, wave, tm);
+        }
+#pragma unroll
+        for (int tn = 0; tn < 4; ++tn) acc[tm][tn] = mma(bf[tn], af, acc[tm][tn]);
+        asm volatile("" : "+v"(acc[tm][0]), "+v"(acc[tm][1]), "+v"(acc[tm][2]), "+v"(acc[tm][3])::"memory");
+        if (tm + 1 < 8) af = af_next;
+      }
+      __builtin_amdgcn_s_waitcnt(0);
+      __syncthreads();
+    };
+    for (int kt = kb0; kt < kb1; kt += 2) {
+      step(std::integral_constant<int, 0>(), kt);
+      if (kt + 1 < kb1) step(std::integral_constant<int, 1>(), kt + 1);
+    }
+  }
+  // lane: rows m0 + wm*128 + tm*16 + lane%16, columns n0 + wn*64 + tn*16 + 4*(lane/16) + r
+  const int64_t mw = m0 + wm * 128 + (lane & 15), nw = n0 + wn * 64 + (lane >> 4) * 4;
+  if constexpr (EPI == EPI_LSE) {
+    float2* red = reinterpret_cast<float2*>(la0);  // [4][256]
+#pragma unroll
+    for (int tm = 0; tm < 8; ++tm) {
+      const int64_t m = mw + tm * 16;
+      const int64_t lab = (m < g.M ? (int64_t)g.y[m] : -1) - g.v0 - nw;  // the label's column, from the lane's first
+      float mx = -__builtin_inff();
+#pragma unroll
+      for (int tn = 0; tn < 4; ++tn)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          if (nw + tn * 16 + r >= g.N) acc[tm][tn][r] = -__builtin_inff();
+          mx = fmaxf(mx, acc[tm][tn][r]);
+          if (lab == tn * 16 + r && m < g.M) g.zl[m] = acc[tm][tn][r];
+        }
+      mx = fmaxf(mx, __shfl_xor(mx, 16));
+      mx = fmaxf(mx, __shfl_xor(mx, 32));
+      const float ref = mx == -__builtin_inff() ? 0.f : mx;
+      float s = 0.f;
+#pragma unroll
+      for (int tn = 0; tn < 4; ++tn)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s += __builtin_amdgcn_exp2f((acc[tm][tn][r] - ref) * LOG2E);
+      s += __shfl_xor(s, 16);
+      s += __shfl_xor(s, 32);
+      if (lane < 16) red[wn * 256 + wm * 128 + tm * 16 + lane] = make_float2(mx, s);
+    }
+    __syncthreads();
+    if (tid < 256 && m0 + tid < g.M) {
+      float2 t[4];
+      float mx = -__builtin_inff();
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        t[i] = red[i * 256 + tid];
+        mx = fmaxf(mx, t[i].x);
+      }
+      const float ref = mx == -__builtin_inff() ? 0.f : mx;
+      float s = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s += t[i].y * __builtin_amdgcn_exp2f((t[i].x - ref) * LOG2E);
+      g.part[(n0 / TN) * g.ldp + m0 + tid] = make_float2(mx, s);
+    }
+  } else if constexpr (EPI == EPI_DZ) {
+    const float c = g.up.common(live);
+#pragma unroll
+    for (int tm = 0; tm < 8; ++tm) {
+      const int64_t m = mw + tm * 16;
+      if (m >= g.M) continue;
+      const int64_t lab = (int64_t)g.y[m] - g.v0 - nw;
+      const float lse = g.lse[m], u = g.up.rest(g.rows[m], c);
+#pragma unroll
+      for (int tn = 0; tn < 4; ++tn) {
+        const int64_t n = nw + tn * 16;
+        float d[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float p = __builtin_amdgcn_exp2f((acc[tm][tn][r] - lse) * LOG2E);
+          d[r] = n + r < g.N ? (lab == tn * 16 + r ? p - 1.0f : p) * u : 0.f;
+        }
+        // the pitch holds whole 64-column steps, zero past the piece
+        if (n < g.ldo) *reinterpret_cast<uint2*>((uint16_t*)g.out + m * g.ldo + n) = make_uint2(pack_bf16(d[0], d[1]), pack_bf16(d[2], d[3]));
+      }
+    }
+  } else if constexpr (EPI == EPI_ACC) {
+    float* o = (float*)g.out + sl * g.slice;
+#pragma unroll
+    for (int tm = 0; tm < 8; ++tm) {
+      const int64_t m = mw + tm * 16;
+      if (m >= g.M) continue;
+#pragma unroll
+      for (int tn = 0; tn < 4; ++tn) {
+        const int64_t n = nw + tn * 16;
+        if (n >= g.ldo) continue;  // the pitch is a multiple of four
+        v4f* q = reinterpret_cast<v4f*>(o + m * g.ldo + n);
+        *q = g.add ? *q + acc[tm][tn] : acc[tm][tn];
+      }
+    }
+  } else {
+    const float c = g.up.common(live);
+#pragma unroll
+    for (int tm = 0; tm < 8; ++tm) {
+      const int64_t m = mw + tm * 16;
+      if (m >= g.M) continue;
+#pragma unroll
+      for (int tn = 0; tn < 4; ++tn) {
+        const int64_t n = nw + tn * 16;
+        acc[tm][tn] *= c;
+        uint16_t* q = (uint16_t*)g.out + m * g.ldo + n;
+        if (g.vec_out && n + 4 <= g.N) {
+          *reinterpret_cast<uint2*>(q) = make_uint2(pack_bf16(acc[tm][tn][0], acc[tm][tn][1]), pack_bf16(acc[tm][tn][2], acc[tm][tn][3]));
+        } else {
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (n + r < g.N) q[r] = f32_to_bf16_bits(acc[tm][tn][r]);
+        }
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// the live rows: pos[t] = place of row t among them (-1: ignored), rows[i] and
+// y[i] (-1: not a word) of the i-th, live[0] how many; one workgroup
+// ---------------------------------------------------------------------------
+constexpr int SCAN = 1024;
+__global__ void __launch_bounds__(SCAN) scan_kernel(const void* targets, int t64, int64_t T, int64_t V, int64_t ignore,
+                                                    int32_t* pos, int32_t* rows, int32_t* y, int32_t* live) {
+  __shared__ int wsum[SCAN / 64];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  int base = 0;
+  for (int64_t t0 = 0; t0 < T; t0 += SCAN) {
+    const int64_t t = t0 + tid;
+    const int64_t v = t < T ? (t64 ? ((const int64_t*)targets)[t] : (int64_t)((const int32_t*)targets)[t]) : ignore;
+    const bool on = t < T && v != ignore;
+    const uint64_t b = __ballot(on);
+    if (lane == 0) wsum[wave] = __popcll(b);
+    __syncthreads();
+    int before = base, all = 0;
+#pragma unroll
+    for (int w = 0; w < SCAN / 64; ++w) {
+      before += w < wave ? wsum[w] : 0;
+      all += wsum[w];
+    }
+    const int at = before + __popcll(b & ((1ull << lane) - 1));
+    if (t < T) pos[t] = on ? at : -1;
+    if (on) {
+      rows[at] = (int32_t)t;
+      y[at] = v >= 0 && v < V ? (int32_t)v : -1;
+    }
+    base += all;
+    __syncthreads();
+  }
+  if (tid == 0) live[0] = base;
+}
+
+// X' rows: 16-byte pieces of the live rows of X, zero past H; a piece of an
+// unaligned or ragged row element by element.  Also what the other kernels
+// expect set: zl (NaN until a tile finds the label) and a zero loss for the
+// ignored rows.
+__global__ void __launch_bounds__(256) gather_kernel(const uint16_t* x, int64_t ldx, int64_t T, int64_t H, int aligned16,
+                                                     const int32_t* pos, uint16_t* xp, int64_t ldp, float* zl, float* loss) {
+  const int64_t t = blockIdx.x;
+  const int at = pos[t];
+  if (at < 0) {
+    if (threadIdx.x == 0 && loss) loss[t] = 0.f;
+    return;
+  }
+  if (threadIdx.x == 0) zl[at] = __builtin_nanf("");
+  const uint16_t* src = x + t * ldx;
+  uint4* dst = reinterpret_cast<uint4*>(xp + (int64_t)at * ldp);
+  for (int64_t c = threadIdx.x; c < ldp / 8; c += blockDim.x) {
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (aligned16 && c * 8 + 8 <= H) {
+      v = *reinterpret_cast<const uint4*>(src + c * 8);
+    } else {
+      uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (c * 8 + i < H) w[i >> 1] |= (uint32_t)src[c * 8 + i] << (16 * (i & 1));
+      v = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    dst[c] = v;
+  }
+}
+
+// lse and loss of the live rows from their pairs: 16 rows by 16 walkers
+__global__ void __launch_bounds__(256) join_kernel(const float2* part, int64_t ldp, int64_t parts, const float* zl,
+                                                   const int32_t* rows, const int32_t* live, float* lse, float* each,
+                                                   float* loss) {
+  __shared__ float2 red[16][17];
+  const int r = threadIdx.x & 15, q = threadIdx.x >> 4;
+  const int64_t m = (int64_t)blockIdx.x * 16 + r;
+  const bool on = m < live[0];
+  if ((int64_t)blockIdx.x * 16 >= live[0]) return;
+  float mx = -__builtin_inff(), s = 0.f;
+  if (on)
+    for (int64_t i = q; i < parts; i += 16) {
+      const float2 t = part[i * ldp + m];
+      const float hi = fmaxf(mx, t.x), ref = hi == -__builtin_inff() ? 0.f : hi;
+      s = s * __builtin_amdgcn_exp2f((mx - ref) * LOG2E) + t.y * __builtin_amdgcn_exp2f((t.x - ref) * LOG2E);
+      mx = hi;
+    }
+  red[q][r] = make_float2(mx, s);
+  __syncthreads();
+  if (q == 0 && on) {
+    for (int i = 1; i < 16; ++i) mx = fmaxf(mx, red[i][r].x);
+    const float ref = mx == -__builtin_inff() ? 0.f : mx;
+    s = 0.f;
+    for (int i = 0; i < 16; ++i) s += red[i][r].y * __builtin_amdgcn_exp2f((red[i][r].x - ref) * LOG2E);
+    const float l = ref + __builtin_amdgcn_logf(s) * LN2, z = zl[m];
+    lse[m] = z != z ? z : l;  // no such word, or its logit is NaN: so is all of the row
+    each[m] = l - z;
+    if (loss) loss[rows[m]] = l - z;
+  }
+}
+
+// the sum or mean of the live rows' losses, in a fixed order; 0 where none is live
+__global__ void __launch_bounds__(1024) total_kernel(const float* each, const int32_t* live, int mean, float* loss) {
+  __shared__ float red[16];
+  const int n = live[0];
+  float s = 0.f;
+  for (int i = threadIdx.x; i < n; i += 1024) s += each[i];
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) s += __shfl_xor(s, d);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    float t = 0.f;
+    for (int i = 0; i < 16; ++i) t += red[i];
+    loss[0] = mean ? t / (float)max(n, 1) : t;
+  }
+}
+
+// the largest finite |du| of the live rows
+__global__ void __launch_bounds__(1024) most_kernel(const float* du, const int32_t* rows, const int32_t* live, float* most) {
+  __shared__ uint32_t red[16];
+  uint32_t m = 0;
+  for (int i = threadIdx.x; i < live[0]; i += 1024) {
+    const uint32_t a = abs_bits(du[rows[i]]);
+    m = a < 0x7F800000u ? max(m, a) : m;
+  }
+  m = wave_max_u32(m);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int i = 1; i < 16; ++i) m = max(m, red[i]);
+    most[0] = __uint_as_float(m);
+  }
+}
+
+// dX rows: the slices summed in order, bf16; zero for the ignored rows
+__global__ void __launch_bounds__(256) scatter_kernel(const float* acc, int64_t ldp, int64_t slice, int slices, Up up,
+                                                      const int32_t* live, const int32_t* pos, int64_t H, uint16_t* dx,
+                                                      int64_t ldx) {
+  const int64_t t = blockIdx.x;
+  const int at = pos[t];
+  const float f = up.common(live[0]);
+  for (int64_t c = (int64_t)threadIdx.x * 4; c < H; c += blockDim.x * 4) {
+    v4f v = {0.f, 0.f, 0.f, 0.f};
+    if (at >= 0)
+      for (int s = 0; s < slices; ++s) v += *reinterpret_cast<const v4f*>(acc + s * slice + (int64_t)at * ldp + c);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (c + i < H) dx[t * ldx + c + i] = f32_to_bf16_bits(at >= 0 ? v[i] * f : 0.f);
+  }
+}
+
+// what the forward leaves for the backward
+struct State {
+  int64_t hp;  // pitch of X', elements
+  int64_t xp, pos, rows, y, lse, live, bytes;
+};
+static State state_of(int64_t T, int64_t H) {
+  State s;
+  s.hp = cdiv(H, 64) * 64;
+  auto up = [](int64_t v) { return cdiv(v, 256) * 256; };
+  s.xp = 0;
+  s.pos = up(T * s.hp * 2);
+  s.rows = s.pos + up(T * 4);
+  s.y = s.rows + up(T * 4);
+  s.lse = s.y + up(T * 4);
+  s.live = s.lse + up(T * 4);
+  s.bytes = s.live + 256;
+  return s;
+}
+
+// forward workspace: the pairs, the label logits, the rows' losses
+static int64_t forward_ws(int64_t T, int64_t V) { return cdiv(V, TN) * T * 8 + 2 * cdiv(T * 4, 256) * 256; }
+
+// backward: pieces of the vocabulary, slices of the dX product, workspace
+struct Plan {
+  int64_t piece, pitch;  // words of a piece, dz's pitch in elements
+  int slices;
+  int64_t dz, acc, most, bytes;
+};
+constexpr int64_t DZ_BYTES = (int64_t)512 << 20;
+static Plan plan_of(int64_t T, int64_t H, int64_t V) {
+  Plan p;
+  const int64_t hp = cdiv(H, 64) * 64, most = std::max<int64_t>(256, DZ_BYTES / (std::max<int64_t>(T, 1) * 2) / 256 * 256);
+  const int64_t n = cdiv(V, most);
+  p.piece = cdiv(cdiv(V, n), 256) * 256;
+  p.pitch = std::min(p.piece, cdiv(V, 64) * 64);
+  const int64_t tiles = cdiv(T, TM) * cdiv(H, TN), steps = cdiv(p.pitch, KSTEP);
+  p.slices = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(split_device_cus() / std::max<int64_t>(tiles, 1), steps / 8), 16));
+  p.dz = cdiv(T * p.pitch * 2, 256) * 256;
+  p.acc = T * hp * 4 * p.slices;
+  p.most = p.dz + p.acc;
+  p.bytes = p.most + 256;
+  return p;
+}
+
+static int check(const char* fn, const void* w, int64_t T, int64_t H, int64_t V, int64_t ldw) {
+  if (T < 0 || H < 1 || V < 1) return fail(NTLB_EINVAL, "%s: bad shape T %lld H %lld V %lld", fn, (long long)T, (long long)H, (long long)V);
+  if (T > (1 << 24) || V > (1 << 30) || H > (1 << 20)) return fail(NTLB_EUNSUPPORTED, "%s: T %lld H %lld V %lld is too large", fn, (long long)T, (long long)H, (long long)V);
+  if (!w || !aligned(w, 16) || ldw < H || ldw % 8) return fail(NTLB_EINVAL, "%s: the weight needs 16-byte rows of at least H values", fn);
+  return NTLB_OK;
+}
+
+}  // namespace xent
+}  // namespace ntlb
+
+using namespace ntlb;
+
+extern "C" int64_t ntlb_linear_xent_state_bytes(int64_t T, int64_t H) { return T < 1 || H < 1 ? 256 : xent::state_of(T, H).bytes; }
+
+extern "C" int64_t ntlb_linear_xent_workspace_bytes(int64_t T, int64_t H, int64_t V, int backward) {
+  if (T < 1 || H < 1 || V < 1) return 0;
+  return backward ? xent::plan_of(T, H, V).bytes : xent::forward_ws(T, V);
+}
+
+extern "C" int ntlb_linear_xent_forward(const uint16_t* x, int64_t ldx, const uint16_t* w, int64_t ldw,
+                                        const void* targets, int targets64, int64_t T, int64_t H, int64_t V,
+                                        int64_t ignore_index, int reduction, float* loss, void* state, void* workspace,
+                                        int64_t ws_bytes, void* stream) {
+  const char* fn = "ntlb_linear_xent_forward";
+  clear_error();
+  if (int rc = xent::check(fn, w, T, H, V, ldw)) return rc;
+  if (reduction < 0 || reduction > 2) return fail(NTLB_EINVAL, "%s: bad reduction %d", fn, reduction);
+  if (!loss || !state || !aligned(state, 256)) return fail(NTLB_EINVAL, "%s: NULL pointer", fn);
+  if (T > 0 && (!x || !targets || (ldx != 0 && ldx < H))) return fail(NTLB_EINVAL, "%s: bad hidden or targets", fn);
+  const int64_t need = T > 0 ? xent::forward_ws(T, V) : 0;
+  if (ws_bytes < need || (need && (!workspace || !aligned(workspace, 16)))) return fail(NTLB_EINVAL, "%s: workspace of %lld bytes, %lld needed", fn, (long long)ws_bytes, (long long)need);
+  hipStream_t st = as_stream(stream);
+  const xent::State s = xent::state_of(std::max<int64_t>(T, 1), H);
+  uint8_t* sp = (uint8_t*)state;
+  int32_t *pos = (int32_t*)(sp + s.pos), *rows = (int32_t*)(sp + s.rows), *y = (int32_t*)(sp + s.y), *live = (int32_t*)(sp + s.live);
+  float* lse = (float*)(sp + s.lse);
+  uint16_t* xp = (uint16_t*)(sp + s.xp);
+  xent::scan_kernel<<<1, xent::SCAN, 0, st>>>(targets, targets64, T, V, ignore_index, pos, rows, y, live);
+  float *zl = nullptr, *each = nullptr;
+  if (T > 0) {
+    const int64_t parts = cdiv(V, xent::TN);
+    float2* part = (float2*)workspace;
+    zl = (float*)((uint8_t*)workspace + parts * T * 8);
+    each = zl + cdiv(T * 4, 256) * 64;
+    const int al = aligned(x, 16) && ldx % 8 == 0;
+    xent::gather_kernel<<<(unsigned)T, 256, 0, st>>>(x, ldx, T, H, al, pos, xp, s.hp, zl, reduction == 0 ? loss : nullptr);
+    xent::Args g{};
+    g.a = {(const uint8_t*)xp, s.hp * 2, T, s.hp};
+    g.b = {(const uint8_t*)w, ldw * 2, V, H};
+    g.M = T; g.N = V; g.live = live; g.group_m = 8; g.part = part; g.ldp = T; g.zl = zl; g.y = y;
+    const int64_t tiles = cdiv(T, xent::TM) * parts;
+    xent::head_kernel<false, false, xent::EPI_LSE><<<(unsigned)tiles, xent::NT, 0, st>>>(g);
+    xent::join_kernel<<<(unsigned)cdiv(T, 16), 256, 0, st>>>(part, T, parts, zl, rows, live, lse, each, reduction == 0 ? loss : nullptr);
+  }
+  if (reduction != 0) xent::total_kernel<<<1, 1024, 0, st>>>(each, live, reduction == 2, loss);
+  return check_launch(fn);
+}
+
+extern "C" int ntlb_linear_xent_backward(const void* state, const uint16_t* w, int64_t ldw, int64_t T, int64_t H,
+                                         int64_t V, int reduction, const float* dloss, uint16_t* dx, int64_t lddx,
+                                         uint16_t* dw, int64_t lddw, void* workspace, int64_t ws_bytes, void* stream) {
+  const char* fn = "ntlb_linear_xent_backward";
+  clear_error();
+  if (int rc = xent::check(fn, w, T, H, V, ldw)) return rc;
+  if (reduction < 0 || reduction > 2) return fail(NTLB_EINVAL, "%s: bad reduction %d", fn, reduction);
+  if (!state || !aligned(state, 256) || (T > 0 && !dloss)) return fail(NTLB_EINVAL, "%s: NULL pointer", fn);
+  if ((dx && lddx < H) || (dw && lddw < H)) return fail(NTLB_EINVAL, "%s: a gradient's pitch is below H", fn);
+  if (T == 0 && !dw) return NTLB_OK;
+  const int64_t Tn = std::max<int64_t>(T, 1);
+  const xent::Plan p = xent::plan_of(Tn, H, V);
+  if (ws_bytes < p.bytes || !workspace || !aligned(workspace, 16)) return fail(NTLB_EINVAL, "%s: workspace of %lld bytes, %lld needed", fn, (long long)ws_bytes, (long long)p.bytes);
+  hipStream_t st = as_stream(stream);
+  const xent::State s = xent::state_of(Tn, H);
+  const uint8_t* sp = (const uint8_t*)state;
+  const int32_t* live = (const int32_t*)(sp + s.live);
+  uint16_t* dz = (uint16_t*)workspace;
+  float* acc = (float*)((uint8_t*)workspace + p.dz);
+  float* most = reduction == 0 ? (float*)((uint8_t*)workspace + p.most) : nullptr;
+  const xent::Up up{dloss, most, reduction == 2};
+  if (most) xent::most_kernel<<<1, 1024, 0, st>>>(dloss, (const int32_t*)(sp + s.rows), live, most);
+  for (int64_t v0 = 0; v0 < V; v0 += p.piece) {
+    const int64_t n = std::min(p.piece, V - v0), np = cdiv(n, 64) * 64;
+    const uint8_t* wp = (const uint8_t*)(w + v0 * ldw);
+    xent::Args g{};
+    g.live = live; g.group_m = 8;
+    g.a = {sp + s.xp, s.hp * 2, Tn, s.hp};
+    g.b = {wp, ldw * 2, n, H};
+    g.M = T; g.N = n; g.y = (const int32_t*)(sp + s.y); g.v0 = v0; g.lse = (const float*)(sp + s.lse);
+    g.rows = (const int32_t*)(sp + s.rows); g.up = up;
+    g.out = dz; g.ldo = np;
+    const int64_t tm = cdiv(T, xent::TM), tn = cdiv(n, xent::TN), th = cdiv(H, xent::TN);
+    if (T > 0) xent::head_kernel<false, false, xent::EPI_DZ><<<(unsigned)(tm * tn), xent::NT, 0, st>>>(g);
+    if (dx && T > 0) {
+      xent::Args x{};
+      x.live = live; x.group_m = 8; x.slices = p.slices;
+      x.a = {(const uint8_t*)dz, np * 2, Tn, np};
+      x.b = {wp, ldw * 2, H, n};
+      x.M = T; x.N = H; x.out = acc; x.ldo = s.hp; x.slice = T * s.hp; x.add = v0 > 0;
+      xent::head_kernel<false, true, xent::EPI_ACC><<<(unsigned)(tm * th * p.slices), xent::NT, 0, st>>>(x);
+    }
+    if (dw) {
+      xent::Args q{};
+      q.live = live; q.group_m = 8;
+      q.a = {(const uint8_t*)dz, np * 2, np, Tn};
+      q.b = {sp + s.xp, s.hp * 2, s.hp, Tn};
+      q.M = n; q.N = H; q.out = dw + v0 * lddw; q.ldo = lddw;
+      q.up = up;
+      q.vec_out = aligned(dw, 8) && lddw % 4 == 0;
+      xent::head_kernel<true, true, xent::EPI_STORE><<<(unsigned)(tn * th), xent::NT, 0, st>>>(q);
+    }
+  }
+  if (dx && T > 0)
+    xent::scatter_kernel<<<(unsigned)T, 256, 0, st>>>(acc, s.hp, T * s.hp, p.slices, up, live, (const int32_t*)(sp + s.pos),
+                                                     H, dx, lddx);
+  return check_launch(fn);
+}

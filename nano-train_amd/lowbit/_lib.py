@@ -143,6 +143,10 @@ SIGNATURES = {
     "ntlb_layer_norm_workspace_bytes": [_I32, _I64, _I64],
     "ntlb_route_topk": [_P, _I32, _I64, _I64, _I64, _I64, _I32, _P, _I64, _I64, _I32, _F32, _P, _P, _P],
     "ntlb_route_topk_backward": [_P, _I32, _I64, _I64, _I64, _I64, _I32, _I32, _F32, _P, _P, _P, _I64, _P],
+    "ntlb_linear_xent_forward": [_P, _I64, _P, _I64, _P, _I32, _I64, _I64, _I64, _I64, _I32, _P, _P, _P, _I64, _P],
+    "ntlb_linear_xent_backward": [_P, _P, _I64, _I64, _I64, _I64, _I32, _P, _P, _I64, _P, _I64, _P, _I64, _P],
+    "ntlb_linear_xent_state_bytes": [_I64, _I64],
+    "ntlb_linear_xent_workspace_bytes": [_I64, _I64, _I64, _I32],
 }
 
 
@@ -160,7 +164,8 @@ class LinearPlan(ctypes.Structure):
 RESTYPES = {"ntlb_gemm_workspace_bytes": _I64, "ntlb_ep_record_bytes": _I64, "ntlb_colsum_workspace_bytes": _I64,
             "ntlb_ep_value_record_bytes": _I64, "ntlb_persistent_quant_ws_words": _I64,
             "ntlb_gemm_lowbit_workspace_bytes": _I64, "ntlb_gemm_dq_workspace_bytes": _I64,
-            "ntlb_layer_norm_workspace_bytes": _I64}
+            "ntlb_layer_norm_workspace_bytes": _I64, "ntlb_linear_xent_state_bytes": _I64,
+            "ntlb_linear_xent_workspace_bytes": _I64}
 
 _lib = None
 _lock = threading.Lock()

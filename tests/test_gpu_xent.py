@@ -1,0 +1,338 @@
+"""GPU tests of lowbit.loss.linear_cross_entropy against the definition in 64 bits.
+
+Bounds, with u = 2^-24 and S_t = max over the words of sum_h |x_th w_vh|: a
+logit adds H exact products in fp32, H roundings of at most u S each, taken as
+independent: off by at most e = 4 sqrt(H) u S (four deviations).  A loss moves
+by at most twice that, plus 16 u of |logsumexp| and the logit (exp, log, the
+joins).  dz = u_t (p - 1[y]) is off by 4 e + 32 u |lse| relative to u_t p and
+rounded to bf16 once (2^-8); dX and dW follow elementwise by the triangle
+inequality over their sums, with 4 sqrt(n) u for the n additions and the
+output's 2^-8.  The roundings of dz and of the output are independent, each of
+at most 2^-8 and 2^-8 / sqrt(3) in the mean square, so a gradient as a whole is
+within 2^-8 in the Frobenius norm.
+"""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+B = 2.0 ** -8
+IGNORE = -100
+
+
+def _inputs(T, H, V, seed, dev, ignored=0.0, scale=1.0):
+    g = torch.Generator().manual_seed(seed)
+    w = (torch.randn(V, H, generator=g) * 0.05).bfloat16()
+    y = torch.randint(0, V, (T,), generator=g)
+    x = ((torch.randn(T, H, generator=g) + 20.0 / math.sqrt(H) * torch.rand(T, 1, generator=g) * w[y].float()) * scale)
+    y = torch.where(torch.rand(T, generator=g) < ignored, IGNORE, y)
+    return x.bfloat16().to(dev), w.to(dev), y.to(dev), g
+
+
+def _check(x, w, y, loss, dx, dw, reduction, dloss, ignore=IGNORE):
+    """loss / dx / dw (each may be None) of 2-D x against 64 bits"""
+    T, H = x.shape
+    V = w.shape[0]
+    live = y != ignore
+    xd, wd = torch.where(live[:, None], x.double(), 0.0), w.double()
+    z = xd @ wd.t()
+    lse = torch.logsumexp(z, 1)
+    at = torch.where(live, y, 0).long()[:, None]
+    each = torch.where(live, lse - z.gather(1, at)[:, 0], 0.0)
+    n = max(1, int(live.sum()))
+    e = 4 * math.sqrt(H) * U * (xd.abs() @ wd.abs().t()).amax(1)
+    off = torch.where(live, 2 * e + 16 * U * (lse.abs() + z.gather(1, at)[:, 0].abs()), 0.0)
+    if loss is not None:
+        if reduction == "none":
+            want, bound = each, off
+        else:
+            div = n if reduction == "mean" else 1
+            want, bound = each.sum() / div, (off.sum() + 4 * math.sqrt(n) * U * each.sum()) / div
+        assert loss.dtype == torch.float32 and ((loss.double() - want).abs() <= bound).all()
+    if dx is None and dw is None:
+        return
+    up = (dloss.double() if reduction == "none" else (dloss.double() / (n if reduction == "mean" else 1)).expand(T))
+    up = torch.where(live, up, 0.0)[:, None]
+    p = torch.softmax(z, 1)
+    dz = p.clone().scatter_add_(1, at, torch.full_like(up, -1.0)) * up
+    err = B * dz.abs() + up.abs() * p * (4 * e + 32 * U * lse.abs())[:, None]
+    for got, want, mag, er, terms in ((dx, lambda m: m @ wd, lambda m: m @ wd.abs(), err, V),
+                                      (dw, lambda m: m.t() @ xd, lambda m: m.t() @ xd.abs(), err, n)):
+        if got is None:
+            continue
+        want = want(dz)
+        bound = mag(er) + 4 * math.sqrt(terms) * U * mag(dz.abs()) + B * want.abs() + 1e-37
+        diff = (got.double() - want).abs()
+        assert got.dtype == torch.bfloat16 and (diff <= bound).all(), float((diff / bound).max())
+        if want.norm() > 0:
+            assert diff.norm() <= B * want.norm(), float(diff.norm() / want.norm())
+
+
+SIZES = [(1, 64, 256), (1, 8, 1), (3, 5, 7), (16, 1024, 3001), (257, 1000, 5003), (300, 513, 700), (64, 72, 260),
+         (1003, 520, 2111), (513, 192, 20011), (37, 2048, 9000), (255, 64, 257), (600, 1541, 500), (2049, 300, 1023)]
+
+
+@pytest.mark.parametrize("T,H,V", SIZES)
+@pytest.mark.parametrize("reduction,ignored", [("mean", 0.0), ("none", 0.4), ("sum", 0.05)])
+def test_loss_and_gradients(gpu_device, T, H, V, reduction, ignored):
+    from lowbit.loss import linear_cross_entropy
+
+    x, w, y, g = _inputs(T, H, V, T + H + V, gpu_device, ignored)
+    with torch.no_grad():
+        l0 = linear_cross_entropy(x, w, y, reduction=reduction)
+    xl, wl = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    loss = linear_cross_entropy(xl, wl, y, reduction=reduction)
+    dl = (torch.randn(T, generator=g) if reduction == "none" else torch.tensor(0.7)).to(gpu_device)
+    dx, dw = torch.autograd.grad(loss, (xl, wl), dl, retain_graph=True)
+    assert loss.shape == ((T,) if reduction == "none" else ()) and torch.equal(loss.detach(), l0)
+    _check(x, w, y, loss.detach(), dx, dw, reduction, dl)
+    again = torch.autograd.grad(loss, (xl, wl), dl)
+    assert torch.equal(dx, again[0]) and torch.equal(dw, again[1])
+
+
+def test_several_pieces_of_the_vocabulary(gpu_device):
+    from lowbit.loss import linear_cross_entropy
+
+    T, H, V = 8192, 64, 40001
+    x, w, y, _ = _inputs(T, H, V, 3, gpu_device, 0.02)
+    xl, wl = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    loss = linear_cross_entropy(xl, wl, y)
+    dx, dw = torch.autograd.grad(loss, (xl, wl))
+    _check(x, w, y, loss.detach(), dx, dw, "mean", torch.ones((), device=gpu_device))
+
+
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+def test_all_ignored(gpu_device, reduction):
+    from lowbit.loss import linear_cross_entropy
+
+    x, w, y, _ = _inputs(70, 96, 300, 4, gpu_device)
+    y[:] = IGNORE
+    xl, wl = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    loss = linear_cross_entropy(xl, wl, y, reduction=reduction)
+    assert not loss.detach().any()
+    loss.sum().backward()
+    assert not xl.grad.any() and not wl.grad.any() and xl.grad.isfinite().all()
+
+
+def test_ignored_rows_cannot_pass_on_a_nan(gpu_device):
+    """ignored rows hold NaN and infinity; the ignore index may lie inside the vocabulary"""
+    from lowbit.loss import linear_cross_entropy
+
+    x, w, y, _ = _inputs(400, 200, 900, 5, gpu_device)
+    y[::3] = 17
+    x[::3] = float("nan")
+    x[3] = float("inf")
+    xl, wl = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    loss = linear_cross_entropy(xl, wl, y, ignore_index=17, reduction="sum")
+    dx, dw = torch.autograd.grad(loss, (xl, wl))
+    assert not dx[::3].any()
+    _check(x.nan_to_num(0.0, 0.0), w, y, loss.detach(), dx, dw, "sum", torch.ones((), device=gpu_device), ignore=17)
+
+
+def test_a_target_outside_the_vocabulary_is_loud(gpu_device):
+    from lowbit.loss import linear_cross_entropy
+
+    x, w, y, _ = _inputs(50, 64, 300, 6, gpu_device)
+    want = linear_cross_entropy(x, w, y, reduction="none")
+    y[7], y[9] = 300, -1
+    xl = x.clone().requires_grad_(True)
+    loss = linear_cross_entropy(xl, w, y, reduction="none")
+    bad = torch.zeros(50, dtype=torch.bool, device=gpu_device)
+    bad[[7, 9]] = True
+    assert loss.detach()[bad].isnan().all() and torch.equal(loss.detach()[~bad], want[~bad])
+    loss.sum().backward()
+    assert xl.grad[bad].isnan().all() and xl.grad[~bad].isfinite().all()
+
+
+def test_nan_and_infinite_rows(gpu_device):
+    from lowbit.loss import linear_cross_entropy
+
+    x, w, y, _ = _inputs(20, 64, 700, 7, gpu_device)
+    want = linear_cross_entropy(x, w, y, reduction="none")
+    x[3, 5], x[8, 0] = float("nan"), float("inf")
+    loss = linear_cross_entropy(x, w, y, reduction="none")
+    bad = torch.zeros(20, dtype=torch.bool, device=gpu_device)
+    bad[[3, 8]] = True
+    assert loss[bad].isnan().all() and torch.equal(loss[~bad], want[~bad])
+
+
+def test_large_logits(gpu_device):
+    """logits of several hundred: exp overflows without the maximum taken off"""
+    from lowbit.loss import linear_cross_entropy
+
+    x, w, y, _ = _inputs(130, 512, 1500, 8, gpu_device, scale=300.0)
+    xl, wl = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    loss = linear_cross_entropy(xl, wl, y, reduction="none")
+    dl = torch.ones(130, device=gpu_device)
+    dx, dw = torch.autograd.grad(loss, (xl, wl), dl)
+    assert loss.max() > 300
+    _check(x, w, y, loss.detach(), dx, dw, "none", dl)
+
+
+@pytest.mark.parametrize("which", ["pitch", "offset", "repeated", "3d", "weight_pitch", "weight_offset", "weight_t",
+                                   "int32", "targets_strided"])
+def test_strides_and_types(gpu_device, which):
+    from lowbit.loss import linear_cross_entropy
+
+    T, H, V = 60, 256, 800
+    x, w, y, _ = _inputs(T, H + 16, V, 9, gpu_device, 0.1)
+    xv, wv, yv = x[:, :H].contiguous(), w[:, :H].contiguous(), y
+    if which == "pitch":
+        xv = x[:, :H]
+    elif which == "offset":
+        xv = x[:, 5:5 + H]
+    elif which == "repeated":
+        xv = x[:1, :H].expand(T, H)
+    elif which == "3d":
+        xv, yv = x[:, :H].reshape(6, 10, H), y.reshape(6, 10)
+    elif which == "weight_pitch":
+        wv = w[:, 8:8 + H]
+    elif which == "weight_offset":
+        wv = w[:, 3:3 + H]
+    elif which == "weight_t":
+        wv = w[:, :H].t().contiguous().t()
+    elif which == "int32":
+        yv = y.int()
+    else:
+        yv = torch.stack([y, y + 1], 1)[:, 0]
+    xl, wl = xv.detach().requires_grad_(True), wv.detach().requires_grad_(True)
+    loss = linear_cross_entropy(xl, wl, yv, reduction="sum")
+    dx, dw = torch.autograd.grad(loss, (xl, wl))
+    assert dx.shape == xv.shape and dw.shape == wv.shape
+    _check(xv.reshape(T, H), wv, yv.reshape(T), loss.detach(), dx.reshape(T, H), dw, "sum",
+           torch.ones((), device=gpu_device))
+
+
+@pytest.mark.parametrize("which", ["hidden", "weight"])
+def test_one_gradient_alone(gpu_device, which):
+    from lowbit.loss import linear_cross_entropy
+
+    x, w, y, _ = _inputs(90, 128, 1000, 10, gpu_device, 0.2)
+    xl, wl = x.clone().requires_grad_(which == "hidden"), w.clone().requires_grad_(which == "weight")
+    loss = linear_cross_entropy(xl, wl, y)
+    loss.backward()
+    assert (xl.grad is None) == (which != "hidden") and (wl.grad is None) == (which != "weight")
+    _check(x, w, y, loss.detach(), xl.grad, wl.grad, "mean", torch.ones((), device=gpu_device))
+
+
+def test_no_positions(gpu_device):
+    from lowbit.loss import linear_cross_entropy
+
+    x = torch.empty(0, 64, device=gpu_device, dtype=torch.bfloat16, requires_grad=True)
+    w = torch.randn(100, 64, device=gpu_device).bfloat16().requires_grad_(True)
+    y = torch.empty(0, dtype=torch.int64, device=gpu_device)
+    for reduction in ("mean", "sum", "none"):
+        loss = linear_cross_entropy(x, w, y, reduction=reduction)
+        dx, dw = torch.autograd.grad(loss.sum(), (x, w))
+        assert float(loss.detach().sum()) == 0 and dx.shape == (0, 64) and not dw.any()
+
+
+def test_gradient_against_differences(gpu_device):
+    """central differences of the kernel's own losses along directions that bf16 holds exactly: x and w are whole
+    multiples of 2^-6 and the steps of 2^-5, all below 2 in magnitude.  The h^2 term is removed by h and 2h; the
+    gradients are bf16 (2^-8 of the magnitudes that meet) and the losses off by 2 e each."""
+    from lowbit.loss import linear_cross_entropy
+
+    T, H, V, h = 20, 32, 50, 2.0 ** -5
+    g = torch.Generator().manual_seed(11)
+    q = lambda *s: (torch.randint(-64, 65, s, generator=g).float() / 64).to(gpu_device)  # noqa: E731
+    x, w = q(T, H), q(V, H)
+    sx = torch.randint(-1, 2, (T, H), generator=g).float().to(gpu_device)
+    sw = torch.randint(-1, 2, (V, H), generator=g).float().to(gpu_device)
+    y = torch.randint(0, V, (T,), generator=g).to(gpu_device)
+    f = lambda a, b: linear_cross_entropy((x + a * sx).bfloat16(), (w + b * sw).bfloat16(), y,  # noqa: E731
+                                          reduction="none").double().sum()
+    xl, wl = x.bfloat16().requires_grad_(True), w.bfloat16().requires_grad_(True)
+    dx, dw = torch.autograd.grad(linear_cross_entropy(xl, wl, y, reduction="sum"), (xl, wl))
+    assert torch.equal((x + 2 * h * sx).bfloat16().float(), x + 2 * h * sx)
+    p = torch.softmax(x.double() @ w.double().t(), 1)
+    dz = p.scatter_add(1, y[:, None], torch.full((T, 1), -1.0, dtype=torch.float64, device=gpu_device)).abs()
+    e = 4 * math.sqrt(H) * U * float((x.abs() @ w.abs().t()).max()) + 32 * U * 10
+    for a, b, got, mag in ((1, 0, (dx.double() * sx).sum(), (dz @ w.double().abs() * sx.abs()).sum()),
+                           (0, 1, (dw.double() * sw).sum(), (dz.t() @ x.double().abs() * sw.abs()).sum())):
+        d1 = (f(a * h, b * h) - f(-a * h, -b * h)) / (2 * h)
+        d2 = (f(2 * a * h, 2 * b * h) - f(-2 * a * h, -2 * b * h)) / (4 * h)
+        # independent roundings of bf16, far fewer than their worst sum: their magnitudes' sum bounds them
+        assert abs(float((4 * d1 - d2) / 3 - got)) <= abs(float(d1 - d2)) + 2 * B * float(mag) + 4 * T * e / h
+
+
+def test_other_stream_and_graph(gpu_device):
+    from lowbit.loss import linear_cross_entropy
+
+    x, w, y, _ = _inputs(100, 320, 3000, 12, gpu_device, 0.3)
+    want = linear_cross_entropy(x, w, y)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = linear_cross_entropy(x, w, y)
+    torch.cuda.current_stream().wait_stream(s)
+    assert torch.equal(got, want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = linear_cross_entropy(x, w, y)
+    for k in range(3):
+        x2, _, y2, _ = _inputs(100, 320, 3000, 20 + k, gpu_device, 0.2 * k)
+        x.copy_(x2)
+        y.copy_(y2)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, linear_cross_entropy(x, w, y))
+
+
+def test_module(gpu_device):
+    from lowbit.loss import LMHeadLoss
+
+    x, w, y, _ = _inputs(30, 64, 500, 13, gpu_device)
+    m = LMHeadLoss(64, 500, weight=torch.nn.Parameter(w))
+    m(x, y).backward()
+    _check(x, w, y, None, None, m.weight.grad, "mean", torch.ones((), device=gpu_device))
+    assert LMHeadLoss(64, 500, device=gpu_device).weight.dtype == torch.bfloat16
+    with pytest.raises(ValueError, match="weight"):
+        LMHeadLoss(64, 501, weight=m.weight)
+
+
+def test_refusals(gpu_device):
+    from lowbit.loss import linear_cross_entropy
+
+    x, w, y, _ = _inputs(4, 64, 100, 14, gpu_device)
+    with pytest.raises(RuntimeError, match="ROCm device"):
+        linear_cross_entropy(x.cpu(), w.cpu(), y.cpu())
+    with pytest.raises(TypeError, match="bfloat16"):
+        linear_cross_entropy(x.float(), w, y)
+    with pytest.raises(TypeError, match="int32 or int64"):
+        linear_cross_entropy(x, w, y.float())
+    with pytest.raises(ValueError, match="reduction"):
+        linear_cross_entropy(x, w, y, reduction="max")
+    with pytest.raises(ValueError, match="weight"):
+        linear_cross_entropy(x, w[:, :32], y)
+    with pytest.raises(ValueError, match="targets"):
+        linear_cross_entropy(x, w, y[:3])
+
+
+@pytest.mark.parametrize("n", [3, 331, 1000])
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_a_common_factor_is_not_rounded(gpu_device, n, reduction):
+    """the factor 1 / n of a mean enters in fp32: rounded into the operands it would scale the whole gradient, so the
+    part of the gradient along the true one is looked at, where independent roundings average out: (dx, want) /
+    (want, want) - 1 is a weighted mean of n * H relative errors of at most 2 * 2^-8 and at most 2^-8 correlated
+    in a row through p - 1; with the labels' p below 1/8 the latter's error is at most 2^-8 / 8"""
+    from lowbit.loss import linear_cross_entropy
+
+    g = torch.Generator().manual_seed(n)
+    H, V = 256, 4000
+    x, w = torch.randn(n, H, generator=g).bfloat16().to(gpu_device), (torch.randn(V, H, generator=g) * 0.05).bfloat16().to(gpu_device)
+    y = torch.randint(0, V, (n,), generator=g).to(gpu_device)
+    xl = x.clone().requires_grad_(True)
+    loss = linear_cross_entropy(xl, w, y, reduction=reduction)
+    (dx,) = torch.autograd.grad(loss, xl, torch.full((n,), 1.0 / n, device=gpu_device) if reduction == "none" else None)
+    p = torch.softmax(x.double() @ w.double().t(), 1)
+    assert p.gather(1, y[:, None]).max() < 0.125
+    want = p.scatter_add(1, y[:, None], torch.full((n, 1), -1.0, dtype=torch.float64, device=gpu_device)) @ w.double() / n
+    part = float((dx.double() * want).sum() / (want * want).sum()) - 1
+    assert abs(part) <= B / 8 + 4 * 2 * B / math.sqrt(n * H)
