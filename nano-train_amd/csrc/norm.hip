@@ -7,7 +7,7 @@
 // and db once to the weights'.
 //
 // HBM-bound: x in, y out; x and dy in, dx out.  A row is read once and stays in
-// registers: RT threads (one wave to eight) hold VPT 16-byte vectors each, and a
+// registers: RT threads (one wave to 16) hold VPT 16-byte vectors each, and a
 // workgroup walks rows with the weights, and in the backward the column sums
 // dw and db, in registers, the next row's loads in flight while this one is
 // reduced.  The variance is the mean of (x - m)^2 over the registers, a second
@@ -48,22 +48,55 @@ __device__ __forceinline__ void renew(Raw& r, float sum) {
   asm("" : "+v"(r.w[0]), "+v"(r.w[1]), "+v"(r.w[2]), "+v"(r.w[3]) : "v"(sum));
 }
 
-// elements [c, c + n) of a row of H elements, zero past it
-template <int DT>
-__device__ __forceinline__ Raw load_vec(const void* row, int c, int H) {
-  constexpr int N = El<DT>::n;
-  Raw r = {{0, 0, 0, 0}};
-  if (c + N <= H) {
-    const u32x4_2 v = *reinterpret_cast<const u32x4_2*>((const uint8_t*)row + (size_t)c * El<DT>::bytes);
+// How a row divides into vectors of n elements: WHOLE: H is a multiple of n;
+// RAGGED: the last vector of a row begins at H - n and shares elements with the
+// one before it; TINY: H < n.  A thread with no vector of its own takes the last
+// one again.  So every access is unconditional and in bounds, and a shared
+// element is computed alike by those that hold it (who may all store it); only
+// sums must count it once.  (A branch around a load or store would make the
+// compiler wait for everything in flight.)
+constexpr int WHOLE = 0, RAGGED = 1, TINY = 2;
+
+template <int DT, int MODE>
+struct Span {
+  static constexpr int N = El<DT>::n;
+  int c;      // first column
+  int first;  // first element of its own
+  int end;    // TINY: elements in the row
+  __device__ __forceinline__ Span(int vec, int H) {
+    const int c0 = vec * N;
+    if constexpr (MODE == TINY) {
+      c = 0;
+      first = vec == 0 ? 0 : N;
+      end = H;
+    } else {
+      c = min(c0, H - N);
+      first = min(c0 - c, N);
+      end = N;
+    }
+  }
+  __device__ __forceinline__ bool own(int i) const {
+    if constexpr (MODE == WHOLE) return first == 0;
+    if constexpr (MODE == RAGGED) return i >= first;
+    return first == 0 && i < end;
+  }
+};
+
+template <int DT, int MODE>
+__device__ __forceinline__ Raw load_vec(const void* row, const Span<DT, MODE>& s) {
+  Raw r;
+  if constexpr (MODE != TINY) {
+    const u32x4_2 v = *reinterpret_cast<const u32x4_2*>((const uint8_t*)row + (uint32_t)s.c * El<DT>::bytes);
     r.w[0] = v[0]; r.w[1] = v[1]; r.w[2] = v[2]; r.w[3] = v[3];
-  } else if (c < H) {
+  } else {
+    r = {{0, 0, 0, 0}};
 #pragma unroll
-    for (int i = 0; i < N; ++i)
-      if (c + i < H) {
+    for (int i = 0; i < El<DT>::n; ++i)
+      if (i < s.end) {
         if constexpr (DT == DT_F32)
-          r.w[i] = ((const uint32_t*)row)[c + i];
+          r.w[i] = ((const uint32_t*)row)[i];
         else
-          r.w[i >> 1] |= (uint32_t)((const uint16_t*)row)[c + i] << (16 * (i & 1));
+          r.w[i >> 1] |= (uint32_t)((const uint16_t*)row)[i] << (16 * (i & 1));
       }
   }
   return r;
@@ -82,9 +115,8 @@ __device__ __forceinline__ void unpack(const Raw& r, float (&f)[El<DT>::n]) {
   }
 }
 
-template <int DT>
-__device__ __forceinline__ void store_vec(void* row, int c, int H, const float (&f)[El<DT>::n]) {
-  constexpr int N = El<DT>::n;
+template <int DT, int MODE>
+__device__ __forceinline__ void store_vec(void* row, const Span<DT, MODE>& s, const float (&f)[El<DT>::n]) {
   uint32_t w[4];
   if constexpr (DT == DT_F32) {
 #pragma unroll
@@ -101,17 +133,18 @@ __device__ __forceinline__ void store_vec(void* row, int c, int H, const float (
       }
     }
   }
-  if (c + N <= H) {
+  if constexpr (MODE != TINY) {
     const u32x4_2 v = {w[0], w[1], w[2], w[3]};
-    *reinterpret_cast<u32x4_2*>((uint8_t*)row + (size_t)c * El<DT>::bytes) = v;
+    // streamed: not read again here (8192 x 7168 bf16 forward: 47 us without the hint, 44 with it)
+    __builtin_nontemporal_store(v, reinterpret_cast<u32x4_2*>((uint8_t*)row + (uint32_t)s.c * El<DT>::bytes));
   } else {
 #pragma unroll
-    for (int i = 0; i < N; ++i)
-      if (c + i < H) {
+    for (int i = 0; i < El<DT>::n; ++i)
+      if (s.own(i)) {
         if constexpr (DT == DT_F32)
-          ((uint32_t*)row)[c + i] = w[i];
+          ((uint32_t*)row)[i] = w[i];
         else
-          ((uint16_t*)row)[c + i] = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
+          ((uint16_t*)row)[i] = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
       }
   }
 }
@@ -168,17 +201,55 @@ struct Args {
   float* part;  // [2][workgroups][H]: dw, db
 };
 
-// a column vector of the weights as floats (w NULL: `none`)
-template <int N>
-__device__ __forceinline__ void load_weights(const void* w, int dt, int c, int H, float none, float (&f)[N]) {
+// the weights of a thread's vectors as floats (w NULL: `none`), there before
+// anything else is issued: the kernel's one branch on types, outside its loop
+template <int WDT, int DT, int RT, int VPT, int MODE>
+__device__ __forceinline__ void load_weights_of(const void* w, int t, int H, float (&f)[VPT][El<DT>::n]) {
+  constexpr int N = El<DT>::n, M = El<WDT>::n;
 #pragma unroll
-  for (int i = 0; i < N; ++i) f[i] = w && c + i < H ? load_elem(w, dt, c + i) : none;
+  for (int v = 0; v < VPT; ++v) {
+    const Span<DT, MODE> s(t + v * RT, H);
+    if constexpr (MODE == TINY || M > N) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) f[v][i] = load_elem(w, WDT, min(s.c + i, H - 1));
+    } else {
+#pragma unroll
+      for (int h = 0; h < N / M; ++h) {
+        Span<WDT, MODE> q(0, H);
+        q.c = s.c + h * M;
+        float u[M];
+        unpack<WDT>(load_vec<WDT, MODE>(w, q), u);
+#pragma unroll
+        for (int i = 0; i < M; ++i) f[v][h * M + i] = u[i];
+      }
+    }
+  }
+}
+template <int DT, int RT, int VPT, int MODE>
+__device__ __forceinline__ void load_weights(const void* w, int dt, int t, int H, float none,
+                                             float (&f)[VPT][El<DT>::n]) {
+  if (!w) {
+#pragma unroll
+    for (int v = 0; v < VPT; ++v)
+#pragma unroll
+      for (int i = 0; i < El<DT>::n; ++i) f[v][i] = none;
+  } else if (dt == DT_F32) {
+    load_weights_of<DT_F32, DT, RT, VPT, MODE>(w, t, H, f);
+  } else if (dt == DT_BF16) {
+    load_weights_of<DT_BF16, DT, RT, VPT, MODE>(w, t, H, f);
+  } else {
+    load_weights_of<DT_F16, DT, RT, VPT, MODE>(w, t, H, f);
+  }
+#pragma unroll
+  for (int v = 0; v < VPT; ++v)
+#pragma unroll
+    for (int i = 0; i < El<DT>::n; ++i) asm volatile("" : "+v"(f[v][i]));
 }
 
 template <int RT>
-constexpr int block_threads() { return RT < 256 ? 256 : RT; }
+constexpr int block_threads() { return RT == 64 ? 256 : RT; }  // one-wave rows share no barrier
 
-template <int DT, int RT, int VPT>
+template <int DT, int RT, int VPT, int MODE>
 __global__ void __launch_bounds__(block_threads<RT>()) forward_kernel(Args g) {
   constexpr int N = El<DT>::n, ROWS = block_threads<RT>() / RT;
   __shared__ float red[2][RT / 64];
@@ -188,42 +259,41 @@ __global__ void __launch_bounds__(block_threads<RT>()) forward_kernel(Args g) {
   int64_t row = (int64_t)blockIdx.x * ROWS + __builtin_amdgcn_readfirstlane(threadIdx.x / RT);
   const float inv = 1.0f / (float)H;
   float w[VPT][N], b[VPT][N];
-#pragma unroll
-  for (int v = 0; v < VPT; ++v) {
-    load_weights(g.w, g.w_dtype, (t + v * RT) * N, H, 1.0f, w[v]);
-    load_weights(g.b, g.w_dtype, (t + v * RT) * N, H, 0.0f, b[v]);
-  }
+  load_weights<DT, RT, VPT, MODE>(g.w, g.w_dtype, t, H, 1.0f, w);
+  load_weights<DT, RT, VPT, MODE>(g.b, g.w_dtype, t, H, 0.0f, b);
   Raw nx[VPT];
   auto fetch = [&](int64_t r) {
     const uint8_t* p = (const uint8_t*)g.x + r * g.ldx;
 #pragma unroll
-    for (int v = 0; v < VPT; ++v) nx[v] = load_vec<DT>(p, (t + v * RT) * N, H);
+    for (int v = 0; v < VPT; ++v) nx[v] = load_vec(p, Span<DT, MODE>(t + v * RT, H));
   };
   if (row < g.T) fetch(row);
   for (; row < g.T; row += stride) {
     Raw x[VPT];
 #pragma unroll
     for (int v = 0; v < VPT; ++v) x[v] = nx[v];
-    if (row + stride < g.T) fetch(row + stride);
+    fetch(min<int64_t>(row + stride, g.T - 1));  // past the end: the last row again
     float s[1] = {0.f};
 #pragma unroll
     for (int v = 0; v < VPT; ++v) {
+      const Span<DT, MODE> sp(t + v * RT, H);
       float f[N];
       unpack<DT>(x[v], f);
 #pragma unroll
-      for (int i = 0; i < N; ++i) s[0] += f[i];
+      for (int i = 0; i < N; ++i) s[0] += sp.own(i) ? f[i] : 0.f;
     }
     row_sum<RT, 1>(s, red[0]);
     const float m = s[0] * inv;
     float q[1] = {0.f};
 #pragma unroll
     for (int v = 0; v < VPT; ++v) {
+      const Span<DT, MODE> sp(t + v * RT, H);
       float f[N];
       renew(x[v], m);
       unpack<DT>(x[v], f);
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        const float d = (t + v * RT) * N + i < H ? f[i] - m : 0.f;
+        const float d = sp.own(i) ? f[i] - m : 0.f;
         q[0] += d * d;
       }
     }
@@ -232,13 +302,12 @@ __global__ void __launch_bounds__(block_threads<RT>()) forward_kernel(Args g) {
     uint8_t* yp = (uint8_t*)g.y + row * g.ldy;
 #pragma unroll
     for (int v = 0; v < VPT; ++v) {
-      const int c = (t + v * RT) * N;
       float f[N];
       renew(x[v], r);
       unpack<DT>(x[v], f);
 #pragma unroll
       for (int i = 0; i < N; ++i) f[i] = (f[i] - m) * r * w[v][i] + b[v][i];
-      if (c < H) store_vec<DT>(yp, c, H, f);
+      store_vec(yp, Span<DT, MODE>(t + v * RT, H), f);
     }
     if (g.mean && t == 0) {
       g.mean[row] = m;
@@ -248,7 +317,7 @@ __global__ void __launch_bounds__(block_threads<RT>()) forward_kernel(Args g) {
 }
 
 // DX: dx is wanted; DW: the partial sums of dw and db are
-template <int DT, int RT, int VPT, bool DX, bool DW>
+template <int DT, int RT, int VPT, int MODE, bool DX, bool DW>
 __global__ void __launch_bounds__(block_threads<RT>()) backward_kernel(Args g) {
   constexpr int N = El<DT>::n, BT = block_threads<RT>(), ROWS = BT / RT;
   __shared__ float red[2][RT / 64 * 2];
@@ -258,12 +327,11 @@ __global__ void __launch_bounds__(block_threads<RT>()) backward_kernel(Args g) {
   int64_t row = (int64_t)blockIdx.x * ROWS + __builtin_amdgcn_readfirstlane(threadIdx.x / RT);
   const float inv = 1.0f / (float)H;
   float w[VPT][N], aw[VPT][N], ab[VPT][N];
+  if constexpr (DX) load_weights<DT, RT, VPT, MODE>(g.w, g.w_dtype, t, H, 1.0f, w);
 #pragma unroll
-  for (int v = 0; v < VPT; ++v) {
-    if constexpr (DX) load_weights(g.w, g.w_dtype, (t + v * RT) * N, H, 1.0f, w[v]);
+  for (int v = 0; v < VPT; ++v)
 #pragma unroll
     for (int i = 0; i < N; ++i) aw[v][i] = ab[v][i] = 0.f;
-  }
   Raw nx[VPT], nd[VPT];
   float nm = 0.f, nr = 0.f;
   auto fetch = [&](int64_t r) {
@@ -271,8 +339,8 @@ __global__ void __launch_bounds__(block_threads<RT>()) backward_kernel(Args g) {
     const uint8_t* d = (const uint8_t*)g.dy + r * g.lddy;
 #pragma unroll
     for (int v = 0; v < VPT; ++v) {
-      nx[v] = load_vec<DT>(p, (t + v * RT) * N, H);
-      nd[v] = load_vec<DT>(d, (t + v * RT) * N, H);
+      nx[v] = load_vec(p, Span<DT, MODE>(t + v * RT, H));
+      nd[v] = load_vec(d, Span<DT, MODE>(t + v * RT, H));
     }
     nm = g.mean[r];
     nr = g.rstd[r];
@@ -280,6 +348,7 @@ __global__ void __launch_bounds__(block_threads<RT>()) backward_kernel(Args g) {
   // eight vectors a thread leave no registers for a row in flight beside this one
   constexpr bool AHEAD = VPT < 8;
   if (AHEAD && row < g.T) fetch(row);
+#pragma unroll 1
   for (int buf = 0; row < g.T; row += stride, buf ^= 1) {
     if (!AHEAD) fetch(row);
     Raw x[VPT], d[VPT];
@@ -289,16 +358,18 @@ __global__ void __launch_bounds__(block_threads<RT>()) backward_kernel(Args g) {
       x[v] = nx[v];
       d[v] = nd[v];
     }
-    if (AHEAD && row + stride < g.T) fetch(row + stride);
+    if (AHEAD) fetch(min<int64_t>(row + stride, g.T - 1));  // past the end: the last row again
     float s[2] = {0.f, 0.f};
 #pragma unroll
     for (int v = 0; v < VPT; ++v) {
       float f[N], e[N];
+      const Span<DT, MODE> sp(t + v * RT, H);
       unpack<DT>(x[v], f);
-      unpack<DT>(d[v], e);  // zero past H: nothing is added there
+      unpack<DT>(d[v], e);
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         const float xh = (f[i] - m) * r;
+        e[i] = sp.own(i) ? e[i] : 0.f;
         if constexpr (DW) {
           aw[v][i] += e[i] * xh;
           ab[v][i] += e[i];
@@ -309,6 +380,10 @@ __global__ void __launch_bounds__(block_threads<RT>()) backward_kernel(Args g) {
           s[1] += u * xh;
         }
       }
+      if constexpr (DW) {  // added here and now: dy and xh are not kept for it
+#pragma unroll
+        for (int i = 0; i < N; ++i) asm volatile("" : "+v"(aw[v][i]), "+v"(ab[v][i]));
+      }
     }
     if constexpr (DX) {
       row_sum<RT, 2>(s, red[buf]);
@@ -316,7 +391,6 @@ __global__ void __launch_bounds__(block_threads<RT>()) backward_kernel(Args g) {
       uint8_t* dp = (uint8_t*)g.y + row * g.ldy;
 #pragma unroll
       for (int v = 0; v < VPT; ++v) {
-        const int c = (t + v * RT) * N;
         float f[N], e[N];
         renew(x[v], s0);
         renew(d[v], s0);
@@ -327,7 +401,7 @@ __global__ void __launch_bounds__(block_threads<RT>()) backward_kernel(Args g) {
           const float xh = (f[i] - m) * r;
           f[i] = r * (e[i] * w[v][i] - s0 - xh * s1);
         }
-        if (c < H) store_vec<DT>(dp, c, H, f);
+        store_vec(dp, Span<DT, MODE>(t + v * RT, H), f);
       }
     }
   }
@@ -336,15 +410,15 @@ __global__ void __launch_bounds__(block_threads<RT>()) backward_kernel(Args g) {
     float* pb = pw + (int64_t)gridDim.x * H;
     if constexpr (ROWS == 1) {
 #pragma unroll
-      for (int v = 0; v < VPT; ++v)
+      for (int v = 0; v < VPT; ++v) {
+        const Span<DT, MODE> sp(t + v * RT, H);
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-          const int c = (t + v * RT) * N + i;
-          if (c < H) {
-            pw[c] = aw[v][i];
-            pb[c] = ab[v][i];
+        for (int i = 0; i < N; ++i)
+          if (sp.own(i)) {
+            pw[sp.c + i] = aw[v][i];
+            pb[sp.c + i] = ab[v][i];
           }
-        }
+      }
     } else {
       // the workgroup's row walkers, summed in their order
       constexpr int W = RT * VPT * N;
@@ -352,9 +426,12 @@ __global__ void __launch_bounds__(block_threads<RT>()) backward_kernel(Args g) {
       for (int k = 0; k < 2; ++k) {
         __syncthreads();
 #pragma unroll
-        for (int v = 0; v < VPT; ++v)
+        for (int v = 0; v < VPT; ++v) {
+          const Span<DT, MODE> sp(t + v * RT, H);
 #pragma unroll
-          for (int i = 0; i < N; ++i) sum[threadIdx.x / RT][(t + v * RT) * N + i] = k ? ab[v][i] : aw[v][i];
+          for (int i = 0; i < N; ++i)
+            if (sp.own(i)) sum[threadIdx.x / RT][sp.c + i] = k ? ab[v][i] : aw[v][i];
+        }
         __syncthreads();
         for (int c = threadIdx.x; c < H; c += BT) {
           float a = sum[0][c];
@@ -367,88 +444,123 @@ __global__ void __launch_bounds__(block_threads<RT>()) backward_kernel(Args g) {
   }
 }
 
-// dw / db (blockIdx.y) of 32 columns: eight walkers down the P partial rows,
-// their sums added in order
-constexpr int FIN_COLS = 32, FIN_WALK = 8;
+// dw / db (blockIdx.y) of 16 columns: 64 walkers down the P partial rows, their
+// sums added in a fixed tree
+constexpr int FIN_COLS = 16, FIN_WALK = 64;
 __global__ void __launch_bounds__(FIN_COLS* FIN_WALK) finish_kernel(const float* part, int P, int H, void* dw, void* db,
                                                                      int w_dtype) {
-  __shared__ float sum[FIN_WALK][FIN_COLS];
+  __shared__ float sum[FIN_WALK / 4][FIN_COLS];
   const int c = blockIdx.x * FIN_COLS + threadIdx.x % FIN_COLS, q = threadIdx.x / FIN_COLS;
   const float* p = part + (int64_t)blockIdx.y * P * H;
   float a = 0.f;
-  if (c < H)
+  if (c < H) {
+#pragma unroll 4
     for (int r = q; r < P; r += FIN_WALK) a += p[(int64_t)r * H + c];
-  sum[q][threadIdx.x % FIN_COLS] = a;
+  }
+  a += __shfl_xor(a, 16);
+  a += __shfl_xor(a, 32);
+  if ((threadIdx.x & 63) < FIN_COLS) sum[threadIdx.x >> 6][threadIdx.x % FIN_COLS] = a;
   __syncthreads();
   void* out = blockIdx.y ? db : dw;
   if (q == 0 && c < H && out) {
 #pragma unroll
-    for (int k = 1; k < FIN_WALK; ++k) a += sum[k][threadIdx.x];
+    for (int k = 1; k < FIN_WALK / 4; ++k) a += sum[k][threadIdx.x];
     store_elem(out, w_dtype, c, a);
   }
 }
 
 constexpr int MAX_H = 16384;
 
-// threads and vectors of a row, by its vectors of 16 bytes
+// Threads and vectors each for a row of nv vectors of 16 bytes, and workgroups
+// per compute unit.  The forward is fastest with four vectors a thread (few
+// waves to reduce over, enough loads in flight), the backward, which holds
+// three times the registers, with one.  us at 8192 x 7168 bf16 (896 vectors),
+// threads x vectors x workgroups: forward 256x4x3 43, 512x2x2 44, 1024x1x2 47;
+// backward 1024x1x1 78, 512x2x1 84, 256x4x2 91.  At 16384 x 2048: forward 64x4 22,
+// 256x1 23; backward 256x1x2 46, 64x4 46.  Few workgroups keep the partial rows of dw and db
+// few: 1024x1x2 took 100.
 struct Shape {
-  int rt, vpt;
+  int rt, vpt, per_cu;
 };
-static Shape shape_for(int dt, int64_t H) {
-  const int64_t nv = cdiv(H * dtype_size(dt), 16);
-  if (nv <= 64) return {64, 1};
-  if (nv <= 128) return {64, 2};
-  if (nv <= 256) return {64, 4};
-  if (nv <= 512) return {256, 2};
-  if (nv <= 1024) return {512, 2};
-  if (nv <= 2048) return {512, 4};
-  return {512, 8};
+static Shape forward_shape(int64_t nv) {
+  if (nv <= 64) return {64, 1, 4};
+  if (nv <= 128) return {64, 2, 4};
+  if (nv <= 256) return {64, 4, 4};
+  if (nv <= 512) return {128, 4, 8};
+  if (nv <= 1024) return {256, 4, 3};
+  if (nv <= 2048) return {512, 4, 2};
+  return {512, 8, 1};
+}
+static Shape backward_shape(int64_t nv) {
+  if (nv <= 64) return {64, 1, 2};
+  if (nv <= 128) return {128, 1, 4};
+  if (nv <= 256) return {256, 1, 2};
+  if (nv <= 512) return {512, 1, 1};
+  if (nv <= 1024) return {1024, 1, 1};
+  if (nv <= 2048) return {512, 4, 1};
+  return {512, 8, 1};
+}
+static int64_t vectors(int dt, int64_t H) { return cdiv(H * dtype_size(dt), 16); }
+static int64_t groups(const Shape& s, int64_t T) {
+  return std::max<int64_t>(1, std::min(cdiv(T, s.rt == 64 ? 4 : 1), (int64_t)split_device_cus() * s.per_cu));
 }
 
-// workgroups: as many as run at once, or fewer
-static int64_t groups_for(const Shape& s, int64_t T, int64_t per_cu) {
-  const int64_t rows = s.rt < 256 ? 256 / s.rt : 1;
-  return std::max<int64_t>(1, std::min(cdiv(T, rows), split_device_cus() * per_cu));
-}
-static int64_t forward_groups(const Shape& s, int64_t T) { return groups_for(s, T, s.rt <= 256 ? 8 : 4); }
-static int64_t backward_groups(const Shape& s, int64_t T) { return groups_for(s, T, s.rt <= 256 ? 2 : 1); }
-
-template <int DT, int RT, int VPT>
+template <int DT, int RT, int VPT, int MODE>
 static void launch_forward(const Args& g, int64_t n, hipStream_t st) {
-  forward_kernel<DT, RT, VPT><<<(unsigned)n, block_threads<RT>(), 0, st>>>(g);
+  forward_kernel<DT, RT, VPT, MODE><<<(unsigned)n, block_threads<RT>(), 0, st>>>(g);
 }
-template <int DT, int RT, int VPT>
+template <int DT, int RT, int VPT, int MODE>
 static void launch_backward(const Args& g, int64_t n, bool dx, bool dw, hipStream_t st) {
   const dim3 grd((unsigned)n), blk(block_threads<RT>());
   if (dx && dw)
-    backward_kernel<DT, RT, VPT, true, true><<<grd, blk, 0, st>>>(g);
+    backward_kernel<DT, RT, VPT, MODE, true, true><<<grd, blk, 0, st>>>(g);
   else if (dx)
-    backward_kernel<DT, RT, VPT, true, false><<<grd, blk, 0, st>>>(g);
+    backward_kernel<DT, RT, VPT, MODE, true, false><<<grd, blk, 0, st>>>(g);
   else
-    backward_kernel<DT, RT, VPT, false, true><<<grd, blk, 0, st>>>(g);
+    backward_kernel<DT, RT, VPT, MODE, false, true><<<grd, blk, 0, st>>>(g);
 }
 
-// f(RT, VPT) as constants for the shape
-#define NTLB_NORM_SHAPES(X) X(64, 1) X(64, 2) X(64, 4) X(256, 2) X(512, 2) X(512, 4)
-template <int DT>
-static bool forward(const Shape& s, const Args& g, int64_t n, hipStream_t st) {
+struct Forward {
+  const Args& g;
+  int64_t n;
+  hipStream_t st;
+  template <int DT, int RT, int VPT, int MODE>
+  void run() const { launch_forward<DT, RT, VPT, MODE>(g, n, st); }
+  template <int DT, int MODE>
+  bool shaped(const Shape& s) const {
 #define NTLB_CASE(RT, VPT) \
-  if (s.rt == RT && s.vpt == VPT) return launch_forward<DT, RT, VPT>(g, n, st), true;
-  NTLB_NORM_SHAPES(NTLB_CASE)
+  if (s.rt == RT && s.vpt == VPT) return run<DT, RT, VPT, MODE>(), true;
+    NTLB_CASE(64, 1) NTLB_CASE(64, 2) NTLB_CASE(64, 4) NTLB_CASE(128, 4) NTLB_CASE(256, 4) NTLB_CASE(512, 4)
+    if constexpr (DT == DT_F32) NTLB_CASE(512, 8)
+    return false;
+  }
+};
+struct Backward {
+  const Args& g;
+  int64_t n;
+  bool dx, dw;
+  hipStream_t st;
+  template <int DT, int RT, int VPT, int MODE>
+  void run() const { launch_backward<DT, RT, VPT, MODE>(g, n, dx, dw, st); }
+  template <int DT, int MODE>
+  bool shaped(const Shape& s) const {
+    NTLB_CASE(64, 1) NTLB_CASE(128, 1) NTLB_CASE(256, 1) NTLB_CASE(512, 1) NTLB_CASE(1024, 1) NTLB_CASE(512, 4)
+    if constexpr (DT == DT_F32) NTLB_CASE(512, 8)
 #undef NTLB_CASE
-  if constexpr (DT == DT_F32)
-    if (s.rt == 512 && s.vpt == 8) return launch_forward<DT, 512, 8>(g, n, st), true;
-  return false;
+    return false;
+  }
+};
+// the kernel of a type, a width and a shape; false if there is none
+template <int DT, typename F>
+static bool dispatch_dt(const Shape& s, int H, const F& f) {
+  if (H < El<DT>::n) return f.template run<DT, 64, 1, TINY>(), true;
+  return H % El<DT>::n ? f.template shaped<DT, RAGGED>(s) : f.template shaped<DT, WHOLE>(s);
 }
-template <int DT>
-static bool backward(const Shape& s, const Args& g, int64_t n, bool dx, bool dw, hipStream_t st) {
-#define NTLB_CASE(RT, VPT) \
-  if (s.rt == RT && s.vpt == VPT) return launch_backward<DT, RT, VPT>(g, n, dx, dw, st), true;
-  NTLB_NORM_SHAPES(NTLB_CASE)
-#undef NTLB_CASE
-  if constexpr (DT == DT_F32)
-    if (s.rt == 512 && s.vpt == 8) return launch_backward<DT, 512, 8>(g, n, dx, dw, st), true;
-  return false;
+template <typename F>
+static bool dispatch(int dt, const Shape& s, int64_t H, const F& f) {
+  if (dt == NTLB_F32) return dispatch_dt<DT_F32>(s, (int)H, f);
+  if (dt == NTLB_BF16) return dispatch_dt<DT_BF16>(s, (int)H, f);
+  return dispatch_dt<DT_F16>(s, (int)H, f);
 }
 
 static int check(const char* fn, const void* x, int dt, int64_t T, int64_t H, int64_t ldx, int wdt) {
@@ -480,19 +592,16 @@ extern "C" int ntlb_layer_norm_forward(const void* x, int x_dtype, int64_t T, in
   norm::Args g{};
   g.x = x; g.ldx = ldx * e; g.w = w; g.b = b; g.w_dtype = w_dtype; g.T = T; g.H = (int)H; g.eps = eps;
   g.y = y; g.ldy = ldy * e; g.mean = mean; g.rstd = rstd;
-  const norm::Shape s = norm::shape_for(x_dtype, H);
-  const int64_t n = norm::forward_groups(s, T);
+  const norm::Shape s = norm::forward_shape(norm::vectors(x_dtype, H));
+  const int64_t n = norm::groups(s, T);
   hipStream_t st = as_stream(stream);
-  const bool ok = x_dtype == NTLB_F32    ? norm::forward<DT_F32>(s, g, n, st)
-                  : x_dtype == NTLB_BF16 ? norm::forward<DT_BF16>(s, g, n, st)
-                                         : norm::forward<DT_F16>(s, g, n, st);
-  if (!ok) return fail(NTLB_EUNSUPPORTED, "%s: no kernel for %lld columns", fn, (long long)H);
+  if (!norm::dispatch(x_dtype, s, H, norm::Forward{g, n, st})) return fail(NTLB_EUNSUPPORTED, "%s: no kernel for %lld columns", fn, (long long)H);
   return check_launch(fn);
 }
 
 extern "C" int64_t ntlb_layer_norm_workspace_bytes(int x_dtype, int64_t T, int64_t H) {
   if (!valid_dtype(x_dtype) || T < 1 || H < 1 || H > norm::MAX_H) return 0;
-  return norm::backward_groups(norm::shape_for(x_dtype, H), T) * H * 8;
+  return norm::groups(norm::backward_shape(norm::vectors(x_dtype, H)), T) * H * 8;
 }
 
 extern "C" int ntlb_layer_norm_backward(const void* x, int x_dtype, int64_t T, int64_t H, int64_t ldx, const void* dy,
@@ -507,8 +616,8 @@ extern "C" int ntlb_layer_norm_backward(const void* x, int x_dtype, int64_t T, i
   if (dx && lddx < H) return fail(NTLB_EINVAL, "%s: dx's row pitch %lld below %lld", fn, (long long)lddx, (long long)H);
   const bool sums = dw || db;
   if (!dx && !sums) return NTLB_OK;
-  const norm::Shape s = norm::shape_for(x_dtype, H);
-  const int64_t n = T > 0 ? norm::backward_groups(s, T) : 0;
+  const norm::Shape s = norm::backward_shape(norm::vectors(x_dtype, H));
+  const int64_t n = T > 0 ? norm::groups(s, T) : 0;
   if (sums && n * H * 8 > ws_bytes) return fail(NTLB_EINVAL, "%s: workspace of %lld bytes, %lld needed", fn, (long long)ws_bytes, (long long)(n * H * 8));
   if (sums && n && (!workspace || !aligned(workspace, 4))) return fail(NTLB_EINVAL, "%s: bad workspace", fn);
   const int64_t e = dtype_size(x_dtype);
@@ -518,10 +627,7 @@ extern "C" int ntlb_layer_norm_backward(const void* x, int x_dtype, int64_t T, i
   g.dy = dy; g.lddy = lddy * e; g.part = (float*)workspace;
   hipStream_t st = as_stream(stream);
   if (T > 0) {
-    const bool ok = x_dtype == NTLB_F32    ? norm::backward<DT_F32>(s, g, n, dx != nullptr, sums, st)
-                    : x_dtype == NTLB_BF16 ? norm::backward<DT_BF16>(s, g, n, dx != nullptr, sums, st)
-                                           : norm::backward<DT_F16>(s, g, n, dx != nullptr, sums, st);
-    if (!ok) return fail(NTLB_EUNSUPPORTED, "%s: no kernel for %lld columns", fn, (long long)H);
+    if (!norm::dispatch(x_dtype, s, H, norm::Backward{g, n, dx != nullptr, sums, st})) return fail(NTLB_EUNSUPPORTED, "%s: no kernel for %lld columns", fn, (long long)H);
     if (int rc = check_launch(fn)) return rc;
   }
   if (sums) {

@@ -30,47 +30,61 @@ def _rows(x: torch.Tensor) -> torch.Tensor:
     return x2
 
 
+def _wdtype(x2, weight, bias) -> int:
+    return ops._dtype_code((weight if weight is not None else bias if bias is not None else x2).dtype)
+
+
 def _forward(x2: torch.Tensor, weight, bias, eps: float, stats: bool):
+    """y and, for the backward, the rows' means and then their 1 / deviations in one tensor"""
     T, H = x2.shape
     y = torch.empty((T, H), dtype=x2.dtype, device=x2.device)
-    mr = torch.empty((2, T), dtype=torch.float32, device=x2.device) if stats else None
-    wdt = ops._dtype_code((weight if weight is not None else bias if bias is not None else x2).dtype)
+    mr = torch.empty(2 * T, dtype=torch.float32, device=x2.device) if stats else None
+    at = mr.data_ptr() if stats else 0
     _lib.call("ntlb_layer_norm_forward", x2.data_ptr(), ops._dtype_code(x2.dtype), T, H, x2.stride(0),
-              ops._ptr(weight), ops._ptr(bias), wdt, eps, y.data_ptr(), H, mr[0].data_ptr() if stats else None,
-              mr[1].data_ptr() if stats else None, ops._stream())
+              ops._ptr(weight), ops._ptr(bias), _wdtype(x2, weight, bias), eps, y.data_ptr(), H, at or None,
+              at + 4 * T if at else None, ops._stream())
     return y, mr
+
+
+def _backward(ctx, dy):
+    x2, weight, bias, mr = ctx.saved_tensors
+    T, H = x2.shape
+    dev = x2.device
+    d2 = _rows(dy)
+    want_x, want_w, want_b = ctx.needs_input_grad[:3]
+    dx = torch.empty((T, H), dtype=x2.dtype, device=dev) if want_x else None
+    dw = torch.empty_like(weight) if want_w else None
+    db = torch.empty_like(bias) if want_b else None
+    xc = ops._dtype_code(x2.dtype)
+    ws, need = None, 0
+    if want_w or want_b:
+        need = _lib.lib().ntlb_layer_norm_workspace_bytes(xc, T, H)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    at = mr.data_ptr()
+    _lib.call("ntlb_layer_norm_backward", x2.data_ptr(), xc, T, H, x2.stride(0), d2.data_ptr(), d2.stride(0), at,
+              at + 4 * T, ops._ptr(weight), _wdtype(x2, weight, bias), ops._ptr(dx), H, ops._ptr(dw), ops._ptr(db),
+              ops._ptr(ws), need, ops._stream())
+    if want_x and dx.shape != ctx.shape:
+        dx = dx.reshape(ctx.shape)
+    return dx, dw, db, None
+
+
+_backward_of_graph = once_differentiable(_backward)
 
 
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
-        x2 = _rows(x.detach())
+        x2 = _rows(x)
         y, mr = _forward(x2, weight, bias, eps, True)
         ctx.save_for_backward(x2, weight, bias, mr)
         ctx.shape = x.shape
-        return y.reshape(x.shape)
+        return y if x.dim() == 2 else y.reshape(x.shape)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
-        x2, weight, bias, mr = ctx.saved_tensors
-        T, H = x2.shape
-        dev = x2.device
-        d2 = _rows(dy)
-        want_x, want_w, want_b = ctx.needs_input_grad[:3]
-        dx = torch.empty((T, H), dtype=x2.dtype, device=dev) if want_x else None
-        dw = torch.empty_like(weight) if want_w else None
-        db = torch.empty_like(bias) if want_b else None
-        wdt = ops._dtype_code((weight if weight is not None else bias if bias is not None else x2).dtype)
-        xc = ops._dtype_code(x2.dtype)
-        ws, need = None, 0
-        if want_w or want_b:
-            need = int(_lib.lib().ntlb_layer_norm_workspace_bytes(xc, T, H))
-            ws = torch.empty(need, dtype=torch.uint8, device=dev)
-        _lib.call("ntlb_layer_norm_backward", x2.data_ptr(), xc, T, H, x2.stride(0), d2.data_ptr(), d2.stride(0),
-                  mr[0].data_ptr(), mr[1].data_ptr(), ops._ptr(weight), wdt, ops._ptr(dx), H, ops._ptr(dw),
-                  ops._ptr(db), ops._ptr(ws), need, ops._stream())
-        return dx.reshape(ctx.shape) if want_x else None, dw, db, None
+        # a gradient that is itself to be differentiated is refused there
+        return (_backward_of_graph if torch.is_grad_enabled() else _backward)(ctx, dy)
 
 
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None, *,
