@@ -58,23 +58,44 @@ __device__ __forceinline__ int sw_perm(int r) { return (r & 7) ^ ((r >> 3) & 1);
 __device__ __forceinline__ int sw(int r, int c) { return r * ROWB + ((c ^ sw_perm(r)) << 4); }
 __device__ __forceinline__ int tr_perm(int k) { return (2 * (k & 3)) ^ (8 * ((k >> 4) & 1)); }
 
+// Where a lane's part of a fragment of 16 operand rows from row0 lies in a
+// stage.  By rows: row0 + lane % 16, bytes 32 g .. of its K step (g = lane / 16),
+// the swizzle the same for all row0.  Transposed: contraction rows 16 g + 4 h + j;
+// row0's chunk is XORed into the address.
 template <bool TR>
-__device__ __forceinline__ v8i frag(const uint8_t* tile, int row0, int lane) {
-  const int g = lane >> 4;
+struct FragAt {
+  uint32_t lo, hi;
+  __device__ __forceinline__ explicit FragAt(int row0, int lane) {
+    const int g = lane >> 4;
+    if constexpr (!TR) {
+      const int r = row0 + (lane & 15);
+      lo = sw(r, 2 * g);
+      hi = sw(r, 2 * g + 1);
+    } else {
+      const int j = (lane >> 2) & 3, q = lane & 3, k = 16 * g + j;
+      lo = k * 512 + ((((row0 >> 3) + (q >> 1)) ^ tr_perm(k)) << 4) + (q & 1) * 8;
+    }
+  }
+  // the address is formed again in every step: hoisted for all row groups, they
+  // would take more registers than there are
+  __device__ __forceinline__ void renew() {
+    if constexpr (TR) asm volatile("" : "+v"(lo));
+  }
+};
+// the fragment `group` groups of 16 rows on
+template <bool TR>
+__device__ __forceinline__ v8i frag(const uint8_t* tile, const FragAt<TR>& at, int group) {
   v8i f;
   if constexpr (!TR) {
-    const int r = row0 + (lane & 15);
-    const uint4 lo = *reinterpret_cast<const uint4*>(tile + sw(r, 2 * g));
-    const uint4 hi = *reinterpret_cast<const uint4*>(tile + sw(r, 2 * g + 1));
+    const uint4 lo = *reinterpret_cast<const uint4*>(tile + at.lo + group * 16 * ROWB);
+    const uint4 hi = *reinterpret_cast<const uint4*>(tile + at.hi + group * 16 * ROWB);
     f[0] = (int)lo.x; f[1] = (int)lo.y; f[2] = (int)lo.z; f[3] = (int)lo.w;
     f[4] = (int)hi.x; f[5] = (int)hi.y; f[6] = (int)hi.z; f[7] = (int)hi.w;
   } else {
-    const int j = (lane >> 2) & 3, q = lane & 3, c = (row0 >> 3) + (q >> 1);
+    const uint8_t* p = tile + (at.lo ^ (uint32_t)(group << 5));
 #pragma unroll
     for (int h = 0; h < 4; ++h) {
-      const int k = 16 * g + 4 * h + j;
-      const v4s v = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-          (lds_v4s_ptr)(tile + k * 512 + ((c ^ tr_perm(k)) << 4) + (q & 1) * 8));
+      const v4s v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s_ptr)(p + h * 2048));
       f[2 * h] = (int)(((uint32_t)(uint16_t)v[1] << 16) | (uint16_t)v[0]);
       f[2 * h + 1] = (int)(((uint32_t)(uint16_t)v[3] << 16) | (uint16_t)v[2]);
     }
@@ -82,11 +103,21 @@ __device__ __forceinline__ v8i frag(const uint8_t* tile, int row0, int lane) {
   return f;
 }
 
+// half a fragment pair's K step: 32 of its 64 contraction values
+template <int HALF>
 __device__ __forceinline__ v4f mma(const v8i& p, const v8i& q, v4f acc) {
-  const v4i pl = {p[0], p[1], p[2], p[3]}, ph = {p[4], p[5], p[6], p[7]};
-  const v4i ql = {q[0], q[1], q[2], q[3]}, qh = {q[4], q[5], q[6], q[7]};
-  acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, pl), __builtin_bit_cast(v8bf, ql), acc, 0, 0, 0);
-  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, ph), __builtin_bit_cast(v8bf, qh), acc, 0, 0, 0);
+  const v4i a = {p[4 * HALF], p[4 * HALF + 1], p[4 * HALF + 2], p[4 * HALF + 3]};
+  const v4i b = {q[4 * HALF], q[4 * HALF + 1], q[4 * HALF + 2], q[4 * HALF + 3]};
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), acc, 0, 0, 0);
+}
+
+// s_waitcnt immediate: at most n vector memory operations outstanding
+constexpr int vmcnt_imm(int n) { return (n & 15) | ((n >> 4) << 14) | 0x0F70; }
+// the workgroup's barrier alone: what must have landed is waited for before it
+__device__ __forceinline__ void barrier() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
 }
 
 __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
@@ -109,52 +140,109 @@ struct Mat {
 // Copies of one K step, global -> LDS: wave w takes copies w + 8j, j = 0..3, of
 // 1 KiB.  Resources begin at the tile (rows) or at the K step (transposed), so
 // offsets stay small whatever the matrix's size.
+// All of a resource is scalar: counts are 32 bits, since comparing 64 would be
+// the vector unit's work and the resource be taken to differ among the lanes.
 struct RowCopy {
   __amdgpu_buffer_rsrc_t rs;
-  uint32_t off, grp;
-  int64_t k;
-  int col;  // first column of the lane's chunk in a step
-  __device__ __forceinline__ void init(const Mat& o, int64_t r0, int wave, int lane) {
+  uint32_t off, pitch;
+  int k, col;  // columns; the first one of the lane's chunk in a step
+  uint32_t at, o;
+  __device__ __forceinline__ void init(const Mat& m, int64_t r0, int wave, int lane) {
     const int xr = wave * 8 + (lane >> 3), c = (lane & 7) ^ sw_perm(xr);
-    const int64_t rows = max<int64_t>(0, min<int64_t>(o.rows - r0, 256));
-    const int64_t last = min<int64_t>(o.pitch, (o.k * 2 + 15) / 16 * 16);
-    const int64_t bytes = rows > 0 ? (rows - 1) * o.pitch + last : 0;
-    rs = __builtin_amdgcn_make_buffer_rsrc((void*)uniform64(o.p + r0 * o.pitch), (short)0, (int)uniform64(bytes), 0x00020000);
-    off = (uint32_t)(xr * o.pitch + c * 16);
-    grp = (uint32_t)(64 * o.pitch);
+    pitch = (uint32_t)m.pitch;
+    k = (int)m.k;
     col = c * 8;
-    k = o.k;
+    off = (uint32_t)xr * pitch + c * 16;
+    const int rows = max(0, min((int)(m.rows - r0), 256));
+    const uint32_t last = min(pitch, (uint32_t)(k * 2 + 15) / 16 * 16);
+    const int bytes = rows > 0 ? (int)((uint32_t)(rows - 1) * pitch + last) : 0;
+    rs = __builtin_amdgcn_make_buffer_rsrc((void*)uniform64(m.p + r0 * m.pitch), (short)0,
+                                           __builtin_amdgcn_readfirstlane(bytes), 0x00020000);
   }
-  __device__ __forceinline__ void issue(uint8_t* stage, int kt, int wave, int j) const {
-    const uint32_t o = (int64_t)kt * KSTEP + col < k ? off : 0x80000000u;
+  // step kt's copies: columns past k read zero
+  __device__ __forceinline__ void set(int kt) {
+    at = (uint32_t)kt * ROWB;
+    o = col < k - kt * KSTEP ? off : 0x80000000u;
+  }
+  __device__ __forceinline__ void issue(uint8_t* stage, int wave, int j) const {
     __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr_t)(stage + (wave + 8 * j) * 1024), 16, o,
-                                             (uint32_t)kt * ROWB + j * grp, 0, 0);
+                                             at + (uint32_t)j * 64 * pitch, 0, 0);
   }
 };
 
 struct TrCopy {
   const uint8_t* p;
-  int64_t pitch, k, last;
-  uint32_t off;
+  uint32_t pitch, last, off;
+  int k;
+  __amdgpu_buffer_rsrc_t rs;
   __device__ static int row0(int wave, int j) { return 2 * (wave & 3) + 16 * (wave >> 2) + 8 * (j & 1) + 32 * (j >> 1); }
-  __device__ __forceinline__ void init(const Mat& o, int64_t r0, int wave, int lane) {
+  __device__ __forceinline__ void init(const Mat& m, int64_t r0, int wave, int lane) {
     const int R = row0(wave, 0) + (lane >> 5), c = (lane & 31) ^ tr_perm(R);
-    p = uniform64(o.p);
-    pitch = uniform64(o.pitch);
-    k = uniform64(o.k);
-    last = min<int64_t>(o.pitch, (o.rows * 2 + 15) / 16 * 16);
-    off = (uint32_t)(R * o.pitch + (r0 + 8 * c) * 2);
+    p = uniform64(m.p + r0 * 2);
+    pitch = (uint32_t)m.pitch;
+    k = __builtin_amdgcn_readfirstlane((int)m.k);
+    // the last stored row ends with the operand's rows, 16 bytes rounded up
+    last = min(pitch, (uint32_t)(m.rows * 2 + 15) / 16 * 16) - (uint32_t)(r0 * 2);
+    off = (uint32_t)R * pitch + 16 * c;
   }
-  __device__ __forceinline__ void issue(uint8_t* stage, int kt, int wave, int j) const {
-    // a tile that overhangs its rows reads into the next stored row, where there is one
-    const int64_t rem = k - (int64_t)kt * KSTEP;
-    const int64_t bytes = rem <= 0 ? 0 : (min<int64_t>(rem, KSTEP + 1) - 1) * pitch + (rem > KSTEP + 1 ? pitch : last);
-    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)(p + (int64_t)kt * KSTEP * pitch), (short)0,
-                                                                        (int)bytes, 0x00020000);
+  // step kt's resource, from its first row's first column of the tile: 64 pitches
+  // where a 65th row holds their end, else to the end of the last row (a tile that
+  // overhangs its rows reads into the next stored row)
+  __device__ __forceinline__ void set(int kt) {
+    const int rem = k - kt * KSTEP;
+    const uint32_t bytes = rem <= 0 ? 0 : rem > KSTEP ? KSTEP * pitch : (uint32_t)(rem - 1) * pitch + last;
+    rs = __builtin_amdgcn_make_buffer_rsrc((void*)uniform64(p + (int64_t)kt * KSTEP * pitch), (short)0,
+                                           __builtin_amdgcn_readfirstlane((int)bytes), 0x00020000);
+  }
+  __device__ __forceinline__ void issue(uint8_t* stage, int wave, int j) const {
     __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr_t)(stage + row0(wave, j) * 512), 16, off,
-                                             (uint32_t)((8 * (j & 1) + 32 * (j >> 1)) * pitch), 0, 0);
+                                             (uint32_t)(8 * (j & 1) + 32 * (j >> 1)) * pitch, 0, 0);
   }
 };
+
+// A wave's 128 x 64 output rows as bf16, 32 rows at a time through its LDS
+// (rows of 64 values and 16 bytes, so that neither side's lanes share banks) to
+// stores of whole 128-byte lines.  value(tm, tn, v): the lane's four of a block.
+template <bool NTS, typename F>
+__device__ __forceinline__ void store_bf16(uint8_t* stage, int lane, int64_t m0, int64_t n0, int64_t M, int64_t N,
+                                           uint16_t* out, int64_t ldo, int vec, F value) {
+  constexpr int PITCH = 64 * 2 + 16;
+#pragma unroll
+  for (int part = 0; part < 4; ++part) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int tn = 0; tn < 4; ++tn) {
+        float v[4];
+        value(part * 2 + t, tn, v);
+        *reinterpret_cast<uint2*>(stage + (t * 16 + (lane & 15)) * PITCH + (tn * 16 + (lane >> 4) * 4) * 2) =
+            make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]));
+      }
+    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): the wave's rows are written
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int row = (lane >> 3) + 8 * j, c = lane & 7;
+      const int64_t m = m0 + part * 32 + row, n = n0 + c * 8;
+      const uint4 q = *reinterpret_cast<const uint4*>(stage + row * PITCH + c * 16);
+      if (m >= M || n >= N) continue;
+      uint16_t* o = out + m * ldo + n;
+      if (vec && n + 8 <= N) {
+        if constexpr (NTS)
+          store16_nt(o, &q);
+        else
+          *reinterpret_cast<uint4*>(o) = q;
+      } else {
+        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (n + i < N) o[i] = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
+      }
+    }
+    __builtin_amdgcn_s_waitcnt(0xC07F);  // read before the next rows overwrite them
+    __builtin_amdgcn_wave_barrier();
+  }
+}
 
 constexpr int EPI_LSE = 0, EPI_DZ = 1, EPI_ACC = 2, EPI_STORE = 3;
 
@@ -187,6 +275,7 @@ struct Args {
   // outputs
   void* out;            // DZ: bf16, ACC: fp32 [slices][..], STORE: bf16
   int64_t ldo;          // elements
+  int64_t cols;         // DZ: columns to store, whole K steps
   int64_t slice;        // elements of a slice
   int add;              // ACC: add to what is there
   int vec_out;
@@ -200,7 +289,7 @@ __global__ void __launch_bounds__(NT, 1) head_kernel(Args g) {
   __shared__ __attribute__((aligned(16))) uint8_t lb1[TILE];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave >> 2, wn = wave & 3;
-  const int live = g.live[0];
+  const int live = __builtin_amdgcn_readfirstlane(g.live[0]);
   // tiles: each XCD walks a contiguous range of a raster of group_m row tiles
   const int num_n = (int)((g.N + TN - 1) / TN);
   const int num_m_all = (int)((g.M + TM - 1) / TM);
@@ -244,46 +333,79 @@ __global__ void __launch_bounds__(NT, 1) head_kernel(Args g) {
   for (int i = 0; i < 8; ++i)
 #pragma unroll
     for (int j = 0; j < 4; ++j) acc[i][j] = (v4f){0.f, 0.f, 0.f, 0.f};
+  // K loop.  A step's fragments stream through registers, A's two row groups
+  // ahead.  The one barrier of a step stands after its last LDS read, before the
+  // products of its last two row groups: those cover the first reads of the next
+  // step, and the copies of the step after it, into the stage just read, have a
+  // whole step's time to land.  So an iteration is: the last two row groups of
+  // step kt - 1 (of zeros, at first), the first six of step kt, the barrier.
   if (kb0 < kb1) {
+    auto copy = [&](uint8_t* na, uint8_t* nb, int j) {
+      ca.issue(na, wave, j);
+      cb.issue(nb, wave, j);
+    };
+    auto rows = [&](int tm, const v8i (&bf)[4], const v8i& a) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      ca.issue(la0, kb0, wave, j);
-      cb.issue(lb0, kb0, wave, j);
-    }
+      for (int tn = 0; tn < 4; ++tn) acc[tm][tn] = mma<0>(bf[tn], a, acc[tm][tn]);
+#pragma unroll
+      for (int tn = 0; tn < 4; ++tn) acc[tm][tn] = mma<1>(bf[tn], a, acc[tm][tn]);
+      asm volatile("" : "+v"(acc[tm][0]), "+v"(acc[tm][1]), "+v"(acc[tm][2]), "+v"(acc[tm][3])::"memory");
+    };
+    ca.set(kb0);
+    cb.set(kb0);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) copy(la0, lb0, j);
+    v8i b0[4], b1[4], af[4];
+    FragAt<TA> fa(wm * 128, lane);
+    FragAt<TB> fb(wn * 64, lane);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) b1[i] = af[i] = (v8i){0, 0, 0, 0, 0, 0, 0, 0};
     __builtin_amdgcn_s_waitcnt(0);
-    __syncthreads();
-    auto step = [&](auto bufc, int kt) {
+    barrier();
+    auto step = [&](auto bufc, int kt, const v8i (&bo)[4], v8i (&bf)[4]) {
       constexpr int BUF = decltype(bufc)::value;
       const uint8_t* ta = BUF ? la1 : la0;
       const uint8_t* tb = BUF ? lb1 : lb0;
-      uint8_t* na = BUF ? la0 : la1;
-      uint8_t* nb = BUF ? lb0 : lb1;
+      uint8_t* oa = BUF ? la0 : la1;
+      uint8_t* ob = BUF ? lb0 : lb1;
       const int kn = min(kt + 1, kb1 - 1);  // the last step copies itself into the idle stage
-      v8i bf[4];
+      fa.renew();
+      fb.renew();
+      ca.set(kn);
+      cb.set(kn);
 #pragma unroll
-      for (int tn = 0; tn < 4; ++tn) bf[tn] = frag<TB>(tb, wn * 64 + tn * 16, lane);
-      v8i af = frag<TA>(ta, wm * 128, lane);
+      for (int tn = 0; tn < 4; ++tn) bf[tn] = frag<TB>(tb, fb, tn);
 #pragma unroll
-      for (int tm = 0; tm < 8; ++tm) {
-        v8i af_next;
-        if (tm + 1 < 8) af_next = frag<TA>(ta, wm * 128 + (tm + 1) * 16, lane);
-        if (tm < 4) {
-          ca.issue(na, kn, wave, tm);
-          cb.issue(nb, kn, wave, tm);
-        }
-#pragma unroll
-        for (int tn = 0; tn < 4; ++tn) acc[tm][tn] = mma(bf[tn], af, acc[tm][tn]);
-        asm volatile("" : "+v"(acc[tm][0]), "+v"(acc[tm][1]), "+v"(acc[tm][2]), "+v"(acc[tm][3])::"memory");
-        if (tm + 1 < 8) af = af_next;
+      for (int i = 0; i < 2; ++i) {
+        af[i] = frag<TA>(ta, fa, i);
+        copy(oa, ob, 2 * i);
+        copy(oa, ob, 2 * i + 1);
+        rows(6 + i, bo, af[2 + i]);
       }
-      __builtin_amdgcn_s_waitcnt(0);
-      __syncthreads();
+#pragma unroll
+      for (int tm = 0; tm < 6; ++tm) {
+        af[(tm + 2) & 3] = frag<TA>(ta, fa, tm + 2);
+        rows(tm, bf, af[tm & 3]);
+      }
+      __builtin_amdgcn_s_waitcnt(0);  // this wave's reads of the stage and its copies into the other are done
+      barrier();
     };
-    for (int kt = kb0; kt < kb1; kt += 2) {
-      step(std::integral_constant<int, 0>(), kt);
-      if (kt + 1 < kb1) step(std::integral_constant<int, 1>(), kt + 1);
+    int kt = kb0;
+    for (; kt + 2 <= kb1; kt += 2) {
+      step(std::integral_constant<int, 0>(), kt, b1, b0);
+      step(std::integral_constant<int, 1>(), kt + 1, b0, b1);
     }
+    if (kt < kb1) {
+      step(std::integral_constant<int, 0>(), kt, b1, b0);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) b1[i] = b0[i];
+    }
+    rows(6, b1, af[2]);
+    rows(7, b1, af[3]);
+    // no wave reads the stages any more, and none copies into them
   }
+  // a wave's 16 KiB of the stages for its output rows
+  uint8_t* stage = (wave < 2 ? la0 : wave < 4 ? lb0 : wave < 6 ? la1 : lb1) + (wave & 1) * (TILE / 2);
   // lane: rows m0 + wm*128 + tm*16 + lane%16, columns n0 + wn*64 + tn*16 + 4*(lane/16) + r
   const int64_t mw = m0 + wm * 128 + (lane & 15), nw = n0 + wn * 64 + (lane >> 4) * 4;
   if constexpr (EPI == EPI_LSE) {
@@ -330,25 +452,23 @@ __global__ void __launch_bounds__(NT, 1) head_kernel(Args g) {
     }
   } else if constexpr (EPI == EPI_DZ) {
     const float c = g.up.common(live);
+    float lse[8], u[8];
+    int lab[8];
 #pragma unroll
     for (int tm = 0; tm < 8; ++tm) {
-      const int64_t m = mw + tm * 16;
-      if (m >= g.M) continue;
-      const int64_t lab = (int64_t)g.y[m] - g.v0 - nw;
-      const float lse = g.lse[m], u = g.up.rest(g.rows[m], c);
-#pragma unroll
-      for (int tn = 0; tn < 4; ++tn) {
-        const int64_t n = nw + tn * 16;
-        float d[4];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const float p = __builtin_amdgcn_exp2f((acc[tm][tn][r] - lse) * LOG2E);
-          d[r] = n + r < g.N ? (lab == tn * 16 + r ? p - 1.0f : p) * u : 0.f;
-        }
-        // the pitch holds whole 64-column steps, zero past the piece
-        if (n < g.ldo) *reinterpret_cast<uint2*>((uint16_t*)g.out + m * g.ldo + n) = make_uint2(pack_bf16(d[0], d[1]), pack_bf16(d[2], d[3]));
-      }
+      const int64_t m = min<int64_t>(mw + tm * 16, g.M - 1);
+      lse[tm] = g.lse[m] * LOG2E;
+      u[tm] = g.up.rest(g.rows[m], c);
+      lab[tm] = (int)(g.y[m] - g.v0 - nw);
     }
+    store_bf16<false>(stage, lane, m0 + wm * 128, n0 + wn * 64, g.M, g.cols, (uint16_t*)g.out, g.ldo, 1, [&](int tm, int tn, float (&v)[4]) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[tm][tn][r], LOG2E, -lse[tm]));
+        // whole K steps are stored, zero past the piece
+        v[r] = nw + tn * 16 + r < g.N ? (lab[tm] == tn * 16 + r ? p - 1.0f : p) * u[tm] : 0.f;
+      }
+    });
   } else if constexpr (EPI == EPI_ACC) {
     float* o = (float*)g.out + sl * g.slice;
 #pragma unroll
@@ -365,24 +485,10 @@ __global__ void __launch_bounds__(NT, 1) head_kernel(Args g) {
     }
   } else {
     const float c = g.up.common(live);
+    store_bf16<true>(stage, lane, m0 + wm * 128, n0 + wn * 64, g.M, g.N, (uint16_t*)g.out, g.ldo, g.vec_out, [&](int tm, int tn, float (&v)[4]) {
 #pragma unroll
-    for (int tm = 0; tm < 8; ++tm) {
-      const int64_t m = mw + tm * 16;
-      if (m >= g.M) continue;
-#pragma unroll
-      for (int tn = 0; tn < 4; ++tn) {
-        const int64_t n = nw + tn * 16;
-        acc[tm][tn] *= c;
-        uint16_t* q = (uint16_t*)g.out + m * g.ldo + n;
-        if (g.vec_out && n + 4 <= g.N) {
-          *reinterpret_cast<uint2*>(q) = make_uint2(pack_bf16(acc[tm][tn][0], acc[tm][tn][1]), pack_bf16(acc[tm][tn][2], acc[tm][tn][3]));
-        } else {
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (n + r < g.N) q[r] = f32_to_bf16_bits(acc[tm][tn][r]);
-        }
-      }
-    }
+      for (int r = 0; r < 4; ++r) v[r] = acc[tm][tn][r] * c;
+    });
   }
 }
 
@@ -426,7 +532,8 @@ __global__ void __launch_bounds__(SCAN) scan_kernel(const void* targets, int t64
 // expect set: zl (NaN until a tile finds the label) and a zero loss for the
 // ignored rows.
 __global__ void __launch_bounds__(256) gather_kernel(const uint16_t* x, int64_t ldx, int64_t T, int64_t H, int aligned16,
-                                                     const int32_t* pos, uint16_t* xp, int64_t ldp, float* zl, float* loss) {
+                                                     const int32_t* pos, uint16_t* xp, int64_t hk, int64_t ldp, float* zl,
+                                                     float* loss) {
   const int64_t t = blockIdx.x;
   const int at = pos[t];
   if (at < 0) {
@@ -436,7 +543,7 @@ __global__ void __launch_bounds__(256) gather_kernel(const uint16_t* x, int64_t 
   if (threadIdx.x == 0) zl[at] = __builtin_nanf("");
   const uint16_t* src = x + t * ldx;
   uint4* dst = reinterpret_cast<uint4*>(xp + (int64_t)at * ldp);
-  for (int64_t c = threadIdx.x; c < ldp / 8; c += blockDim.x) {
+  for (int64_t c = threadIdx.x; c < hk / 8; c += blockDim.x) {
     uint4 v = make_uint4(0, 0, 0, 0);
     if (aligned16 && c * 8 + 8 <= H) {
       v = *reinterpret_cast<const uint4*>(src + c * 8);
@@ -533,14 +640,21 @@ __global__ void __launch_bounds__(256) scatter_kernel(const float* acc, int64_t 
   }
 }
 
+// Pitch of a matrix of the kernels' own with `steps` 128-byte K steps: an odd
+// number of them.  A tile reads one step of 256 rows at a time, and rows a power
+// of two apart lie in few of the memory's channels (dz of 65536 words in 4096
+// rows: its products took PLACEHOLDER).
+static int64_t odd_pitch(int64_t cols) { return (cdiv(cols, 64) | 1) * 64; }
+
 // what the forward leaves for the backward
 struct State {
-  int64_t hp;  // pitch of X', elements
+  int64_t hk, hp;  // columns of X', whole K steps; its pitch, elements
   int64_t xp, pos, rows, y, lse, live, bytes;
 };
 static State state_of(int64_t T, int64_t H) {
   State s;
-  s.hp = cdiv(H, 64) * 64;
+  s.hk = cdiv(H, 64) * 64;
+  s.hp = odd_pitch(H);
   auto up = [](int64_t v) { return cdiv(v, 256) * 256; };
   s.xp = 0;
   s.pos = up(T * s.hp * 2);
@@ -564,12 +678,22 @@ struct Plan {
 constexpr int64_t DZ_BYTES = (int64_t)512 << 20;
 static Plan plan_of(int64_t T, int64_t H, int64_t V) {
   Plan p;
-  const int64_t hp = cdiv(H, 64) * 64, most = std::max<int64_t>(256, DZ_BYTES / (std::max<int64_t>(T, 1) * 2) / 256 * 256);
+  const int64_t hp = cdiv(H, 64) * 64, most = std::min<int64_t>(1 << 20, std::max<int64_t>(256, DZ_BYTES / (std::max<int64_t>(T, 1) * 2) / 256 * 256));
   const int64_t n = cdiv(V, most);
   p.piece = cdiv(cdiv(V, n), 256) * 256;
-  p.pitch = std::min(p.piece, cdiv(V, 64) * 64);
+  p.pitch = odd_pitch(std::min(p.piece, V));
   const int64_t tiles = cdiv(T, TM) * cdiv(H, TN), steps = cdiv(p.pitch, KSTEP);
-  p.slices = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(split_device_cus() / std::max<int64_t>(tiles, 1), steps / 8), 16));
+  // ranges that fill the last round of tiles, at least 16 steps each; each range
+  // costs about four steps more (its fp32 tile read, written and summed)
+  const int64_t cus = split_device_cus();
+  double best = 1e30;
+  for (int n = 1; n <= 16 && (n == 1 || steps / n >= 16); ++n) {
+    const double t = (double)cdiv(tiles * n, cus) * ((double)steps / n + 4);
+    if (t < best * 0.98) {
+      best = t;
+      p.slices = n;
+    }
+  }
   p.dz = cdiv(T * p.pitch * 2, 256) * 256;
   p.acc = T * hp * 4 * p.slices;
   p.most = p.dz + p.acc;
@@ -580,7 +704,7 @@ static Plan plan_of(int64_t T, int64_t H, int64_t V) {
 static int check(const char* fn, const void* w, int64_t T, int64_t H, int64_t V, int64_t ldw) {
   if (T < 0 || H < 1 || V < 1) return fail(NTLB_EINVAL, "%s: bad shape T %lld H %lld V %lld", fn, (long long)T, (long long)H, (long long)V);
   if (T > (1 << 24) || V > (1 << 30) || H > (1 << 20)) return fail(NTLB_EUNSUPPORTED, "%s: T %lld H %lld V %lld is too large", fn, (long long)T, (long long)H, (long long)V);
-  if (!w || !aligned(w, 16) || ldw < H || ldw % 8) return fail(NTLB_EINVAL, "%s: the weight needs 16-byte rows of at least H values", fn);
+  if (!w || !aligned(w, 16) || ldw < H || ldw % 8 || ldw > (1 << 22)) return fail(NTLB_EINVAL, "%s: the weight needs 16-byte rows of at least H values", fn);
   return NTLB_OK;
 }
 
@@ -622,9 +746,9 @@ extern "C" int ntlb_linear_xent_forward(const uint16_t* x, int64_t ldx, const ui
     zl = (float*)((uint8_t*)workspace + parts * T * 8);
     each = zl + cdiv(T * 4, 256) * 64;
     const int al = aligned(x, 16) && ldx % 8 == 0;
-    xent::gather_kernel<<<(unsigned)T, 256, 0, st>>>(x, ldx, T, H, al, pos, xp, s.hp, zl, reduction == 0 ? loss : nullptr);
+    xent::gather_kernel<<<(unsigned)T, 256, 0, st>>>(x, ldx, T, H, al, pos, xp, s.hk, s.hp, zl, reduction == 0 ? loss : nullptr);
     xent::Args g{};
-    g.a = {(const uint8_t*)xp, s.hp * 2, T, s.hp};
+    g.a = {(const uint8_t*)xp, s.hp * 2, T, s.hk};
     g.b = {(const uint8_t*)w, ldw * 2, V, H};
     g.M = T; g.N = V; g.live = live; g.group_m = 8; g.part = part; g.ldp = T; g.zl = zl; g.y = y;
     const int64_t tiles = cdiv(T, xent::TM) * parts;
@@ -662,34 +786,34 @@ extern "C" int ntlb_linear_xent_backward(const void* state, const uint16_t* w, i
     const uint8_t* wp = (const uint8_t*)(w + v0 * ldw);
     xent::Args g{};
     g.live = live; g.group_m = 8;
-    g.a = {sp + s.xp, s.hp * 2, Tn, s.hp};
+    g.a = {sp + s.xp, s.hp * 2, Tn, s.hk};
     g.b = {wp, ldw * 2, n, H};
     g.M = T; g.N = n; g.y = (const int32_t*)(sp + s.y); g.v0 = v0; g.lse = (const float*)(sp + s.lse);
     g.rows = (const int32_t*)(sp + s.rows); g.up = up;
-    g.out = dz; g.ldo = np;
+    g.out = dz; g.ldo = p.pitch; g.cols = np;
     const int64_t tm = cdiv(T, xent::TM), tn = cdiv(n, xent::TN), th = cdiv(H, xent::TN);
     if (T > 0) xent::head_kernel<false, false, xent::EPI_DZ><<<(unsigned)(tm * tn), xent::NT, 0, st>>>(g);
     if (dx && T > 0) {
       xent::Args x{};
       x.live = live; x.group_m = 8; x.slices = p.slices;
-      x.a = {(const uint8_t*)dz, np * 2, Tn, np};
+      x.a = {(const uint8_t*)dz, p.pitch * 2, Tn, np};
       x.b = {wp, ldw * 2, H, n};
-      x.M = T; x.N = H; x.out = acc; x.ldo = s.hp; x.slice = T * s.hp; x.add = v0 > 0;
+      x.M = T; x.N = H; x.out = acc; x.ldo = s.hk; x.slice = T * s.hk; x.add = v0 > 0;
       xent::head_kernel<false, true, xent::EPI_ACC><<<(unsigned)(tm * th * p.slices), xent::NT, 0, st>>>(x);
     }
     if (dw) {
       xent::Args q{};
       q.live = live; q.group_m = 8;
-      q.a = {(const uint8_t*)dz, np * 2, np, Tn};
-      q.b = {sp + s.xp, s.hp * 2, s.hp, Tn};
+      q.a = {(const uint8_t*)dz, p.pitch * 2, np, Tn};
+      q.b = {sp + s.xp, s.hp * 2, s.hk, Tn};
       q.M = n; q.N = H; q.out = dw + v0 * lddw; q.ldo = lddw;
       q.up = up;
-      q.vec_out = aligned(dw, 8) && lddw % 4 == 0;
+      q.vec_out = aligned(dw, 16) && lddw % 8 == 0;
       xent::head_kernel<true, true, xent::EPI_STORE><<<(unsigned)(tn * th), xent::NT, 0, st>>>(q);
     }
   }
   if (dx && T > 0)
-    xent::scatter_kernel<<<(unsigned)T, 256, 0, st>>>(acc, s.hp, T * s.hp, p.slices, up, live, (const int32_t*)(sp + s.pos),
+    xent::scatter_kernel<<<(unsigned)T, 256, 0, st>>>(acc, s.hk, T * s.hk, p.slices, up, live, (const int32_t*)(sp + s.pos),
                                                      H, dx, lddx);
   return check_launch(fn);
 }
