@@ -43,6 +43,7 @@ struct Args {
   int64_t T;
   int E, k, sigmoid, renorm;
   int G, Gk, gsize, gmagic;  // e / gsize == (e * gmagic) >> 20
+  int per, gshift;           // where groups are runs of lanes: experts of a lane, log2 of a group's lanes
   float scale;
   const float* bias;
   int32_t* ids;  // [T, k]
@@ -111,14 +112,14 @@ __device__ __forceinline__ void store_row(void* z, int64_t at, int l, int E, con
         vec v;
 #pragma unroll
         for (int i = 0; i < V; ++i) v[i] = f[c * V + i];
-        *reinterpret_cast<vec*>((float*)z + at + e) = v;
+        __builtin_nontemporal_store(v, reinterpret_cast<vec*>((float*)z + at + e));
       } else {
         typedef uint16_t vec __attribute__((ext_vector_type(V), aligned(2)));
         vec v;
 #pragma unroll
         for (int i = 0; i < V; ++i)
           v[i] = DT == DT_BF16 ? f32_to_bf16_bits(f[c * V + i]) : __half_as_ushort(f32_to_f16(f[c * V + i]));
-        *reinterpret_cast<vec*>((uint16_t*)z + at + e) = v;
+        __builtin_nontemporal_store(v, reinterpret_cast<vec*>((uint16_t*)z + at + e));
       }
     } else {
 #pragma unroll
@@ -130,12 +131,16 @@ __device__ __forceinline__ void store_row(void* z, int64_t at, int l, int E, con
 
 // the value of the partner lane of step S: lane ^ 1, ^ 2, 7 - lane, 15 - lane
 // (in its row of 16), then lane ^ 16, lane ^ 32
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, CTRL, 0xF, 0xF, true);
+}
 template <int S>
 __device__ __forceinline__ uint32_t partner(uint32_t v) {
-  if constexpr (S == 0) return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xF, 0xF, false);
-  if constexpr (S == 1) return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xF, 0xF, false);
-  if constexpr (S == 2) return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x141, 0xF, 0xF, false);
-  if constexpr (S == 3) return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x140, 0xF, 0xF, false);
+  if constexpr (S == 0) return dpp<0xB1>(v);
+  if constexpr (S == 1) return dpp<0x4E>(v);
+  if constexpr (S == 2) return dpp<0x141>(v);
+  if constexpr (S == 3) return dpp<0x140>(v);
   if constexpr (S == 4) return (uint32_t)__shfl_xor((int)v, 16);
   return (uint32_t)__shfl_xor((int)v, 32);
 }
@@ -177,46 +182,70 @@ __device__ __forceinline__ float token_max(float v) {
   return v;
 }
 
-// scores of the lane's elements; those past E are 0.  Softmax of a row of
-// -infinities is 0 everywhere.
+// score(z) of one expert, given what is common to the token: sigmoid, or the
+// softmax's maximum and 1 / sum.  Softmax of a row of -infinities is 0 everywhere.
+struct Common {
+  float m, inv;
+};
+__device__ __forceinline__ float score(float z, int sigmoid, const Common& c) {
+  return sigmoid ? __builtin_amdgcn_rcpf(1.0f + exp_f32(-z)) : exp_f32(z - c.m) * c.inv;
+}
+// scores of the lane's elements; those past E are 0
 template <int LPT, int J>
-__device__ __forceinline__ void scores(const float (&z)[J], int sigmoid, float (&p)[J]) {
+__device__ __forceinline__ Common scores(const float (&z)[J], int sigmoid, float (&p)[J]) {
+  Common c{0.f, 0.f};
   if (sigmoid) {
 #pragma unroll
-    for (int j = 0; j < J; ++j) p[j] = __builtin_amdgcn_rcpf(1.0f + exp_f32(-z[j]));
-    return;
+    for (int j = 0; j < J; ++j) p[j] = score(z[j], 1, c);
+    return c;
   }
-  float m = z[0];
+  c.m = z[0];
 #pragma unroll
-  for (int j = 1; j < J; ++j) m = max_nan(m, z[j]);
-  m = token_max<LPT>(m);
-  m = m == -__builtin_inff() ? 0.f : m;
+  for (int j = 1; j < J; ++j) c.m = max_nan(c.m, z[j]);
+  c.m = token_max<LPT>(c.m);
+  c.m = c.m == -__builtin_inff() ? 0.f : c.m;
   float s = 0.f;
 #pragma unroll
   for (int j = 0; j < J; ++j) {
-    p[j] = exp_f32(z[j] - m);
+    p[j] = exp_f32(z[j] - c.m);
     s += p[j];
   }
   s = token_sum<LPT>(s);
-  const float inv = s == 0.f ? 0.f : 1.0f / s;
+  c.inv = s == 0.f ? 0.f : 1.0f / s;
 #pragma unroll
-  for (int j = 0; j < J; ++j) p[j] *= inv;
+  for (int j = 0; j < J; ++j) p[j] *= c.inv;
+  return c;
 }
 
-// the order of a choice as a 32-bit whole number: -inf lowest (and above 0),
-// -0 as 0, NaN highest
+// the order of a choice as a 32-bit whole number: -inf lowest (and above 0), NaN
+// highest; a choice, p + bias with p >= 0, is never -0
 __device__ __forceinline__ uint32_t order_bits(float c) {
-  const uint32_t s = __float_as_uint(c + 0.0f);
+  const uint32_t s = __float_as_uint(c);
   const uint32_t u = s ^ ((uint32_t)((int32_t)s >> 31) | 0x80000000u);
   return c != c ? 0xFFFFFFFFu : u;
+}
+__device__ __forceinline__ float order_value(uint32_t u) {  // of order_bits, NaN for NaN
+  return __uint_as_float((u & 0x80000000u) ? u ^ 0x80000000u : ~u);
 }
 __device__ __forceinline__ double make_key(uint32_t order, int e) {
   const uint32_t hi = order >> 2, lo = (order << 30) | (uint32_t)(1023 - e);
   return __longlong_as_double((long long)(((uint64_t)hi << 32) | lo));
 }
 
+// the instructions themselves: keys are no NaNs, and the compiler would first
+// make sure of it, value by value
+__device__ __forceinline__ double max64(double a, double b) {
+  double r;
+  asm("v_max_f64 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+  return r;
+}
+__device__ __forceinline__ double min64(double a, double b) {
+  double r;
+  asm("v_min_f64 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+  return r;
+}
 __device__ __forceinline__ void exchange(double& a, double& b) {
-  const double hi = __builtin_fmax(a, b), lo = __builtin_fmin(a, b);
+  const double hi = max64(a, b), lo = min64(a, b);
   a = hi;
   b = lo;
 }
@@ -255,7 +284,7 @@ __device__ __forceinline__ void merge_round(double* v) {
 #pragma unroll
     for (int i = 0; i < L; ++i) o[i] = partner<S>(v[i]);
 #pragma unroll
-    for (int i = 0; i < L; ++i) v[i] = __builtin_fmax(v[i], o[L - 1 - i]);
+    for (int i = 0; i < L; ++i) v[i] = max64(v[i], o[L - 1 - i]);
     bitonic<L>(v);
   }
 }
@@ -277,17 +306,17 @@ __device__ __forceinline__ void lane_list(double* v) {
 #pragma unroll
     for (int c = 1; c < J / KN; ++c) {
 #pragma unroll
-      for (int i = 0; i < KN; ++i) v[i] = __builtin_fmax(v[i], v[c * KN + KN - 1 - i]);
+      for (int i = 0; i < KN; ++i) v[i] = max64(v[i], v[c * KN + KN - 1 - i]);
       bitonic<KN>(v);
     }
   }
 }
 
-// place of element e in a token's LDS row: four words of skew per 32, so that
-// the walkers of the groups start in different banks
-__device__ __forceinline__ int slot(int e) { return e + ((e >> 5) << 2); }
+// place of expert e in a token's LDS row: four words of skew per 16, so that
+// lanes that read runs of 16 start in different banks
+__device__ __forceinline__ int slot(int e) { return e + ((e >> 4) << 2); }
 template <int LPT, int J>
-constexpr int row_words() { return LPT * J + LPT * J / 8; }
+constexpr int row_words() { return LPT * J + LPT * J / 4; }
 
 // a wave's LDS traffic is in order; this keeps the compiler's order too
 __device__ __forceinline__ void wave_fence() {
@@ -295,70 +324,141 @@ __device__ __forceinline__ void wave_fence() {
   __builtin_amdgcn_wave_barrier();
 }
 
-template <int DT, int LPT, int J, int KN>
+template <int LPT, int J, typename T>
+__device__ __forceinline__ void to_lds(T* row, int l, const T (&f)[J]) {
+  constexpr int V = Lay<LPT, J>::V;
+  typedef T vec __attribute__((ext_vector_type(V)));
+#pragma unroll
+  for (int c = 0; c < J / V; ++c) {
+    vec v;
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = f[c * V + i];
+    *reinterpret_cast<vec*>(row + slot(Lay<LPT, J>::e(l, c * V))) = v;
+  }
+}
+
+// the two highest, a >= b, of a, b and v
+__device__ __forceinline__ void top2(uint32_t& a, uint32_t& b, uint32_t v) {
+  b = max(min(a, v), b);
+  a = max(a, v);
+}
+// a group's score, as its order
+__device__ __forceinline__ uint32_t group_order(uint32_t a, uint32_t b, int gsize) {
+  return gsize == 1 ? a : order_bits(order_value(a) + order_value(b));
+}
+// how many of the other lanes' groups come before this lane's (each once for
+// each of its lanes): earlier holds bit R where the lane R round the row of 16
+// lies in an earlier group
+template <int R>
+__device__ __forceinline__ int groups_before(uint32_t order, uint32_t earlier) {
+  if constexpr (R > 15) {
+    return 0;
+  } else {
+    // an equal group counts if it is the earlier one
+    return (dpp<0x120 + R>(order) > order - ((earlier >> R) & 1u) ? 1 : 0) + groups_before<R + 1>(order, earlier);
+  }
+}
+
+// GM: how the groups are chosen.  NONE: all are kept; LANES: a group is 16 / G
+// lanes of a row of 16, each reading its E / 16 experts in a row (LPT 16, E a
+// multiple of 16, G a power of two); WALK: any other, each walked by one lane
+constexpr int NONE = 0, LANES = 1, WALK = 2;
+
+template <int DT, int LPT, int J, int KN, int GM>
 __global__ void __launch_bounds__(64 * WAVES) forward_kernel(Args g) {
   constexpr int TPW = 64 / LPT, W = row_words<LPT, J>(), STEPS = LPT == 64 ? 6 : 4;
   constexpr int NL = J > KN ? J : KN;
-  __shared__ __attribute__((aligned(16))) float rows[WAVES][TPW][W];
+  __shared__ __attribute__((aligned(16))) uint32_t rows[GM == NONE ? 1 : WAVES][TPW][GM == NONE ? 4 : W];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane % LPT, sub = lane / LPT;
-  float* row = rows[wave][sub];
+  uint32_t* row = rows[GM == NONE ? 0 : wave][sub];
   const int E = g.E;
-  float bias[J];
+  uint32_t earlier = 0;  // LANES: bit R, whether lane (l - R) % 16 lies in an earlier group
+  if constexpr (GM == LANES) {
 #pragma unroll
-  for (int j = 0; j < J; ++j) {
-    const int e = Lay<LPT, J>::e(l, j);
-    bias[j] = g.bias && e < E ? g.bias[e] : 0.f;
+    for (int r = 1; r < 16; ++r) earlier |= (((l - r) & 15) >> g.gshift < l >> g.gshift ? 1u : 0u) << r;
   }
   const int64_t step = (int64_t)gridDim.x * WAVES * TPW;
   // the loop's bound is the wave's, not the lane's: every lane takes part in
   // the exchanges, those of tokens past T on a copy of the last one
   for (int64_t t0 = ((int64_t)blockIdx.x * WAVES + wave) * TPW; t0 < g.T; t0 += step) {
     const int64_t t = min<int64_t>(t0 + sub, g.T - 1);
-    float z[J], p[J];
-    load_row<DT, LPT, J>(g.z, t * g.ldz, l, E, -__builtin_inff(), z);
-    scores<LPT, J>(z, g.sigmoid, p);
-    double key[NL];
-    if (g.G > 1) {
-      wave_fence();
+    uint32_t o[J];  // the choices' order
+    Common common;
+    {
+      float z[J], p[J];
+      load_row<DT, LPT, J>(g.z, t * g.ldz, l, E, -__builtin_inff(), z);
+      common = scores<LPT, J>(z, g.sigmoid, p);
+      if (g.bias) {
+        load_row<DT_F32, LPT, J>(g.bias, 0, l, E, 0.f, z);
 #pragma unroll
-      for (int j = 0; j < J; ++j) row[slot(Lay<LPT, J>::e(l, j))] = p[j] + bias[j];
-      wave_fence();
-      // lane l walks group l: its two highest choices (NaN counts as highest)
-      float a = -__builtin_inff(), b = a;
-      if (l < g.G) {
-        for (int i = 0; i < g.gsize; ++i) {
-          const float v = row[slot(l * g.gsize + i)];
-          const float low = max_nan(a, v) == a && a == a ? v : a;  // the lower of a and v
-          a = max_nan(a, v);
-          b = max_nan(b, low);
-        }
+        for (int j = 0; j < J; ++j) p[j] += z[j];
       }
-      const float sc = g.gsize == 1 ? a : a + b;
-      const uint32_t o = l < g.G ? order_bits(sc) : 0u;
+#pragma unroll
+      for (int j = 0; j < J; ++j) o[j] = order_bits(p[j]);
+    }
+    double key[NL];
+    if constexpr (GM == LANES) {
+      wave_fence();
+      to_lds<LPT, J>(row, l, o);
+      wave_fence();
+      // from here the lane holds experts l * per ... in a row
+      const int e0 = l * g.per;
+      uint32_t a = 0, b = 0;
+      if (g.per == J) {
+#pragma unroll
+        for (int j = 0; j < J; ++j) o[j] = row[slot(l * J + j)];
+      } else {
+#pragma unroll
+        for (int j = 0; j < J; ++j) o[j] = j < g.per ? row[slot(e0 + j)] : 0u;
+      }
+#pragma unroll
+      for (int j = 0; j < J; ++j) top2(a, b, o[j]);
+      if (g.gshift > 0) {
+        const uint32_t oa = partner<0>(a), ob = partner<0>(b);
+        top2(a, b, oa);
+        b = max(b, ob);
+      }
+      if (g.gshift > 1) {
+        const uint32_t oa = partner<1>(a), ob = partner<1>(b);
+        top2(a, b, oa);
+        b = max(b, ob);
+      }
+      if (g.gshift > 2) {
+        const uint32_t oa = partner<2>(a), ob = partner<2>(b);
+        top2(a, b, oa);
+        b = max(b, ob);
+      }
+      const bool in = groups_before<1>(group_order(a, b, g.gsize), earlier) < g.Gk << g.gshift;
+#pragma unroll
+      for (int j = 0; j < J; ++j) key[j] = make_key(in ? o[j] : 0u, e0 + j);  // below any expert's where dropped
+    } else if constexpr (GM == WALK) {
+      wave_fence();
+      to_lds<LPT, J>(row, l, o);
+      wave_fence();
+      uint32_t a = 0, b = 0;
+      if (l < g.G)
+        for (int i = 0; i < g.gsize; ++i) top2(a, b, row[slot(l * g.gsize + i)]);
+      const uint32_t go = l < g.G ? group_order(a, b, g.gsize) : 0u;
       int rank = 0;
       for (int q = 0; q < g.G; ++q) {
-        const uint32_t oq = (uint32_t)__shfl((int)o, sub * LPT + q);
-        rank += oq > o || (oq == o && q < l);
+        const uint32_t oq = (uint32_t)__shfl((int)go, sub * LPT + q);
+        rank += oq > go || (oq == go && q < l);
       }
       const uint64_t vote = __ballot(l < g.G && rank < g.Gk);
       const uint32_t kept = (uint32_t)(vote >> (sub * LPT)) & 0xFFFFu;
 #pragma unroll
       for (int j = 0; j < J; ++j) {
         const int e = Lay<LPT, J>::e(l, j);
-        const bool in = e < E && ((kept >> ((e * g.gmagic) >> 20)) & 1u);
-        key[j] = in ? make_key(order_bits(p[j] + bias[j]), e) : 0.0;
+        const bool in = e < E && ((kept >> (__umul24(e, g.gmagic) >> 20)) & 1u);
+        key[j] = make_key(in ? o[j] : 0u, e);
       }
     } else {
 #pragma unroll
       for (int j = 0; j < J; ++j) {
         const int e = Lay<LPT, J>::e(l, j);
-        key[j] = e < E ? make_key(order_bits(p[j] + bias[j]), e) : 0.0;
+        key[j] = make_key(e < E ? o[j] : 0u, e);
       }
     }
-    wave_fence();
-#pragma unroll
-    for (int j = 0; j < J; ++j) row[slot(Lay<LPT, J>::e(l, j))] = p[j];
-    wave_fence();
     lane_list<J, KN>(key);
     merge_lanes<(J < KN ? J : KN), KN, 0, STEPS>(key);
     // lane i takes the i-th of the list
@@ -367,7 +467,8 @@ __global__ void __launch_bounds__(64 * WAVES) forward_kernel(Args g) {
     for (int i = 0; i < KN; ++i) lo = l == i ? (uint32_t)__double_as_longlong(key[i]) : lo;
     const int id = 1023 - (int)(lo & 1023u);
     const bool mine = l < g.k;
-    float q = mine ? row[slot(min(id, E - 1))] : 0.f;
+    float q = 0.f;
+    if (mine) q = score(load_elem(g.z, DT, t * g.ldz + min(id, E - 1)), g.sigmoid, common);
     if (g.renorm) {
       const float s = token_sum<LPT>(q) + RENORM_EPS;
       q = q / s;
@@ -381,7 +482,7 @@ __global__ void __launch_bounds__(64 * WAVES) forward_kernel(Args g) {
 
 template <int DT, int LPT, int J, bool SIG>
 __global__ void __launch_bounds__(64 * WAVES) backward_kernel(Args g) {
-  constexpr int TPW = 64 / LPT, W = row_words<LPT, J>();
+  constexpr int TPW = 64 / LPT, W = row_words<LPT, J>(), V = Lay<LPT, J>::V;
   __shared__ __attribute__((aligned(16))) float rows[WAVES][TPW][W];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane % LPT, sub = lane / LPT;
   float* row = rows[wave][sub];
@@ -392,11 +493,11 @@ __global__ void __launch_bounds__(64 * WAVES) backward_kernel(Args g) {
     const bool mine = l < g.k;
     const int id = mine ? min(max(g.ids[t * g.k + l], 0), E - 1) : 0;
     float d = mine ? g.scale * g.dw[t * g.k + l] : 0.f;
+    const float zc = mine ? load_elem(g.z, DT, t * g.ldz + id) : 0.f;
     float p[J], q = 0.f, q1 = 0.f;  // q: the chosen score, q1: 1 - q
     if constexpr (SIG) {
       // only the chosen logits matter
       if (mine) {
-        const float zc = load_elem(g.z, DT, t * g.ldz + id);
         const float ex = exp_f32(-__builtin_fabsf(zc));
         const float r = __builtin_amdgcn_rcpf(1.0f + ex);
         q = zc < 0.f ? ex * r : r;
@@ -407,12 +508,8 @@ __global__ void __launch_bounds__(64 * WAVES) backward_kernel(Args g) {
     } else {
       float z[J];
       load_row<DT, LPT, J>(g.z, t * g.ldz, l, E, -__builtin_inff(), z);
-      scores<LPT, J>(z, 0, p);
-      wave_fence();
-#pragma unroll
-      for (int j = 0; j < J; ++j) row[slot(Lay<LPT, J>::e(l, j))] = p[j];
-      wave_fence();
-      if (mine) q = row[slot(id)];
+      const Common c = scores<LPT, J>(z, 0, p);
+      if (mine) q = score(zc, 0, c);
     }
     if (g.renorm) {
       const float s = token_sum<LPT>(q) + RENORM_EPS;
@@ -429,24 +526,45 @@ __global__ void __launch_bounds__(64 * WAVES) backward_kernel(Args g) {
       for (int j = 0; j < J; ++j) p[j] = -p[j] * s;
     }
     wave_fence();
-#pragma unroll
-    for (int j = 0; j < J; ++j) row[slot(Lay<LPT, J>::e(l, j))] = p[j];
+    to_lds<LPT, J>(row, l, p);
     wave_fence();
     if (mine) row[slot(id)] = own;
     wave_fence();
+    typedef float vec __attribute__((ext_vector_type(V)));
 #pragma unroll
-    for (int j = 0; j < J; ++j) p[j] = row[slot(Lay<LPT, J>::e(l, j))];
+    for (int c = 0; c < J / V; ++c) {
+      const vec v = *reinterpret_cast<const vec*>(row + slot(Lay<LPT, J>::e(l, c * V)));
+#pragma unroll
+      for (int i = 0; i < V; ++i) p[c * V + i] = v[i];
+    }
     if (t0 + sub < g.T) store_row<DT, LPT, J>(g.dz, t * g.lddz, l, E, p);
   }
 }
 
 static unsigned groups_for(int64_t T, int lpt) {
   const int64_t per = WAVES * (64 / lpt);
-  return (unsigned)std::max<int64_t>(1, std::min<int64_t>(cdiv(T, per), split_device_cus() * 8));
+  return (unsigned)std::max<int64_t>(1, std::min<int64_t>(cdiv(T, per), split_device_cus() * 16));
+}
+
+template <int DT, int LPT, int J, int KN>
+static void launch_forward(const Args& g, unsigned n, hipStream_t st) {
+  if constexpr (LPT == 16) {
+    if (g.G > 1 && g.E % 16 == 0 && 16 % g.G == 0) {
+      forward_kernel<DT, LPT, J, KN, LANES><<<n, 64 * WAVES, 0, st>>>(g);
+      return;
+    }
+  }
+  if (g.G > 1)
+    forward_kernel<DT, LPT, J, KN, WALK><<<n, 64 * WAVES, 0, st>>>(g);
+  else
+    forward_kernel<DT, LPT, J, KN, NONE><<<n, 64 * WAVES, 0, st>>>(g);
 }
 
 template <int DT, int LPT, int J>
-static void launch(const Args& g, bool back, hipStream_t st) {
+static void launch(const Args& a, bool back, hipStream_t st) {
+  Args g = a;
+  g.per = g.E / 16;
+  g.gshift = g.G > 8 ? 0 : g.G > 4 ? 1 : g.G > 2 ? 2 : 3;
   const unsigned n = groups_for(g.T, LPT);
   if (back) {
     if (g.sigmoid)
@@ -454,11 +572,11 @@ static void launch(const Args& g, bool back, hipStream_t st) {
     else
       backward_kernel<DT, LPT, J, false><<<n, 64 * WAVES, 0, st>>>(g);
   } else if (g.k <= 4) {
-    forward_kernel<DT, LPT, J, 4><<<n, 64 * WAVES, 0, st>>>(g);
+    launch_forward<DT, LPT, J, 4>(g, n, st);
   } else if (g.k <= 8) {
-    forward_kernel<DT, LPT, J, 8><<<n, 64 * WAVES, 0, st>>>(g);
+    launch_forward<DT, LPT, J, 8>(g, n, st);
   } else {
-    forward_kernel<DT, LPT, J, 16><<<n, 64 * WAVES, 0, st>>>(g);
+    launch_forward<DT, LPT, J, 16>(g, n, st);
   }
 }
 
