@@ -48,7 +48,7 @@ typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) void* lds_ptr_t;
 typedef __attribute__((address_space(3))) v4s* lds_v4s_ptr;
 
-constexpr int TM = 256, TN = 256, ROWB = 128, KSTEP = 64, TILE = 256 * ROWB, NT = 512;
+constexpr int ROWB = 128, KSTEP = 64;  // bytes and values of a row's K step
 constexpr float LOG2E = 1.44269502e+00f, LN2 = 6.93147182e-01f;
 
 // LDS stages and fragments as in gemm_dq.hip: row-major [256][128 bytes] with
@@ -62,7 +62,7 @@ __device__ __forceinline__ int tr_perm(int k) { return (2 * (k & 3)) ^ (8 * ((k 
 // stage.  By rows: row0 + lane % 16, bytes 32 g .. of its K step (g = lane / 16),
 // the swizzle the same for all row0.  Transposed: contraction rows 16 g + 4 h + j;
 // row0's chunk is XORed into the address.
-template <bool TR>
+template <bool TR, int D>
 struct FragAt {
   uint32_t lo, hi;
   __device__ __forceinline__ explicit FragAt(int row0, int lane) {
@@ -73,7 +73,7 @@ struct FragAt {
       hi = sw(r, 2 * g + 1);
     } else {
       const int j = (lane >> 2) & 3, q = lane & 3, k = 16 * g + j;
-      lo = k * 512 + ((((row0 >> 3) + (q >> 1)) ^ tr_perm(k)) << 4) + (q & 1) * 8;
+      lo = k * (2 * D) + ((((row0 >> 3) + (q >> 1)) ^ tr_perm(k)) << 4) + (q & 1) * 8;
     }
   }
   // the address is formed again in every step: hoisted for all row groups, they
@@ -83,8 +83,8 @@ struct FragAt {
   }
 };
 // the fragment `group` groups of 16 rows on
-template <bool TR>
-__device__ __forceinline__ v8i frag(const uint8_t* tile, const FragAt<TR>& at, int group) {
+template <bool TR, int D>
+__device__ __forceinline__ v8i frag(const uint8_t* tile, const FragAt<TR, D>& at, int group) {
   v8i f;
   if constexpr (!TR) {
     const uint4 lo = *reinterpret_cast<const uint4*>(tile + at.lo + group * 16 * ROWB);
@@ -95,7 +95,7 @@ __device__ __forceinline__ v8i frag(const uint8_t* tile, const FragAt<TR>& at, i
     const uint8_t* p = tile + (at.lo ^ (uint32_t)(group << 5));
 #pragma unroll
     for (int h = 0; h < 4; ++h) {
-      const v4s v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s_ptr)(p + h * 2048));
+      const v4s v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s_ptr)(p + h * (8 * D)));
       f[2 * h] = (int)(((uint32_t)(uint16_t)v[1] << 16) | (uint16_t)v[0]);
       f[2 * h + 1] = (int)(((uint32_t)(uint16_t)v[3] << 16) | (uint16_t)v[2]);
     }
@@ -137,12 +137,14 @@ struct Mat {
   int64_t k;      // contraction
 };
 
-// Copies of one K step, global -> LDS: wave w takes copies w + 8j, j = 0..3, of
-// 1 KiB.  Resources begin at the tile (rows) or at the K step (transposed), so
+// Copies of one K step of a tile of D rows, global -> LDS: four of 1 KiB for each
+// of the D / 32 waves.  Resources begin at the tile (rows) or at the K step (transposed), so
 // offsets stay small whatever the matrix's size.
 // All of a resource is scalar: counts are 32 bits, since comparing 64 would be
 // the vector unit's work and the resource be taken to differ among the lanes.
+template <int D>
 struct RowCopy {
+  static constexpr int NW = D / 32;
   __amdgpu_buffer_rsrc_t rs;
   uint32_t off, pitch;
   int k, col;  // columns; the first one of the lane's chunk in a step
@@ -153,7 +155,7 @@ struct RowCopy {
     k = (int)m.k;
     col = c * 8;
     off = (uint32_t)xr * pitch + c * 16;
-    const int rows = max(0, min((int)(m.rows - r0), 256));
+    const int rows = max(0, min((int)(m.rows - r0), D));
     const uint32_t last = min(pitch, (uint32_t)(k * 2 + 15) / 16 * 16);
     const int bytes = rows > 0 ? (int)((uint32_t)(rows - 1) * pitch + last) : 0;
     rs = __builtin_amdgcn_make_buffer_rsrc((void*)uniform64(m.p + r0 * m.pitch), (short)0,
@@ -165,19 +167,25 @@ struct RowCopy {
     o = col < k - kt * KSTEP ? off : 0x80000000u;
   }
   __device__ __forceinline__ void issue(uint8_t* stage, int wave, int j) const {
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr_t)(stage + (wave + 8 * j) * 1024), 16, o,
-                                             at + (uint32_t)j * 64 * pitch, 0, 0);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr_t)(stage + (wave + NW * j) * 1024), 16, o,
+                                             at + (uint32_t)j * (8 * NW) * pitch, 0, 0);
   }
 };
 
+template <int D>
 struct TrCopy {
   const uint8_t* p;
   uint32_t pitch, last, off;
   int k;
   __amdgpu_buffer_rsrc_t rs;
-  __device__ static int row0(int wave, int j) { return 2 * (wave & 3) + 16 * (wave >> 2) + 8 * (j & 1) + 32 * (j >> 1); }
+  // the first of the rows of a wave's copy j (two of 512 bytes or four of 256):
+  // bit 4, which the swizzle looks at, is the wave's, so its lanes' offsets serve all j
+  __device__ static int row0(int wave, int j) {
+    return (D == 256 ? 2 * (wave & 3) + 16 * (wave >> 2) + 8 * (j & 1) : 8 * (wave >> 1) + 16 * (wave & 1) + 4 * (j & 1)) +
+           32 * (j >> 1);
+  }
   __device__ __forceinline__ void init(const Mat& m, int64_t r0, int wave, int lane) {
-    const int R = row0(wave, 0) + (lane >> 5), c = (lane & 31) ^ tr_perm(R);
+    const int R = row0(wave, 0) + lane / (D / 8), c = lane % (D / 8) ^ tr_perm(R);
     p = uniform64(m.p + r0 * 2);
     pitch = (uint32_t)m.pitch;
     k = __builtin_amdgcn_readfirstlane((int)m.k);
@@ -195,20 +203,20 @@ struct TrCopy {
                                            __builtin_amdgcn_readfirstlane((int)bytes), 0x00020000);
   }
   __device__ __forceinline__ void issue(uint8_t* stage, int wave, int j) const {
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr_t)(stage + row0(wave, j) * 512), 16, off,
-                                             (uint32_t)(8 * (j & 1) + 32 * (j >> 1)) * pitch, 0, 0);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr_t)(stage + row0(wave, j) * (2 * D)), 16, off,
+                                             (uint32_t)(row0(0, j)) * pitch, 0, 0);
   }
 };
 
-// A wave's 128 x 64 output rows as bf16, 32 rows at a time through its LDS
+// A wave's 16 MT x 64 output rows as bf16, 32 rows at a time through its LDS
 // (rows of 64 values and 16 bytes, so that neither side's lanes share banks) to
 // stores of whole 128-byte lines.  value(tm, tn, v): the lane's four of a block.
-template <bool NTS, typename F>
+template <int MT, bool NTS, typename F>
 __device__ __forceinline__ void store_bf16(uint8_t* stage, int lane, int64_t m0, int64_t n0, int64_t M, int64_t N,
                                            uint16_t* out, int64_t ldo, int vec, F value) {
   constexpr int PITCH = 64 * 2 + 16;
 #pragma unroll
-  for (int part = 0; part < 4; ++part) {
+  for (int part = 0; part < MT / 2; ++part) {
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -281,14 +289,17 @@ struct Args {
   int vec_out;
 };
 
-template <bool TA, bool TB, int EPI>
-__global__ void __launch_bounds__(NT, 1) head_kernel(Args g) {
+// D x D output tiles: 256, eight waves of 128 x 64, one workgroup a compute unit;
+// 128, four waves of 64 x 64, two workgroups
+template <int D, bool TA, bool TB, int EPI>
+__global__ void __launch_bounds__(2 * D, D == 256 ? 1 : 2) head_kernel(Args g) {
+  constexpr int TM = D, TN = D, TILE = D * ROWB, WAVES_N = D / 64, MT = D / 32;
   __shared__ __attribute__((aligned(16))) uint8_t la0[TILE];
   __shared__ __attribute__((aligned(16))) uint8_t lb0[TILE];
   __shared__ __attribute__((aligned(16))) uint8_t la1[TILE];
   __shared__ __attribute__((aligned(16))) uint8_t lb1[TILE];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int wm = wave >> 2, wn = wave & 3;
+  const int wm = wave / WAVES_N, wn = wave % WAVES_N;
   const int live = __builtin_amdgcn_readfirstlane(g.live[0]);
   // tiles: each XCD walks a contiguous range of a raster of group_m row tiles
   const int num_n = (int)((g.N + TN - 1) / TN);
@@ -324,13 +335,13 @@ __global__ void __launch_bounds__(NT, 1) head_kernel(Args g) {
   const int kb0 = EPI == EPI_ACC ? (int)((int64_t)sl * nk / g.slices) : 0;
   const int kb1 = EPI == EPI_ACC ? (int)((int64_t)(sl + 1) * nk / g.slices) : nk;
 
-  typename std::conditional<TA, TrCopy, RowCopy>::type ca;
-  typename std::conditional<TB, TrCopy, RowCopy>::type cb;
+  typename std::conditional<TA, TrCopy<D>, RowCopy<D>>::type ca;
+  typename std::conditional<TB, TrCopy<D>, RowCopy<D>>::type cb;
   ca.init(g.a, m0, wave, lane);
   cb.init(g.b, n0, wave, lane);
-  v4f acc[8][4];
+  v4f acc[MT][4];
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
+  for (int i = 0; i < MT; ++i)
 #pragma unroll
     for (int j = 0; j < 4; ++j) acc[i][j] = (v4f){0.f, 0.f, 0.f, 0.f};
   // K loop.  A step's fragments stream through registers, A's two row groups
@@ -338,7 +349,7 @@ __global__ void __launch_bounds__(NT, 1) head_kernel(Args g) {
   // products of its last two row groups: those cover the first reads of the next
   // step, and the copies of the step after it, into the stage just read, have a
   // whole step's time to land.  So an iteration is: the last two row groups of
-  // step kt - 1 (of zeros, at first), the first six of step kt, the barrier.
+  // step kt - 1 (of zeros, at first), the others of step kt, the barrier.
   if (kb0 < kb1) {
     auto copy = [&](uint8_t* na, uint8_t* nb, int j) {
       ca.issue(na, wave, j);
@@ -356,8 +367,8 @@ __global__ void __launch_bounds__(NT, 1) head_kernel(Args g) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) copy(la0, lb0, j);
     v8i b0[4], b1[4], af[4];
-    FragAt<TA> fa(wm * 128, lane);
-    FragAt<TB> fb(wn * 64, lane);
+    FragAt<TA, D> fa(wm * 16 * MT, lane);
+    FragAt<TB, D> fb(wn * 64, lane);
 #pragma unroll
     for (int i = 0; i < 4; ++i) b1[i] = af[i] = (v8i){0, 0, 0, 0, 0, 0, 0, 0};
     __builtin_amdgcn_s_waitcnt(0);
@@ -374,17 +385,17 @@ __global__ void __launch_bounds__(NT, 1) head_kernel(Args g) {
       ca.set(kn);
       cb.set(kn);
 #pragma unroll
-      for (int tn = 0; tn < 4; ++tn) bf[tn] = frag<TB>(tb, fb, tn);
+      for (int tn = 0; tn < 4; ++tn) bf[tn] = frag(tb, fb, tn);
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        af[i] = frag<TA>(ta, fa, i);
+        af[i] = frag(ta, fa, i);
         copy(oa, ob, 2 * i);
         copy(oa, ob, 2 * i + 1);
-        rows(6 + i, bo, af[2 + i]);
+        rows(MT - 2 + i, bo, af[2 + i]);
       }
 #pragma unroll
-      for (int tm = 0; tm < 6; ++tm) {
-        af[(tm + 2) & 3] = frag<TA>(ta, fa, tm + 2);
+      for (int tm = 0; tm < MT - 2; ++tm) {
+        af[(tm + 2) & 3] = frag(ta, fa, tm + 2);
         rows(tm, bf, af[tm & 3]);
       }
       __builtin_amdgcn_s_waitcnt(0);  // this wave's reads of the stage and its copies into the other are done
@@ -400,18 +411,19 @@ __global__ void __launch_bounds__(NT, 1) head_kernel(Args g) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) b1[i] = b0[i];
     }
-    rows(6, b1, af[2]);
-    rows(7, b1, af[3]);
+    rows(MT - 2, b1, af[2]);
+    rows(MT - 1, b1, af[3]);
     // no wave reads the stages any more, and none copies into them
   }
   // a wave's 16 KiB of the stages for its output rows
-  uint8_t* stage = (wave < 2 ? la0 : wave < 4 ? lb0 : wave < 6 ? la1 : lb1) + (wave & 1) * (TILE / 2);
-  // lane: rows m0 + wm*128 + tm*16 + lane%16, columns n0 + wn*64 + tn*16 + 4*(lane/16) + r
-  const int64_t mw = m0 + wm * 128 + (lane & 15), nw = n0 + wn * 64 + (lane >> 4) * 4;
+  constexpr int PER = TILE / 16384;
+  uint8_t* stage = (wave / PER == 0 ? la0 : wave / PER == 1 ? lb0 : wave / PER == 2 ? la1 : lb1) + (wave % PER) * 16384;
+  // lane: rows m0 + wm*16*MT + tm*16 + lane%16, columns n0 + wn*64 + tn*16 + 4*(lane/16) + r
+  const int64_t mw = m0 + wm * 16 * MT + (lane & 15), nw = n0 + wn * 64 + (lane >> 4) * 4;
   if constexpr (EPI == EPI_LSE) {
-    float2* red = reinterpret_cast<float2*>(la0);  // [4][256]
+    float2* red = reinterpret_cast<float2*>(la0);  // [WAVES_N][D]
 #pragma unroll
-    for (int tm = 0; tm < 8; ++tm) {
+    for (int tm = 0; tm < MT; ++tm) {
       const int64_t m = mw + tm * 16;
       const int64_t lab = (m < g.M ? (int64_t)g.y[m] : -1) - g.v0 - nw;  // the label's column, from the lane's first
       float mx = -__builtin_inff();
@@ -433,35 +445,35 @@ __global__ void __launch_bounds__(NT, 1) head_kernel(Args g) {
         for (int r = 0; r < 4; ++r) s += __builtin_amdgcn_exp2f((acc[tm][tn][r] - ref) * LOG2E);
       s += __shfl_xor(s, 16);
       s += __shfl_xor(s, 32);
-      if (lane < 16) red[wn * 256 + wm * 128 + tm * 16 + lane] = make_float2(mx, s);
+      if (lane < 16) red[wn * D + wm * 16 * MT + tm * 16 + lane] = make_float2(mx, s);
     }
     __syncthreads();
-    if (tid < 256 && m0 + tid < g.M) {
-      float2 t[4];
+    if (tid < D && m0 + tid < g.M) {
+      float2 t[WAVES_N];
       float mx = -__builtin_inff();
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        t[i] = red[i * 256 + tid];
+      for (int i = 0; i < WAVES_N; ++i) {
+        t[i] = red[i * D + tid];
         mx = fmaxf(mx, t[i].x);
       }
       const float ref = mx == -__builtin_inff() ? 0.f : mx;
       float s = 0.f;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) s += t[i].y * __builtin_amdgcn_exp2f((t[i].x - ref) * LOG2E);
+      for (int i = 0; i < WAVES_N; ++i) s += t[i].y * __builtin_amdgcn_exp2f((t[i].x - ref) * LOG2E);
       g.part[(n0 / TN) * g.ldp + m0 + tid] = make_float2(mx, s);
     }
   } else if constexpr (EPI == EPI_DZ) {
     const float c = g.up.common(live);
-    float lse[8], u[8];
-    int lab[8];
+    float lse[MT], u[MT];
+    int lab[MT];
 #pragma unroll
-    for (int tm = 0; tm < 8; ++tm) {
+    for (int tm = 0; tm < MT; ++tm) {
       const int64_t m = min<int64_t>(mw + tm * 16, g.M - 1);
       lse[tm] = g.lse[m] * LOG2E;
       u[tm] = g.up.rest(g.rows[m], c);
       lab[tm] = (int)(g.y[m] - g.v0 - nw);
     }
-    store_bf16<false>(stage, lane, m0 + wm * 128, n0 + wn * 64, g.M, g.cols, (uint16_t*)g.out, g.ldo, 1, [&](int tm, int tn, float (&v)[4]) {
+    store_bf16<MT, false>(stage, lane, m0 + wm * 16 * MT, n0 + wn * 64, g.M, g.cols, (uint16_t*)g.out, g.ldo, 1, [&](int tm, int tn, float (&v)[4]) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[tm][tn][r], LOG2E, -lse[tm]));
@@ -472,7 +484,7 @@ __global__ void __launch_bounds__(NT, 1) head_kernel(Args g) {
   } else if constexpr (EPI == EPI_ACC) {
     float* o = (float*)g.out + sl * g.slice;
 #pragma unroll
-    for (int tm = 0; tm < 8; ++tm) {
+    for (int tm = 0; tm < MT; ++tm) {
       const int64_t m = mw + tm * 16;
       if (m >= g.M) continue;
 #pragma unroll
@@ -485,7 +497,7 @@ __global__ void __launch_bounds__(NT, 1) head_kernel(Args g) {
     }
   } else {
     const float c = g.up.common(live);
-    store_bf16<true>(stage, lane, m0 + wm * 128, n0 + wn * 64, g.M, g.N, (uint16_t*)g.out, g.ldo, g.vec_out, [&](int tm, int tn, float (&v)[4]) {
+    store_bf16<MT, true>(stage, lane, m0 + wm * 16 * MT, n0 + wn * 64, g.M, g.N, (uint16_t*)g.out, g.ldo, g.vec_out, [&](int tm, int tn, float (&v)[4]) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) v[r] = acc[tm][tn][r] * c;
     });
@@ -666,36 +678,73 @@ static State state_of(int64_t T, int64_t H) {
   return s;
 }
 
-// forward workspace: the pairs, the label logits, the rows' losses
-static int64_t forward_ws(int64_t T, int64_t V) { return cdiv(V, TN) * T * 8 + 2 * cdiv(T * 4, 256) * 256; }
+// relative times of a K step: 256 x 256 tiles, one 128 x 128 tile alone on a
+// compute unit, two side by side
+constexpr double BIG_STEP = 1.0, LONE_STEP = 0.5, PAIR_STEP = 0.68;
 
-// backward: pieces of the vocabulary, slices of the dX product, workspace
+// The tile of a product of M x N over `steps` K steps: the one whose rounds of
+// workgroups (one or two to a compute unit) take less time
+static int tile_for(int64_t M, int64_t N) {
+  const int64_t cus = split_device_cus();
+  const double big = (double)cdiv(cdiv(M, 256) * cdiv(N, 256), cus) * BIG_STEP;
+  const int64_t small = cdiv(M, 128) * cdiv(N, 128);
+  const double little = small <= cus ? LONE_STEP : (double)cdiv(small, 2 * cus) * PAIR_STEP;
+  return little < big ? 128 : 256;
+}
+
+// The parts of a D-tiled product's contraction of `steps`: ranges that fill the
+// last round of workgroups, at least 16 steps each; each range costs about four
+// steps more (its fp32 tile read, written and summed)
+static int ranges_for(int D, int64_t M, int64_t N, int64_t steps) {
+  const int64_t tiles = cdiv(M, D) * cdiv(N, D), room = split_device_cus() * (D == 128 ? 2 : 1);
+  int best_n = 1;
+  double best = 1e30;
+  for (int n = 1; n <= 16 && (n == 1 || steps / n >= 16); ++n) {
+    const double t = (double)cdiv(tiles * n, room) * ((double)steps / n + 4);
+    if (t < best * 0.98) {
+      best = t;
+      best_n = n;
+    }
+  }
+  return best_n;
+}
+
+// one product
+template <bool TA, bool TB, int EPI>
+static void launch_head(int D, const Args& g, hipStream_t st) {
+  const unsigned n = (unsigned)(cdiv(g.M, D) * cdiv(g.N, D) * (EPI == EPI_ACC ? g.slices : 1));
+  if (D == 256)
+    head_kernel<256, TA, TB, EPI><<<n, 512, 0, st>>>(g);
+  else
+    head_kernel<128, TA, TB, EPI><<<n, 256, 0, st>>>(g);
+}
+
+// forward workspace: the pairs, the label logits, the rows' losses
+static int64_t forward_parts(int64_t T, int64_t V) { return cdiv(V, tile_for(T, V)); }
+static int64_t forward_ws(int64_t T, int64_t V) { return forward_parts(T, V) * T * 8 + 2 * cdiv(T * 4, 256) * 256; }
+
+// backward: pieces of the vocabulary, tiles, ranges of the dX product, workspace
 struct Plan {
   int64_t piece, pitch;  // words of a piece, dz's pitch in elements
-  int slices;
+  int dz_tile, dx_tile, dw_tile, slices;
   int64_t dz, acc, most, bytes;
 };
 constexpr int64_t DZ_BYTES = (int64_t)512 << 20;
 static Plan plan_of(int64_t T, int64_t H, int64_t V) {
   Plan p;
-  const int64_t hp = cdiv(H, 64) * 64, most = std::min<int64_t>(1 << 20, std::max<int64_t>(256, DZ_BYTES / (std::max<int64_t>(T, 1) * 2) / 256 * 256));
-  const int64_t n = cdiv(V, most);
-  p.piece = cdiv(cdiv(V, n), 256) * 256;
-  p.pitch = odd_pitch(std::min(p.piece, V));
-  const int64_t tiles = cdiv(T, TM) * cdiv(H, TN), steps = cdiv(p.pitch, KSTEP);
-  // ranges that fill the last round of tiles, at least 16 steps each; each range
-  // costs about four steps more (its fp32 tile read, written and summed)
-  const int64_t cus = split_device_cus();
-  double best = 1e30;
-  for (int n = 1; n <= 16 && (n == 1 || steps / n >= 16); ++n) {
-    const double t = (double)cdiv(tiles * n, cus) * ((double)steps / n + 4);
-    if (t < best * 0.98) {
-      best = t;
-      p.slices = n;
-    }
-  }
+  const int64_t hk = cdiv(H, 64) * 64;
+  const int64_t words = std::min<int64_t>(1 << 20, std::max<int64_t>(256, DZ_BYTES / (T * 2) / 256 * 256));
+  p.piece = cdiv(cdiv(V, cdiv(V, words)), 256) * 256;
+  const int64_t cols = std::min(p.piece, V);
+  p.pitch = odd_pitch(cols);
+  p.dz_tile = tile_for(T, cols);
+  p.dw_tile = tile_for(cols, H);
+  // dX: ranges can fill the chip with either tile; the small one where the large one's are too short
+  const int64_t steps = cdiv(cols, KSTEP);
+  p.dx_tile = cdiv(T, 256) * cdiv(H, 256) * std::max<int64_t>(1, steps / 16) < split_device_cus() || T <= 128 ? 128 : 256;
+  p.slices = ranges_for(p.dx_tile, T, H, steps);
   p.dz = cdiv(T * p.pitch * 2, 256) * 256;
-  p.acc = T * hp * 4 * p.slices;
+  p.acc = T * hk * 4 * p.slices;
   p.most = p.dz + p.acc;
   p.bytes = p.most + 256;
   return p;
@@ -741,7 +790,7 @@ extern "C" int ntlb_linear_xent_forward(const uint16_t* x, int64_t ldx, const ui
   xent::scan_kernel<<<1, xent::SCAN, 0, st>>>(targets, targets64, T, V, ignore_index, pos, rows, y, live);
   float *zl = nullptr, *each = nullptr;
   if (T > 0) {
-    const int64_t parts = cdiv(V, xent::TN);
+    const int64_t parts = xent::forward_parts(T, V);
     float2* part = (float2*)workspace;
     zl = (float*)((uint8_t*)workspace + parts * T * 8);
     each = zl + cdiv(T * 4, 256) * 64;
@@ -751,8 +800,7 @@ extern "C" int ntlb_linear_xent_forward(const uint16_t* x, int64_t ldx, const ui
     g.a = {(const uint8_t*)xp, s.hp * 2, T, s.hk};
     g.b = {(const uint8_t*)w, ldw * 2, V, H};
     g.M = T; g.N = V; g.live = live; g.group_m = 8; g.part = part; g.ldp = T; g.zl = zl; g.y = y;
-    const int64_t tiles = cdiv(T, xent::TM) * parts;
-    xent::head_kernel<false, false, xent::EPI_LSE><<<(unsigned)tiles, xent::NT, 0, st>>>(g);
+    xent::launch_head<false, false, xent::EPI_LSE>(xent::tile_for(T, V), g, st);
     xent::join_kernel<<<(unsigned)cdiv(T, 16), 256, 0, st>>>(part, T, parts, zl, rows, live, lse, each, reduction == 0 ? loss : nullptr);
   }
   if (reduction != 0) xent::total_kernel<<<1, 1024, 0, st>>>(each, live, reduction == 2, loss);
@@ -791,15 +839,14 @@ extern "C" int ntlb_linear_xent_backward(const void* state, const uint16_t* w, i
     g.M = T; g.N = n; g.y = (const int32_t*)(sp + s.y); g.v0 = v0; g.lse = (const float*)(sp + s.lse);
     g.rows = (const int32_t*)(sp + s.rows); g.up = up;
     g.out = dz; g.ldo = p.pitch; g.cols = np;
-    const int64_t tm = cdiv(T, xent::TM), tn = cdiv(n, xent::TN), th = cdiv(H, xent::TN);
-    if (T > 0) xent::head_kernel<false, false, xent::EPI_DZ><<<(unsigned)(tm * tn), xent::NT, 0, st>>>(g);
+    if (T > 0) xent::launch_head<false, false, xent::EPI_DZ>(p.dz_tile, g, st);
     if (dx && T > 0) {
       xent::Args x{};
       x.live = live; x.group_m = 8; x.slices = p.slices;
       x.a = {(const uint8_t*)dz, p.pitch * 2, Tn, np};
       x.b = {wp, ldw * 2, H, n};
       x.M = T; x.N = H; x.out = acc; x.ldo = s.hk; x.slice = T * s.hk; x.add = v0 > 0;
-      xent::head_kernel<false, true, xent::EPI_ACC><<<(unsigned)(tm * th * p.slices), xent::NT, 0, st>>>(x);
+      xent::launch_head<false, true, xent::EPI_ACC>(p.dx_tile, x, st);
     }
     if (dw) {
       xent::Args q{};
@@ -809,7 +856,7 @@ extern "C" int ntlb_linear_xent_backward(const void* state, const uint16_t* w, i
       q.M = n; q.N = H; q.out = dw + v0 * lddw; q.ldo = lddw;
       q.up = up;
       q.vec_out = aligned(dw, 16) && lddw % 8 == 0;
-      xent::head_kernel<true, true, xent::EPI_STORE><<<(unsigned)(tn * th), xent::NT, 0, st>>>(q);
+      xent::launch_head<true, true, xent::EPI_STORE>(p.dw_tile, q, st);
     }
   }
   if (dx && T > 0)
