@@ -2,7 +2,8 @@
 
 Each csrc/*.hip file is compiled to an object in parallel with hipcc for
 gfx950 only, then linked into nano-train_amd/lowbit/libntlowbit.so next to the
-Python package that loads it.  Packed-FP32 instruction selection is disabled
+Python package that loads it; csrc/binding/autograd.cpp becomes
+lowbit/_autograd.so, the Python module of the C++ autograd nodes.  Packed-FP32 instruction selection is disabled
 for all device code (-Xclang -target-feature -Xclang -packed-fp32-ops).  The
 compiler's per-kernel resource report (registers, scratch, occupancy) is kept
 in _build/kernel_resources.json for the register checks in the tests.
@@ -22,6 +23,8 @@ CSRC = os.path.join(HERE, "csrc")
 OBJ_DIR = os.path.join(HERE, "_build")
 RESOURCES = os.path.join(OBJ_DIR, "kernel_resources.json")
 LIB = os.path.join(HERE, "lowbit", "libntlowbit.so")
+BINDING = os.path.join(CSRC, "binding", "autograd.cpp")
+AUTOGRAD = os.path.join(HERE, "lowbit", "_autograd.so")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 ARCH = "gfx950"
 
@@ -84,11 +87,34 @@ def _compile(src: str):
     return obj, _resources(res.stderr)
 
 
+def _compile_binding() -> None:
+    """The Python module of the C++ autograd nodes: host code over torch's C++
+    API, linked to torch only (it is handed the C-ABI's addresses)."""
+    import sysconfig
+
+    import torch
+
+    at = os.path.dirname(torch.__file__)
+    inc = [os.path.join(at, "include"), os.path.join(at, "include", "torch", "csrc", "api", "include"),
+           sysconfig.get_paths()["include"], os.path.join(os.path.dirname(os.path.dirname(HIPCC)), "include")]
+    tmp = AUTOGRAD + ".tmp"
+    cmd = ["g++", "-std=c++17", "-O2", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *(f"-isystem{i}" for i in inc), "-Wall",
+           BINDING, "-o", tmp, f"-L{os.path.join(at, 'lib')}", "-ltorch", "-ltorch_cpu", "-ltorch_hip",
+           "-ltorch_python", "-lc10", "-lc10_hip"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"g++ failed for {BINDING}:\n{res.stderr}")
+    os.replace(tmp, AUTOGRAD)
+
+
 def build(verbose: bool = False) -> str:
     os.makedirs(OBJ_DIR, exist_ok=True)
     srcs = sources()
-    with cf.ThreadPoolExecutor(max_workers=min(8, len(srcs))) as ex:
+    with cf.ThreadPoolExecutor(max_workers=min(8, len(srcs) + 1)) as ex:
+        binding = ex.submit(_compile_binding)
         done = list(ex.map(_compile, srcs))
+        binding.result()
     objs = [o for o, _ in done]
     resources = {}
     for _, r in done:

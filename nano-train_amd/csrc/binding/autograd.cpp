@@ -1,0 +1,392 @@
+// Autograd nodes of the norm, the router and the head loss: the Python module
+// lowbit._autograd.
+//
+// These operators are short: at ordinary sizes a training step's kernels take
+// less time than a Python forward and backward around them (the backward runs on
+// the engine's thread, where Python first has to be entered).  So their nodes are
+// C++.  The kernels stay behind the C-ABI of include/ntlowbit.h: bind() is
+// handed the addresses of its functions in the library that lowbit._lib has
+// loaded, so this module links to no kernel and there is one library at a time.
+// Arguments are checked in Python, where an operator is called.
+#include <ATen/ATen.h>
+#include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+#include <c10/core/DeviceGuard.h>
+#include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/utils/object_ptr.h>
+
+#include <algorithm>
+#include <optional>
+#include <string>
+#include <tuple>
+#include <vector>
+
+#include "../../../include/ntlowbit.h"
+
+namespace {
+
+using at::Tensor;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+using Maybe = std::optional<Tensor>;
+
+struct Abi {
+  decltype(&ntlb_last_error) last_error;
+  decltype(&ntlb_layer_norm_forward) norm_forward;
+  decltype(&ntlb_layer_norm_backward) norm_backward;
+  decltype(&ntlb_layer_norm_workspace_bytes) norm_workspace;
+  decltype(&ntlb_route_topk) route;
+  decltype(&ntlb_route_topk_backward) route_backward;
+  decltype(&ntlb_linear_xent_forward) xent_forward;
+  decltype(&ntlb_linear_xent_backward) xent_backward;
+  decltype(&ntlb_linear_xent_state_bytes) xent_state;
+  decltype(&ntlb_linear_xent_workspace_bytes) xent_workspace;
+} abi = {};
+
+void check(const char* fn, int rc) {
+  if (rc == NTLB_OK) return;
+  const std::string msg = std::string(fn) + " failed (" + std::to_string(rc) + "): " + abi.last_error();
+  if (rc == NTLB_EINVAL) C10_THROW_ERROR(ValueError, msg);
+  C10_THROW_ERROR(Error, msg);
+}
+
+int dtype_of(const Tensor& t) {
+  switch (t.scalar_type()) {
+    case at::kFloat: return NTLB_F32;
+    case at::kBFloat16: return NTLB_BF16;
+    case at::kHalf: return NTLB_F16;
+    default: C10_THROW_ERROR(TypeError, "expected float32, bfloat16 or float16");
+  }
+}
+
+void* stream_of(const Tensor& t) {
+  return (void*)c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(t.device().index()).stream();
+}
+
+void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+void* ptr(const Maybe& t) { return t ? t->data_ptr() : nullptr; }
+
+Tensor scratch(int64_t bytes, const Tensor& like) { return at::empty({bytes}, like.options().dtype(at::kByte)); }
+
+// t as [rows, columns] with unit stride along the columns and rows one behind the
+// other (or one row repeated): a copy only where no view gives that
+Tensor rows_of(const Tensor& t) {
+  Tensor r = t.dim() == 2 ? t : t.reshape({t.numel() / t.size(-1), t.size(-1)});
+  if (r.stride(1) != 1 || (r.stride(0) != 0 && r.stride(0) < r.size(1))) r = r.contiguous();
+  return r;
+}
+Tensor shaped(const Tensor& t, at::IntArrayRef sizes) { return t.sizes() == sizes ? t : t.reshape(sizes); }
+
+bool wanted(const Tensor& t) { return t.defined() && t.requires_grad(); }
+bool wanted(const Maybe& t) { return t && t->requires_grad(); }
+
+// The gradients are no functions of the graph: where one is being recorded, they
+// carry an error for whoever differentiates them
+variable_list once(variable_list grads) {
+  if (!at::GradMode::is_enabled()) return grads;
+  for (Tensor& g : grads) {
+    if (!g.defined()) continue;
+    torch::autograd::DelayedError err("the gradients of this operator cannot be differentiated again", 1);
+    g = err({g.detach().set_requires_grad(true)})[0];
+  }
+  return grads;
+}
+
+// ---------------------------------------------------------------------------
+struct LayerNorm : torch::autograd::Function<LayerNorm> {
+  static int weight_dtype(const Tensor& x, const Maybe& w, const Maybe& b) { return dtype_of(w ? *w : b ? *b : x); }
+
+  // mr: the rows' means, then 1 / their deviations (undefined: not kept)
+  static Tensor run(const Tensor& x2, const Maybe& w, const Maybe& b, double eps, const Tensor& mr) {
+    const int64_t T = x2.size(0), H = x2.size(1);
+    Tensor y = at::empty({T, H}, x2.options());
+    float* m = mr.defined() ? mr.data_ptr<float>() : nullptr;
+    check("ntlb_layer_norm_forward",
+          abi.norm_forward(x2.data_ptr(), dtype_of(x2), T, H, x2.stride(0), ptr(w), ptr(b), weight_dtype(x2, w, b),
+                           (float)eps, y.data_ptr(), H, m, m ? m + T : nullptr, stream_of(x2)));
+    return y;
+  }
+
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Maybe& w, const Maybe& b, double eps) {
+    ctx->set_materialize_grads(false);
+    const c10::DeviceGuard guard(x.device());
+    const Tensor x2 = rows_of(x);
+    const Tensor mr = at::empty({std::max<int64_t>(1, 2 * x2.size(0))}, x2.options().dtype(at::kFloat));
+    Tensor y = run(x2, w, b, eps, mr);
+    ctx->save_for_backward({x2, w ? *w : Tensor(), b ? *b : Tensor(), mr});
+    ctx->saved_data["sizes"] = x.sizes();
+    return shaped(y, x.sizes());
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    if (!grads[0].defined()) return variable_list(4);
+    const variable_list s = ctx->get_saved_variables();
+    const Tensor &x2 = s[0], &w = s[1], &b = s[2], &mr = s[3];
+    const c10::DeviceGuard guard(x2.device());
+    const int64_t T = x2.size(0), H = x2.size(1);
+    const at::AutoDispatchBelowADInplaceOrView below;
+    const Tensor d2 = rows_of(grads[0]);
+    Tensor dx, dw, db, ws;
+    // (inputs are counted without those that are None)
+    if (ctx->needs_input_grad(0)) dx = at::empty({T, H}, x2.options());
+    if (w.defined() && ctx->needs_input_grad(1)) dw = at::empty_like(w);
+    if (b.defined() && ctx->needs_input_grad(w.defined() ? 2 : 1)) db = at::empty_like(b);
+    int64_t need = 0;
+    if (dw.defined() || db.defined()) {
+      need = abi.norm_workspace(dtype_of(x2), T, H);
+      ws = scratch(need, x2);
+    }
+    const float* m = mr.data_ptr<float>();
+    check("ntlb_layer_norm_backward",
+          abi.norm_backward(x2.data_ptr(), dtype_of(x2), T, H, x2.stride(0), d2.data_ptr(), d2.stride(0), m, m + T,
+                            ptr(w), dtype_of(w.defined() ? w : b.defined() ? b : x2), ptr(dx), H, ptr(dw), ptr(db),
+                            ptr(ws), need, stream_of(x2)));
+    if (dx.defined()) dx = shaped(dx, ctx->saved_data["sizes"].toIntVector());
+    return once({dx, dw, db, Tensor()});
+  }
+};
+
+// ---------------------------------------------------------------------------
+struct RouteConfig {
+  int64_t k, sigmoid, groups, kept, renorm;
+  double scale;
+};
+
+struct Route : torch::autograd::Function<Route> {
+  static std::tuple<Tensor, Tensor> run(const Tensor& z, const Maybe& bias, const RouteConfig& c) {
+    const int64_t T = z.size(0);
+    Tensor ids = at::empty({T, c.k}, z.options().dtype(at::kInt));
+    Tensor w = at::empty({T, c.k}, z.options().dtype(at::kFloat));
+    check("ntlb_route_topk",
+          abi.route(z.data_ptr(), dtype_of(z), T, z.size(1), z.stride(0), c.k, (int)c.sigmoid, (const float*)ptr(bias),
+                    c.groups, c.kept, (int)c.renorm, (float)c.scale, ids.data_ptr<int32_t>(), w.data_ptr<float>(),
+                    stream_of(z)));
+    return {ids, w};
+  }
+  static variable_list lead(const Tensor& logits, const std::tuple<Tensor, Tensor>& r, int64_t k) {
+    std::vector<int64_t> sizes = logits.sizes().vec();
+    sizes.back() = k;
+    return {shaped(std::get<0>(r), sizes), shaped(std::get<1>(r), sizes)};
+  }
+
+  static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Maybe& bias, int64_t k,
+                               int64_t sigmoid, int64_t groups, int64_t kept, int64_t renorm, double scale) {
+    ctx->set_materialize_grads(false);
+    const c10::DeviceGuard guard(logits.device());
+    const Tensor z = rows_of(logits);
+    const auto r = run(z, bias, {k, sigmoid, groups, kept, renorm, scale});
+    ctx->save_for_backward({z, std::get<0>(r)});
+    ctx->saved_data["sizes"] = logits.sizes();
+    ctx->saved_data["sigmoid"] = sigmoid;
+    ctx->saved_data["renorm"] = renorm;
+    ctx->saved_data["scale"] = scale;
+    const variable_list out = lead(logits, r, k);
+    ctx->mark_non_differentiable({out[0]});
+    return out;
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    if (!grads[1].defined()) return variable_list(8);
+    const variable_list s = ctx->get_saved_variables();
+    const Tensor &z = s[0], &ids = s[1];
+    const c10::DeviceGuard guard(z.device());
+    const at::AutoDispatchBelowADInplaceOrView below;
+    const int64_t T = z.size(0), E = z.size(1);
+    const Tensor dw = grads[1].contiguous();
+    Tensor dz = at::empty({T, E}, z.options());
+    check("ntlb_route_topk_backward",
+          abi.route_backward(z.data_ptr(), dtype_of(z), T, E, z.stride(0), ids.size(1),
+                             (int)ctx->saved_data["sigmoid"].toInt(), (int)ctx->saved_data["renorm"].toInt(),
+                             (float)ctx->saved_data["scale"].toDouble(), ids.data_ptr<int32_t>(), dw.data_ptr<float>(),
+                             dz.data_ptr(), E, stream_of(z)));
+    dz = shaped(dz, ctx->saved_data["sizes"].toIntVector());
+    return once({dz, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()});
+  }
+};
+
+// ---------------------------------------------------------------------------
+struct LinearXent : torch::autograd::Function<LinearXent> {
+  // w: weight in 16-byte rows; reduction 0 none, 1 sum, 2 mean
+  static std::tuple<Tensor, Tensor> run(const Tensor& x2, const Tensor& w, const Tensor& targets, int64_t ignore,
+                                        int64_t reduction) {
+    const int64_t T = x2.size(0), H = x2.size(1), V = w.size(0);
+    const Tensor y = targets.reshape({T}).contiguous();
+    const Tensor state = scratch(abi.xent_state(T, H), x2);
+    const int64_t need = abi.xent_workspace(T, H, V, 0);
+    const Tensor ws = scratch(std::max<int64_t>(need, 16), x2);
+    Tensor loss = at::empty({reduction ? 1 : std::max<int64_t>(T, 1)}, x2.options().dtype(at::kFloat));
+    check("ntlb_linear_xent_forward",
+          abi.xent_forward((const uint16_t*)x2.data_ptr(), x2.stride(0), (const uint16_t*)w.data_ptr(), w.stride(0),
+                           y.data_ptr(), y.scalar_type() == at::kLong, T, H, V, ignore, (int)reduction,
+                           loss.data_ptr<float>(), state.data_ptr(), ws.data_ptr(), need, stream_of(x2)));
+    return {reduction ? loss.reshape({}) : shaped(T ? loss : loss.slice(0, 0, 0), targets.sizes()), state};
+  }
+
+  static Tensor forward(AutogradContext* ctx, const Tensor& hidden, const Tensor& weight, const Tensor& w,
+                        const Tensor& targets, int64_t ignore, int64_t reduction) {
+    ctx->set_materialize_grads(false);
+    const c10::DeviceGuard guard(hidden.device());
+    const Tensor x2 = rows_of(hidden);
+    const auto [loss, state] = run(x2, w, targets, ignore, reduction);
+    ctx->save_for_backward({w, state});
+    ctx->saved_data["sizes"] = hidden.sizes();
+    ctx->saved_data["T"] = x2.size(0);
+    ctx->saved_data["H"] = x2.size(1);
+    ctx->saved_data["reduction"] = reduction;
+    return loss;
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    if (!grads[0].defined()) return variable_list(6);
+    const variable_list s = ctx->get_saved_variables();
+    const Tensor &w = s[0], &state = s[1];
+    const c10::DeviceGuard guard(w.device());
+    const at::AutoDispatchBelowADInplaceOrView below;
+    const int64_t T = ctx->saved_data["T"].toInt(), H = ctx->saved_data["H"].toInt(), V = w.size(0);
+    const int64_t reduction = ctx->saved_data["reduction"].toInt();
+    const Tensor dl = grads[0].reshape({-1}).contiguous();
+    Tensor dx, dw;
+    if (ctx->needs_input_grad(0)) dx = at::empty({T, H}, w.options());
+    if (ctx->needs_input_grad(1)) dw = at::empty({V, H}, w.options());
+    const int64_t need = abi.xent_workspace(std::max<int64_t>(T, 1), H, V, 1);
+    const Tensor ws = scratch(need, w);
+    check("ntlb_linear_xent_backward",
+          abi.xent_backward(state.data_ptr(), (const uint16_t*)w.data_ptr(), w.stride(0), T, H, V, (int)reduction,
+                            dl.data_ptr<float>(), (uint16_t*)ptr(dx), H, (uint16_t*)ptr(dw), H, ws.data_ptr(), need,
+                            stream_of(w)));
+    if (dx.defined()) dx = shaped(dx, ctx->saved_data["sizes"].toIntVector());
+    return once({dx, dw, Tensor(), Tensor(), Tensor(), Tensor()});
+  }
+};
+
+// ---------------------------------------------------------------------------
+// Python
+// ---------------------------------------------------------------------------
+Maybe maybe(PyObject* o) { return o == Py_None ? Maybe() : Maybe(THPVariable_Unpack(o)); }
+
+void count(Py_ssize_t n, Py_ssize_t want) {
+  if (n != want) C10_THROW_ERROR(TypeError, "wrong number of arguments");
+}
+int64_t integer(PyObject* o) {
+  const int64_t v = PyLong_AsLongLong(o);
+  if (v == -1 && PyErr_Occurred()) throw python_error();
+  return v;
+}
+double real(PyObject* o) {
+  const double v = PyFloat_AsDouble(o);
+  if (v == -1.0 && PyErr_Occurred()) throw python_error();
+  return v;
+}
+struct NoGil {  // kernels are launched without the interpreter's lock
+  PyThreadState* save = PyEval_SaveThread();
+  ~NoGil() { PyEval_RestoreThread(save); }
+};
+
+// layer_norm(x, weight | None, bias | None, eps)
+PyObject* py_layer_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  count(n, 4);
+  const Tensor& x = THPVariable_Unpack(a[0]);
+  const Maybe w = maybe(a[1]), b = maybe(a[2]);
+  const double eps = real(a[3]);
+  Tensor y;
+  {
+    const NoGil nogil;
+    if (at::GradMode::is_enabled() && (wanted(x) || wanted(w) || wanted(b))) {
+      y = LayerNorm::apply(x, w, b, eps);
+    } else {
+      const at::AutoDispatchBelowADInplaceOrView below;
+      const c10::DeviceGuard guard(x.device());
+      y = shaped(LayerNorm::run(rows_of(x), w, b, eps, Tensor()), x.sizes());
+    }
+  }
+  return THPVariable_Wrap(y);
+  END_HANDLE_TH_ERRORS
+}
+
+// route(logits, bias | None, k, sigmoid, groups, kept, renorm, scale) -> (ids, weights)
+PyObject* py_route(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  count(n, 8);
+  const Tensor& z = THPVariable_Unpack(a[0]);
+  const Maybe bias = maybe(a[1]);
+  const RouteConfig c{integer(a[2]), integer(a[3]), integer(a[4]), integer(a[5]), integer(a[6]), real(a[7])};
+  variable_list r;
+  {
+    const NoGil nogil;
+    if (at::GradMode::is_enabled() && wanted(z)) {
+      r = Route::apply(z, bias, c.k, c.sigmoid, c.groups, c.kept, c.renorm, c.scale);
+    } else {
+      const at::AutoDispatchBelowADInplaceOrView below;
+      const c10::DeviceGuard guard(z.device());
+      r = Route::lead(z, Route::run(rows_of(z), bias, c), c.k);
+    }
+  }
+  THPObjectPtr ids(THPVariable_Wrap(r[0])), w(THPVariable_Wrap(r[1]));
+  if (!ids || !w) throw python_error();
+  return PyTuple_Pack(2, ids.get(), w.get());
+  END_HANDLE_TH_ERRORS
+}
+
+// linear_xent(hidden, weight, weight in 16-byte rows, targets, ignore_index, reduction)
+PyObject* py_linear_xent(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  count(n, 6);
+  const Tensor &x = THPVariable_Unpack(a[0]), &weight = THPVariable_Unpack(a[1]), &w = THPVariable_Unpack(a[2]),
+               &y = THPVariable_Unpack(a[3]);
+  const int64_t ignore = integer(a[4]), reduction = integer(a[5]);
+  Tensor loss;
+  {
+    const NoGil nogil;
+    if (at::GradMode::is_enabled() && (wanted(x) || wanted(weight))) {
+      loss = LinearXent::apply(x, weight, w.detach(), y, ignore, reduction);
+    } else {
+      const at::AutoDispatchBelowADInplaceOrView below;
+      const c10::DeviceGuard guard(x.device());
+      loss = std::get<0>(LinearXent::run(rows_of(x), w, y, ignore, reduction));
+    }
+  }
+  return THPVariable_Wrap(loss);
+  END_HANDLE_TH_ERRORS
+}
+
+// bind({name: address}): the C-ABI's functions
+template <typename F>
+void take(PyObject* table, const char* name, F& f) {
+  PyObject* v = PyDict_GetItemString(table, name);  // borrowed
+  if (!v) C10_THROW_ERROR(ValueError, std::string("no address of ") + name);
+  f = reinterpret_cast<F>((uintptr_t)PyLong_AsUnsignedLongLong(v));
+  if (PyErr_Occurred()) throw python_error();
+}
+PyObject* py_bind(PyObject*, PyObject* table) {
+  HANDLE_TH_ERRORS
+  if (!PyDict_Check(table)) C10_THROW_ERROR(TypeError, "bind takes a dict of addresses");
+  Abi a{};
+  take(table, "ntlb_last_error", a.last_error);
+  take(table, "ntlb_layer_norm_forward", a.norm_forward);
+  take(table, "ntlb_layer_norm_backward", a.norm_backward);
+  take(table, "ntlb_layer_norm_workspace_bytes", a.norm_workspace);
+  take(table, "ntlb_route_topk", a.route);
+  take(table, "ntlb_route_topk_backward", a.route_backward);
+  take(table, "ntlb_linear_xent_forward", a.xent_forward);
+  take(table, "ntlb_linear_xent_backward", a.xent_backward);
+  take(table, "ntlb_linear_xent_state_bytes", a.xent_state);
+  take(table, "ntlb_linear_xent_workspace_bytes", a.xent_workspace);
+  abi = a;
+  Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
+}
+
+PyMethodDef methods[] = {
+    {"bind", py_bind, METH_O, nullptr},
+    {"layer_norm", (PyCFunction)(void (*)(void))py_layer_norm, METH_FASTCALL, nullptr},
+    {"route", (PyCFunction)(void (*)(void))py_route, METH_FASTCALL, nullptr},
+    {"linear_xent", (PyCFunction)(void (*)(void))py_linear_xent, METH_FASTCALL, nullptr},
+    {nullptr, nullptr, 0, nullptr}};
+PyModuleDef module = {PyModuleDef_HEAD_INIT, "_autograd", nullptr, -1, methods};
+
+}  // namespace
+
+PyMODINIT_FUNC PyInit__autograd(void) { return PyModule_Create(&module); }

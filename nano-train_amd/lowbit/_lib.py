@@ -200,6 +200,29 @@ def lib() -> ctypes.CDLL:
     return _lib
 
 
+_autograd = None
+
+
+def autograd():
+    """The C++ autograd nodes (csrc/binding/autograd.cpp), bound to the loaded
+    library's functions; raises if either is missing."""
+    global _autograd
+    if _autograd is not None:
+        return _autograd
+    L = lib()
+    with _lock:
+        if _autograd is None:
+            try:
+                from . import _autograd as mod
+            except ImportError as exc:
+                raise RuntimeError("the autograd module is not built or does not load; build it with "
+                                   f"`python nano-train_amd/build.py` ({exc})") from exc
+            names = [n for n in SIGNATURES if n.startswith(("ntlb_layer_norm", "ntlb_route", "ntlb_linear_xent"))]
+            mod.bind({n: ctypes.cast(getattr(L, n), ctypes.c_void_p).value for n in [*names, "ntlb_last_error"]})
+            _autograd = mod
+    return _autograd
+
+
 def call(name: str, *args) -> None:
     """Call an entry point and raise on a non-zero status."""
     rc = getattr(_lib or lib(), name)(*args)

@@ -12,54 +12,11 @@ from typing import Optional
 
 import torch
 import torch.nn as nn
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 from . import ops
-from .norm import _rows
 
 _REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
-
-
-def _forward(x2, w, targets, ignore_index: int, reduction: int):
-    T, H = x2.shape
-    V = w.shape[0]
-    L = _lib.lib()
-    dev = x2.device
-    state = torch.empty(int(L.ntlb_linear_xent_state_bytes(T, H)), dtype=torch.uint8, device=dev)
-    need = int(L.ntlb_linear_xent_workspace_bytes(T, H, V, 0))
-    ws = torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
-    loss = torch.empty(max(T, 1) if reduction == 0 else 1, dtype=torch.float32, device=dev)
-    _lib.call("ntlb_linear_xent_forward", x2.data_ptr(), x2.stride(0), w.data_ptr(), w.stride(0), targets.data_ptr(),
-              int(targets.dtype == torch.int64), T, H, V, ignore_index, reduction, loss.data_ptr(), state.data_ptr(),
-              ws.data_ptr(), need, ops._stream())
-    return (loss if T else loss[:0]) if reduction == 0 else loss, state
-
-
-class _LinearCrossEntropy(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, hidden, weight, targets, ignore_index, reduction):
-        x2 = _rows(hidden.detach())
-        w = ops._pad_cols(weight.detach(), 8)
-        loss, state = _forward(x2, w, targets.reshape(-1).contiguous(), ignore_index, reduction)
-        ctx.save_for_backward(w, state)
-        ctx.meta = (hidden.shape, x2.shape[0], weight.shape, reduction)
-        return loss.reshape(targets.shape if reduction == 0 else ())
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dloss):
-        w, state = ctx.saved_tensors
-        shape, T, (V, H), reduction = ctx.meta
-        dev = w.device
-        dloss = dloss.reshape(-1).contiguous()
-        dx = torch.empty((T, H), dtype=torch.bfloat16, device=dev) if ctx.needs_input_grad[0] else None
-        dw = torch.empty((V, H), dtype=torch.bfloat16, device=dev) if ctx.needs_input_grad[1] else None
-        need = int(_lib.lib().ntlb_linear_xent_workspace_bytes(max(T, 1), H, V, 1))
-        ws = torch.empty(need, dtype=torch.uint8, device=dev)
-        _lib.call("ntlb_linear_xent_backward", state.data_ptr(), w.data_ptr(), w.stride(0), T, H, V, reduction,
-                  dloss.data_ptr(), ops._ptr(dx), H, ops._ptr(dw), H, ws.data_ptr(), need, ops._stream())
-        return dx.reshape(shape) if dx is not None else None, dw, None, None, None
 
 
 def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, *,
@@ -91,12 +48,11 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: to
         raise ValueError(f"targets must be {tuple(hidden.shape[:-1])}, not {tuple(targets.shape)}")
     if not (hidden.device == weight.device == targets.device):
         raise ValueError(f"hidden, weight and targets are on {hidden.device}, {weight.device} and {targets.device}")
-    red = _REDUCTIONS[reduction]
-    if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
-        return _LinearCrossEntropy.apply(hidden, weight, targets, int(ignore_index), red)
-    loss, _ = _forward(_rows(hidden), ops._pad_cols(weight, 8), targets.reshape(-1).contiguous(),
-                       int(ignore_index), red)
-    return loss.reshape(targets.shape if red == 0 else ())
+    w = weight
+    if w.stride(1) != 1 or w.stride(0) % 8 or w.shape[1] % 8 or w.data_ptr() % 16 or w.stride(0) < w.shape[1]:
+        w = ops._pad_cols(weight.detach(), 8)
+    return (_lib._autograd or _lib.autograd()).linear_xent(hidden, weight, w, targets, ignore_index,
+                                                           _REDUCTIONS[reduction])
 
 
 class LMHeadLoss(nn.Module):

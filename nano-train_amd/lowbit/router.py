@@ -14,49 +14,14 @@ from typing import Optional
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 from . import ops
-from .norm import _rows
 
 MAX_EXPERTS = 1024
 MAX_TOP_K = 16
 MAX_GROUPS = 16
 _SCORES = {"softmax": 0, "sigmoid": 1}
-
-
-def _forward(z: torch.Tensor, k: int, sigmoid: int, bias, groups: int, kept: int, renorm: int, scale: float):
-    T, E = z.shape
-    ids = torch.empty((T, k), dtype=torch.int32, device=z.device)
-    w = torch.empty((T, k), dtype=torch.float32, device=z.device)
-    _lib.call("ntlb_route_topk", z.data_ptr(), ops._dtype_code(z.dtype), T, E, z.stride(0), k, sigmoid, ops._ptr(bias),
-              groups, kept, renorm, scale, ids.data_ptr(), w.data_ptr(), ops._stream())
-    return ids, w
-
-
-class _Route(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, bias, k, sigmoid, groups, kept, renorm, scale):
-        z = _rows(logits.detach())
-        ids, w = _forward(z, k, sigmoid, bias, groups, kept, renorm, scale)
-        ctx.save_for_backward(z, ids)
-        ctx.cfg = (k, sigmoid, renorm, scale, logits.shape)
-        ctx.mark_non_differentiable(ids)
-        lead = logits.shape[:-1]
-        return ids.reshape(*lead, k), w.reshape(*lead, k)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, _d_ids, dw):
-        z, ids = ctx.saved_tensors
-        k, sigmoid, renorm, scale, shape = ctx.cfg
-        T, E = z.shape
-        dw = dw.contiguous()
-        dz = torch.empty((T, E), dtype=z.dtype, device=z.device)
-        _lib.call("ntlb_route_topk_backward", z.data_ptr(), ops._dtype_code(z.dtype), T, E, z.stride(0), k, sigmoid,
-                  renorm, scale, ids.data_ptr(), dw.data_ptr(), dz.data_ptr(), E, ops._stream())
-        return dz.reshape(shape), None, None, None, None, None, None, None
 
 
 def route_tokens(logits: torch.Tensor, top_k: int, *, score: str = "softmax", bias: Optional[torch.Tensor] = None,
@@ -76,33 +41,31 @@ def route_tokens(logits: torch.Tensor, top_k: int, *, score: str = "softmax", bi
     Experts that must not be chosen take bias -inf: they are chosen only when
     fewer than top_k others remain.  NaN logits order highest; ids are always
     distinct and in range.  E <= 1024, top_k <= 16, n_groups <= 16."""
-    ops._require_device(logits, bias)
+    if not logits.is_cuda:
+        ops._require_device(logits)
     if score not in _SCORES:
         raise ValueError(f"unknown score {score!r}; expected 'softmax' or 'sigmoid'")
-    if logits.dim() < 1 or not 1 <= logits.shape[-1] <= MAX_EXPERTS:
+    E = logits.shape[-1] if logits.dim() else 0
+    if not 1 <= E <= MAX_EXPERTS:
         raise ValueError(f"logits must be [..., E] with 1 to {MAX_EXPERTS} experts, not {tuple(logits.shape)}")
     ops._dtype_code(logits.dtype)
-    E = logits.shape[-1]
     kept = n_groups if topk_groups is None else topk_groups
     if not 1 <= n_groups <= MAX_GROUPS or E % n_groups:
         raise ValueError(f"{E} experts cannot form {n_groups} equal groups (at most {MAX_GROUPS})")
     if not 1 <= kept <= n_groups:
         raise ValueError(f"topk_groups must be 1 to {n_groups}, not {kept}")
-    if not 1 <= top_k <= min(MAX_TOP_K, kept * (E // n_groups)):
-        raise ValueError(f"top_k must be 1 to {min(MAX_TOP_K, kept * (E // n_groups))}, not {top_k}")
+    most = min(MAX_TOP_K, kept * (E // n_groups))
+    if not 1 <= top_k <= most:
+        raise ValueError(f"top_k must be 1 to {most}, not {top_k}")
     if bias is not None:
-        if bias.shape != (E,) or bias.dtype != torch.float32 or bias.device != logits.device:
+        if bias.dtype != torch.float32 or bias.dim() != 1 or bias.shape[0] != E or bias.device != logits.device:
             raise ValueError(f"bias must be float32 [{E}] on {logits.device}, not {bias.dtype} {tuple(bias.shape)} "
                              f"on {bias.device}")
         bias = bias.detach()
         if bias.stride(0) != 1:
             bias = bias.contiguous()
-    args = (int(top_k), _SCORES[score], bias, int(n_groups), int(kept), int(bool(renormalize)), float(scale))
-    if torch.is_grad_enabled() and logits.requires_grad:
-        return _Route.apply(logits, bias, args[0], args[1], *args[3:])
-    ids, w = _forward(_rows(logits), *args)
-    lead = logits.shape[:-1]
-    return ids.reshape(*lead, top_k), w.reshape(*lead, top_k)
+    return (_lib._autograd or _lib.autograd()).route(logits, bias, top_k, _SCORES[score], n_groups, kept,
+                                                     bool(renormalize), scale)
 
 
 class TopKRouter(nn.Module):
