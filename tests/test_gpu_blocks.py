@@ -1,0 +1,79 @@
+"""GPU tests of the MoE block and the small language model: norm, router, experts and head loss in one training step."""
+
+from __future__ import annotations
+
+import os
+import sys
+
+import pytest
+import torch
+
+from conftest import PKG_PARENT
+
+pytestmark = pytest.mark.gpu
+sys.path.insert(0, os.path.join(PKG_PARENT, "examples"))
+
+
+def _block(dev, **kw):
+    from lowbit.blocks import MoEBlock
+
+    torch.manual_seed(3)
+    return MoEBlock(256, 128, 8, 2, device=dev, **kw)
+
+
+def test_block_is_its_parts(gpu_device):
+    """the block's output and gradients are those of its operators called one by one"""
+    from lowbit import moe
+    from lowbit.norm import layer_norm
+    from lowbit.router import route_tokens
+
+    b = _block(gpu_device, score="sigmoid", n_groups=4, topk_groups=2, scale=1.5)
+    x = torch.randn(3, 50, 256, device=gpu_device).bfloat16().requires_grad_(True)
+    dy = torch.randn(3, 50, 256, device=gpu_device).bfloat16()
+    y = b(x)
+    y.backward(dy)
+    x2 = x.detach().clone().requires_grad_(True)
+    p = {n: q.detach().clone().requires_grad_(True) for n, q in b.named_parameters()}
+    t = layer_norm(x2, p["norm.weight"], p["norm.bias"]).reshape(-1, 256)
+    ids, w = route_tokens(torch.nn.functional.linear(t.float(), p["router.weight"]), 2, score="sigmoid", n_groups=4,
+                          topk_groups=2, scale=1.5)
+    want = x2 + moe.local_moe(t, ids, w, p["w_gate_up"], p["w_down"]).reshape(x.shape)
+    want.backward(dy)
+    assert torch.equal(y.detach(), want.detach()) and torch.equal(b.last_ids, ids)
+    assert torch.equal(x.grad, x2.grad)
+    for n, q in b.named_parameters():
+        assert torch.equal(q.grad, p[n].grad) and q.grad.any(), n
+
+
+def test_block_with_a_capacity_and_no_gradients(gpu_device):
+    b = _block(gpu_device, capacity_factor=1.0, fmt="int_grid")
+    x = torch.randn(64, 256, device=gpu_device).bfloat16()
+    with torch.no_grad():
+        y = b(x)
+        one = b(x[:1])
+    assert y.isfinite().all() and one.shape == (1, 256)
+
+
+def test_block_refusals(gpu_device):
+    from lowbit.blocks import MoEBlock
+
+    with pytest.raises(ValueError, match="multiples of 128"):
+        MoEBlock(200, 128, 8, 2, device=gpu_device)
+    with pytest.raises(ValueError, match="top_k"):
+        MoEBlock(256, 128, 16, 9, device=gpu_device)
+
+
+def test_small_model_learns(gpu_device):
+    """60 steps on a next-word permutation of 500 words: from ln 500 (6.2) or above to below a third of it, the balance
+    bias moves, and single tokens score the right word above another"""
+    import moe_lm
+
+    losses, model, step_of = moe_lm.train(60)
+    assert losses[0] > 5.5 and sum(losses[-5:]) / 5 < 2.1, (losses[0], losses[-5:])
+    assert model.blocks[0].router.balance_bias.any()
+    words = torch.arange(0, 40, device=gpu_device)[:, None]
+    right = model.score(words, step_of[:40, None].cuda())
+    wrong = model.score(words, ((step_of[:40, None] + 1) % 500).cuda())
+    assert (right > wrong).float().mean() > 0.9
+    one = model.score(words[:1], step_of[:1, None].cuda())
+    assert one.shape == (1, 1)
