@@ -111,8 +111,6 @@ __device__ __forceinline__ v4f mma(const v8i& p, const v8i& q, v4f acc) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), acc, 0, 0, 0);
 }
 
-// s_waitcnt immediate: at most n vector memory operations outstanding
-constexpr int vmcnt_imm(int n) { return (n & 15) | ((n >> 4) << 14) | 0x0F70; }
 // the workgroup's barrier alone: what must have landed is waited for before it
 __device__ __forceinline__ void barrier() {
   asm volatile("" ::: "memory");
@@ -125,14 +123,15 @@ __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
   return __builtin_bit_cast(uint32_t, p);
 }
 
-// One operand: bf16, 16-byte aligned with whole 16-byte rows.
-//   stored by rows: [rows, cols], the contraction along cols; columns at or past
-//     cols read zero, rows past rows too
-//   transposed: [k, rows], the contraction down the rows; stored rows at or past
-//     k read zero
+// One operand, bf16: rows by contraction ([rows, k]) or, transposed, the other
+// way ([k, rows]).  The user's weight lies by rows, 16-byte aligned, whole 16-byte
+// rows; what lies at or past rows or k reads zero.  The kernels' own X' and dz lie
+// in blocks: 64 columns of all rows, 128 bytes a row, one block after another, so
+// that the step of a tile is one run of 32 KiB (or, transposed, a run of 8 KiB of
+// each of four blocks) and not 256 rows a pitch apart.
 struct Mat {
   const uint8_t* p;
-  int64_t pitch;  // bytes
+  int64_t pitch;  // bytes: of a row, or of a block
   int64_t rows;   // of the operand
   int64_t k;      // contraction
 };
@@ -205,6 +204,55 @@ struct TrCopy {
   __device__ __forceinline__ void issue(uint8_t* stage, int wave, int j) const {
     __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr_t)(stage + row0(wave, j) * (2 * D)), 16, off,
                                              (uint32_t)(row0(0, j)) * pitch, 0, 0);
+  }
+};
+
+// by rows, in blocks of the contraction
+template <int D>
+struct BlockRowCopy {
+  static constexpr int NW = D / 32;
+  const uint8_t* p;
+  int64_t pitch;
+  int bytes;
+  uint32_t off;
+  __amdgpu_buffer_rsrc_t rs;
+  __device__ __forceinline__ void init(const Mat& m, int64_t r0, int wave, int lane) {
+    const int xr = wave * 8 + (lane >> 3), c = (lane & 7) ^ sw_perm(xr);
+    p = uniform64(m.p + r0 * ROWB);
+    pitch = m.pitch;
+    bytes = __builtin_amdgcn_readfirstlane(max(0, min((int)(m.rows - r0), D)) * ROWB);
+    off = (uint32_t)(xr * ROWB + c * 16);
+  }
+  __device__ __forceinline__ void set(int kt) {
+    rs = __builtin_amdgcn_make_buffer_rsrc((void*)uniform64(p + kt * pitch), (short)0, bytes, 0x00020000);
+  }
+  __device__ __forceinline__ void issue(uint8_t* stage, int wave, int j) const {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr_t)(stage + (wave + NW * j) * 1024), 16, off, j * (8 * NW * ROWB), 0, 0);
+  }
+};
+
+// transposed, in blocks of the operand's rows: the contraction's rows up to the
+// next 64 are there, zero
+template <int D>
+struct BlockTrCopy {
+  const uint8_t* p;
+  uint32_t bytes, off;
+  __amdgpu_buffer_rsrc_t rs;
+  __device__ __forceinline__ void init(const Mat& m, int64_t r0, int wave, int lane) {
+    const int R = TrCopy<D>::row0(wave, 0) + lane / (D / 8), c = lane % (D / 8) ^ tr_perm(R);
+    p = uniform64(m.p + (r0 / 64) * m.pitch);
+    const int blocks = min((int)((m.rows - r0 + 63) / 64), D / 64);
+    bytes = __builtin_amdgcn_readfirstlane(m.k > 0 && blocks > 0 ? (uint32_t)blocks * (uint32_t)m.pitch : 0);
+    off = (uint32_t)(c >> 3) * (uint32_t)m.pitch + (uint32_t)(R * ROWB + (c & 7) * 16);
+  }
+  __device__ __forceinline__ void set(int kt) {
+    const uint32_t at = (uint32_t)kt * (KSTEP * ROWB);
+    rs = __builtin_amdgcn_make_buffer_rsrc((void*)uniform64(p + at), (short)0,
+                                           __builtin_amdgcn_readfirstlane((int)(bytes > at ? bytes - at : 0)), 0x00020000);
+  }
+  __device__ __forceinline__ void issue(uint8_t* stage, int wave, int j) const {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr_t)(stage + TrCopy<D>::row0(wave, j) * (2 * D)), 16, off,
+                                             TrCopy<D>::row0(0, j) * ROWB, 0, 0);
   }
 };
 
@@ -282,8 +330,8 @@ struct Args {
   Up up;
   // outputs
   void* out;            // DZ: bf16, ACC: fp32 [slices][..], STORE: bf16
-  int64_t ldo;          // elements
-  int64_t cols;         // DZ: columns to store, whole K steps
+  int64_t ldo;          // elements; DZ: of a block
+  int64_t cols;         // DZ: columns to store, whole blocks
   int64_t slice;        // elements of a slice
   int add;              // ACC: add to what is there
   int vec_out;
@@ -335,8 +383,9 @@ __global__ void __launch_bounds__(2 * D, D == 256 ? 1 : 2) head_kernel(Args g) {
   const int kb0 = EPI == EPI_ACC ? (int)((int64_t)sl * nk / g.slices) : 0;
   const int kb1 = EPI == EPI_ACC ? (int)((int64_t)(sl + 1) * nk / g.slices) : nk;
 
-  typename std::conditional<TA, TrCopy<D>, RowCopy<D>>::type ca;
-  typename std::conditional<TB, TrCopy<D>, RowCopy<D>>::type cb;
+  // A is X' or dz, B the weight or (with A transposed) X'
+  typename std::conditional<TA, BlockTrCopy<D>, BlockRowCopy<D>>::type ca;
+  typename std::conditional<TA, BlockTrCopy<D>, typename std::conditional<TB, TrCopy<D>, RowCopy<D>>::type>::type cb;
   ca.init(g.a, m0, wave, lane);
   cb.init(g.b, n0, wave, lane);
   v4f acc[MT][4];
@@ -466,18 +515,21 @@ __global__ void __launch_bounds__(2 * D, D == 256 ? 1 : 2) head_kernel(Args g) {
     const float c = g.up.common(live);
     float lse[MT], u[MT];
     int lab[MT];
+    // dz's rows up to the next 64 are read, zero past the live ones; so are whole
+    // blocks, zero past the piece
 #pragma unroll
     for (int tm = 0; tm < MT; ++tm) {
-      const int64_t m = min<int64_t>(mw + tm * 16, g.M - 1);
-      lse[tm] = g.lse[m] * LOG2E;
-      u[tm] = g.up.rest(g.rows[m], c);
-      lab[tm] = (int)(g.y[m] - g.v0 - nw);
+      const bool on = mw + tm * 16 < g.M;
+      const int64_t m = on ? mw + tm * 16 : 0;
+      lse[tm] = on ? g.lse[m] * LOG2E : __builtin_inff();
+      u[tm] = on ? g.up.rest(g.rows[m], c) : 0.f;
+      lab[tm] = on ? (int)(g.y[m] - g.v0 - nw) : -1;
     }
-    store_bf16<MT, false>(stage, lane, m0 + wm * 16 * MT, n0 + wn * 64, g.M, g.cols, (uint16_t*)g.out, g.ldo, 1, [&](int tm, int tn, float (&v)[4]) {
+    const int64_t block = n0 / 64 + wn;
+    store_bf16<MT, false>(stage, lane, m0 + wm * 16 * MT, 0, (g.M + 63) / 64 * 64, g.cols - block * 64, (uint16_t*)g.out + block * g.ldo, 64, 1, [&](int tm, int tn, float (&v)[4]) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[tm][tn][r], LOG2E, -lse[tm]));
-        // whole K steps are stored, zero past the piece
         v[r] = nw + tn * 16 + r < g.N ? (lab[tm] == tn * 16 + r ? p - 1.0f : p) * u[tm] : 0.f;
       }
     });
@@ -539,34 +591,35 @@ __global__ void __launch_bounds__(SCAN) scan_kernel(const void* targets, int t64
   if (tid == 0) live[0] = base;
 }
 
-// X' rows: 16-byte pieces of the live rows of X, zero past H; a piece of an
-// unaligned or ragged row element by element.  Also what the other kernels
-// expect set: zl (NaN until a tile finds the label) and a zero loss for the
-// ignored rows.
+// X': 16-byte pieces of the live rows of X into blocks of 64 columns, zero past
+// H and, by the last 63 workgroups, in the rows up to the next 64; a piece of an
+// unaligned or ragged row element by element.  Also what the other kernels expect
+// set: zl (NaN until a tile finds the label) and a zero loss for the ignored rows.
 __global__ void __launch_bounds__(256) gather_kernel(const uint16_t* x, int64_t ldx, int64_t T, int64_t H, int aligned16,
-                                                     const int32_t* pos, uint16_t* xp, int64_t hk, int64_t ldp, float* zl,
-                                                     float* loss) {
+                                                     const int32_t* pos, const int32_t* live, uint16_t* xp, int64_t hk,
+                                                     int64_t block, float* zl, float* loss) {
   const int64_t t = blockIdx.x;
-  const int at = pos[t];
+  const bool past = t >= T;
+  const int64_t at = past ? live[0] + (t - T) : pos[t];
+  if (past && at >= (live[0] + 63) / 64 * 64) return;
   if (at < 0) {
     if (threadIdx.x == 0 && loss) loss[t] = 0.f;
     return;
   }
-  if (threadIdx.x == 0) zl[at] = __builtin_nanf("");
+  if (threadIdx.x == 0 && !past) zl[at] = __builtin_nanf("");
   const uint16_t* src = x + t * ldx;
-  uint4* dst = reinterpret_cast<uint4*>(xp + (int64_t)at * ldp);
   for (int64_t c = threadIdx.x; c < hk / 8; c += blockDim.x) {
     uint4 v = make_uint4(0, 0, 0, 0);
-    if (aligned16 && c * 8 + 8 <= H) {
+    if (!past && aligned16 && c * 8 + 8 <= H) {
       v = *reinterpret_cast<const uint4*>(src + c * 8);
-    } else {
+    } else if (!past) {
       uint32_t w[4] = {0, 0, 0, 0};
 #pragma unroll
       for (int i = 0; i < 8; ++i)
         if (c * 8 + i < H) w[i >> 1] |= (uint32_t)src[c * 8 + i] << (16 * (i & 1));
       v = make_uint4(w[0], w[1], w[2], w[3]);
     }
-    dst[c] = v;
+    *reinterpret_cast<uint4*>(xp + (c >> 3) * block + at * 64 + (c & 7) * 8) = v;
   }
 }
 
@@ -652,24 +705,21 @@ __global__ void __launch_bounds__(256) scatter_kernel(const float* acc, int64_t 
   }
 }
 
-// Pitch of a matrix of the kernels' own with `steps` 128-byte K steps: an odd
-// number of them.  A tile reads one step of 256 rows at a time, and rows a power
-// of two apart lie in few of the memory's channels (dz of 65536 words in 4096
-// rows: its products took PLACEHOLDER).
-static int64_t odd_pitch(int64_t cols) { return (cdiv(cols, 64) | 1) * 64; }
+// elements of a block of X' or dz: 64 columns of T rows, whole 64 of them
+static int64_t block_of(int64_t T) { return cdiv(T, 64) * 64 * 64; }
 
 // what the forward leaves for the backward
 struct State {
-  int64_t hk, hp;  // columns of X', whole K steps; its pitch, elements
+  int64_t hk, block;  // columns of X', whole blocks; elements of one
   int64_t xp, pos, rows, y, lse, live, bytes;
 };
 static State state_of(int64_t T, int64_t H) {
   State s;
   s.hk = cdiv(H, 64) * 64;
-  s.hp = odd_pitch(H);
+  s.block = block_of(T);
   auto up = [](int64_t v) { return cdiv(v, 256) * 256; };
   s.xp = 0;
-  s.pos = up(T * s.hp * 2);
+  s.pos = up(s.hk / 64 * s.block * 2);
   s.rows = s.pos + up(T * 4);
   s.y = s.rows + up(T * 4);
   s.lse = s.y + up(T * 4);
@@ -725,7 +775,7 @@ static int64_t forward_ws(int64_t T, int64_t V) { return forward_parts(T, V) * T
 
 // backward: pieces of the vocabulary, tiles, ranges of the dX product, workspace
 struct Plan {
-  int64_t piece, pitch;  // words of a piece, dz's pitch in elements
+  int64_t piece, block;  // words of a piece, elements of a block of dz
   int dz_tile, dx_tile, dw_tile, slices;
   int64_t dz, acc, most, bytes;
 };
@@ -736,14 +786,14 @@ static Plan plan_of(int64_t T, int64_t H, int64_t V) {
   const int64_t words = std::min<int64_t>(1 << 20, std::max<int64_t>(256, DZ_BYTES / (T * 2) / 256 * 256));
   p.piece = cdiv(cdiv(V, cdiv(V, words)), 256) * 256;
   const int64_t cols = std::min(p.piece, V);
-  p.pitch = odd_pitch(cols);
+  p.block = block_of(T);
   p.dz_tile = tile_for(T, cols);
   p.dw_tile = tile_for(cols, H);
   // dX: ranges can fill the chip with either tile; the small one where the large one's are too short
   const int64_t steps = cdiv(cols, KSTEP);
   p.dx_tile = cdiv(T, 256) * cdiv(H, 256) * std::max<int64_t>(1, steps / 16) < split_device_cus() || T <= 128 ? 128 : 256;
   p.slices = ranges_for(p.dx_tile, T, H, steps);
-  p.dz = cdiv(T * p.pitch * 2, 256) * 256;
+  p.dz = cdiv(cols, 64) * p.block * 2;
   p.acc = T * hk * 4 * p.slices;
   p.most = p.dz + p.acc;
   p.bytes = p.most + 256;
@@ -752,7 +802,7 @@ static Plan plan_of(int64_t T, int64_t H, int64_t V) {
 
 static int check(const char* fn, const void* w, int64_t T, int64_t H, int64_t V, int64_t ldw) {
   if (T < 0 || H < 1 || V < 1) return fail(NTLB_EINVAL, "%s: bad shape T %lld H %lld V %lld", fn, (long long)T, (long long)H, (long long)V);
-  if (T > (1 << 24) || V > (1 << 30) || H > (1 << 20)) return fail(NTLB_EUNSUPPORTED, "%s: T %lld H %lld V %lld is too large", fn, (long long)T, (long long)H, (long long)V);
+  if (T > (1 << 22) || V > (1 << 30) || H > (1 << 20)) return fail(NTLB_EUNSUPPORTED, "%s: T %lld H %lld V %lld is too large", fn, (long long)T, (long long)H, (long long)V);
   if (!w || !aligned(w, 16) || ldw < H || ldw % 8 || ldw > (1 << 22)) return fail(NTLB_EINVAL, "%s: the weight needs 16-byte rows of at least H values", fn);
   return NTLB_OK;
 }
@@ -795,9 +845,9 @@ extern "C" int ntlb_linear_xent_forward(const uint16_t* x, int64_t ldx, const ui
     zl = (float*)((uint8_t*)workspace + parts * T * 8);
     each = zl + cdiv(T * 4, 256) * 64;
     const int al = aligned(x, 16) && ldx % 8 == 0;
-    xent::gather_kernel<<<(unsigned)T, 256, 0, st>>>(x, ldx, T, H, al, pos, xp, s.hk, s.hp, zl, reduction == 0 ? loss : nullptr);
+    xent::gather_kernel<<<(unsigned)T + 63, 256, 0, st>>>(x, ldx, T, H, al, pos, live, xp, s.hk, s.block, zl, reduction == 0 ? loss : nullptr);
     xent::Args g{};
-    g.a = {(const uint8_t*)xp, s.hp * 2, T, s.hk};
+    g.a = {(const uint8_t*)xp, s.block * 2, T, s.hk};
     g.b = {(const uint8_t*)w, ldw * 2, V, H};
     g.M = T; g.N = V; g.live = live; g.group_m = 8; g.part = part; g.ldp = T; g.zl = zl; g.y = y;
     xent::launch_head<false, false, xent::EPI_LSE>(xent::tile_for(T, V), g, st);
@@ -834,16 +884,16 @@ extern "C" int ntlb_linear_xent_backward(const void* state, const uint16_t* w, i
     const uint8_t* wp = (const uint8_t*)(w + v0 * ldw);
     xent::Args g{};
     g.live = live; g.group_m = 8;
-    g.a = {sp + s.xp, s.hp * 2, Tn, s.hk};
+    g.a = {sp + s.xp, s.block * 2, Tn, s.hk};
     g.b = {wp, ldw * 2, n, H};
     g.M = T; g.N = n; g.y = (const int32_t*)(sp + s.y); g.v0 = v0; g.lse = (const float*)(sp + s.lse);
     g.rows = (const int32_t*)(sp + s.rows); g.up = up;
-    g.out = dz; g.ldo = p.pitch; g.cols = np;
+    g.out = dz; g.ldo = p.block; g.cols = np;
     if (T > 0) xent::launch_head<false, false, xent::EPI_DZ>(p.dz_tile, g, st);
     if (dx && T > 0) {
       xent::Args x{};
       x.live = live; x.group_m = 8; x.slices = p.slices;
-      x.a = {(const uint8_t*)dz, p.pitch * 2, Tn, np};
+      x.a = {(const uint8_t*)dz, p.block * 2, Tn, np};
       x.b = {wp, ldw * 2, H, n};
       x.M = T; x.N = H; x.out = acc; x.ldo = s.hk; x.slice = T * s.hk; x.add = v0 > 0;
       xent::launch_head<false, true, xent::EPI_ACC>(p.dx_tile, x, st);
@@ -851,8 +901,8 @@ extern "C" int ntlb_linear_xent_backward(const void* state, const uint16_t* w, i
     if (dw) {
       xent::Args q{};
       q.live = live; q.group_m = 8;
-      q.a = {(const uint8_t*)dz, p.pitch * 2, np, Tn};
-      q.b = {sp + s.xp, s.hp * 2, s.hk, Tn};
+      q.a = {(const uint8_t*)dz, p.block * 2, np, Tn};
+      q.b = {sp + s.xp, s.block * 2, s.hk, Tn};
       q.M = n; q.N = H; q.out = dw + v0 * lddw; q.ldo = lddw;
       q.up = up;
       q.vec_out = aligned(dw, 16) && lddw % 8 == 0;
