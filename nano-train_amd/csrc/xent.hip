@@ -405,11 +405,16 @@ __global__ void __launch_bounds__(2 * D, D == 256 ? 1 : 2) head_kernel(Args g) {
       cb.issue(nb, wave, j);
     };
     auto rows = [&](int tm, const v8i (&bf)[4], const v8i& a) {
+      // one operand by rows, one transposed: the products before the other wave's
+      // reads (4096 x 7168 over 65536: 2.85 ms, without 3.10; of two operands read
+      // alike 4096 x 65536 over 7168 5.48 and 5.41 ms, 65536 x 7168 over 4096 2.89 and 2.69)
+      if (TB && !TA) __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int tn = 0; tn < 4; ++tn) acc[tm][tn] = mma<0>(bf[tn], a, acc[tm][tn]);
 #pragma unroll
       for (int tn = 0; tn < 4; ++tn) acc[tm][tn] = mma<1>(bf[tn], a, acc[tm][tn]);
       asm volatile("" : "+v"(acc[tm][0]), "+v"(acc[tm][1]), "+v"(acc[tm][2]), "+v"(acc[tm][3])::"memory");
+      if (TB && !TA) __builtin_amdgcn_s_setprio(0);
     };
     ca.set(kb0);
     cb.set(kb0);
@@ -558,18 +563,29 @@ __global__ void __launch_bounds__(2 * D, D == 256 ? 1 : 2) head_kernel(Args g) {
 
 // ---------------------------------------------------------------------------
 // the live rows: pos[t] = place of row t among them (-1: ignored), rows[i] and
-// y[i] (-1: not a word) of the i-th, live[0] how many; one workgroup
+// y[i] (-1: not a word) of the i-th, live[0] how many.  One workgroup; up to HERE
+// rows each of gather_kernel's counts for itself (16 rows: 5.0 us, with this
+// launch 4.7 + 4.9; 1003 rows 5.0 and 2.4 + 3.6).
 // ---------------------------------------------------------------------------
-constexpr int SCAN = 1024;
-__global__ void __launch_bounds__(SCAN) scan_kernel(const void* targets, int t64, int64_t T, int64_t V, int64_t ignore,
-                                                    int32_t* pos, int32_t* rows, int32_t* y, int32_t* live) {
+constexpr int SCAN = 1024, HERE = 1024;
+struct Targets {
+  const void* p;
+  int wide;
+  int64_t T, V, ignore;
+  __device__ int64_t at(int64_t t) const { return t >= T ? ignore : wide ? ((const int64_t*)p)[t] : (int64_t)((const int32_t*)p)[t]; }
+  __device__ int32_t word(int64_t v) const { return v >= 0 && v < V ? (int32_t)v : -1; }
+};
+struct Live {
+  int32_t *pos, *rows, *y, *live;
+};
+
+__global__ void __launch_bounds__(SCAN) scan_kernel(Targets tg, Live o) {
   __shared__ int wsum[SCAN / 64];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   int base = 0;
-  for (int64_t t0 = 0; t0 < T; t0 += SCAN) {
-    const int64_t t = t0 + tid;
-    const int64_t v = t < T ? (t64 ? ((const int64_t*)targets)[t] : (int64_t)((const int32_t*)targets)[t]) : ignore;
-    const bool on = t < T && v != ignore;
+  for (int64_t t0 = 0; t0 < tg.T; t0 += SCAN) {
+    const int64_t t = t0 + tid, v = tg.at(t);
+    const bool on = v != tg.ignore;
     const uint64_t b = __ballot(on);
     if (lane == 0) wsum[wave] = __popcll(b);
     __syncthreads();
@@ -580,28 +596,61 @@ __global__ void __launch_bounds__(SCAN) scan_kernel(const void* targets, int t64
       all += wsum[w];
     }
     const int at = before + __popcll(b & ((1ull << lane) - 1));
-    if (t < T) pos[t] = on ? at : -1;
+    if (t < tg.T) o.pos[t] = on ? at : -1;
     if (on) {
-      rows[at] = (int32_t)t;
-      y[at] = v >= 0 && v < V ? (int32_t)v : -1;
+      o.rows[at] = (int32_t)t;
+      o.y[at] = tg.word(v);
     }
     base += all;
     __syncthreads();
   }
-  if (tid == 0) live[0] = base;
+  if (tid == 0) o.live[0] = base;
 }
 
 // X': 16-byte pieces of the live rows of X into blocks of 64 columns, zero past
 // H and, by the last 63 workgroups, in the rows up to the next 64; a piece of an
 // unaligned or ragged row element by element.  Also what the other kernels expect
 // set: zl (NaN until a tile finds the label) and a zero loss for the ignored rows.
-__global__ void __launch_bounds__(256) gather_kernel(const uint16_t* x, int64_t ldx, int64_t T, int64_t H, int aligned16,
-                                                     const int32_t* pos, const int32_t* live, uint16_t* xp, int64_t hk,
-                                                     int64_t block, float* zl, float* loss) {
+template <bool COUNT>
+__global__ void __launch_bounds__(256) gather_kernel(const uint16_t* x, int64_t ldx, int64_t H, int aligned16, Targets tg,
+                                                     Live o, uint16_t* xp, int64_t hk, int64_t block, float* zl, float* loss) {
   const int64_t t = blockIdx.x;
-  const bool past = t >= T;
-  const int64_t at = past ? live[0] + (t - T) : pos[t];
-  if (past && at >= (live[0] + 63) / 64 * 64) return;
+  const bool past = t >= tg.T;
+  int at, n;
+  if constexpr (COUNT) {
+    __shared__ int2 red[4];
+    const int64_t v = tg.at(t);
+    int2 c = make_int2(0, 0);
+    for (int i = threadIdx.x; i < tg.T; i += 256) {
+      const bool on = tg.at(i) != tg.ignore;
+      c.x += on && i < t;
+      c.y += on;
+    }
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+      c.x += __shfl_xor(c.x, d);
+      c.y += __shfl_xor(c.y, d);
+    }
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = c;
+    __syncthreads();
+    at = red[0].x + red[1].x + red[2].x + red[3].x;
+    n = red[0].y + red[1].y + red[2].y + red[3].y;
+    const bool on = v != tg.ignore;
+    if (threadIdx.x == 0) {
+      if (!past) o.pos[t] = on ? at : -1;
+      if (on) {
+        o.rows[at] = (int32_t)t;
+        o.y[at] = tg.word(v);
+      }
+      if (t == 0) o.live[0] = n;
+    }
+    if (!on) at = -1;
+  } else {
+    n = o.live[0];
+    at = past ? -1 : o.pos[t];
+  }
+  if (past) at = n + (int)(t - tg.T);
+  if (past && at >= (n + 63) / 64 * 64) return;
   if (at < 0) {
     if (threadIdx.x == 0 && loss) loss[t] = 0.f;
     return;
@@ -619,42 +668,48 @@ __global__ void __launch_bounds__(256) gather_kernel(const uint16_t* x, int64_t 
         if (c * 8 + i < H) w[i >> 1] |= (uint32_t)src[c * 8 + i] << (16 * (i & 1));
       v = make_uint4(w[0], w[1], w[2], w[3]);
     }
-    *reinterpret_cast<uint4*>(xp + (c >> 3) * block + at * 64 + (c & 7) * 8) = v;
+    *reinterpret_cast<uint4*>(xp + (c >> 3) * block + (int64_t)at * 64 + (c & 7) * 8) = v;
   }
 }
 
-// lse and loss of the live rows from their pairs: 16 rows by 16 walkers
-__global__ void __launch_bounds__(256) join_kernel(const float2* part, int64_t ldp, int64_t parts, const float* zl,
-                                                   const int32_t* rows, const int32_t* live, float* lse, float* each,
-                                                   float* loss) {
-  __shared__ float2 red[16][17];
-  const int r = threadIdx.x & 15, q = threadIdx.x >> 4;
-  const int64_t m = (int64_t)blockIdx.x * 16 + r;
-  const bool on = m < live[0];
-  if ((int64_t)blockIdx.x * 16 >= live[0]) return;
-  float mx = -__builtin_inff(), s = 0.f;
+// (max, sum) of two sets
+__device__ __forceinline__ float2 merge(float2 a, float2 b) {
+  const float hi = fmaxf(a.x, b.x), ref = hi == -__builtin_inff() ? 0.f : hi;
+  return make_float2(hi, a.y * __builtin_amdgcn_exp2f((a.x - ref) * LOG2E) + b.y * __builtin_amdgcn_exp2f((b.x - ref) * LOG2E));
+}
+
+// lse and loss of the live rows from their pairs, R rows by Q walkers
+template <int R, int Q>
+__global__ void __launch_bounds__(R * Q) join_kernel(const float2* part, int64_t ldp, int64_t parts, const float* zl,
+                                                     const int32_t* rows, const int32_t* live, float* lse, float* each,
+                                                     float* loss) {
+  constexpr int WAVES = R * Q / 64;
+  __shared__ float2 red[WAVES][R];
+  const int tid = threadIdx.x, r = tid % R, q = tid / R, n = live[0];
+  const int64_t m = (int64_t)blockIdx.x * R + r;
+  const bool on = m < n;
+  float2 p = make_float2(-__builtin_inff(), 0.f);
   if (on)
-    for (int64_t i = q; i < parts; i += 16) {
-      const float2 t = part[i * ldp + m];
-      const float hi = fmaxf(mx, t.x), ref = hi == -__builtin_inff() ? 0.f : hi;
-      s = s * __builtin_amdgcn_exp2f((mx - ref) * LOG2E) + t.y * __builtin_amdgcn_exp2f((t.x - ref) * LOG2E);
-      mx = hi;
-    }
-  red[q][r] = make_float2(mx, s);
+#pragma unroll 4
+    for (int64_t i = q; i < parts; i += Q) p = merge(p, part[i * ldp + m]);
+#pragma unroll
+  for (int d = R; d < 64; d *= 2) p = merge(p, make_float2(__shfl_xor(p.x, d), __shfl_xor(p.y, d)));
+  if ((tid & 63) < R) red[tid >> 6][r] = p;
   __syncthreads();
   if (q == 0 && on) {
-    for (int i = 1; i < 16; ++i) mx = fmaxf(mx, red[i][r].x);
-    const float ref = mx == -__builtin_inff() ? 0.f : mx;
-    s = 0.f;
-    for (int i = 0; i < 16; ++i) s += red[i][r].y * __builtin_amdgcn_exp2f((red[i][r].x - ref) * LOG2E);
-    const float l = ref + __builtin_amdgcn_logf(s) * LN2, z = zl[m];
+#pragma unroll
+    for (int i = 1; i < WAVES; ++i) p = merge(p, red[i][r]);
+    const float ref = p.x == -__builtin_inff() ? 0.f : p.x;
+    const float l = ref + __builtin_amdgcn_logf(p.y) * LN2, z = zl[m];
     lse[m] = z != z ? z : l;  // no such word, or its logit is NaN: so is all of the row
     each[m] = l - z;
     if (loss) loss[rows[m]] = l - z;
   }
 }
 
-// the sum or mean of the live rows' losses, in a fixed order; 0 where none is live
+// the sum or mean of the live rows' losses, in a fixed order; 0 where none is
+// live.  A launch of its own, 2 us: the join's last workgroup cannot know that it
+// is the last without a fence in each, 15 us for 4096 rows.
 __global__ void __launch_bounds__(1024) total_kernel(const float* each, const int32_t* live, int mean, float* loss) {
   __shared__ float red[16];
   const int n = live[0];
@@ -834,26 +889,38 @@ extern "C" int ntlb_linear_xent_forward(const uint16_t* x, int64_t ldx, const ui
   hipStream_t st = as_stream(stream);
   const xent::State s = xent::state_of(std::max<int64_t>(T, 1), H);
   uint8_t* sp = (uint8_t*)state;
-  int32_t *pos = (int32_t*)(sp + s.pos), *rows = (int32_t*)(sp + s.rows), *y = (int32_t*)(sp + s.y), *live = (int32_t*)(sp + s.live);
+  const xent::Targets tg{targets, targets64, T, V, ignore_index};
+  const xent::Live o{(int32_t*)(sp + s.pos), (int32_t*)(sp + s.rows), (int32_t*)(sp + s.y), (int32_t*)(sp + s.live)};
   float* lse = (float*)(sp + s.lse);
   uint16_t* xp = (uint16_t*)(sp + s.xp);
-  xent::scan_kernel<<<1, xent::SCAN, 0, st>>>(targets, targets64, T, V, ignore_index, pos, rows, y, live);
-  float *zl = nullptr, *each = nullptr;
+  const int64_t parts = T > 0 ? xent::forward_parts(T, V) : 0;
+  float2* part = (float2*)workspace;
+  float* zl = T > 0 ? (float*)((uint8_t*)workspace + parts * T * 8) : nullptr;
+  float* each = T > 0 ? zl + cdiv(T * 4, 256) * 64 : nullptr;
+  float* rows_loss = reduction == 0 ? loss : nullptr;
+  const int al = aligned(x, 16) && ldx % 8 == 0;
+  if (T > xent::HERE) {
+    xent::scan_kernel<<<1, xent::SCAN, 0, st>>>(tg, o);
+    xent::gather_kernel<false><<<(unsigned)T + 63, 256, 0, st>>>(x, ldx, H, al, tg, o, xp, s.hk, s.block, zl, rows_loss);
+  } else {
+    xent::gather_kernel<true><<<(unsigned)T + 63, 256, 0, st>>>(x, ldx, H, al, tg, o, xp, s.hk, s.block, zl, rows_loss);
+  }
   if (T > 0) {
-    const int64_t parts = xent::forward_parts(T, V);
-    float2* part = (float2*)workspace;
-    zl = (float*)((uint8_t*)workspace + parts * T * 8);
-    each = zl + cdiv(T * 4, 256) * 64;
-    const int al = aligned(x, 16) && ldx % 8 == 0;
-    xent::gather_kernel<<<(unsigned)T + 63, 256, 0, st>>>(x, ldx, T, H, al, pos, live, xp, s.hk, s.block, zl, reduction == 0 ? loss : nullptr);
     xent::Args g{};
     g.a = {(const uint8_t*)xp, s.block * 2, T, s.hk};
     g.b = {(const uint8_t*)w, ldw * 2, V, H};
-    g.M = T; g.N = V; g.live = live; g.group_m = 8; g.part = part; g.ldp = T; g.zl = zl; g.y = y;
+    g.M = T; g.N = V; g.live = o.live; g.group_m = 8; g.part = part; g.ldp = T; g.zl = zl; g.y = o.y;
     xent::launch_head<false, false, xent::EPI_LSE>(xent::tile_for(T, V), g, st);
-    xent::join_kernel<<<(unsigned)cdiv(T, 16), 256, 0, st>>>(part, T, parts, zl, rows, live, lse, each, reduction == 0 ? loss : nullptr);
   }
-  if (reduction != 0) xent::total_kernel<<<1, 1024, 0, st>>>(each, live, reduction == 2, loss);
+  if (T > 0) {
+    // many pairs of few rows: more walkers to a row (16 rows of 1024 pairs: 5.6 us, by
+    // 16 walkers 27; 4096 rows of 256: 8.5 and 6.7)
+    if (parts > 128 && T <= 1024)
+      xent::join_kernel<4, 256><<<(unsigned)cdiv(T, 4), 1024, 0, st>>>(part, T, parts, zl, o.rows, o.live, lse, each, rows_loss);
+    else
+      xent::join_kernel<16, 16><<<(unsigned)cdiv(T, 16), 256, 0, st>>>(part, T, parts, zl, o.rows, o.live, lse, each, rows_loss);
+  }
+  if (reduction != 0) xent::total_kernel<<<1, 1024, 0, st>>>(each, o.live, reduction == 2, loss);
   return check_launch(fn);
 }
 
