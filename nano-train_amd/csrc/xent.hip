@@ -319,7 +319,7 @@ struct Args {
   int slices;           // ACC: ranges of the contraction, one after another in the grid
   int group_m;          // raster: row tiles side by side
   // LSE
-  float2* part;         // [column tiles][ldp] (max, sum)
+  float2* part;         // [column tiles][ldp] (ref, sum)
   int64_t ldp;
   float* zl;            // [M] the label's logit
   const int32_t* y;     // labels of the live rows, < 0: none
@@ -336,6 +336,14 @@ struct Args {
   int add;              // ACC: add to what is there
   int vec_out;
 };
+
+// A set of logits z: the largest z log2(e), ref, and the sum of 2^(z log2(e) - ref).
+// Rounded once, ref is the same number for whoever adds to the sum, so its
+// rounding costs nothing.
+__device__ __forceinline__ float2 merge(float2 a, float2 b) {
+  const float hi = fmaxf(a.x, b.x), ref = hi == -__builtin_inff() ? 0.f : hi;
+  return make_float2(hi, a.y * __builtin_amdgcn_exp2f(a.x - ref) + b.y * __builtin_amdgcn_exp2f(b.x - ref));
+}
 
 // D x D output tiles: 256, eight waves of 128 x 64, one workgroup a compute unit;
 // 128, four waves of 64 x 64, two workgroups
@@ -474,47 +482,54 @@ __global__ void __launch_bounds__(2 * D, D == 256 ? 1 : 2) head_kernel(Args g) {
   uint8_t* stage = (wave / PER == 0 ? la0 : wave / PER == 1 ? lb0 : wave / PER == 2 ? la1 : lb1) + (wave % PER) * 16384;
   // lane: rows m0 + wm*16*MT + tm*16 + lane%16, columns n0 + wn*64 + tn*16 + 4*(lane/16) + r
   const int64_t mw = m0 + wm * 16 * MT + (lane & 15), nw = n0 + wn * 64 + (lane >> 4) * 4;
+  // Few waves hold columns past N or a row's label: what either asks of each value
+  // stands behind a test of the whole wave
+  const int cols = (int)min<int64_t>(64, g.N - (n0 + wn * 64)) - (lane >> 4) * 4;  // of N, from the lane's first
+  const bool edge = g.N - (n0 + wn * 64) < 64;
   if constexpr (EPI == EPI_LSE) {
     float2* red = reinterpret_cast<float2*>(la0);  // [WAVES_N][D]
+    int lab[MT];  // the label's column, from the lane's first
+#pragma unroll
+    for (int tm = 0; tm < MT; ++tm) lab[tm] = mw + tm * 16 < g.M ? (int)(g.y[mw + tm * 16] - nw) : -1;
 #pragma unroll
     for (int tm = 0; tm < MT; ++tm) {
-      const int64_t m = mw + tm * 16;
-      const int64_t lab = (m < g.M ? (int64_t)g.y[m] : -1) - g.v0 - nw;  // the label's column, from the lane's first
+      if (__any(lab[tm] >= 0 && lab[tm] < 64)) {
+#pragma unroll
+        for (int tn = 0; tn < 4; ++tn)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (lab[tm] == tn * 16 + r) g.zl[mw + tm * 16] = acc[tm][tn][r];
+      }
+      if (edge) {
+#pragma unroll
+        for (int tn = 0; tn < 4; ++tn)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (tn * 16 + r >= cols) acc[tm][tn][r] = -__builtin_inff();
+      }
       float mx = -__builtin_inff();
 #pragma unroll
       for (int tn = 0; tn < 4; ++tn)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          if (nw + tn * 16 + r >= g.N) acc[tm][tn][r] = -__builtin_inff();
-          mx = fmaxf(mx, acc[tm][tn][r]);
-          if (lab == tn * 16 + r && m < g.M) g.zl[m] = acc[tm][tn][r];
-        }
+        for (int r = 0; r < 4; ++r) mx = fmaxf(mx, acc[tm][tn][r]);
       mx = fmaxf(mx, __shfl_xor(mx, 16));
-      mx = fmaxf(mx, __shfl_xor(mx, 32));
+      mx = fmaxf(mx, __shfl_xor(mx, 32)) * LOG2E;
       const float ref = mx == -__builtin_inff() ? 0.f : mx;
       float s = 0.f;
 #pragma unroll
       for (int tn = 0; tn < 4; ++tn)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) s += __builtin_amdgcn_exp2f((acc[tm][tn][r] - ref) * LOG2E);
+        for (int r = 0; r < 4; ++r) s += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[tm][tn][r], LOG2E, -ref));
       s += __shfl_xor(s, 16);
       s += __shfl_xor(s, 32);
       if (lane < 16) red[wn * D + wm * 16 * MT + tm * 16 + lane] = make_float2(mx, s);
     }
     __syncthreads();
     if (tid < D && m0 + tid < g.M) {
-      float2 t[WAVES_N];
-      float mx = -__builtin_inff();
+      float2 t = red[tid];
 #pragma unroll
-      for (int i = 0; i < WAVES_N; ++i) {
-        t[i] = red[i * D + tid];
-        mx = fmaxf(mx, t[i].x);
-      }
-      const float ref = mx == -__builtin_inff() ? 0.f : mx;
-      float s = 0.f;
-#pragma unroll
-      for (int i = 0; i < WAVES_N; ++i) s += t[i].y * __builtin_amdgcn_exp2f((t[i].x - ref) * LOG2E);
-      g.part[(n0 / TN) * g.ldp + m0 + tid] = make_float2(mx, s);
+      for (int i = 1; i < WAVES_N; ++i) t = merge(t, red[i * D + tid]);
+      g.part[(n0 / TN) * g.ldp + m0 + tid] = t;
     }
   } else if constexpr (EPI == EPI_DZ) {
     const float c = g.up.common(live);
@@ -530,13 +545,32 @@ __global__ void __launch_bounds__(2 * D, D == 256 ? 1 : 2) head_kernel(Args g) {
       u[tm] = on ? g.up.rest(g.rows[m], c) : 0.f;
       lab[tm] = on ? (int)(g.y[m] - g.v0 - nw) : -1;
     }
+#pragma unroll
+    for (int tm = 0; tm < MT; ++tm) {
+#pragma unroll
+      for (int tn = 0; tn < 4; ++tn)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          acc[tm][tn][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[tm][tn][r], LOG2E, -lse[tm]));
+      if (__any(lab[tm] >= 0 && lab[tm] < 64)) {
+#pragma unroll
+        for (int tn = 0; tn < 4; ++tn)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (lab[tm] == tn * 16 + r) acc[tm][tn][r] -= 1.0f;
+      }
+      if (edge) {
+#pragma unroll
+        for (int tn = 0; tn < 4; ++tn)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (tn * 16 + r >= cols) acc[tm][tn][r] = 0.f;
+      }
+    }
     const int64_t block = n0 / 64 + wn;
     store_bf16<MT, false>(stage, lane, m0 + wm * 16 * MT, 0, (g.M + 63) / 64 * 64, g.cols - block * 64, (uint16_t*)g.out + block * g.ldo, 64, 1, [&](int tm, int tn, float (&v)[4]) {
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[tm][tn][r], LOG2E, -lse[tm]));
-        v[r] = nw + tn * 16 + r < g.N ? (lab[tm] == tn * 16 + r ? p - 1.0f : p) * u[tm] : 0.f;
-      }
+      for (int r = 0; r < 4; ++r) v[r] = acc[tm][tn][r] * u[tm];
     });
   } else if constexpr (EPI == EPI_ACC) {
     float* o = (float*)g.out + sl * g.slice;
@@ -672,12 +706,6 @@ __global__ void __launch_bounds__(256) gather_kernel(const uint16_t* x, int64_t 
   }
 }
 
-// (max, sum) of two sets
-__device__ __forceinline__ float2 merge(float2 a, float2 b) {
-  const float hi = fmaxf(a.x, b.x), ref = hi == -__builtin_inff() ? 0.f : hi;
-  return make_float2(hi, a.y * __builtin_amdgcn_exp2f((a.x - ref) * LOG2E) + b.y * __builtin_amdgcn_exp2f((b.x - ref) * LOG2E));
-}
-
 // lse and loss of the live rows from their pairs, R rows by Q walkers
 template <int R, int Q>
 __global__ void __launch_bounds__(R * Q) join_kernel(const float2* part, int64_t ldp, int64_t parts, const float* zl,
@@ -700,7 +728,7 @@ __global__ void __launch_bounds__(R * Q) join_kernel(const float2* part, int64_t
 #pragma unroll
     for (int i = 1; i < WAVES; ++i) p = merge(p, red[i][r]);
     const float ref = p.x == -__builtin_inff() ? 0.f : p.x;
-    const float l = ref + __builtin_amdgcn_logf(p.y) * LN2, z = zl[m];
+    const float l = (ref + __builtin_amdgcn_logf(p.y)) * LN2, z = zl[m];
     lse[m] = z != z ? z : l;  // no such word, or its logit is NaN: so is all of the row
     each[m] = l - z;
     if (loss) loss[rows[m]] = l - z;
