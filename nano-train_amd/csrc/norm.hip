@@ -17,7 +17,7 @@
 // which a second kernel sums in a fixed order: the result does not depend on
 // how the workgroups are scheduled.
 // Measured (a large copy runs at 5.3 TB/s): 8192 x 7168 bf16 forward 38.6 us (6.1
-// TB/s), backward 70.5 (5.0) and 6.8 for dw and db's sums; 65536 x 512 fp16
+// TB/s), backward 70.1 (5.0) and 4.6 for dw and db's sums; 65536 x 512 fp16
 // forward 23.6 us (5.7), backward 34.9 (5.8) and 4.0; one row of 7168 3.3 us, the
 // launch and the latency of one pass.
 #include <hip/hip_runtime.h>
@@ -448,28 +448,34 @@ __global__ void __launch_bounds__(block_threads<RT>()) backward_kernel(Args g) {
   }
 }
 
-// dw / db (blockIdx.y) of 16 columns: 64 walkers down the P partial rows, their
-// sums added in a fixed tree
-constexpr int FIN_COLS = 16, FIN_WALK = 64;
-__global__ void __launch_bounds__(FIN_COLS* FIN_WALK) finish_kernel(const float* part, int P, int H, void* dw, void* db,
-                                                                     int w_dtype) {
-  __shared__ float sum[FIN_WALK / 4][FIN_COLS];
-  const int c = blockIdx.x * FIN_COLS + threadIdx.x % FIN_COLS, q = threadIdx.x / FIN_COLS;
+// dw / db (blockIdx.y) of 32 columns, two a thread, so that a partial row's piece
+// is a whole line: 64 walkers down the P partial rows, their sums added in a fixed
+// tree (256 rows of 7168: 4.6 us, by 16 columns, one a thread, 6.8)
+constexpr int FIN_COLS = 32, FIN_WALK = 64;
+__global__ void __launch_bounds__(FIN_COLS / 2 * FIN_WALK) finish_kernel(const float* part, int P, int H, void* dw, void* db,
+                                                                          int w_dtype) {
+  typedef float f2 __attribute__((ext_vector_type(2), aligned(4)));
+  constexpr int PAIRS = FIN_COLS / 2;
+  __shared__ f2 sum[FIN_WALK / 4][PAIRS];
+  const int c = blockIdx.x * FIN_COLS + threadIdx.x % PAIRS * 2, q = threadIdx.x / PAIRS;
   const float* p = part + (int64_t)blockIdx.y * P * H;
-  float a = 0.f;
-  if (c < H) {
+  f2 a = {0.f, 0.f};
+  if (c + 1 < H) {
 #pragma unroll 4
-    for (int r = q; r < P; r += FIN_WALK) a += p[(int64_t)r * H + c];
+    for (int r = q; r < P; r += FIN_WALK) a += *reinterpret_cast<const f2*>(p + (int64_t)r * H + c);
+  } else if (c < H) {
+    for (int r = q; r < P; r += FIN_WALK) a[0] += p[(int64_t)r * H + c];
   }
-  a += __shfl_xor(a, 16);
-  a += __shfl_xor(a, 32);
-  if ((threadIdx.x & 63) < FIN_COLS) sum[threadIdx.x >> 6][threadIdx.x % FIN_COLS] = a;
+#pragma unroll
+  for (int d = PAIRS; d < 64; d *= 2) a += (f2){__shfl_xor(a[0], d), __shfl_xor(a[1], d)};
+  if ((threadIdx.x & 63) < PAIRS) sum[threadIdx.x >> 6][threadIdx.x % PAIRS] = a;
   __syncthreads();
   void* out = blockIdx.y ? db : dw;
   if (q == 0 && c < H && out) {
 #pragma unroll
     for (int k = 1; k < FIN_WALK / 4; ++k) a += sum[k][threadIdx.x];
-    store_elem(out, w_dtype, c, a);
+    store_elem(out, w_dtype, c, a[0]);
+    if (c + 1 < H) store_elem(out, w_dtype, c + 1, a[1]);
   }
 }
 
@@ -635,7 +641,7 @@ extern "C" int ntlb_layer_norm_backward(const void* x, int x_dtype, int64_t T, i
     if (int rc = check_launch(fn)) return rc;
   }
   if (sums) {
-    const dim3 grd((unsigned)cdiv(H, norm::FIN_COLS), 2), blk(norm::FIN_COLS * norm::FIN_WALK);
+    const dim3 grd((unsigned)cdiv(H, norm::FIN_COLS), 2), blk(norm::FIN_COLS / 2 * norm::FIN_WALK);
     norm::finish_kernel<<<grd, blk, 0, st>>>((const float*)workspace, (int)n, (int)H, dw, db, w_dtype);
     return check_launch(fn);
   }
