@@ -1054,7 +1054,7 @@ int ntlb_route_topk_backward(const void* logits, int dtype, int64_t T, int64_t E
  * Ignored rows of x are not read.  state (ntlb_linear_xent_state_bytes, 256-byte
  * aligned) holds what the backward needs: the live rows of x among it, not w.
  * workspace: ntlb_linear_xent_workspace_bytes(T, H, V, 0), 16-byte aligned,
- * contents free.
+ * contents free.  T <= 2^22, V <= 2^30, H <= 2^20, ldw <= 2^22.
  */
 int ntlb_linear_xent_forward(const uint16_t* x, int64_t ldx, const uint16_t* w, int64_t ldw, const void* targets,
                              int targets64, int64_t T, int64_t H, int64_t V, int64_t ignore_index, int reduction,

@@ -336,3 +336,59 @@ def test_a_common_factor_is_not_rounded(gpu_device, n, reduction):
     want = p.scatter_add(1, y[:, None], torch.full((n, 1), -1.0, dtype=torch.float64, device=gpu_device)) @ w.double() / n
     part = float((dx.double() * want).sum() / (want * want).sum()) - 1
     assert abs(part) <= B / 8 + 4 * 2 * B / math.sqrt(n * H)
+
+
+@pytest.mark.parametrize("live", [1, 63, 64, 65, 128, 129])
+@pytest.mark.parametrize("T", [200, 1100])
+def test_memory_past_the_live_rows_takes_no_part(gpu_device, T, live):
+    """the contraction over positions ends inside a block of 64: whatever the workspace held there before, here NaN"""
+    from lowbit.loss import linear_cross_entropy
+
+    x, w, y, _ = _inputs(T, 200, 3000, live, gpu_device)
+    y[torch.randperm(T, generator=torch.Generator().manual_seed(live))[live:].to(gpu_device)] = IGNORE
+    x[y == IGNORE] = float("nan")
+    xl, wl = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    for _ in range(2):
+        torch.cuda.empty_cache()
+        junk = [torch.full((16 << 20,), float("nan"), device=gpu_device) for _ in range(4)]
+        junk += [torch.full((64 << 10,), float("nan"), device=gpu_device) for _ in range(64)]
+        del junk
+        loss = linear_cross_entropy(xl, wl, y)
+        dx, dw = torch.autograd.grad(loss, (xl, wl))
+        _check(torch.where((y == IGNORE)[:, None], torch.zeros_like(x), x), w, y, loss.detach(), dx, dw, "mean",
+               torch.ones((), device=gpu_device))
+
+
+@pytest.mark.parametrize("T", [1, 5, 1000])
+@pytest.mark.parametrize("scale", [1.0, 30.0])
+def test_few_rows_of_many_words(gpu_device, T, scale):
+    """hundreds of tiles' pairs to a row, of far apart maxima"""
+    from lowbit.loss import linear_cross_entropy
+
+    x, w, y, _ = _inputs(T, 64, 40001, T, gpu_device, 0.2, scale)
+    for reduction in ("none", "sum"):
+        with torch.no_grad():
+            _check(x, w, y, linear_cross_entropy(x, w, y, reduction=reduction), None, None, reduction, None)
+    w2 = w.clone()
+    w2[:39000] = -float("inf")  # rows of -inf, inf and NaN products: the pairs of whole tiles hold no number
+    x2 = x.abs()
+    x2[x2 == 0] = 1.0
+    live = y != IGNORE
+    y2 = torch.where(live, 39000 + y % 1001, y)
+    z = x2.double() @ w[39000:].double().t()
+    want = torch.logsumexp(z, 1) - z.gather(1, torch.where(live, y2 - 39000, 0)[:, None])[:, 0]
+    with torch.no_grad():
+        got = linear_cross_entropy(x2, w2, y2, reduction="none").double()
+    e = 4 * math.sqrt(64) * U * (x2.double().abs() @ w[39000:].double().abs().t()).amax(1)
+    bound = 2 * e + 16 * U * (torch.logsumexp(z, 1).abs() + z.abs().amax(1))
+    assert ((got - want).abs() <= bound)[live].all() and (got[~live] == 0).all()
+
+
+def test_too_large_is_refused():
+    """before anything is read or launched"""
+    from lowbit import _lib
+
+    p = 4096
+    for T, H, V, ldw in (((1 << 22) + 1, 64, 64, 64), (8, (1 << 20) + 8, 64, (1 << 20) + 8), (8, 64, (1 << 30) + 1, 64)):
+        with pytest.raises(_lib.LowBitKernelError, match="too large"):
+            _lib.call("ntlb_linear_xent_forward", p, H, p, ldw, p, 1, T, H, V, -100, 2, p, p, p, 1 << 60, 0)
