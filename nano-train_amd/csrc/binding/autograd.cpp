@@ -9,15 +9,20 @@
 // loaded, so this module links to no kernel and there is one library at a time.
 // Arguments are checked in Python, where an operator is called.
 #include <ATen/ATen.h>
+#include <ATen/hip/EmptyTensor.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <c10/core/DeviceGuard.h>
 #include <torch/csrc/Exceptions.h>
-#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/autograd/saved_variable.h>
 #include <torch/csrc/utils/object_ptr.h>
 
 #include <algorithm>
+#include <memory>
+#include <mutex>
 #include <optional>
 #include <string>
 #include <tuple>
@@ -28,9 +33,9 @@
 namespace {
 
 using at::Tensor;
-using torch::autograd::AutogradContext;
+using torch::autograd::Node;
+using torch::autograd::SavedVariable;
 using torch::autograd::variable_list;
-using Maybe = std::optional<Tensor>;
 
 struct Abi {
   decltype(&ntlb_last_error) last_error;
@@ -66,9 +71,12 @@ void* stream_of(const Tensor& t) {
 }
 
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
-void* ptr(const Maybe& t) { return t ? t->data_ptr() : nullptr; }
 
-Tensor scratch(int64_t bytes, const Tensor& like) { return at::empty({bytes}, like.options().dtype(at::kByte)); }
+// memory of like's device, past the dispatcher
+Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const Tensor& like) {
+  return Tensor(at::detail::empty_cuda(sizes, type, like.device(), std::nullopt));
+}
+Tensor scratch(int64_t bytes, const Tensor& like) { return fresh({bytes}, at::kByte, like); }
 
 // t as [rows, columns] with unit stride along the columns and rows one behind the
 // other (or one row repeated): a copy only where no view gives that
@@ -80,7 +88,6 @@ Tensor rows_of(const Tensor& t) {
 Tensor shaped(const Tensor& t, at::IntArrayRef sizes) { return t.sizes() == sizes ? t : t.reshape(sizes); }
 
 bool wanted(const Tensor& t) { return t.defined() && t.requires_grad(); }
-bool wanted(const Maybe& t) { return t && t->requires_grad(); }
 
 // The gradients are no functions of the graph: where one is being recorded, they
 // carry an error for whoever differentiates them
@@ -94,14 +101,29 @@ variable_list once(variable_list grads) {
   return grads;
 }
 
+// What the backward is to read of t: t itself, whose changes in place are then
+// noticed, where `used` (its rows) is a view of it, else the copy
+SavedVariable kept(const Tensor& t, const Tensor& used) { return SavedVariable(used.is_alias_of(t) ? t : used, false); }
+
+// The nodes are torch's own kind, not its custom functions, whose context of named
+// values and wrapping of results take 8 us a step
+template <typename N>
+std::shared_ptr<N> make_node(torch::autograd::edge_list edges) {
+  std::shared_ptr<N> node(new N(), torch::autograd::deleteNode);
+  node->set_next_edges(std::move(edges));
+  return node;
+}
+
 // ---------------------------------------------------------------------------
-struct LayerNorm : torch::autograd::Function<LayerNorm> {
-  static int weight_dtype(const Tensor& x, const Maybe& w, const Maybe& b) { return dtype_of(w ? *w : b ? *b : x); }
+struct LayerNorm {
+  static int weight_dtype(const Tensor& x, const Tensor& w, const Tensor& b) {
+    return dtype_of(w.defined() ? w : b.defined() ? b : x);
+  }
 
   // mr: the rows' means, then 1 / their deviations (undefined: not kept)
-  static Tensor run(const Tensor& x2, const Maybe& w, const Maybe& b, double eps, const Tensor& mr) {
+  static Tensor run(const Tensor& x2, const Tensor& w, const Tensor& b, double eps, const Tensor& mr) {
     const int64_t T = x2.size(0), H = x2.size(1);
-    Tensor y = at::empty({T, H}, x2.options());
+    Tensor y = fresh({T, H}, x2.scalar_type(), x2);
     float* m = mr.defined() ? mr.data_ptr<float>() : nullptr;
     check("ntlb_layer_norm_forward",
           abi.norm_forward(x2.data_ptr(), dtype_of(x2), T, H, x2.stride(0), ptr(w), ptr(b), weight_dtype(x2, w, b),
@@ -109,42 +131,61 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
     return y;
   }
 
-  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Maybe& w, const Maybe& b, double eps) {
-    ctx->set_materialize_grads(false);
-    const c10::DeviceGuard guard(x.device());
-    const Tensor x2 = rows_of(x);
-    const Tensor mr = at::empty({std::max<int64_t>(1, 2 * x2.size(0))}, x2.options().dtype(at::kFloat));
-    Tensor y = run(x2, w, b, eps, mr);
-    ctx->save_for_backward({x2, w ? *w : Tensor(), b ? *b : Tensor(), mr});
-    ctx->saved_data["sizes"] = x.sizes();
-    return shaped(y, x.sizes());
-  }
+  struct Backward : Node {
+    SavedVariable x, w, b;
+    Tensor mr;
 
-  static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    if (!grads[0].defined()) return variable_list(4);
-    const variable_list s = ctx->get_saved_variables();
-    const Tensor &x2 = s[0], &w = s[1], &b = s[2], &mr = s[3];
-    const c10::DeviceGuard guard(x2.device());
-    const int64_t T = x2.size(0), H = x2.size(1);
-    const at::AutoDispatchBelowADInplaceOrView below;
-    const Tensor d2 = rows_of(grads[0]);
-    Tensor dx, dw, db, ws;
-    // (inputs are counted without those that are None)
-    if (ctx->needs_input_grad(0)) dx = at::empty({T, H}, x2.options());
-    if (w.defined() && ctx->needs_input_grad(1)) dw = at::empty_like(w);
-    if (b.defined() && ctx->needs_input_grad(w.defined() ? 2 : 1)) db = at::empty_like(b);
-    int64_t need = 0;
-    if (dw.defined() || db.defined()) {
-      need = abi.norm_workspace(dtype_of(x2), T, H);
-      ws = scratch(need, x2);
+    variable_list apply(variable_list&& grads) override {
+      const std::lock_guard<std::mutex> lock(mutex_);
+      if (!grads[0].defined()) return variable_list(3);
+      const Tensor xt = x.unpack(), wt = w.unpack(), bt = b.unpack();
+      const c10::DeviceGuard guard(xt.device());
+      const at::AutoDispatchBelowADInplaceOrView below;
+      const Tensor x2 = rows_of(xt), d2 = rows_of(grads[0]);
+      const int64_t T = x2.size(0), H = x2.size(1);
+      Tensor dx, dw, db, ws;
+      if (task_should_compute_output(0)) dx = fresh({T, H}, x2.scalar_type(), x2);
+      if (wt.defined() && task_should_compute_output(1)) dw = fresh({H}, wt.scalar_type(), x2);
+      if (bt.defined() && task_should_compute_output(2)) db = fresh({H}, bt.scalar_type(), x2);
+      int64_t need = 0;
+      if (dw.defined() || db.defined()) {
+        need = abi.norm_workspace(dtype_of(x2), T, H);
+        ws = scratch(need, x2);
+      }
+      const float* m = mr.data_ptr<float>();
+      check("ntlb_layer_norm_backward",
+            abi.norm_backward(x2.data_ptr(), dtype_of(x2), T, H, x2.stride(0), d2.data_ptr(), d2.stride(0), m, m + T,
+                              ptr(wt), weight_dtype(x2, wt, bt), ptr(dx), H, ptr(dw), ptr(db), ptr(ws), need,
+                              stream_of(x2)));
+      if (dx.defined()) dx = shaped(dx, xt.sizes());
+      return once({dx, dw, db});
     }
-    const float* m = mr.data_ptr<float>();
-    check("ntlb_layer_norm_backward",
-          abi.norm_backward(x2.data_ptr(), dtype_of(x2), T, H, x2.stride(0), d2.data_ptr(), d2.stride(0), m, m + T,
-                            ptr(w), dtype_of(w.defined() ? w : b.defined() ? b : x2), ptr(dx), H, ptr(dw), ptr(db),
-                            ptr(ws), need, stream_of(x2)));
-    if (dx.defined()) dx = shaped(dx, ctx->saved_data["sizes"].toIntVector());
-    return once({dx, dw, db, Tensor()});
+    void release_variables() override {
+      const std::lock_guard<std::mutex> lock(mutex_);
+      x.reset_data();
+      w.reset_data();
+      b.reset_data();
+      mr.reset();
+    }
+    std::string name() const override { return "LayerNormBackward"; }
+  };
+
+  static Tensor forward(const Tensor& x, const Tensor& w, const Tensor& b, double eps) {
+    const c10::DeviceGuard guard(x.device());
+    Tensor y, x2, mr;
+    {
+      const at::AutoDispatchBelowADInplaceOrView below;
+      x2 = rows_of(x);
+      mr = fresh({std::max<int64_t>(1, 2 * x2.size(0))}, at::kFloat, x2);
+      y = shaped(run(x2, w, b, eps, mr), x.sizes());
+    }
+    auto node = make_node<Backward>(torch::autograd::collect_next_edges(x, w, b));
+    node->x = kept(x, x2);
+    node->w = SavedVariable(w, false);
+    node->b = SavedVariable(b, false);
+    node->mr = mr;
+    torch::autograd::set_history(y, node);
+    return y;
   }
 };
 
@@ -154,60 +195,71 @@ struct RouteConfig {
   double scale;
 };
 
-struct Route : torch::autograd::Function<Route> {
-  static std::tuple<Tensor, Tensor> run(const Tensor& z, const Maybe& bias, const RouteConfig& c) {
+struct Route {
+  static std::tuple<Tensor, Tensor> run(const Tensor& z, const Tensor& bias, const RouteConfig& c) {
     const int64_t T = z.size(0);
-    Tensor ids = at::empty({T, c.k}, z.options().dtype(at::kInt));
-    Tensor w = at::empty({T, c.k}, z.options().dtype(at::kFloat));
+    Tensor ids = fresh({T, c.k}, at::kInt, z);
+    Tensor w = fresh({T, c.k}, at::kFloat, z);
     check("ntlb_route_topk",
           abi.route(z.data_ptr(), dtype_of(z), T, z.size(1), z.stride(0), c.k, (int)c.sigmoid, (const float*)ptr(bias),
                     c.groups, c.kept, (int)c.renorm, (float)c.scale, ids.data_ptr<int32_t>(), w.data_ptr<float>(),
                     stream_of(z)));
     return {ids, w};
   }
-  static variable_list lead(const Tensor& logits, const std::tuple<Tensor, Tensor>& r, int64_t k) {
+  // the results in the logits' leading shape
+  static std::tuple<Tensor, Tensor> lead(const Tensor& logits, const std::tuple<Tensor, Tensor>& r, int64_t k) {
+    if (logits.dim() == 2) return r;
     std::vector<int64_t> sizes = logits.sizes().vec();
     sizes.back() = k;
     return {shaped(std::get<0>(r), sizes), shaped(std::get<1>(r), sizes)};
   }
 
-  static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Maybe& bias, int64_t k,
-                               int64_t sigmoid, int64_t groups, int64_t kept, int64_t renorm, double scale) {
-    ctx->set_materialize_grads(false);
-    const c10::DeviceGuard guard(logits.device());
-    const Tensor z = rows_of(logits);
-    const auto r = run(z, bias, {k, sigmoid, groups, kept, renorm, scale});
-    ctx->save_for_backward({z, std::get<0>(r)});
-    ctx->saved_data["sizes"] = logits.sizes();
-    ctx->saved_data["sigmoid"] = sigmoid;
-    ctx->saved_data["renorm"] = renorm;
-    ctx->saved_data["scale"] = scale;
-    const variable_list out = lead(logits, r, k);
-    ctx->mark_non_differentiable({out[0]});
-    return out;
-  }
+  struct Backward : Node {
+    SavedVariable z, ids;
+    RouteConfig c;
 
-  static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    if (!grads[1].defined()) return variable_list(8);
-    const variable_list s = ctx->get_saved_variables();
-    const Tensor &z = s[0], &ids = s[1];
-    const c10::DeviceGuard guard(z.device());
-    const at::AutoDispatchBelowADInplaceOrView below;
-    const int64_t T = z.size(0), E = z.size(1);
-    const Tensor dw = grads[1].contiguous();
-    Tensor dz = at::empty({T, E}, z.options());
-    check("ntlb_route_topk_backward",
-          abi.route_backward(z.data_ptr(), dtype_of(z), T, E, z.stride(0), ids.size(1),
-                             (int)ctx->saved_data["sigmoid"].toInt(), (int)ctx->saved_data["renorm"].toInt(),
-                             (float)ctx->saved_data["scale"].toDouble(), ids.data_ptr<int32_t>(), dw.data_ptr<float>(),
-                             dz.data_ptr(), E, stream_of(z)));
-    dz = shaped(dz, ctx->saved_data["sizes"].toIntVector());
-    return once({dz, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()});
+    variable_list apply(variable_list&& grads) override {
+      const std::lock_guard<std::mutex> lock(mutex_);
+      if (!grads[0].defined()) return variable_list(1);
+      const Tensor zt = z.unpack(), it = ids.unpack();
+      const c10::DeviceGuard guard(zt.device());
+      const at::AutoDispatchBelowADInplaceOrView below;
+      const Tensor z2 = rows_of(zt), dw = grads[0].contiguous();
+      const int64_t T = z2.size(0), E = z2.size(1);
+      Tensor dz = fresh({T, E}, z2.scalar_type(), z2);
+      check("ntlb_route_topk_backward",
+            abi.route_backward(z2.data_ptr(), dtype_of(z2), T, E, z2.stride(0), c.k, (int)c.sigmoid, (int)c.renorm,
+                               (float)c.scale, it.data_ptr<int32_t>(), dw.data_ptr<float>(), dz.data_ptr(), E,
+                               stream_of(z2)));
+      return once({shaped(dz, zt.sizes())});
+    }
+    void release_variables() override {
+      const std::lock_guard<std::mutex> lock(mutex_);
+      z.reset_data();
+      ids.reset_data();
+    }
+    std::string name() const override { return "RouteBackward"; }
+  };
+
+  static std::tuple<Tensor, Tensor> forward(const Tensor& logits, const Tensor& bias, const RouteConfig& c) {
+    const c10::DeviceGuard guard(logits.device());
+    Tensor z, ids, w;
+    {
+      const at::AutoDispatchBelowADInplaceOrView below;
+      z = rows_of(logits);
+      std::tie(ids, w) = lead(logits, run(z, bias, c), c.k);
+    }
+    auto node = make_node<Backward>(torch::autograd::collect_next_edges(logits));
+    node->z = kept(logits, z);
+    node->ids = SavedVariable(ids, false);
+    node->c = c;
+    torch::autograd::set_history(w, node);
+    return {ids, w};
   }
 };
 
 // ---------------------------------------------------------------------------
-struct LinearXent : torch::autograd::Function<LinearXent> {
+struct LinearXent {
   // w: weight in 16-byte rows; reduction 0 none, 1 sum, 2 mean
   static std::tuple<Tensor, Tensor> run(const Tensor& x2, const Tensor& w, const Tensor& targets, int64_t ignore,
                                         int64_t reduction) {
@@ -216,7 +268,7 @@ struct LinearXent : torch::autograd::Function<LinearXent> {
     const Tensor state = scratch(abi.xent_state(T, H), x2);
     const int64_t need = abi.xent_workspace(T, H, V, 0);
     const Tensor ws = scratch(std::max<int64_t>(need, 16), x2);
-    Tensor loss = at::empty({reduction ? 1 : std::max<int64_t>(T, 1)}, x2.options().dtype(at::kFloat));
+    Tensor loss = fresh({reduction ? 1 : std::max<int64_t>(T, 1)}, at::kFloat, x2);
     check("ntlb_linear_xent_forward",
           abi.xent_forward((const uint16_t*)x2.data_ptr(), x2.stride(0), (const uint16_t*)w.data_ptr(), w.stride(0),
                            y.data_ptr(), y.scalar_type() == at::kLong, T, H, V, ignore, (int)reduction,
@@ -224,47 +276,63 @@ struct LinearXent : torch::autograd::Function<LinearXent> {
     return {reduction ? loss.reshape({}) : shaped(T ? loss : loss.slice(0, 0, 0), targets.sizes()), state};
   }
 
-  static Tensor forward(AutogradContext* ctx, const Tensor& hidden, const Tensor& weight, const Tensor& w,
-                        const Tensor& targets, int64_t ignore, int64_t reduction) {
-    ctx->set_materialize_grads(false);
-    const c10::DeviceGuard guard(hidden.device());
-    const Tensor x2 = rows_of(hidden);
-    const auto [loss, state] = run(x2, w, targets, ignore, reduction);
-    ctx->save_for_backward({w, state});
-    ctx->saved_data["sizes"] = hidden.sizes();
-    ctx->saved_data["T"] = x2.size(0);
-    ctx->saved_data["H"] = x2.size(1);
-    ctx->saved_data["reduction"] = reduction;
-    return loss;
-  }
+  struct Backward : Node {
+    SavedVariable w;
+    Tensor state;
+    std::vector<int64_t> sizes;  // of hidden
+    int64_t T, reduction;
 
-  static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    if (!grads[0].defined()) return variable_list(6);
-    const variable_list s = ctx->get_saved_variables();
-    const Tensor &w = s[0], &state = s[1];
-    const c10::DeviceGuard guard(w.device());
-    const at::AutoDispatchBelowADInplaceOrView below;
-    const int64_t T = ctx->saved_data["T"].toInt(), H = ctx->saved_data["H"].toInt(), V = w.size(0);
-    const int64_t reduction = ctx->saved_data["reduction"].toInt();
-    const Tensor dl = grads[0].reshape({-1}).contiguous();
-    Tensor dx, dw;
-    if (ctx->needs_input_grad(0)) dx = at::empty({T, H}, w.options());
-    if (ctx->needs_input_grad(1)) dw = at::empty({V, H}, w.options());
-    const int64_t need = abi.xent_workspace(std::max<int64_t>(T, 1), H, V, 1);
-    const Tensor ws = scratch(need, w);
-    check("ntlb_linear_xent_backward",
-          abi.xent_backward(state.data_ptr(), (const uint16_t*)w.data_ptr(), w.stride(0), T, H, V, (int)reduction,
-                            dl.data_ptr<float>(), (uint16_t*)ptr(dx), H, (uint16_t*)ptr(dw), H, ws.data_ptr(), need,
-                            stream_of(w)));
-    if (dx.defined()) dx = shaped(dx, ctx->saved_data["sizes"].toIntVector());
-    return once({dx, dw, Tensor(), Tensor(), Tensor(), Tensor()});
+    variable_list apply(variable_list&& grads) override {
+      const std::lock_guard<std::mutex> lock(mutex_);
+      if (!grads[0].defined()) return variable_list(2);
+      const Tensor wt = w.unpack();
+      const c10::DeviceGuard guard(wt.device());
+      const at::AutoDispatchBelowADInplaceOrView below;
+      const int64_t H = sizes.back(), V = wt.size(0);
+      const Tensor dl = grads[0].reshape({-1}).contiguous();
+      Tensor dx, dw;
+      if (task_should_compute_output(0)) dx = fresh({T, H}, wt.scalar_type(), wt);
+      if (task_should_compute_output(1)) dw = fresh({V, H}, wt.scalar_type(), wt);
+      const int64_t need = abi.xent_workspace(std::max<int64_t>(T, 1), H, V, 1);
+      const Tensor ws = scratch(need, wt);
+      check("ntlb_linear_xent_backward",
+            abi.xent_backward(state.data_ptr(), (const uint16_t*)wt.data_ptr(), wt.stride(0), T, H, V, (int)reduction,
+                              dl.data_ptr<float>(), (uint16_t*)ptr(dx), H, (uint16_t*)ptr(dw), H, ws.data_ptr(), need,
+                              stream_of(wt)));
+      if (dx.defined()) dx = shaped(dx, sizes);
+      return once({dx, dw});
+    }
+    void release_variables() override {
+      const std::lock_guard<std::mutex> lock(mutex_);
+      w.reset_data();
+      state.reset();
+    }
+    std::string name() const override { return "LinearXentBackward"; }
+  };
+
+  static Tensor forward(const Tensor& hidden, const Tensor& weight, const Tensor& w, const Tensor& targets,
+                        int64_t ignore, int64_t reduction) {
+    const c10::DeviceGuard guard(hidden.device());
+    Tensor loss, state;
+    {
+      const at::AutoDispatchBelowADInplaceOrView below;
+      std::tie(loss, state) = run(rows_of(hidden), w, targets, ignore, reduction);
+    }
+    auto node = make_node<Backward>(torch::autograd::collect_next_edges(hidden, weight));
+    node->w = SavedVariable(w, false);
+    node->state = state;
+    node->sizes = hidden.sizes().vec();
+    node->T = hidden.numel() / hidden.size(-1);
+    node->reduction = reduction;
+    torch::autograd::set_history(loss, node);
+    return loss;
   }
 };
 
 // ---------------------------------------------------------------------------
 // Python
 // ---------------------------------------------------------------------------
-Maybe maybe(PyObject* o) { return o == Py_None ? Maybe() : Maybe(THPVariable_Unpack(o)); }
+Tensor maybe(PyObject* o) { return o == Py_None ? Tensor() : THPVariable_Unpack(o); }
 
 void count(Py_ssize_t n, Py_ssize_t want) {
   if (n != want) C10_THROW_ERROR(TypeError, "wrong number of arguments");
@@ -289,13 +357,13 @@ PyObject* py_layer_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   count(n, 4);
   const Tensor& x = THPVariable_Unpack(a[0]);
-  const Maybe w = maybe(a[1]), b = maybe(a[2]);
+  const Tensor w = maybe(a[1]), b = maybe(a[2]);
   const double eps = real(a[3]);
   Tensor y;
   {
     const NoGil nogil;
     if (at::GradMode::is_enabled() && (wanted(x) || wanted(w) || wanted(b))) {
-      y = LayerNorm::apply(x, w, b, eps);
+      y = LayerNorm::forward(x, w, b, eps);
     } else {
       const at::AutoDispatchBelowADInplaceOrView below;
       const c10::DeviceGuard guard(x.device());
@@ -311,20 +379,20 @@ PyObject* py_route(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   count(n, 8);
   const Tensor& z = THPVariable_Unpack(a[0]);
-  const Maybe bias = maybe(a[1]);
+  const Tensor bias = maybe(a[1]);
   const RouteConfig c{integer(a[2]), integer(a[3]), integer(a[4]), integer(a[5]), integer(a[6]), real(a[7])};
-  variable_list r;
+  std::tuple<Tensor, Tensor> r;
   {
     const NoGil nogil;
     if (at::GradMode::is_enabled() && wanted(z)) {
-      r = Route::apply(z, bias, c.k, c.sigmoid, c.groups, c.kept, c.renorm, c.scale);
+      r = Route::forward(z, bias, c);
     } else {
       const at::AutoDispatchBelowADInplaceOrView below;
       const c10::DeviceGuard guard(z.device());
       r = Route::lead(z, Route::run(rows_of(z), bias, c), c.k);
     }
   }
-  THPObjectPtr ids(THPVariable_Wrap(r[0])), w(THPVariable_Wrap(r[1]));
+  THPObjectPtr ids(THPVariable_Wrap(std::get<0>(r))), w(THPVariable_Wrap(std::get<1>(r)));
   if (!ids || !w) throw python_error();
   return PyTuple_Pack(2, ids.get(), w.get());
   END_HANDLE_TH_ERRORS
@@ -341,7 +409,7 @@ PyObject* py_linear_xent(PyObject*, PyObject* const* a, Py_ssize_t n) {
   {
     const NoGil nogil;
     if (at::GradMode::is_enabled() && (wanted(x) || wanted(weight))) {
-      loss = LinearXent::apply(x, weight, w.detach(), y, ignore, reduction);
+      loss = LinearXent::forward(x, weight, w, y, ignore, reduction);
     } else {
       const at::AutoDispatchBelowADInplaceOrView below;
       const c10::DeviceGuard guard(x.device());

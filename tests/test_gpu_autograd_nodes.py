@@ -1,0 +1,109 @@
+"""The C++ autograd nodes of norm, router and head loss as autograd's own rules
+see them: changes in place are noticed, a freed graph is refused, a retained one
+runs again, and only the gradients asked for are formed."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+def _norm(dev, lead=(6,)):
+    from lowbit.norm import layer_norm
+
+    ins = [torch.randn(*lead, 40, device=dev).requires_grad_(True), torch.randn(40, device=dev).requires_grad_(True),
+           torch.randn(40, device=dev).requires_grad_(True)]
+    return ins, lambda x, w, b: layer_norm(x, w, b)
+
+
+def _route(dev, lead=(6,)):
+    from lowbit.router import route_tokens
+
+    return [torch.randn(*lead, 20, device=dev).requires_grad_(True)], lambda z: route_tokens(z, 4)[1]
+
+
+def _xent(dev, lead=(6,)):
+    from lowbit.loss import linear_cross_entropy
+
+    y = torch.randint(0, 90, lead, device=dev)
+    ins = [torch.randn(*lead, 40, device=dev).bfloat16().requires_grad_(True),
+           torch.randn(90, 40, device=dev).bfloat16().requires_grad_(True)]
+    return ins, lambda x, w: linear_cross_entropy(x, w, y, reduction="none")
+
+
+ALL = pytest.mark.parametrize("make", [_norm, _route, _xent])
+
+
+@ALL
+@pytest.mark.parametrize("lead", [(6,), (2, 3)])
+def test_a_change_in_place_is_noticed(gpu_device, make, lead):
+    ins, f = make(gpu_device, lead)
+    # the head's hidden rows are copied in the forward: they may change
+    for i in range(1 if make is _xent else 0, 1 if make is _route else 2):
+        leaves = [t.detach().clone().requires_grad_(True) for t in ins]
+        moved = [t * 1 for t in leaves]
+        out = f(*moved)
+        with torch.no_grad():
+            moved[i].mul_(2)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            torch.autograd.grad(out.sum(), leaves)
+
+
+@ALL
+def test_a_graph_is_used_once_unless_kept(gpu_device, make):
+    ins, f = make(gpu_device)
+    up = torch.randn_like(f(*ins))
+    out = f(*ins)
+    first = torch.autograd.grad(out, ins, up, retain_graph=True)
+    again = torch.autograd.grad(out, ins, up)
+    for a, b, t in zip(first, again, ins):
+        assert a.shape == t.shape and a.dtype == t.dtype and torch.equal(a, b)
+    with pytest.raises(RuntimeError, match="second time"):
+        torch.autograd.grad(out, ins, up)
+
+
+@ALL
+def test_gradients_asked_for_alone(gpu_device, make):
+    ins, f = make(gpu_device)
+    up = torch.randn_like(f(*ins))
+    every = torch.autograd.grad(f(*ins), ins, up)
+    for i, t in enumerate(ins):
+        (one,) = torch.autograd.grad(f(*ins), t, up)
+        assert torch.equal(one, every[i])
+        alone = [u if j == i else u.detach() for j, u in enumerate(ins)]
+        f(*alone).backward(up)
+        assert torch.equal(t.grad, every[i]) and all(u.grad is None for j, u in enumerate(ins) if j != i)
+        t.grad = None
+
+
+@ALL
+def test_outputs_may_change_in_place_and_graphs_join(gpu_device, make):
+    """the result is an ordinary part of a graph: it may be scaled in place, hooked, and used twice"""
+    ins, f = make(gpu_device)
+    up = torch.randn_like(f(*ins))
+    every = torch.autograd.grad(f(*ins), ins, up)
+    out = f(*ins)
+    assert out.requires_grad and not out.is_leaf and "Backward" in out.grad_fn.name()
+    seen = []
+    out.register_hook(lambda g: seen.append(g.clone()))
+    got = torch.autograd.grad((out * 0.5 + out * 0.5), ins, up)
+    assert len(seen) == 1 and torch.allclose(seen[0], up)
+    for a, b in zip(got, every):
+        assert torch.allclose(a.float(), b.float(), rtol=2.0 ** -7, atol=1e-6)
+    scaled = f(*ins).mul_(2.0)  # 2 is exact in every type
+    for a, b in zip(torch.autograd.grad(scaled, ins, up / 2), every):
+        assert torch.equal(a, b)
+    with torch.no_grad():
+        assert not f(*ins).requires_grad
+    with torch.inference_mode():
+        assert f(*ins).is_inference()
+    assert not f(*[t.detach() for t in ins]).requires_grad
+
+
+def test_ids_are_not_differentiable(gpu_device):
+    from lowbit.router import route_tokens
+
+    ids, w = route_tokens(torch.randn(5, 12, device=gpu_device, requires_grad=True), 3)
+    assert not ids.requires_grad and w.requires_grad
