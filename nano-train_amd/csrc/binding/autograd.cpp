@@ -106,7 +106,7 @@ variable_list once(variable_list grads) {
 SavedVariable kept(const Tensor& t, const Tensor& used) { return SavedVariable(used.is_alias_of(t) ? t : used, false); }
 
 // The nodes are torch's own kind, not its custom functions, whose context of named
-// values and wrapping of results take 8 us a step
+// values and wrapping of results take 3 us more of a router step's 51
 template <typename N>
 std::shared_ptr<N> make_node(torch::autograd::edge_list edges) {
   std::shared_ptr<N> node(new N(), torch::autograd::deleteNode);
