@@ -40,6 +40,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "ntlb_device.h"
@@ -356,15 +357,12 @@ __device__ __forceinline__ float2 merge(float2 a, float2 b) {
   return make_float2(hi, a.y * __builtin_amdgcn_exp2f(a.x - ref) + b.y * __builtin_amdgcn_exp2f(b.x - ref));
 }
 
-// D x D output tiles: 256, eight waves of 128 x 64, one workgroup a compute unit;
-// 128, four waves of 64 x 64, two workgroups
+// One output tile of D x D, the pid-th of its product: 256, eight waves of 128 x
+// 64, one workgroup a compute unit; 128, four waves of 64 x 64, two workgroups.
+// la0 ... lb1: two stages of both operands, TILE bytes each.
 template <int D, bool TA, bool TB, int EPI>
-__global__ void __launch_bounds__(2 * D, D == 256 ? 1 : 2) head_kernel(Args g) {
+__device__ __forceinline__ void head_tile(Args g, int pid, uint8_t* la0, uint8_t* lb0, uint8_t* la1, uint8_t* lb1) {
   constexpr int TM = D, TN = D, TILE = D * ROWB, WAVES_N = D / 64, MT = D / 32;
-  __shared__ __attribute__((aligned(16))) uint8_t la0[TILE];
-  __shared__ __attribute__((aligned(16))) uint8_t lb0[TILE];
-  __shared__ __attribute__((aligned(16))) uint8_t la1[TILE];
-  __shared__ __attribute__((aligned(16))) uint8_t lb1[TILE];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / WAVES_N, wn = wave % WAVES_N;
   const int live = __builtin_amdgcn_readfirstlane(g.live[0]);
@@ -372,7 +370,6 @@ __global__ void __launch_bounds__(2 * D, D == 256 ? 1 : 2) head_kernel(Args g) {
   const int num_n = (int)((g.N + TN - 1) / TN);
   const int num_m_all = (int)((g.M + TM - 1) / TM);
   const int num_m = EPI == EPI_STORE ? num_m_all : (live + TM - 1) / TM;
-  int pid = (int)blockIdx.x;
   int sl = 0;
   if constexpr (EPI == EPI_ACC) {
     const int tiles = num_m * num_n;
@@ -604,6 +601,29 @@ __global__ void __launch_bounds__(2 * D, D == 256 ? 1 : 2) head_kernel(Args g) {
       for (int r = 0; r < 4; ++r) v[r] = acc[tm][tn][r] * c;
     });
   }
+}
+
+#define STAGES(D)                                            \
+  __shared__ __attribute__((aligned(16))) uint8_t la0[D * ROWB]; \
+  __shared__ __attribute__((aligned(16))) uint8_t lb0[D * ROWB]; \
+  __shared__ __attribute__((aligned(16))) uint8_t la1[D * ROWB]; \
+  __shared__ __attribute__((aligned(16))) uint8_t lb1[D * ROWB]
+
+template <int D, bool TA, bool TB, int EPI>
+__global__ void __launch_bounds__(2 * D, D == 256 ? 1 : 2) head_kernel(Args g) {
+  STAGES(D);
+  head_tile<D, TA, TB, EPI>(g, (int)blockIdx.x, la0, lb0, la1, lb1);
+}
+
+// dX's tiles (the first nx, a multiple of 8, workgroups) and dW's in one grid
+template <int D>
+__global__ void __launch_bounds__(2 * D, D == 256 ? 1 : 2) gradients_kernel(Args x, Args w, int nx) {
+  STAGES(D);
+  const int pid = (int)blockIdx.x;
+  if (pid < nx)
+    head_tile<D, false, true, EPI_ACC>(x, pid, la0, lb0, la1, lb1);
+  else
+    head_tile<D, true, true, EPI_STORE>(w, pid - nx, la0, lb0, la1, lb1);
 }
 
 // ---------------------------------------------------------------------------
@@ -866,6 +886,56 @@ static void launch_head(int D, const Args& g, hipStream_t st) {
     head_kernel<128, TA, TB, EPI><<<n, 256, 0, st>>>(g);
 }
 
+static void launch_pair(int D, const Args& x, const Args& w, hipStream_t st) {
+  const int64_t nx = cdiv(cdiv(x.M, D) * cdiv(x.N, D) * x.slices, 8) * 8, nw = cdiv(w.M, D) * cdiv(w.N, D);
+  if (D == 256)
+    gradients_kernel<256><<<(unsigned)(nx + nw), 512, 0, st>>>(x, w, (int)nx);
+  else
+    gradients_kernel<128><<<(unsigned)(nx + nw), 256, 0, st>>>(x, w, (int)nx);
+}
+
+// dX's and dW's products in one launch, where the tiles of one fill the rounds
+// that the other leaves open: the tile and dX's ranges of least time.  That of a
+// step, of an item's beginning and end in steps, of the memory's part and of
+// adding a range's values are fitted to 17 shapes by both tiles and 1 to 16 ranges
+// (off by 12%; the choice is within 13% of the best, 4% on average).  us of the
+// choice, and of two launches with tiles of their own: 1003 rows, 1000 wide,
+// 10007 words 52 and 65; 64, 1024, 32000 34 and 48; 600, 768, 50257 98 and 145;
+// 2048, 2048, 32768 430 and 466; 4096, 4096, 16384 819 and 870.
+struct Pair {
+  int tile, slices;
+};
+static Pair pair_of(int64_t T, int64_t H, int64_t cols) {
+  const int64_t cus = split_device_cus();
+  const double memory = 4.0 * (double)cols * (double)(H + T) / 5.14e6;  // W, dW; dz twice
+  Pair best{256, 1};
+  double t_best = 1e30;
+  for (int D = 256; D >= 128; D /= 2) {
+    const double step = D == 256 ? 1.33 : 0.83, over_x = D == 256 ? 10.6 : 5.1, over_w = D == 256 ? 3.9 : 5.1;
+    const int64_t steps = cdiv(cols, KSTEP), nw = cdiv(cols, D) * cdiv(H, D);
+    const double tw = step * ((double)cdiv(T, KSTEP) + over_w);
+    for (int n = 1; n <= 16 && (n == 1 || steps / n >= 8); ++n) {
+      const int64_t nx = cdiv(T, D) * cdiv(H, D) * n, room = cus * (D == 128 && nx + nw > cus ? 2 : 1), x = nx % room;
+      const double tx = step * ((double)steps / n + over_x);
+      // dX's whole rounds, then the rest of it beside dW
+      double t = (double)(nx / room) * tx - 8;
+      if (x == 0)
+        t += (double)cdiv(nw, room) * tw;
+      else if ((double)(room - x) * (int64_t)(tx / tw) >= (double)nw)
+        t += tx;
+      else
+        t += std::max(tx, ((double)x * tx + (double)nw * tw) / (double)room + 0.5 * tw);
+      const double a = t * t, b = memory * memory;
+      t = std::sqrt(std::sqrt(a * a + b * b)) + 1.45e-6 * (double)T * (double)(H * n);
+      if (t < t_best) {
+        t_best = t;
+        best = {D, n};
+      }
+    }
+  }
+  return best;
+}
+
 // forward workspace: the pairs, the label logits, the rows' losses
 static int64_t forward_parts(int64_t T, int64_t V) { return cdiv(V, tile_for(T, V)); }
 static int64_t forward_ws(int64_t T, int64_t V) { return forward_parts(T, V) * T * 8 + 2 * cdiv(T * 4, 256) * 256; }
@@ -874,6 +944,7 @@ static int64_t forward_ws(int64_t T, int64_t V) { return forward_parts(T, V) * T
 struct Plan {
   int64_t piece, block;  // words of a piece, elements of a block of dz
   int dz_tile, dx_tile, dw_tile, slices;
+  Pair pair;  // where both gradients are wanted
   int64_t dz, acc, most, bytes;
 };
 constexpr int64_t DZ_BYTES = (int64_t)512 << 20;
@@ -890,8 +961,9 @@ static Plan plan_of(int64_t T, int64_t H, int64_t V) {
   const int64_t steps = cdiv(cols, KSTEP);
   p.dx_tile = cdiv(T, 256) * cdiv(H, 256) * std::max<int64_t>(1, steps / 16) < split_device_cus() || T <= 128 ? 128 : 256;
   p.slices = ranges_for(p.dx_tile, T, H, steps);
+  p.pair = pair_of(T, H, cols);
   p.dz = cdiv(cols, 64) * p.block * 2;
-  p.acc = T * hk * 4 * p.slices;
+  p.acc = T * hk * 4 * std::max(p.slices, p.pair.slices);
   p.most = p.dz + p.acc;
   p.bytes = p.most + 256;
   return p;
@@ -975,7 +1047,7 @@ extern "C" int ntlb_linear_xent_backward(const void* state, const uint16_t* w, i
   if (reduction < 0 || reduction > 2) return fail(NTLB_EINVAL, "%s: bad reduction %d", fn, reduction);
   if (!state || !aligned(state, 256) || (T > 0 && !dloss)) return fail(NTLB_EINVAL, "%s: NULL pointer", fn);
   if ((dx && lddx < H) || (dw && lddw < H)) return fail(NTLB_EINVAL, "%s: a gradient's pitch is below H", fn);
-  if (T == 0 && !dw) return NTLB_OK;
+  if ((T == 0 || !dx) && !dw) return NTLB_OK;
   const int64_t Tn = std::max<int64_t>(T, 1);
   const xent::Plan p = xent::plan_of(Tn, H, V);
   if (ws_bytes < p.bytes || !workspace || !aligned(workspace, 16)) return fail(NTLB_EINVAL, "%s: workspace of %lld bytes, %lld needed", fn, (long long)ws_bytes, (long long)p.bytes);
@@ -987,6 +1059,8 @@ extern "C" int ntlb_linear_xent_backward(const void* state, const uint16_t* w, i
   float* acc = (float*)((uint8_t*)workspace + p.dz);
   float* most = reduction == 0 ? (float*)((uint8_t*)workspace + p.most) : nullptr;
   const xent::Up up{dloss, most, reduction == 2};
+  const bool both = dx && dw && T > 0;
+  const int slices = both ? p.pair.slices : p.slices;
   if (most) xent::most_kernel<<<1, 1024, 0, st>>>(dloss, (const int32_t*)(sp + s.rows), live, most);
   for (int64_t v0 = 0; v0 < V; v0 += p.piece) {
     const int64_t n = std::min(p.piece, V - v0), np = cdiv(n, 64) * 64;
@@ -999,27 +1073,26 @@ extern "C" int ntlb_linear_xent_backward(const void* state, const uint16_t* w, i
     g.rows = (const int32_t*)(sp + s.rows); g.up = up;
     g.out = dz; g.ldo = p.block; g.cols = np;
     if (T > 0) xent::launch_head<false, false, xent::EPI_DZ>(p.dz_tile, g, st);
-    if (dx && T > 0) {
-      xent::Args x{};
-      x.live = live; x.group_m = 8; x.slices = p.slices;
-      x.a = {(const uint8_t*)dz, p.block * 2, Tn, np};
-      x.b = {wp, ldw * 2, H, n};
-      x.M = T; x.N = H; x.out = acc; x.ldo = s.hk; x.slice = T * s.hk; x.add = v0 > 0;
-      xent::launch_head<false, true, xent::EPI_ACC>(p.dx_tile, x, st);
-    }
-    if (dw) {
-      xent::Args q{};
-      q.live = live; q.group_m = 8;
-      q.a = {(const uint8_t*)dz, p.block * 2, np, Tn};
-      q.b = {sp + s.xp, s.block * 2, s.hk, Tn};
-      q.M = n; q.N = H; q.out = dw + v0 * lddw; q.ldo = lddw;
-      q.up = up;
-      q.vec_out = aligned(dw, 16) && lddw % 8 == 0;
+    xent::Args x{}, q{};
+    x.live = live; x.group_m = 8; x.slices = slices;
+    x.a = {(const uint8_t*)dz, p.block * 2, Tn, np};
+    x.b = {wp, ldw * 2, H, n};
+    x.M = T; x.N = H; x.out = acc; x.ldo = s.hk; x.slice = T * s.hk; x.add = v0 > 0;
+    q.live = live; q.group_m = 8;
+    q.a = {(const uint8_t*)dz, p.block * 2, np, Tn};
+    q.b = {sp + s.xp, s.block * 2, s.hk, Tn};
+    q.M = n; q.N = H; q.out = dw + v0 * lddw; q.ldo = lddw;
+    q.up = up;
+    q.vec_out = aligned(dw, 16) && lddw % 8 == 0;
+    if (both)
+      xent::launch_pair(p.pair.tile, x, q, st);
+    else if (dw)
       xent::launch_head<true, true, xent::EPI_STORE>(p.dw_tile, q, st);
-    }
+    else if (dx)
+      xent::launch_head<false, true, xent::EPI_ACC>(p.dx_tile, x, st);
   }
   if (dx && T > 0)
-    xent::scatter_kernel<<<(unsigned)T, 256, 0, st>>>(acc, s.hk, T * s.hk, p.slices, up, live, (const int32_t*)(sp + s.pos),
+    xent::scatter_kernel<<<(unsigned)T, 256, 0, st>>>(acc, s.hk, T * s.hk, slices, up, live, (const int32_t*)(sp + s.pos),
                                                      H, dx, lddx);
   return check_launch(fn);
 }
