@@ -328,7 +328,9 @@ struct Args {
   Mat a, b;
   int64_t M, N;
   const int32_t* live;  // device: the number of live rows (rows of A for LSE / DZ / ACC, the contraction for STORE)
-  int slices;           // ACC: ranges of the contraction, one after another in the grid
+  int slices;           // ACC, and LSE and DZ by small tiles: ranges of the contraction
+  float4* part_z;       // LSE, DZ with ranges: their sums, [tile][range][16 v4f][thread]
+  uint32_t* count;      // ... of each tile, how many are there (0 before and after)
   int group_m;          // raster: row tiles side by side
   // LSE
   float2* part;         // [column tiles][ldp] (ref, sum)
@@ -357,12 +359,56 @@ __device__ __forceinline__ float2 merge(float2 a, float2 b) {
   return make_float2(hi, a.y * __builtin_amdgcn_exp2f(a.x - ref) + b.y * __builtin_amdgcn_exp2f(b.x - ref));
 }
 
+// Where the small tiles of z are too few for the chip, a tile's contraction is
+// divided among `slices` workgroups: each leaves its sums, and the last to arrive
+// adds all of them, in the ranges' order, and goes on.  Nobody waits.  Only groups
+// of 16 rows that hold live ones travel.
+template <int MT>
+__device__ __forceinline__ bool exchange(v4f (&acc)[MT][4], float4* part, uint32_t* count, int slices, int sl, int groups, int tid) {
+  constexpr int THREADS = 256, PER = MT * 4 * THREADS;
+  __shared__ int last;
+  part += tid;
+#pragma unroll
+  for (int tm = 0; tm < MT; ++tm)
+    if (tm < groups)
+#pragma unroll
+      for (int tn = 0; tn < 4; ++tn)
+        part[sl * PER + (tm * 4 + tn) * THREADS] = make_float4(acc[tm][tn][0], acc[tm][tn][1], acc[tm][tn][2], acc[tm][tn][3]);
+  __syncthreads();  // the stores of all waves are in this XCD's L2; the release writes them back
+  if (tid == 0) last = __hip_atomic_fetch_add(count, 1u, __ATOMIC_RELEASE, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)(slices - 1);
+  __syncthreads();
+  if (!last) return false;
+  if (tid == 0) __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+  __syncthreads();
+#pragma unroll
+  for (int tm = 0; tm < MT; ++tm)
+    if (tm < groups) {
+#pragma unroll
+      for (int tn = 0; tn < 4; ++tn) acc[tm][tn] = (v4f){0.f, 0.f, 0.f, 0.f};
+      for (int c0 = 0; c0 < slices; c0 += 4) {
+        float4 v[4][4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int tn = 0; tn < 4; ++tn) v[c][tn] = part[min(c0 + c, slices - 1) * PER + (tm * 4 + tn) * THREADS];
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          if (c0 + c < slices)
+#pragma unroll
+            for (int tn = 0; tn < 4; ++tn) acc[tm][tn] += (v4f){v[c][tn].x, v[c][tn].y, v[c][tn].z, v[c][tn].w};
+      }
+    }
+  if (tid == 0) atomicExch(count, 0u);  // ready for the next product
+  return true;
+}
+
 // One output tile of D x D, the pid-th of its product: 256, eight waves of 128 x
 // 64, one workgroup a compute unit; 128, four waves of 64 x 64, two workgroups.
 // la0 ... lb1: two stages of both operands, TILE bytes each.
 template <int D, bool TA, bool TB, int EPI>
 __device__ __forceinline__ void head_tile(Args g, int pid, uint8_t* la0, uint8_t* lb0, uint8_t* la1, uint8_t* lb1) {
   constexpr int TM = D, TN = D, TILE = D * ROWB, WAVES_N = D / 64, MT = D / 32;
+  constexpr bool SPLIT = D == 128 && (EPI == EPI_LSE || EPI == EPI_DZ), RANGES = SPLIT || EPI == EPI_ACC;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / WAVES_N, wn = wave % WAVES_N;
   const int live = __builtin_amdgcn_readfirstlane(g.live[0]);
@@ -380,10 +426,15 @@ __device__ __forceinline__ void head_tile(Args g, int pid, uint8_t* la0, uint8_t
     sl = q / tiles;
     pid = q - sl * tiles;
   } else {
-    const int nwg = num_m * num_n;
+    const int nwg = num_m * num_n * (SPLIT ? g.slices : 1);
     if (pid >= nwg) return;
     const int xcd = pid & 7, per = nwg >> 3, extra = nwg & 7;
     pid = xcd * per + min(xcd, extra) + (pid >> 3);
+    if constexpr (SPLIT) {
+      const int q = pid / g.slices;
+      sl = pid - q * g.slices;
+      pid = q;
+    }
   }
   const int group = pid / (g.group_m * num_n), first_m = group * g.group_m;
   const int gsize = min(num_m - first_m, g.group_m), in_group = pid - group * g.group_m * num_n;
@@ -396,8 +447,8 @@ __device__ __forceinline__ void head_tile(Args g, int pid, uint8_t* la0, uint8_t
     g.a.rows = live;
   }
   const int nk = max(1, (int)((g.a.k + KSTEP - 1) / KSTEP));
-  const int kb0 = EPI == EPI_ACC ? (int)((int64_t)sl * nk / g.slices) : 0;
-  const int kb1 = EPI == EPI_ACC ? (int)((int64_t)(sl + 1) * nk / g.slices) : nk;
+  const int kb0 = RANGES ? (int)((int64_t)sl * nk / g.slices) : 0;
+  const int kb1 = RANGES ? (int)((int64_t)(sl + 1) * nk / g.slices) : nk;
 
   // A is X' or dz, B the weight or (with A transposed) X'
   typename std::conditional<TA, BlockTrCopy<D>, BlockRowCopy<D>>::type ca;
@@ -484,6 +535,10 @@ __device__ __forceinline__ void head_tile(Args g, int pid, uint8_t* la0, uint8_t
     rows(MT - 2, b1, af[2]);
     rows(MT - 1, b1, af[3]);
     // no wave reads the stages any more, and none copies into them
+  }
+  if constexpr (SPLIT) {
+    const int groups = min((int)(g.M - m0 - wm * 16 * MT + 15) / 16, MT);
+    if (g.slices > 1 && !exchange<MT>(acc, g.part_z + (int64_t)pid * g.slices * (MT * 4 * 256), g.count + pid, g.slices, sl, groups, tid)) return;
   }
   // a wave's 16 KiB of the stages for its output rows
   constexpr int PER = TILE / 16384;
@@ -632,7 +687,7 @@ __global__ void __launch_bounds__(2 * D, D == 256 ? 1 : 2) gradients_kernel(Args
 // rows each of gather_kernel's counts for itself (16 rows: 5.0 us, with this
 // launch 4.7 + 4.9; 1003 rows 5.0 and 2.4 + 3.6).
 // ---------------------------------------------------------------------------
-constexpr int SCAN = 1024, HERE = 1024;
+constexpr int SCAN = 1024, HERE = 1024, COUNTERS = 1024;
 struct Targets {
   const void* p;
   int wide;
@@ -675,11 +730,15 @@ __global__ void __launch_bounds__(SCAN) scan_kernel(Targets tg, Live o) {
 // X': 16-byte pieces of the live rows of X into blocks of 64 columns, zero past
 // H and, by the last 63 workgroups, in the rows up to the next 64; a piece of an
 // unaligned or ragged row element by element.  Also what the other kernels expect
-// set: zl (NaN until a tile finds the label) and a zero loss for the ignored rows.
+// set: zl (NaN until a tile finds the label), a zero loss for the ignored rows and
+// the counters of the ranges.
 template <bool COUNT>
 __global__ void __launch_bounds__(256) gather_kernel(const uint16_t* x, int64_t ldx, int64_t H, int aligned16, Targets tg,
-                                                     Live o, uint16_t* xp, int64_t hk, int64_t block, float* zl, float* loss) {
+                                                     Live o, uint16_t* xp, int64_t hk, int64_t block, float* zl, float* loss,
+                                                     uint32_t* count) {
   const int64_t t = blockIdx.x;
+  if (t == 0 && count)
+    for (int i = threadIdx.x; i < COUNTERS; i += 256) count[i] = 0;
   const bool past = t >= tg.T;
   int at, n;
   if constexpr (COUNT) {
@@ -785,9 +844,13 @@ __global__ void __launch_bounds__(1024) total_kernel(const float* each, const in
   }
 }
 
-// the largest finite |du| of the live rows
-__global__ void __launch_bounds__(1024) most_kernel(const float* du, const int32_t* rows, const int32_t* live, float* most) {
+// the largest finite |du| of the live rows, if `most` is given, and the counters of
+// the ranges cleared, if there are any
+__global__ void __launch_bounds__(1024) most_kernel(const float* du, const int32_t* rows, const int32_t* live, float* most,
+                                                    uint32_t* count) {
   __shared__ uint32_t red[16];
+  if (count) count[threadIdx.x] = 0;
+  if (!most) return;
   uint32_t m = 0;
   for (int i = threadIdx.x; i < live[0]; i += 1024) {
     const uint32_t a = abs_bits(du[rows[i]]);
@@ -879,7 +942,7 @@ static int ranges_for(int D, int64_t M, int64_t N, int64_t steps) {
 // one product
 template <bool TA, bool TB, int EPI>
 static void launch_head(int D, const Args& g, hipStream_t st) {
-  const unsigned n = (unsigned)(cdiv(g.M, D) * cdiv(g.N, D) * (EPI == EPI_ACC ? g.slices : 1));
+  const unsigned n = (unsigned)(cdiv(g.M, D) * cdiv(g.N, D) * (EPI == EPI_STORE ? 1 : g.slices));
   if (D == 256)
     head_kernel<256, TA, TB, EPI><<<n, 512, 0, st>>>(g);
   else
@@ -936,16 +999,44 @@ static Pair pair_of(int64_t T, int64_t H, int64_t cols) {
   return best;
 }
 
-// forward workspace: the pairs, the label logits, the rows' losses
+// Ranges of the contraction for the logits of `cols` words by small tiles: of
+// least time, in us 0.5 a step, and for more than one 4, 1.2 a range of 128 rows
+// and 0.03 a workgroup, whose release and place in the count the others share.
+// Forward by one range and by the choice: 3 rows, 6413 wide, 265 words 71 us and
+// 17; 5, 4208, 2904 48 and 19; 1, 7168, 4096 75 and 25; 1000, 7168, 1000 81 and 45;
+// 16, 4096, 16384 46 and 34; 1000, 1024, 500, by one, 18 (by two 19).
+static int logit_slices(int64_t T, int64_t H, int64_t cols) {
+  if (tile_for(T, cols) != 128) return 1;
+  const int64_t tiles = cdiv(T, 128) * cdiv(cols, 128), steps = cdiv(H, KSTEP);
+  const double rows = (double)cdiv(std::min<int64_t>(T, 128), 16) / 8;
+  int best = 1;
+  double t_best = 0.5 * (double)steps;
+  for (int n = 2; n <= std::min<int64_t>(16, steps) && tiles * n <= 2 * split_device_cus() && tiles <= COUNTERS; ++n) {
+    const double t = 0.5 * (double)steps / n + 4 + 1.2 * n * rows + 0.03 * (double)(tiles * n);
+    if (t < t_best) {
+      t_best = t;
+      best = n;
+    }
+  }
+  return best;
+}
+// the bytes of their counters and sums
+static int64_t slices_bytes(int64_t T, int64_t cols, int slices) {
+  return slices < 2 ? 0 : COUNTERS * 4 + cdiv(T, 128) * cdiv(cols, 128) * slices * 65536;
+}
+
+// forward workspace: the pairs, the label logits, the rows' losses, the ranges' sums
 static int64_t forward_parts(int64_t T, int64_t V) { return cdiv(V, tile_for(T, V)); }
-static int64_t forward_ws(int64_t T, int64_t V) { return forward_parts(T, V) * T * 8 + 2 * cdiv(T * 4, 256) * 256; }
+static int64_t forward_sums(int64_t T, int64_t V) { return cdiv(forward_parts(T, V) * T * 8, 256) * 256 + 2 * cdiv(T * 4, 256) * 256; }
+static int64_t forward_ws(int64_t T, int64_t H, int64_t V) { return forward_sums(T, V) + slices_bytes(T, V, logit_slices(T, H, V)); }
 
 // backward: pieces of the vocabulary, tiles, ranges of the dX product, workspace
 struct Plan {
   int64_t piece, block;  // words of a piece, elements of a block of dz
   int dz_tile, dx_tile, dw_tile, slices;
   Pair pair;  // where both gradients are wanted
-  int64_t dz, acc, most, bytes;
+  int dz_slices;
+  int64_t dz, acc, most, sums, bytes;
 };
 constexpr int64_t DZ_BYTES = (int64_t)512 << 20;
 static Plan plan_of(int64_t T, int64_t H, int64_t V) {
@@ -965,7 +1056,9 @@ static Plan plan_of(int64_t T, int64_t H, int64_t V) {
   p.dz = cdiv(cols, 64) * p.block * 2;
   p.acc = T * hk * 4 * std::max(p.slices, p.pair.slices);
   p.most = p.dz + p.acc;
-  p.bytes = p.most + 256;
+  p.dz_slices = logit_slices(T, H, cols);
+  p.sums = p.most + 256;
+  p.bytes = p.sums + slices_bytes(T, cols, p.dz_slices);
   return p;
 }
 
@@ -985,7 +1078,7 @@ extern "C" int64_t ntlb_linear_xent_state_bytes(int64_t T, int64_t H) { return T
 
 extern "C" int64_t ntlb_linear_xent_workspace_bytes(int64_t T, int64_t H, int64_t V, int backward) {
   if (T < 1 || H < 1 || V < 1) return 0;
-  return backward ? xent::plan_of(T, H, V).bytes : xent::forward_ws(T, V);
+  return backward ? xent::plan_of(T, H, V).bytes : xent::forward_ws(T, H, V);
 }
 
 extern "C" int ntlb_linear_xent_forward(const uint16_t* x, int64_t ldx, const uint16_t* w, int64_t ldw,
@@ -998,7 +1091,7 @@ extern "C" int ntlb_linear_xent_forward(const uint16_t* x, int64_t ldx, const ui
   if (reduction < 0 || reduction > 2) return fail(NTLB_EINVAL, "%s: bad reduction %d", fn, reduction);
   if (!loss || !state || !aligned(state, 256)) return fail(NTLB_EINVAL, "%s: NULL pointer", fn);
   if (T > 0 && (!x || !targets || (ldx != 0 && ldx < H))) return fail(NTLB_EINVAL, "%s: bad hidden or targets", fn);
-  const int64_t need = T > 0 ? xent::forward_ws(T, V) : 0;
+  const int64_t need = T > 0 ? xent::forward_ws(T, H, V) : 0;
   if (ws_bytes < need || (need && (!workspace || !aligned(workspace, 16)))) return fail(NTLB_EINVAL, "%s: workspace of %lld bytes, %lld needed", fn, (long long)ws_bytes, (long long)need);
   hipStream_t st = as_stream(stream);
   const xent::State s = xent::state_of(std::max<int64_t>(T, 1), H);
@@ -1009,21 +1102,24 @@ extern "C" int ntlb_linear_xent_forward(const uint16_t* x, int64_t ldx, const ui
   uint16_t* xp = (uint16_t*)(sp + s.xp);
   const int64_t parts = T > 0 ? xent::forward_parts(T, V) : 0;
   float2* part = (float2*)workspace;
-  float* zl = T > 0 ? (float*)((uint8_t*)workspace + parts * T * 8) : nullptr;
+  float* zl = T > 0 ? (float*)((uint8_t*)workspace + cdiv(parts * T * 8, 256) * 256) : nullptr;
   float* each = T > 0 ? zl + cdiv(T * 4, 256) * 64 : nullptr;
+  const int slices = T > 0 ? xent::logit_slices(T, H, V) : 1;
+  uint32_t* count = slices > 1 ? (uint32_t*)((uint8_t*)workspace + xent::forward_sums(T, V)) : nullptr;
   float* rows_loss = reduction == 0 ? loss : nullptr;
   const int al = aligned(x, 16) && ldx % 8 == 0;
   if (T > xent::HERE) {
     xent::scan_kernel<<<1, xent::SCAN, 0, st>>>(tg, o);
-    xent::gather_kernel<false><<<(unsigned)T + 63, 256, 0, st>>>(x, ldx, H, al, tg, o, xp, s.hk, s.block, zl, rows_loss);
+    xent::gather_kernel<false><<<(unsigned)T + 63, 256, 0, st>>>(x, ldx, H, al, tg, o, xp, s.hk, s.block, zl, rows_loss, count);
   } else {
-    xent::gather_kernel<true><<<(unsigned)T + 63, 256, 0, st>>>(x, ldx, H, al, tg, o, xp, s.hk, s.block, zl, rows_loss);
+    xent::gather_kernel<true><<<(unsigned)T + 63, 256, 0, st>>>(x, ldx, H, al, tg, o, xp, s.hk, s.block, zl, rows_loss, count);
   }
   if (T > 0) {
     xent::Args g{};
     g.a = {(const uint8_t*)xp, s.block * 2, T, s.hk};
     g.b = {(const uint8_t*)w, ldw * 2, V, H};
     g.M = T; g.N = V; g.live = o.live; g.group_m = 8; g.part = part; g.ldp = T; g.zl = zl; g.y = o.y;
+    g.slices = slices; g.count = count; g.part_z = count ? (float4*)(count + xent::COUNTERS) : nullptr;
     xent::launch_head<false, false, xent::EPI_LSE>(xent::tile_for(T, V), g, st);
   }
   if (T > 0) {
@@ -1061,7 +1157,8 @@ extern "C" int ntlb_linear_xent_backward(const void* state, const uint16_t* w, i
   const xent::Up up{dloss, most, reduction == 2};
   const bool both = dx && dw && T > 0;
   const int slices = both ? p.pair.slices : p.slices;
-  if (most) xent::most_kernel<<<1, 1024, 0, st>>>(dloss, (const int32_t*)(sp + s.rows), live, most);
+  uint32_t* count = p.dz_slices > 1 ? (uint32_t*)((uint8_t*)workspace + p.sums) : nullptr;
+  if (most || count) xent::most_kernel<<<1, xent::COUNTERS, 0, st>>>(dloss, (const int32_t*)(sp + s.rows), live, most, count);
   for (int64_t v0 = 0; v0 < V; v0 += p.piece) {
     const int64_t n = std::min(p.piece, V - v0), np = cdiv(n, 64) * 64;
     const uint8_t* wp = (const uint8_t*)(w + v0 * ldw);
@@ -1072,6 +1169,7 @@ extern "C" int ntlb_linear_xent_backward(const void* state, const uint16_t* w, i
     g.M = T; g.N = n; g.y = (const int32_t*)(sp + s.y); g.v0 = v0; g.lse = (const float*)(sp + s.lse);
     g.rows = (const int32_t*)(sp + s.rows); g.up = up;
     g.out = dz; g.ldo = p.block; g.cols = np;
+    g.slices = p.dz_slices; g.count = count; g.part_z = count ? (float4*)(count + xent::COUNTERS) : nullptr;
     if (T > 0) xent::launch_head<false, false, xent::EPI_DZ>(p.dz_tile, g, st);
     xent::Args x{}, q{};
     x.live = live; x.group_m = 8; x.slices = slices;

@@ -392,3 +392,29 @@ def test_too_large_is_refused():
     for T, H, V, ldw in (((1 << 22) + 1, 64, 64, 64), (8, (1 << 20) + 8, 64, (1 << 20) + 8), (8, 64, (1 << 30) + 1, 64)):
         with pytest.raises(_lib.LowBitKernelError, match="too large"):
             _lib.call("ntlb_linear_xent_forward", p, H, p, ldw, p, 1, T, H, V, -100, 2, p, p, p, 1 << 60, 0)
+
+
+@pytest.mark.parametrize("T,H,V", [(1, 7168, 300), (3, 6413, 265), (16, 4096, 1000), (17, 2000, 129), (129, 2500, 700), (300, 5000, 257)])
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_a_divided_contraction(gpu_device, T, H, V, reduction):
+    """few tiles of long rows, whose contraction workgroups share: the sums come in a fixed order, call after call and
+    whatever the memory held, with ignored rows and none at all"""
+    from lowbit.loss import linear_cross_entropy
+
+    x, w, y, g = _inputs(T, H, V, T + H, gpu_device, 0.3)
+    dl = (torch.randn(T, generator=g) if reduction == "none" else torch.tensor(1.3)).to(gpu_device)
+    first = None
+    for k in range(4):
+        junk = torch.full((8 << 20,), float("nan"), device=gpu_device)
+        del junk
+        xl, wl = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+        loss = linear_cross_entropy(xl, wl, y, reduction=reduction)
+        got = (loss.detach(), *torch.autograd.grad(loss, (xl, wl), dl))
+        first = first or got
+        assert all(torch.equal(a, b) for a, b in zip(got, first))
+    _check(x, w, y, *first, reduction, dl)
+    none = torch.full_like(y, IGNORE)
+    xl, wl = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    loss = linear_cross_entropy(xl, wl, none, reduction=reduction)
+    assert (loss == 0).all()
+    assert all((t == 0).all() for t in torch.autograd.grad(loss, (xl, wl), dl))
