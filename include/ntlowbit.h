@@ -1043,6 +1043,13 @@ int ntlb_route_topk_backward(const void* logits, int dtype, int64_t T, int64_t E
                              void* dlogits, int64_t ldd, void* stream);
 
 /*
+ * out [R, ldo] = x [R, H] (16-bit values, pitch ldx in elements, any alignment),
+ * zero from column H on: rows as the head's product below takes them.  ldo % 8 ==
+ * 0, out 16-byte aligned.
+ */
+int ntlb_pad_rows(const uint16_t* x, int64_t ldx, int64_t R, int64_t H, uint16_t* out, int64_t ldo, void* stream);
+
+/*
  * Softmax cross entropy of a linear head without its logits: with z = X W^T
  * (x bf16 [T, H], pitch ldx, 0 for one row repeated; w bf16 [V, H], 16-byte
  * aligned with ldw % 8 == 0, its columns from H to the next multiple of 8

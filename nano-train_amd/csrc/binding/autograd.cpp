@@ -44,6 +44,7 @@ struct Abi {
   decltype(&ntlb_layer_norm_workspace_bytes) norm_workspace;
   decltype(&ntlb_route_topk) route;
   decltype(&ntlb_route_topk_backward) route_backward;
+  decltype(&ntlb_pad_rows) pad_rows;
   decltype(&ntlb_linear_xent_forward) xent_forward;
   decltype(&ntlb_linear_xent_backward) xent_backward;
   decltype(&ntlb_linear_xent_state_bytes) xent_state;
@@ -260,6 +261,17 @@ struct Route {
 
 // ---------------------------------------------------------------------------
 struct LinearXent {
+  // weight in rows of whole 16-byte pieces
+  static Tensor padded(const Tensor& weight) {
+    const c10::DeviceGuard guard(weight.device());
+    const at::AutoDispatchBelowADInplaceOrView below;
+    const Tensor w = rows_of(weight);
+    Tensor out = fresh({w.size(0), (w.size(1) + 7) / 8 * 8}, w.scalar_type(), w);
+    check("ntlb_pad_rows", abi.pad_rows((const uint16_t*)w.data_ptr(), w.stride(0), w.size(0), w.size(1),
+                                        (uint16_t*)out.data_ptr(), out.size(1), stream_of(w)));
+    return out;
+  }
+
   // w: weight in 16-byte rows; reduction 0 none, 1 sum, 2 mean
   static std::tuple<Tensor, Tensor> run(const Tensor& x2, const Tensor& w, const Tensor& targets, int64_t ignore,
                                         int64_t reduction) {
@@ -398,16 +410,17 @@ PyObject* py_route(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// linear_xent(hidden, weight, weight in 16-byte rows, targets, ignore_index, reduction)
+// linear_xent(hidden, weight, whether it is in 16-byte rows, targets, ignore_index, reduction)
 PyObject* py_linear_xent(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   count(n, 6);
-  const Tensor &x = THPVariable_Unpack(a[0]), &weight = THPVariable_Unpack(a[1]), &w = THPVariable_Unpack(a[2]),
-               &y = THPVariable_Unpack(a[3]);
+  const Tensor &x = THPVariable_Unpack(a[0]), &weight = THPVariable_Unpack(a[1]), &y = THPVariable_Unpack(a[3]);
+  const bool fits = a[2] == Py_True;
   const int64_t ignore = integer(a[4]), reduction = integer(a[5]);
   Tensor loss;
   {
     const NoGil nogil;
+    const Tensor w = fits ? weight : LinearXent::padded(weight);
     if (at::GradMode::is_enabled() && (wanted(x) || wanted(weight))) {
       loss = LinearXent::forward(x, weight, w, y, ignore, reduction);
     } else {
@@ -438,6 +451,7 @@ PyObject* py_bind(PyObject*, PyObject* table) {
   take(table, "ntlb_layer_norm_workspace_bytes", a.norm_workspace);
   take(table, "ntlb_route_topk", a.route);
   take(table, "ntlb_route_topk_backward", a.route_backward);
+  take(table, "ntlb_pad_rows", a.pad_rows);
   take(table, "ntlb_linear_xent_forward", a.xent_forward);
   take(table, "ntlb_linear_xent_backward", a.xent_backward);
   take(table, "ntlb_linear_xent_state_bytes", a.xent_state);

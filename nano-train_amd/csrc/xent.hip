@@ -60,6 +60,10 @@ typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) void* lds_ptr_t;
 typedef __attribute__((address_space(3))) v4s* lds_v4s_ptr;
 
+// the user's rows begin at any element
+typedef uint32_t u32x4_2 __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t u32x2_2 __attribute__((ext_vector_type(2), aligned(2)));
+
 constexpr int ROWB = 128, KSTEP = 64;  // bytes and values of a row's K step
 constexpr float LOG2E = 1.44269502e+00f, LN2 = 6.93147182e-01f;
 
@@ -273,7 +277,7 @@ struct BlockTrCopy {
 // stores of whole 128-byte lines.  value(tm, tn, v): the lane's four of a block.
 template <int MT, bool NTS, typename F>
 __device__ __forceinline__ void store_bf16(uint8_t* stage, int lane, int64_t m0, int64_t n0, int64_t M, int64_t N,
-                                           uint16_t* out, int64_t ldo, int vec, F value) {
+                                           uint16_t* out, int64_t ldo, F value) {
   constexpr int PITCH = 64 * 2 + 16;
 #pragma unroll
   for (int part = 0; part < MT / 2; ++part) {
@@ -295,11 +299,12 @@ __device__ __forceinline__ void store_bf16(uint8_t* stage, int lane, int64_t m0,
       const uint4 q = *reinterpret_cast<const uint4*>(stage + row * PITCH + c * 16);
       if (m >= M || n >= N) continue;
       uint16_t* o = out + m * ldo + n;
-      if (vec && n + 8 <= N) {
+      if (n + 8 <= N) {
+        const u32x4_2 v = {q.x, q.y, q.z, q.w};
         if constexpr (NTS)
-          store16_nt(o, &q);
+          __builtin_nontemporal_store(v, reinterpret_cast<u32x4_2*>(o));
         else
-          *reinterpret_cast<uint4*>(o) = q;
+          *reinterpret_cast<u32x4_2*>(o) = v;
       } else {
         const uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
@@ -348,7 +353,6 @@ struct Args {
   int64_t cols;         // DZ: columns to store, whole blocks
   int64_t slice;        // elements of a slice
   int add;              // ACC: add to what is there
-  int vec_out;
 };
 
 // A set of logits z: the largest z log2(e), ref, and the sum of 2^(z log2(e) - ref).
@@ -631,7 +635,7 @@ __device__ __forceinline__ void head_tile(Args g, int pid, uint8_t* la0, uint8_t
       }
     }
     const int64_t block = n0 / 64 + wn;
-    store_bf16<MT, false>(stage, lane, m0 + wm * 16 * MT, 0, (g.M + 63) / 64 * 64, g.cols - block * 64, (uint16_t*)g.out + block * g.ldo, 64, 1, [&](int tm, int tn, float (&v)[4]) {
+    store_bf16<MT, false>(stage, lane, m0 + wm * 16 * MT, 0, (g.M + 63) / 64 * 64, g.cols - block * 64, (uint16_t*)g.out + block * g.ldo, 64, [&](int tm, int tn, float (&v)[4]) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) v[r] = acc[tm][tn][r] * u[tm];
     });
@@ -651,7 +655,7 @@ __device__ __forceinline__ void head_tile(Args g, int pid, uint8_t* la0, uint8_t
     }
   } else {
     const float c = g.up.common(live);
-    store_bf16<MT, true>(stage, lane, m0 + wm * 16 * MT, n0 + wn * 64, g.M, g.N, (uint16_t*)g.out, g.ldo, g.vec_out, [&](int tm, int tn, float (&v)[4]) {
+    store_bf16<MT, true>(stage, lane, m0 + wm * 16 * MT, n0 + wn * 64, g.M, g.N, (uint16_t*)g.out, g.ldo, [&](int tm, int tn, float (&v)[4]) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) v[r] = acc[tm][tn][r] * c;
     });
@@ -727,13 +731,39 @@ __global__ void __launch_bounds__(SCAN) scan_kernel(Targets tg, Live o) {
   if (tid == 0) o.live[0] = base;
 }
 
+// eight values of a row of H from column c, zero past H; rows begin anywhere
+__device__ __forceinline__ uint4 piece_of(const uint16_t* row, int64_t c, int64_t H) {
+  if (c + 8 <= H) {
+    const u32x4_2 v = *reinterpret_cast<const u32x4_2*>(row + c);
+    return make_uint4(v[0], v[1], v[2], v[3]);
+  }
+  uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (c + i < H) w[i >> 1] |= (uint32_t)row[c + i] << (16 * (i & 1));
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// rows of any pitch into rows of whole 16-byte pieces, zero past H: HBM-bound
+// (42508 rows of 345: 14.3 us, 4.1 TB/s).  A workgroup takes `per` rows.
+__global__ void __launch_bounds__(256) pad_kernel(const uint16_t* x, int64_t ldx, int64_t R, int64_t H, uint16_t* out,
+                                                  int64_t ldo, int per) {
+  const int pieces = (int)(ldo / 8);
+  const int64_t r0 = (int64_t)blockIdx.x * per;
+  const int n = (int)min<int64_t>(per, R - r0) * pieces;
+#pragma unroll 4
+  for (int i = threadIdx.x; i < n; i += 256) {
+    const int r = i / pieces, c = i - r * pieces;
+    reinterpret_cast<uint4*>(out + (r0 + r) * ldo)[c] = piece_of(x + (r0 + r) * ldx, (int64_t)c * 8, H);
+  }
+}
+
 // X': 16-byte pieces of the live rows of X into blocks of 64 columns, zero past
-// H and, by the last 63 workgroups, in the rows up to the next 64; a piece of an
-// unaligned or ragged row element by element.  Also what the other kernels expect
+// H and, by the last 63 workgroups, in the rows up to the next 64.  Also what the other kernels expect
 // set: zl (NaN until a tile finds the label), a zero loss for the ignored rows and
 // the counters of the ranges.
 template <bool COUNT>
-__global__ void __launch_bounds__(256) gather_kernel(const uint16_t* x, int64_t ldx, int64_t H, int aligned16, Targets tg,
+__global__ void __launch_bounds__(256) gather_kernel(const uint16_t* x, int64_t ldx, int64_t H, Targets tg,
                                                      Live o, uint16_t* xp, int64_t hk, int64_t block, float* zl, float* loss,
                                                      uint32_t* count) {
   const int64_t t = blockIdx.x;
@@ -782,16 +812,7 @@ __global__ void __launch_bounds__(256) gather_kernel(const uint16_t* x, int64_t 
   if (threadIdx.x == 0 && !past) zl[at] = __builtin_nanf("");
   const uint16_t* src = x + t * ldx;
   for (int64_t c = threadIdx.x; c < hk / 8; c += blockDim.x) {
-    uint4 v = make_uint4(0, 0, 0, 0);
-    if (!past && aligned16 && c * 8 + 8 <= H) {
-      v = *reinterpret_cast<const uint4*>(src + c * 8);
-    } else if (!past) {
-      uint32_t w[4] = {0, 0, 0, 0};
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (c * 8 + i < H) w[i >> 1] |= (uint32_t)src[c * 8 + i] << (16 * (i & 1));
-      v = make_uint4(w[0], w[1], w[2], w[3]);
-    }
+    const uint4 v = past ? make_uint4(0, 0, 0, 0) : piece_of(src, c * 8, H);
     *reinterpret_cast<uint4*>(xp + (c >> 3) * block + (int64_t)at * 64 + (c & 7) * 8) = v;
   }
 }
@@ -874,11 +895,19 @@ __global__ void __launch_bounds__(256) scatter_kernel(const float* acc, int64_t 
   const float f = up.common(live[0]);
   for (int64_t c = (int64_t)threadIdx.x * 4; c < H; c += blockDim.x * 4) {
     v4f v = {0.f, 0.f, 0.f, 0.f};
-    if (at >= 0)
+    if (at >= 0) {
+#pragma unroll 4
       for (int s = 0; s < slices; ++s) v += *reinterpret_cast<const v4f*>(acc + s * slice + (int64_t)at * ldp + c);
+      v *= f;
+    }
+    uint16_t* o = dx + t * ldx + c;
+    if (c + 4 <= H) {
+      *reinterpret_cast<u32x2_2*>(o) = (u32x2_2){pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])};
+    } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (c + i < H) dx[t * ldx + c + i] = f32_to_bf16_bits(at >= 0 ? v[i] * f : 0.f);
+      for (int i = 0; i < 4; ++i)
+        if (c + i < H) o[i] = f32_to_bf16_bits(v[i]);
+    }
   }
 }
 
@@ -1074,6 +1103,18 @@ static int check(const char* fn, const void* w, int64_t T, int64_t H, int64_t V,
 
 using namespace ntlb;
 
+extern "C" int ntlb_pad_rows(const uint16_t* x, int64_t ldx, int64_t R, int64_t H, uint16_t* out, int64_t ldo, void* stream) {
+  const char* fn = "ntlb_pad_rows";
+  clear_error();
+  if (R < 0 || H < 1 || ldx < 0 || ldo < H || ldo % 8) return fail(NTLB_EINVAL, "%s: bad shape R %lld H %lld ldx %lld ldo %lld", fn, (long long)R, (long long)H, (long long)ldx, (long long)ldo);
+  if (ldo > (1 << 22) || R > ((int64_t)1 << 31) - 1) return fail(NTLB_EUNSUPPORTED, "%s: R %lld ldo %lld is too large", fn, (long long)R, (long long)ldo);
+  if (R == 0) return NTLB_OK;
+  if (!x || !out || !aligned(out, 16)) return fail(NTLB_EINVAL, "%s: bad pointer", fn);
+  const int per = (int)std::max<int64_t>(1, 2048 / (ldo / 8));
+  xent::pad_kernel<<<(unsigned)cdiv(R, per), 256, 0, as_stream(stream)>>>(x, ldx, R, H, out, ldo, per);
+  return check_launch(fn);
+}
+
 extern "C" int64_t ntlb_linear_xent_state_bytes(int64_t T, int64_t H) { return T < 1 || H < 1 ? 256 : xent::state_of(T, H).bytes; }
 
 extern "C" int64_t ntlb_linear_xent_workspace_bytes(int64_t T, int64_t H, int64_t V, int backward) {
@@ -1107,12 +1148,11 @@ extern "C" int ntlb_linear_xent_forward(const uint16_t* x, int64_t ldx, const ui
   const int slices = T > 0 ? xent::logit_slices(T, H, V) : 1;
   uint32_t* count = slices > 1 ? (uint32_t*)((uint8_t*)workspace + xent::forward_sums(T, V)) : nullptr;
   float* rows_loss = reduction == 0 ? loss : nullptr;
-  const int al = aligned(x, 16) && ldx % 8 == 0;
   if (T > xent::HERE) {
     xent::scan_kernel<<<1, xent::SCAN, 0, st>>>(tg, o);
-    xent::gather_kernel<false><<<(unsigned)T + 63, 256, 0, st>>>(x, ldx, H, al, tg, o, xp, s.hk, s.block, zl, rows_loss, count);
+    xent::gather_kernel<false><<<(unsigned)T + 63, 256, 0, st>>>(x, ldx, H, tg, o, xp, s.hk, s.block, zl, rows_loss, count);
   } else {
-    xent::gather_kernel<true><<<(unsigned)T + 63, 256, 0, st>>>(x, ldx, H, al, tg, o, xp, s.hk, s.block, zl, rows_loss, count);
+    xent::gather_kernel<true><<<(unsigned)T + 63, 256, 0, st>>>(x, ldx, H, tg, o, xp, s.hk, s.block, zl, rows_loss, count);
   }
   if (T > 0) {
     xent::Args g{};
@@ -1181,7 +1221,6 @@ extern "C" int ntlb_linear_xent_backward(const void* state, const uint16_t* w, i
     q.b = {sp + s.xp, s.block * 2, s.hk, Tn};
     q.M = n; q.N = H; q.out = dw + v0 * lddw; q.ldo = lddw;
     q.up = up;
-    q.vec_out = aligned(dw, 16) && lddw % 8 == 0;
     if (both)
       xent::launch_pair(p.pair.tile, x, q, st);
     else if (dw)

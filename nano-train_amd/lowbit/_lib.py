@@ -143,6 +143,7 @@ SIGNATURES = {
     "ntlb_layer_norm_workspace_bytes": [_I32, _I64, _I64],
     "ntlb_route_topk": [_P, _I32, _I64, _I64, _I64, _I64, _I32, _P, _I64, _I64, _I32, _F32, _P, _P, _P],
     "ntlb_route_topk_backward": [_P, _I32, _I64, _I64, _I64, _I64, _I32, _I32, _F32, _P, _P, _P, _I64, _P],
+    "ntlb_pad_rows": [_P, _I64, _I64, _I64, _P, _I64, _P],
     "ntlb_linear_xent_forward": [_P, _I64, _P, _I64, _P, _I32, _I64, _I64, _I64, _I64, _I32, _P, _P, _P, _I64, _P],
     "ntlb_linear_xent_backward": [_P, _P, _I64, _I64, _I64, _I64, _I32, _P, _P, _I64, _P, _I64, _P, _I64, _P],
     "ntlb_linear_xent_state_bytes": [_I64, _I64],
@@ -217,7 +218,8 @@ def autograd():
             except ImportError as exc:
                 raise RuntimeError("the autograd module is not built or does not load; build it with "
                                    f"`python nano-train_amd/build.py` ({exc})") from exc
-            names = [n for n in SIGNATURES if n.startswith(("ntlb_layer_norm", "ntlb_route", "ntlb_linear_xent"))]
+            names = [n for n in SIGNATURES
+                     if n.startswith(("ntlb_layer_norm", "ntlb_route", "ntlb_linear_xent", "ntlb_pad_rows"))]
             mod.bind({n: ctypes.cast(getattr(L, n), ctypes.c_void_p).value for n in [*names, "ntlb_last_error"]})
             _autograd = mod
     return _autograd

@@ -418,3 +418,27 @@ def test_a_divided_contraction(gpu_device, T, H, V, reduction):
     loss = linear_cross_entropy(xl, wl, none, reduction=reduction)
     assert (loss == 0).all()
     assert all((t == 0).all() for t in torch.autograd.grad(loss, (xl, wl), dl))
+
+
+@pytest.mark.parametrize("R,H,pitch,off", [(1, 1, 1, 0), (5, 7, 7, 1), (70000, 3, 5, 0), (300, 345, 345, 0), (33, 1000, 1003, 3), (9, 8, 8, 2),
+                                           (4, 20001, 20001, 0)])
+def test_pad_rows(gpu_device, R, H, pitch, off):
+    """each value to its place, zeros past H, nothing past the rows"""
+    from lowbit import _lib
+
+    src = torch.randint(-32768, 32767, (off + R * pitch,), dtype=torch.int16, device=gpu_device)
+    Hp = (H + 7) // 8 * 8 + 8 * (R % 2)
+    out = torch.full((R + 1, Hp), 77, dtype=torch.int16, device=gpu_device)
+    s = torch.cuda.current_stream().cuda_stream
+    _lib.call("ntlb_pad_rows", src.data_ptr() + 2 * off, pitch, R, H, out.data_ptr(), Hp, s)
+    x = src[off:].as_strided((R, H), (pitch, 1)) if pitch else None
+    assert torch.equal(out[:R, :H], x) and (out[:R, H:] == 0).all() and (out[R] == 77).all()
+
+
+def test_pad_rows_refuses():
+    from lowbit import _lib
+
+    for args in ((4096, 8, -1, 8, 4096, 8, 0), (4096, 8, 4, 8, 4096, 7, 0), (4096, 8, 4, 9, 4096, 8, 0), (4096, 8, 4, 8, 4098, 8, 0),
+                 (0, 8, 4, 8, 4096, 8, 0)):
+        with pytest.raises(ValueError, match="ntlb_pad_rows"):
+            _lib.call("ntlb_pad_rows", *args)
