@@ -1029,19 +1029,20 @@ static Pair pair_of(int64_t T, int64_t H, int64_t cols) {
 }
 
 // Ranges of the contraction for the logits of `cols` words by small tiles: of
-// least time, in us 0.5 a step, and for more than one 4, 1.2 a range of 128 rows
-// and 0.03 a workgroup, whose release and place in the count the others share.
-// Forward by one range and by the choice: 3 rows, 6413 wide, 265 words 71 us and
-// 17; 5, 4208, 2904 48 and 19; 1, 7168, 4096 75 and 25; 1000, 7168, 1000 81 and 45;
-// 16, 4096, 16384 46 and 34; 1000, 1024, 500, by one, 18 (by two 19).
+// least time, in us 0.63 a step, and for more than one range 1.34 for each 128
+// rows of one, which the last to arrive reads, and 0.029 (twice that with 128 rows)
+// a workgroup, whose release all share: fitted to 14 shapes by 1 to 16 ranges, off
+// by 5%.  Forward by one range and by the choice: 3 rows, 6413 wide, 265 words 71
+// us and 17; 5, 4208, 2904 48 and 19; 1, 7168, 4096 75 and 25; 1000, 7168, 1000
+// 81 and 45; 16, 4096, 16384 46 and 34; 1000, 1024, 500, by one, 18 (by two 19).
 static int logit_slices(int64_t T, int64_t H, int64_t cols) {
   if (tile_for(T, cols) != 128) return 1;
   const int64_t tiles = cdiv(T, 128) * cdiv(cols, 128), steps = cdiv(H, KSTEP);
   const double rows = (double)cdiv(std::min<int64_t>(T, 128), 16) / 8;
   int best = 1;
-  double t_best = 0.5 * (double)steps;
+  double t_best = 0.63 * (double)steps;
   for (int n = 2; n <= std::min<int64_t>(16, steps) && tiles * n <= 2 * split_device_cus() && tiles <= COUNTERS; ++n) {
-    const double t = 0.5 * (double)steps / n + 4 + 1.2 * n * rows + 0.03 * (double)(tiles * n);
+    const double t = 0.63 * (double)steps / n + 1.34 * n * rows + 0.029 * (double)(tiles * n) * (1 + rows);
     if (t < t_best) {
       t_best = t;
       best = n;
