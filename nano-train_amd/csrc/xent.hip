@@ -334,8 +334,9 @@ struct Args {
   int64_t M, N;
   const int32_t* live;  // device: the number of live rows (rows of A for LSE / DZ / ACC, the contraction for STORE)
   int slices;           // ACC, and LSE and DZ by small tiles: ranges of the contraction
-  float4* part_z;       // LSE, DZ with ranges: their sums, [tile][range][16 v4f][thread]
-  uint32_t* count;      // ... of each tile, how many are there (0 before and after)
+  int base;             // LSE, DZ by small tiles: the tiles before this one are not divided
+  float4* part_z;       // LSE, DZ with ranges: their sums, [tile - base][range][16 v4f][thread]
+  uint32_t* count;      // ... of each divided tile, how many are there (0 before and after)
   int group_m;          // raster: row tiles side by side
   // LSE
   float2* part;         // [column tiles][ldp] (ref, sum)
@@ -420,7 +421,7 @@ __device__ __forceinline__ void head_tile(Args g, int pid, uint8_t* la0, uint8_t
   const int num_n = (int)((g.N + TN - 1) / TN);
   const int num_m_all = (int)((g.M + TM - 1) / TM);
   const int num_m = EPI == EPI_STORE ? num_m_all : (live + TM - 1) / TM;
-  int sl = 0;
+  int sl = 0, parts = EPI == EPI_ACC ? g.slices : 1;
   if constexpr (EPI == EPI_ACC) {
     const int tiles = num_m * num_n;
     if (pid >= tiles * g.slices) return;
@@ -430,15 +431,19 @@ __device__ __forceinline__ void head_tile(Args g, int pid, uint8_t* la0, uint8_t
     sl = q / tiles;
     pid = q - sl * tiles;
   } else {
-    const int nwg = num_m * num_n * (SPLIT ? g.slices : 1);
-    if (pid >= nwg) return;
-    const int xcd = pid & 7, per = nwg >> 3, extra = nwg & 7;
+    const int tiles = num_m * num_n, base = SPLIT ? min(g.base, tiles) : tiles;
+    const bool divided = SPLIT && pid >= base;
+    if (divided) parts = g.slices;
+    const int first = divided ? base : 0, n = divided ? (tiles - base) * parts : base;
+    pid -= first;
+    if (pid >= n) return;
+    const int xcd = pid & 7, per = n >> 3, extra = n & 7;
     pid = xcd * per + min(xcd, extra) + (pid >> 3);
-    if constexpr (SPLIT) {
-      const int q = pid / g.slices;
-      sl = pid - q * g.slices;
-      pid = q;
+    if (divided) {
+      sl = pid % parts;
+      pid /= parts;
     }
+    pid += first;
   }
   const int group = pid / (g.group_m * num_n), first_m = group * g.group_m;
   const int gsize = min(num_m - first_m, g.group_m), in_group = pid - group * g.group_m * num_n;
@@ -451,8 +456,8 @@ __device__ __forceinline__ void head_tile(Args g, int pid, uint8_t* la0, uint8_t
     g.a.rows = live;
   }
   const int nk = max(1, (int)((g.a.k + KSTEP - 1) / KSTEP));
-  const int kb0 = RANGES ? (int)((int64_t)sl * nk / g.slices) : 0;
-  const int kb1 = RANGES ? (int)((int64_t)(sl + 1) * nk / g.slices) : nk;
+  const int kb0 = RANGES ? (int)((int64_t)sl * nk / parts) : 0;
+  const int kb1 = RANGES ? (int)((int64_t)(sl + 1) * nk / parts) : nk;
 
   // A is X' or dz, B the weight or (with A transposed) X'
   typename std::conditional<TA, BlockTrCopy<D>, BlockRowCopy<D>>::type ca;
@@ -542,7 +547,8 @@ __device__ __forceinline__ void head_tile(Args g, int pid, uint8_t* la0, uint8_t
   }
   if constexpr (SPLIT) {
     const int groups = min((int)(g.M - m0 - wm * 16 * MT + 15) / 16, MT);
-    if (g.slices > 1 && !exchange<MT>(acc, g.part_z + (int64_t)pid * g.slices * (MT * 4 * 256), g.count + pid, g.slices, sl, groups, tid)) return;
+    const int64_t tile = pid - g.base;
+    if (parts > 1 && !exchange<MT>(acc, g.part_z + tile * parts * (MT * 4 * 256), g.count + tile, parts, sl, groups, tid)) return;
   }
   // a wave's 16 KiB of the stages for its output rows
   constexpr int PER = TILE / 16384;
@@ -971,7 +977,8 @@ static int ranges_for(int D, int64_t M, int64_t N, int64_t steps) {
 // one product
 template <bool TA, bool TB, int EPI>
 static void launch_head(int D, const Args& g, hipStream_t st) {
-  const unsigned n = (unsigned)(cdiv(g.M, D) * cdiv(g.N, D) * (EPI == EPI_STORE ? 1 : g.slices));
+  const int64_t tiles = cdiv(g.M, D) * cdiv(g.N, D), base = std::min<int64_t>(g.base, tiles);
+  const unsigned n = (unsigned)(EPI == EPI_ACC ? tiles * g.slices : EPI == EPI_STORE ? tiles : base + (tiles - base) * g.slices);
   if (D == 256)
     head_kernel<256, TA, TB, EPI><<<n, 512, 0, st>>>(g);
   else
@@ -1028,44 +1035,48 @@ static Pair pair_of(int64_t T, int64_t H, int64_t cols) {
   return best;
 }
 
-// Ranges of the contraction for the logits of `cols` words by small tiles: of
-// least time, in us 0.63 a step, and for more than one range 1.34 for each 128
-// rows of one, which the last to arrive reads, and 0.029 (twice that with 128 rows)
-// a workgroup, whose release all share: fitted to 14 shapes by 1 to 16 ranges, off
-// by 5%.  Forward by one range and by the choice: 3 rows, 6413 wide, 265 words 71
-// us and 17; 5, 4208, 2904 48 and 19; 1, 7168, 4096 75 and 25; 1000, 7168, 1000
-// 81 and 45; 16, 4096, 16384 46 and 34; 1000, 1024, 500, by one, 18 (by two 19).
-static int logit_slices(int64_t T, int64_t H, int64_t cols) {
-  if (tile_for(T, cols) != 128) return 1;
-  const int64_t tiles = cdiv(T, 128) * cdiv(cols, 128), steps = cdiv(H, KSTEP);
+// The logits of `cols` words by small tiles: what the tiles past the last whole
+// round (two workgroups to a compute unit) are divided into, if that leaves the
+// chip room: the ranges of least time, in us 0.63 a step, and for more than one
+// range 1.34 for each 128 rows of one, which the last to arrive reads, and 0.029
+// (twice that with 128 rows) a workgroup, whose release all share: fitted to 14
+// shapes by 1 to 16 ranges, off by 5%.  Forward by one range and by the choice: 3
+// rows, 6413 wide, 265 words 71 us and 17; 5, 4208, 2904 48 and 19; 1, 7168, 4096
+// 75 and 25; 1000, 7168, 1000 81 and 45; 16, 4096, 16384 46 and 34; 1000, 1024,
+// 500, by one, 18 (by two 19); 54 tiles past the first 512: 4, 3600, 72400 145 and 113.
+struct Ranges {
+  int base = 0, n = 1;  // tiles that are not divided, ranges of the others
+  int64_t tiles = 0;    // that are
+  int64_t bytes() const { return n < 2 ? 0 : COUNTERS * 4 + tiles * n * 65536; }
+};
+static Ranges logit_ranges(int64_t T, int64_t H, int64_t cols) {
+  Ranges best;
+  if (tile_for(T, cols) != 128) return best;
+  const int64_t room = 2 * split_device_cus(), all = cdiv(T, 128) * cdiv(cols, 128), tiles = all % room, steps = cdiv(H, KSTEP);
+  if (tiles == 0 || tiles > COUNTERS || all - tiles > (1 << 30)) return best;
   const double rows = (double)cdiv(std::min<int64_t>(T, 128), 16) / 8;
-  int best = 1;
   double t_best = 0.63 * (double)steps;
-  for (int n = 2; n <= std::min<int64_t>(16, steps) && tiles * n <= 2 * split_device_cus() && tiles <= COUNTERS; ++n) {
+  for (int n = 2; n <= std::min<int64_t>(16, steps) && tiles * n <= room; ++n) {
     const double t = 0.63 * (double)steps / n + 1.34 * n * rows + 0.029 * (double)(tiles * n) * (1 + rows);
     if (t < t_best) {
       t_best = t;
-      best = n;
+      best = {(int)(all - tiles), n, tiles};
     }
   }
   return best;
-}
-// the bytes of their counters and sums
-static int64_t slices_bytes(int64_t T, int64_t cols, int slices) {
-  return slices < 2 ? 0 : COUNTERS * 4 + cdiv(T, 128) * cdiv(cols, 128) * slices * 65536;
 }
 
 // forward workspace: the pairs, the label logits, the rows' losses, the ranges' sums
 static int64_t forward_parts(int64_t T, int64_t V) { return cdiv(V, tile_for(T, V)); }
 static int64_t forward_sums(int64_t T, int64_t V) { return cdiv(forward_parts(T, V) * T * 8, 256) * 256 + 2 * cdiv(T * 4, 256) * 256; }
-static int64_t forward_ws(int64_t T, int64_t H, int64_t V) { return forward_sums(T, V) + slices_bytes(T, V, logit_slices(T, H, V)); }
+static int64_t forward_ws(int64_t T, int64_t H, int64_t V) { return forward_sums(T, V) + logit_ranges(T, H, V).bytes(); }
 
 // backward: pieces of the vocabulary, tiles, ranges of the dX product, workspace
 struct Plan {
   int64_t piece, block;  // words of a piece, elements of a block of dz
   int dz_tile, dx_tile, dw_tile, slices;
   Pair pair;  // where both gradients are wanted
-  int dz_slices;
+  Ranges ranges;  // of the whole pieces' logits
   int64_t dz, acc, most, sums, bytes;
 };
 constexpr int64_t DZ_BYTES = (int64_t)512 << 20;
@@ -1086,9 +1097,9 @@ static Plan plan_of(int64_t T, int64_t H, int64_t V) {
   p.dz = cdiv(cols, 64) * p.block * 2;
   p.acc = T * hk * 4 * std::max(p.slices, p.pair.slices);
   p.most = p.dz + p.acc;
-  p.dz_slices = logit_slices(T, H, cols);
+  p.ranges = logit_ranges(T, H, cols);
   p.sums = p.most + 256;
-  p.bytes = p.sums + slices_bytes(T, cols, p.dz_slices);
+  p.bytes = p.sums + p.ranges.bytes();
   return p;
 }
 
@@ -1146,8 +1157,8 @@ extern "C" int ntlb_linear_xent_forward(const uint16_t* x, int64_t ldx, const ui
   float2* part = (float2*)workspace;
   float* zl = T > 0 ? (float*)((uint8_t*)workspace + cdiv(parts * T * 8, 256) * 256) : nullptr;
   float* each = T > 0 ? zl + cdiv(T * 4, 256) * 64 : nullptr;
-  const int slices = T > 0 ? xent::logit_slices(T, H, V) : 1;
-  uint32_t* count = slices > 1 ? (uint32_t*)((uint8_t*)workspace + xent::forward_sums(T, V)) : nullptr;
+  const xent::Ranges ranges = T > 0 ? xent::logit_ranges(T, H, V) : xent::Ranges{};
+  uint32_t* count = ranges.n > 1 ? (uint32_t*)((uint8_t*)workspace + xent::forward_sums(T, V)) : nullptr;
   float* rows_loss = reduction == 0 ? loss : nullptr;
   if (T > xent::HERE) {
     xent::scan_kernel<<<1, xent::SCAN, 0, st>>>(tg, o);
@@ -1160,7 +1171,7 @@ extern "C" int ntlb_linear_xent_forward(const uint16_t* x, int64_t ldx, const ui
     g.a = {(const uint8_t*)xp, s.block * 2, T, s.hk};
     g.b = {(const uint8_t*)w, ldw * 2, V, H};
     g.M = T; g.N = V; g.live = o.live; g.group_m = 8; g.part = part; g.ldp = T; g.zl = zl; g.y = o.y;
-    g.slices = slices; g.count = count; g.part_z = count ? (float4*)(count + xent::COUNTERS) : nullptr;
+    g.slices = ranges.n; g.base = ranges.base; g.count = count; g.part_z = count ? (float4*)(count + xent::COUNTERS) : nullptr;
     xent::launch_head<false, false, xent::EPI_LSE>(xent::tile_for(T, V), g, st);
   }
   if (T > 0) {
@@ -1198,7 +1209,7 @@ extern "C" int ntlb_linear_xent_backward(const void* state, const uint16_t* w, i
   const xent::Up up{dloss, most, reduction == 2};
   const bool both = dx && dw && T > 0;
   const int slices = both ? p.pair.slices : p.slices;
-  uint32_t* count = p.dz_slices > 1 ? (uint32_t*)((uint8_t*)workspace + p.sums) : nullptr;
+  uint32_t* count = p.ranges.n > 1 ? (uint32_t*)((uint8_t*)workspace + p.sums) : nullptr;
   if (most || count) xent::most_kernel<<<1, xent::COUNTERS, 0, st>>>(dloss, (const int32_t*)(sp + s.rows), live, most, count);
   for (int64_t v0 = 0; v0 < V; v0 += p.piece) {
     const int64_t n = std::min(p.piece, V - v0), np = cdiv(n, 64) * 64;
@@ -1210,7 +1221,9 @@ extern "C" int ntlb_linear_xent_backward(const void* state, const uint16_t* w, i
     g.M = T; g.N = n; g.y = (const int32_t*)(sp + s.y); g.v0 = v0; g.lse = (const float*)(sp + s.lse);
     g.rows = (const int32_t*)(sp + s.rows); g.up = up;
     g.out = dz; g.ldo = p.block; g.cols = np;
-    g.slices = p.dz_slices; g.count = count; g.part_z = count ? (float4*)(count + xent::COUNTERS) : nullptr;
+    // (the last piece may have fewer tiles than the others' base, or fewer past it)
+    g.slices = p.ranges.n; g.base = p.ranges.base; g.count = count;
+    g.part_z = count ? (float4*)(count + xent::COUNTERS) : nullptr;
     if (T > 0) xent::launch_head<false, false, xent::EPI_DZ>(p.dz_tile, g, st);
     xent::Args x{}, q{};
     x.live = live; x.group_m = 8; x.slices = slices;

@@ -394,7 +394,8 @@ def test_too_large_is_refused():
             _lib.call("ntlb_linear_xent_forward", p, H, p, ldw, p, 1, T, H, V, -100, 2, p, p, p, 1 << 60, 0)
 
 
-@pytest.mark.parametrize("T,H,V", [(1, 7168, 300), (3, 6413, 265), (16, 4096, 1000), (17, 2000, 129), (129, 2500, 700), (300, 5000, 257)])
+@pytest.mark.parametrize("T,H,V", [(1, 7168, 300), (3, 6413, 265), (16, 4096, 1000), (17, 2000, 129), (129, 2500, 700), (300, 5000, 257),
+                                   (5, 1280, 66001)])
 @pytest.mark.parametrize("reduction", ["mean", "none"])
 def test_a_divided_contraction(gpu_device, T, H, V, reduction):
     """few tiles of long rows, whose contraction workgroups share: the sums come in a fixed order, call after call and
