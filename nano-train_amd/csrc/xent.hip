@@ -28,15 +28,15 @@
 // for each row, their largest magnitude), which the outputs take in fp32.
 //
 // Measured, 3891 live rows of 4096, 7168 wide, 131072 words in two pieces: logits
-// and their sums 5.41 ms (1.35 PFLOP/s), per piece logits and dz 2.74 (1.34), dX
-// 2.83 (1.29), dW 2.74 (1.34); the library's product of the forward's operands
-// runs at 1.49.  Both are held by the chip's power: under such a load its clock
-// falls from 2.4 to about 1.8 GHz.  With all copies from the nearest cache (the
-// same step again and again) the four would take 5.24, 2.63, 2.48 and 2.45 ms: the
-// wait for memory is what is left of dX and dW.  Four waves of 128 x 128 instead of
-// eight of 128 x 64 read less of LDS, but one wave a SIMD has no other to hide its
-// waits: 5.79, 2.86, 3.20 and 3.05.  16 rows of 4096 x 131072 words: 187 us, 5.7
-// TB/s of weights.
+// and their sums 5.41 to 5.51 ms (1.35 PFLOP/s), per piece logits and dz 2.74 to
+// 2.79 (1.33), dX and dW 5.52 (1.33; in launches of their own 2.83 and 2.74); the
+// library's product of the forward's operands runs at 1.49.  All are held by the
+// chip's power: under such a load its clock falls from 2.4 to about 1.8 GHz.  With
+// all copies from the nearest cache (the same step again and again) the four would
+// take 5.24, 2.63, 2.48 and 2.45 ms: the wait for memory is what is left of dX and
+// dW.  Four waves of 128 x 128 instead of eight of 128 x 64 read less of LDS, but
+// one wave a SIMD has no other to hide its waits: 5.79, 2.86, 3.20 and 3.05.  16
+// rows of 4096 x 131072 words: 175 to 187 us, 5.7 to 6.1 TB/s of weights.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
