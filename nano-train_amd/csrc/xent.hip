@@ -823,13 +823,16 @@ __global__ void __launch_bounds__(256) gather_kernel(const uint16_t* x, int64_t 
   }
 }
 
-// lse and loss of the live rows from their pairs, R rows by Q walkers
-template <int R, int Q>
+// lse and loss of the live rows from their pairs, R rows by Q walkers; TOTAL: of
+// all rows, in one workgroup, and then their sum or mean in a fixed order (0 where
+// none is live)
+template <int R, int Q, bool TOTAL>
 __global__ void __launch_bounds__(R * Q) join_kernel(const float2* part, int64_t ldp, int64_t parts, const float* zl,
-                                                     const int32_t* rows, const int32_t* live, float* lse, float* each,
-                                                     float* loss) {
+                                                     const int32_t* rows, const int32_t* live, int mean, float* lse,
+                                                     float* each, float* loss) {
   constexpr int WAVES = R * Q / 64;
   __shared__ float2 red[WAVES][R];
+  __shared__ float losses[R];
   const int tid = threadIdx.x, r = tid % R, q = tid / R, n = live[0];
   const int64_t m = (int64_t)blockIdx.x * R + r;
   const bool on = m < n;
@@ -847,14 +850,27 @@ __global__ void __launch_bounds__(R * Q) join_kernel(const float2* part, int64_t
     const float ref = p.x == -__builtin_inff() ? 0.f : p.x;
     const float l = (ref + __builtin_amdgcn_logf(p.y)) * LN2, z = zl[m];
     lse[m] = z != z ? z : l;  // no such word, or its logit is NaN: so is all of the row
-    each[m] = l - z;
-    if (loss) loss[rows[m]] = l - z;
+    if constexpr (TOTAL) {
+      losses[r] = l - z;
+    } else {
+      each[m] = l - z;
+      if (loss) loss[rows[m]] = l - z;
+    }
+  }
+  if constexpr (TOTAL) {
+    __syncthreads();
+    if (tid < 64) {
+      float s = tid < n ? losses[tid % R] : 0.f;
+#pragma unroll
+      for (int d = 1; d < 64; d *= 2) s += __shfl_xor(s, d);
+      if (tid == 0) loss[0] = mean ? s / (float)max(n, 1) : s;
+    }
   }
 }
 
-// the sum or mean of the live rows' losses, in a fixed order; 0 where none is
-// live.  A launch of its own, 2 us: the join's last workgroup cannot know that it
-// is the last without a fence in each, 15 us for 4096 rows.
+// the sum or mean of more rows' losses, in a fixed order; 0 where none is live.  A
+// launch of its own, 2 us: the join's last workgroup cannot know that it is the
+// last without a fence in each, 15 us for 4096 rows.
 __global__ void __launch_bounds__(1024) total_kernel(const float* each, const int32_t* live, int mean, float* loss) {
   __shared__ float red[16];
   const int n = live[0];
@@ -1174,15 +1190,20 @@ extern "C" int ntlb_linear_xent_forward(const uint16_t* x, int64_t ldx, const ui
     g.slices = ranges.n; g.base = ranges.base; g.count = count; g.part_z = count ? (float4*)(count + xent::COUNTERS) : nullptr;
     xent::launch_head<false, false, xent::EPI_LSE>(xent::tile_for(T, V), g, st);
   }
-  if (T > 0) {
-    // many pairs of few rows: more walkers to a row (16 rows of 1024 pairs: 5.6 us, by
-    // 16 walkers 27; 4096 rows of 256: 8.5 and 6.7)
+  const int mean = reduction == 2;
+  // up to 64 rows one workgroup does it all; many pairs of few rows: more walkers to
+  // a row (16 rows of 1024 pairs: 5.6 us, by 16 walkers 27; 4096 rows of 256: 8.5 and 6.7)
+  if (reduction != 0 && T <= 16)
+    xent::join_kernel<16, 64, true><<<1, 1024, 0, st>>>(part, T, parts, zl, o.rows, o.live, mean, lse, nullptr, loss);
+  else if (reduction != 0 && T <= 64 && parts <= 256)
+    xent::join_kernel<64, 16, true><<<1, 1024, 0, st>>>(part, T, parts, zl, o.rows, o.live, mean, lse, nullptr, loss);
+  else if (T > 0) {
     if (parts > 128 && T <= 1024)
-      xent::join_kernel<4, 256><<<(unsigned)cdiv(T, 4), 1024, 0, st>>>(part, T, parts, zl, o.rows, o.live, lse, each, rows_loss);
+      xent::join_kernel<4, 256, false><<<(unsigned)cdiv(T, 4), 1024, 0, st>>>(part, T, parts, zl, o.rows, o.live, mean, lse, each, rows_loss);
     else
-      xent::join_kernel<16, 16><<<(unsigned)cdiv(T, 16), 256, 0, st>>>(part, T, parts, zl, o.rows, o.live, lse, each, rows_loss);
+      xent::join_kernel<16, 16, false><<<(unsigned)cdiv(T, 16), 256, 0, st>>>(part, T, parts, zl, o.rows, o.live, mean, lse, each, rows_loss);
+    if (reduction != 0) xent::total_kernel<<<1, 1024, 0, st>>>(each, o.live, mean, loss);
   }
-  if (reduction != 0) xent::total_kernel<<<1, 1024, 0, st>>>(each, o.live, reduction == 2, loss);
   return check_launch(fn);
 }
 
