@@ -1061,7 +1061,8 @@ int ntlb_pad_rows(const uint16_t* x, int64_t ldx, int64_t R, int64_t H, uint16_t
  * Ignored rows of x are not read.  state (ntlb_linear_xent_state_bytes, 256-byte
  * aligned) holds what the backward needs: the live rows of x among it, not w.
  * workspace: ntlb_linear_xent_workspace_bytes(T, H, V, 0), 16-byte aligned,
- * contents free.  T <= 2^22, V <= 2^30, H <= 2^20, ldw <= 2^22.
+ * contents free.  T <= 2^22, V <= 2^30, H <= 2^20, ldw <= 2^22, and of tiles of
+ * 128 x 128 at most 2^23 in T x V and V x H, 2^19 in T x H.
  */
 int ntlb_linear_xent_forward(const uint16_t* x, int64_t ldx, const uint16_t* w, int64_t ldw, const void* targets,
                              int targets64, int64_t T, int64_t H, int64_t V, int64_t ignore_index, int reduction,

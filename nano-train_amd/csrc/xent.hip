@@ -1119,9 +1119,16 @@ static Plan plan_of(int64_t T, int64_t H, int64_t V) {
   return p;
 }
 
+// every product's grid, of up to 512 threads a tile and 16 ranges, below 2^32 threads
+static bool grids_fit(int64_t T, int64_t H, int64_t V) {
+  auto tiles = [](int64_t a, int64_t b) { return cdiv(a, 128) * cdiv(b, 128); };
+  const int64_t most = 1 << 23;  // of 256 threads: 128 x 128, or four of 512
+  return tiles(T, V) <= most && tiles(V, H) <= most && tiles(T, H) <= most / 16;
+}
+
 static int check(const char* fn, const void* w, int64_t T, int64_t H, int64_t V, int64_t ldw) {
   if (T < 0 || H < 1 || V < 1) return fail(NTLB_EINVAL, "%s: bad shape T %lld H %lld V %lld", fn, (long long)T, (long long)H, (long long)V);
-  if (T > (1 << 22) || V > (1 << 30) || H > (1 << 20)) return fail(NTLB_EUNSUPPORTED, "%s: T %lld H %lld V %lld is too large", fn, (long long)T, (long long)H, (long long)V);
+  if (T > (1 << 22) || V > (1 << 30) || H > (1 << 20) || !grids_fit(T, H, V)) return fail(NTLB_EUNSUPPORTED, "%s: T %lld H %lld V %lld is too large", fn, (long long)T, (long long)H, (long long)V);
   if (!w || !aligned(w, 16) || ldw < H || ldw % 8 || ldw > (1 << 22)) return fail(NTLB_EINVAL, "%s: the weight needs 16-byte rows of at least H values", fn);
   return NTLB_OK;
 }

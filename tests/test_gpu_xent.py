@@ -389,7 +389,8 @@ def test_too_large_is_refused():
     from lowbit import _lib
 
     p = 4096
-    for T, H, V, ldw in (((1 << 22) + 1, 64, 64, 64), (8, (1 << 20) + 8, 64, (1 << 20) + 8), (8, 64, (1 << 30) + 1, 64)):
+    for T, H, V, ldw in (((1 << 22) + 1, 64, 64, 64), (8, (1 << 20) + 8, 64, (1 << 20) + 8), (8, 64, (1 << 30) + 1, 64),
+                         (1 << 22, 64, 1 << 19, 64), (8, 1 << 20, 1 << 18, 1 << 20), (1 << 22, 4096, 64, 4096)):
         with pytest.raises(_lib.LowBitKernelError, match="too large"):
             _lib.call("ntlb_linear_xent_forward", p, H, p, ldw, p, 1, T, H, V, -100, 2, p, p, p, 1 << 60, 0)
 
