@@ -444,3 +444,48 @@ def test_pad_rows_refuses():
                  (0, 8, 4, 8, 4096, 8, 0)):
         with pytest.raises(ValueError, match="ntlb_pad_rows"):
             _lib.call("ntlb_pad_rows", *args)
+
+
+@pytest.mark.parametrize("T,H,V", [(5, 4096, 300), (40, 2048, 1000), (1100, 256, 3000), (20, 1280, 66001)])
+@pytest.mark.parametrize("reduction", [0, 2])
+def test_both_directions_replay_in_a_graph(gpu_device, T, H, V, reduction):
+    """the calls of a step captured once, with contractions divided or not, and replayed over new values and dirty
+    memory: every replay equals the eager step"""
+    from lowbit import _lib
+    from lowbit.loss import linear_cross_entropy
+
+    L = _lib.lib()
+    new = lambda n: torch.full((n,), 255, dtype=torch.uint8, device=gpu_device)  # noqa: E731
+    x, w, y, _ = _inputs(T, H, V, 1, gpu_device, 0.3)
+    loss = torch.empty(T if reduction == 0 else 1, device=gpu_device)
+    dl = torch.rand(T if reduction == 0 else 1, device=gpu_device)
+    dx, dw = torch.empty_like(x), torch.empty_like(w)
+    state, fws, bws = (new(n) for n in (L.ntlb_linear_xent_state_bytes(T, H), max(16, L.ntlb_linear_xent_workspace_bytes(T, H, V, 0)),
+                                        L.ntlb_linear_xent_workspace_bytes(T, H, V, 1)))
+
+    def step():
+        s = torch.cuda.current_stream().cuda_stream
+        _lib.call("ntlb_linear_xent_forward", x.data_ptr(), H, w.data_ptr(), H, y.data_ptr(), 1, T, H, V, IGNORE, reduction,
+                  loss.data_ptr(), state.data_ptr(), fws.data_ptr(), fws.numel(), s)
+        _lib.call("ntlb_linear_xent_backward", state.data_ptr(), w.data_ptr(), H, T, H, V, reduction, dl.data_ptr(),
+                  dx.data_ptr(), H, dw.data_ptr(), H, bws.data_ptr(), bws.numel(), s)
+
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for k in range(4):
+        x2, w2, y2, _ = _inputs(T, H, V, 30 + k, gpu_device, 0.25 * k)
+        x.copy_(x2)
+        w.copy_(w2)
+        y.copy_(y2)
+        state.fill_(255)
+        fws.fill_(255)
+        bws.fill_(255)
+        graph.replay()
+        torch.cuda.synchronize()
+        xl, wl = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+        want = linear_cross_entropy(xl, wl, y, reduction=("none", "sum", "mean")[reduction])
+        gx, gw = torch.autograd.grad(want, (xl, wl), dl if reduction == 0 else dl[0])
+        assert torch.equal(loss, want.detach().reshape(-1)) and torch.equal(dx, gx) and torch.equal(dw, gw)
