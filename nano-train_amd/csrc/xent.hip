@@ -332,7 +332,7 @@ struct Up {
 struct Args {
   Mat a, b;
   int64_t M, N;
-  const int32_t* live;  // device: the number of live rows (rows of A for LSE / DZ / ACC, the contraction for STORE)
+  const int32_t* live;  // device: the rows in use (of A for LSE / DZ / ACC, of the contraction for STORE)
   int slices;           // ACC, and LSE and DZ by small tiles: ranges of the contraction
   int base;             // LSE, DZ by small tiles: the tiles before this one are not divided
   float4* part_z;       // LSE, DZ with ranges: their sums, [tile - base][range][16 v4f][thread]
@@ -348,6 +348,8 @@ struct Args {
   const float* lse;
   const int32_t* rows;
   Up up;
+  int half;             // DZ: the row that the rest of row 0's values goes to, or 0
+  const int32_t* n;     // STORE: the number of live rows
   // outputs
   void* out;            // DZ: bf16, ACC: fp32 [slices][..], STORE: bf16
   int64_t ldo;          // elements; DZ: of a block
@@ -641,10 +643,21 @@ __device__ __forceinline__ void head_tile(Args g, int pid, uint8_t* la0, uint8_t
       }
     }
     const int64_t block = n0 / 64 + wn;
-    store_bf16<MT, false>(stage, lane, m0 + wm * 16 * MT, 0, (g.M + 63) / 64 * 64, g.cols - block * 64, (uint16_t*)g.out + block * g.ldo, 64, [&](int tm, int tn, float (&v)[4]) {
+    const bool rest = D == 128 && g.half;  // (up to 64 rows always take the small tiles)
+    const int64_t end = rest ? g.half : (g.M + 63) / 64 * 64;
+    uint16_t* o = (uint16_t*)g.out + block * g.ldo;
+    store_bf16<MT, false>(stage, lane, m0 + wm * 16 * MT, 0, end, g.cols - block * 64, o, 64, [&](int tm, int tn, float (&v)[4]) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) v[r] = acc[tm][tn][r] * u[tm];
     });
+    if (rest)
+      store_bf16<MT, false>(stage, lane, m0 + wm * 16 * MT, 0, end, g.cols - block * 64, o + g.half * 64, 64, [&](int tm, int tn, float (&v)[4]) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float w = acc[tm][tn][r] * u[tm], hi = (float)(__bf16)w;
+          v[r] = __builtin_fabsf(hi) < __builtin_inff() ? w - hi : 0.f;  // what is no number is in the first half
+        }
+      });
   } else if constexpr (EPI == EPI_ACC) {
     float* o = (float*)g.out + sl * g.slice;
 #pragma unroll
@@ -660,7 +673,7 @@ __device__ __forceinline__ void head_tile(Args g, int pid, uint8_t* la0, uint8_t
       }
     }
   } else {
-    const float c = g.up.common(live);
+    const float c = g.up.common(g.n[0]);
     store_bf16<MT, true>(stage, lane, m0 + wm * 16 * MT, n0 + wn * 64, g.M, g.N, (uint16_t*)g.out, g.ldo, [&](int tm, int tn, float (&v)[4]) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) v[r] = acc[tm][tn][r] * c;
@@ -693,7 +706,7 @@ __global__ void __launch_bounds__(2 * D, D == 256 ? 1 : 2) gradients_kernel(Args
 
 // ---------------------------------------------------------------------------
 // the live rows: pos[t] = place of row t among them (-1: ignored), rows[i] and
-// y[i] (-1: not a word) of the i-th, live[0] how many.  One workgroup; up to HERE
+// y[i] (-1: not a word) of the i-th, live[0] how many, live[1] the rows of dz.  One workgroup; up to HERE
 // rows each of gather_kernel's counts for itself (16 rows: 5.0 us, with this
 // launch 4.7 + 4.9; 1003 rows 5.0 and 2.4 + 3.6).
 // ---------------------------------------------------------------------------
@@ -734,7 +747,7 @@ __global__ void __launch_bounds__(SCAN) scan_kernel(Targets tg, Live o) {
     base += all;
     __syncthreads();
   }
-  if (tid == 0) o.live[0] = base;
+  if (tid == 0) o.live[0] = o.live[1] = base;
 }
 
 // eight values of a row of H from column c, zero past H; rows begin anywhere
@@ -765,13 +778,14 @@ __global__ void __launch_bounds__(256) pad_kernel(const uint16_t* x, int64_t ldx
 }
 
 // X': 16-byte pieces of the live rows of X into blocks of 64 columns, zero past
-// H and, by the last 63 workgroups, in the rows up to the next 64.  Also what the other kernels expect
+// H and, by the last 63 workgroups, in the rows up to the next 64; with `half`, twice,
+// `half` rows on again.  Also what the other kernels expect
 // set: zl (NaN until a tile finds the label), a zero loss for the ignored rows and
 // the counters of the ranges.
 template <bool COUNT>
 __global__ void __launch_bounds__(256) gather_kernel(const uint16_t* x, int64_t ldx, int64_t H, Targets tg,
                                                      Live o, uint16_t* xp, int64_t hk, int64_t block, float* zl, float* loss,
-                                                     uint32_t* count) {
+                                                     uint32_t* count, int half) {
   const int64_t t = blockIdx.x;
   if (t == 0 && count)
     for (int i = threadIdx.x; i < COUNTERS; i += 256) count[i] = 0;
@@ -802,7 +816,10 @@ __global__ void __launch_bounds__(256) gather_kernel(const uint16_t* x, int64_t 
         o.rows[at] = (int32_t)t;
         o.y[at] = tg.word(v);
       }
-      if (t == 0) o.live[0] = n;
+      if (t == 0) {
+        o.live[0] = n;
+        o.live[1] = half && n ? half + n : n;
+      }
     }
     if (!on) at = -1;
   } else {
@@ -810,7 +827,7 @@ __global__ void __launch_bounds__(256) gather_kernel(const uint16_t* x, int64_t 
     at = past ? -1 : o.pos[t];
   }
   if (past) at = n + (int)(t - tg.T);
-  if (past && at >= (n + 63) / 64 * 64) return;
+  if (past && at >= (half ? half : (n + 63) / 64 * 64)) return;
   if (at < 0) {
     if (threadIdx.x == 0 && loss) loss[t] = 0.f;
     return;
@@ -819,7 +836,9 @@ __global__ void __launch_bounds__(256) gather_kernel(const uint16_t* x, int64_t 
   const uint16_t* src = x + t * ldx;
   for (int64_t c = threadIdx.x; c < hk / 8; c += blockDim.x) {
     const uint4 v = past ? make_uint4(0, 0, 0, 0) : piece_of(src, c * 8, H);
-    *reinterpret_cast<uint4*>(xp + (c >> 3) * block + (int64_t)at * 64 + (c & 7) * 8) = v;
+    uint4* o = reinterpret_cast<uint4*>(xp + (c >> 3) * block + (int64_t)at * 64 + (c & 7) * 8);
+    o[0] = v;
+    if (half) o[half * 8] = v;
   }
 }
 
@@ -909,7 +928,7 @@ __global__ void __launch_bounds__(1024) most_kernel(const float* du, const int32
 }
 
 // dX rows: the slices summed in order, bf16; zero for the ignored rows
-__global__ void __launch_bounds__(256) scatter_kernel(const float* acc, int64_t ldp, int64_t slice, int slices, Up up,
+__global__ void __launch_bounds__(256) scatter_kernel(const float* acc, int64_t ldp, int64_t slice, int slices, int half, Up up,
                                                       const int32_t* live, const int32_t* pos, int64_t H, uint16_t* dx,
                                                       int64_t ldx) {
   const int64_t t = blockIdx.x;
@@ -920,6 +939,9 @@ __global__ void __launch_bounds__(256) scatter_kernel(const float* acc, int64_t 
     if (at >= 0) {
 #pragma unroll 4
       for (int s = 0; s < slices; ++s) v += *reinterpret_cast<const v4f*>(acc + s * slice + (int64_t)at * ldp + c);
+      if (half)
+#pragma unroll 4
+        for (int s = 0; s < slices; ++s) v += *reinterpret_cast<const v4f*>(acc + s * slice + (int64_t)(half + at) * ldp + c);
       v *= f;
     }
     uint16_t* o = dx + t * ldx + c;
@@ -933,8 +955,15 @@ __global__ void __launch_bounds__(256) scatter_kernel(const float* acc, int64_t 
   }
 }
 
-// elements of a block of X' or dz: 64 columns of T rows, whole 64 of them
-static int64_t block_of(int64_t T) { return cdiv(T, 64) * 64 * 64; }
+// Up to 64 rows, whose tiles and steps have room for it, dz's rounding to bf16 is
+// not left out: row `half` + i holds what row i's values lack, beside X' row i
+// again, and both products sum the two.  (Of few values the gradients would
+// otherwise be off by up to 1.9 times their own rounding; of many it is 1.4 times.)
+static int half_of(int64_t T) { return T <= 32 ? 32 : T <= 64 ? 64 : 0; }
+// rows of dz as dX's product has them
+static int64_t dz_rows(int64_t T) { return half_of(T) + T; }
+// elements of a block of X' or dz: 64 columns of the rows, whole 64 of them
+static int64_t block_of(int64_t T) { return half_of(T) ? 2 * half_of(T) * 64 : cdiv(T, 64) * 64 * 64; }
 
 // what the forward leaves for the backward
 struct State {
@@ -1111,7 +1140,7 @@ static Plan plan_of(int64_t T, int64_t H, int64_t V) {
   p.slices = ranges_for(p.dx_tile, T, H, steps);
   p.pair = pair_of(T, H, cols);
   p.dz = cdiv(cols, 64) * p.block * 2;
-  p.acc = T * hk * 4 * std::max(p.slices, p.pair.slices);
+  p.acc = dz_rows(T) * hk * 4 * std::max(p.slices, p.pair.slices);
   p.most = p.dz + p.acc;
   p.ranges = logit_ranges(T, H, cols);
   p.sums = p.most + 256;
@@ -1185,9 +1214,9 @@ extern "C" int ntlb_linear_xent_forward(const uint16_t* x, int64_t ldx, const ui
   float* rows_loss = reduction == 0 ? loss : nullptr;
   if (T > xent::HERE) {
     xent::scan_kernel<<<1, xent::SCAN, 0, st>>>(tg, o);
-    xent::gather_kernel<false><<<(unsigned)T + 63, 256, 0, st>>>(x, ldx, H, tg, o, xp, s.hk, s.block, zl, rows_loss, count);
+    xent::gather_kernel<false><<<(unsigned)T + 63, 256, 0, st>>>(x, ldx, H, tg, o, xp, s.hk, s.block, zl, rows_loss, count, xent::half_of(T));
   } else {
-    xent::gather_kernel<true><<<(unsigned)T + 63, 256, 0, st>>>(x, ldx, H, tg, o, xp, s.hk, s.block, zl, rows_loss, count);
+    xent::gather_kernel<true><<<(unsigned)T + 63, 256, 0, st>>>(x, ldx, H, tg, o, xp, s.hk, s.block, zl, rows_loss, count, xent::half_of(T));
   }
   if (T > 0) {
     xent::Args g{};
@@ -1250,15 +1279,16 @@ extern "C" int ntlb_linear_xent_backward(const void* state, const uint16_t* w, i
     g.rows = (const int32_t*)(sp + s.rows); g.up = up;
     g.out = dz; g.ldo = p.block; g.cols = np;
     // (the last piece may have fewer tiles than the others' base, or fewer past it)
+    g.half = xent::half_of(T);
     g.slices = p.ranges.n; g.base = p.ranges.base; g.count = count;
     g.part_z = count ? (float4*)(count + xent::COUNTERS) : nullptr;
     if (T > 0) xent::launch_head<false, false, xent::EPI_DZ>(p.dz_tile, g, st);
     xent::Args x{}, q{};
-    x.live = live; x.group_m = 8; x.slices = slices;
+    x.live = live + 1; x.group_m = 8; x.slices = slices;
     x.a = {(const uint8_t*)dz, p.block * 2, Tn, np};
     x.b = {wp, ldw * 2, H, n};
-    x.M = T; x.N = H; x.out = acc; x.ldo = s.hk; x.slice = T * s.hk; x.add = v0 > 0;
-    q.live = live; q.group_m = 8;
+    x.M = xent::dz_rows(T); x.N = H; x.out = acc; x.ldo = s.hk; x.slice = x.M * s.hk; x.add = v0 > 0;
+    q.live = live + 1; q.n = live; q.group_m = 8;
     q.a = {(const uint8_t*)dz, p.block * 2, np, Tn};
     q.b = {sp + s.xp, s.block * 2, s.hk, Tn};
     q.M = n; q.N = H; q.out = dw + v0 * lddw; q.ldo = lddw;
@@ -1271,7 +1301,7 @@ extern "C" int ntlb_linear_xent_backward(const void* state, const uint16_t* w, i
       xent::launch_head<false, true, xent::EPI_ACC>(p.dx_tile, x, st);
   }
   if (dx && T > 0)
-    xent::scatter_kernel<<<(unsigned)T, 256, 0, st>>>(acc, s.hk, T * s.hk, slices, up, live, (const int32_t*)(sp + s.pos),
+    xent::scatter_kernel<<<(unsigned)T, 256, 0, st>>>(acc, s.hk, xent::dz_rows(T) * s.hk, slices, xent::half_of(T), up, live, (const int32_t*)(sp + s.pos),
                                                      H, dx, lddx);
   return check_launch(fn);
 }
