@@ -1074,7 +1074,8 @@ int ntlb_linear_xent_forward(const uint16_t* x, int64_t ldx, const uint16_t* w, 
  *   dx = dz W (bf16 [T, H], zero in ignored rows), dw = dz^T X (bf16 [V, H]),
  * either NULL if not wanted.  The logits are formed again piece by piece of the
  * vocabulary; dz, without the rows' common factor, is rounded to bf16 as the
- * operand of the two products.  w must be as in the forward.  workspace: ntlb_linear_xent_workspace_bytes(T, H, V, 1).
+ * operand of the two products (up to 64 rows: to two bf16 values, whose sum
+ * holds 16 bits).  w must be as in the forward.  workspace: ntlb_linear_xent_workspace_bytes(T, H, V, 1).
  */
 int ntlb_linear_xent_backward(const void* state, const uint16_t* w, int64_t ldw, int64_t T, int64_t H, int64_t V,
                               int reduction, const float* dloss, uint16_t* dx, int64_t lddx, uint16_t* dw,

@@ -25,7 +25,8 @@
 // large values, p - 1 at the labels, would not be if they held the factor 1 / n of
 // a mean: every one of them would be off by the same part, and so the whole
 // gradient.  So dz is formed without the rows' common factor (for u of its own
-// for each row, their largest magnitude), which the outputs take in fp32.
+// for each row, their largest magnitude), which the outputs take in fp32.  Up to 64
+// rows dz is two bf16 values, at no product's cost.
 //
 // Measured, 3891 live rows of 4096, 7168 wide, 131072 words in two pieces: logits
 // and their sums 5.41 to 5.51 ms (1.35 PFLOP/s), per piece logits and dz 2.74 to
