@@ -518,9 +518,12 @@ __global__ void __launch_bounds__(64 * WAVES) backward_kernel(Args g) {
       if (mine) q = score(zc, 0, c);
     }
     if (g.renorm) {
+      // relative to the first chosen one's gradient, so that what all have in common
+      // does not cancel: d - sum(d q) / s = c - sum(c q) / s + d0 eps / s for c = d - d0
+      const float d0 = g.scale * g.dw[t * g.k], c = mine ? d - d0 : 0.f;
       const float s = token_sum<LPT>(q) + RENORM_EPS;
-      const float a = token_sum<LPT>(d * q);
-      d = mine ? (d - a / s) / s : 0.f;
+      const float a = token_sum<LPT>(c * q);
+      d = mine ? (c - a / s + d0 * (RENORM_EPS / s)) / s : 0.f;
     }
     float own;  // the gradient at a chosen logit
     if constexpr (SIG) {

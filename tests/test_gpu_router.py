@@ -328,3 +328,23 @@ def test_refusals(gpu_device):
         route_tokens(z.double(), 2)
     with pytest.raises(RuntimeError, match="balance bias"):
         TopKRouter(8, 4, 2, device=gpu_device).update_bias(torch.zeros(1, 2, device=gpu_device))
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("k", [2, 5])
+def test_gradients_nearly_alike_do_not_cancel(gpu_device, score, k):
+    """dw of one large value and small differences: the renormalised weights' sum is one, so the large value has no part in
+    the gradient.  Formed from differences, each of a few roundings, what is left is off by roundings of the differences'
+    size; the sum d p would be off by roundings of the large value, a thousand times more"""
+    from lowbit.router import route_tokens
+
+    g = torch.Generator().manual_seed(k)
+    z = torch.randn(64, 40, generator=g).to(gpu_device).requires_grad_(True)
+    dw = (1024.0 + torch.randint(-64, 65, (64, k), generator=g) / 64.0).to(gpu_device)  # exact in fp32
+    ids, w = route_tokens(z, k, score=score)
+    (dz,) = torch.autograd.grad(w, z, dw)
+    zd = z.detach().double().requires_grad_(True)
+    p = (torch.softmax(zd, 1) if score == "softmax" else torch.sigmoid(zd)).gather(1, ids.long())
+    (want,) = torch.autograd.grad(p / p.sum(1, keepdim=True), zd, dw.double())
+    # |c| <= 2; c, its mean, their difference, p and its factors: at most 64 roundings of values below 4 |dw/dz|
+    assert (dz.double() - want).abs().max() <= 64 * U * 4
