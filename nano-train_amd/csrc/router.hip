@@ -60,16 +60,16 @@ struct Args {
 };
 
 // exp(x), within two units of the last place: v_exp_f32 of x log2(e) with the
-// product's rounding error put back to first order.  Underflows to 0 below
-// about -87, overflows to infinity; NaN stays.
+// product's rounding error put back to first order.  From |x| of about 88.7 on
+// there is nothing to put back: 0 or infinity (whose correction would be infinity
+// times 0, or less infinity: NaN), and NaN stays.
 __device__ __forceinline__ float exp_f32(float x) {
   constexpr float L = 1.44269502e+00f, L_LO = 1.92596303e-08f, LN2 = 6.93147182e-01f;
   const float t = x * L;
   float r = __builtin_fmaf(x, L, -t);
   r = __builtin_fmaf(x, L_LO, r) * LN2;
-  r = __builtin_fabsf(t) < 256.f ? r : 0.f;  // t infinite: r is NaN
   const float e = __builtin_amdgcn_exp2f(t);
-  return __builtin_fmaf(e, r, e);
+  return __builtin_fabsf(t) < 128.f ? __builtin_fmaf(e, r, e) : e;
 }
 
 // Lane l of a token's LPT lanes holds elements e(l, j): chunks of V consecutive

@@ -348,3 +348,68 @@ def test_gradients_nearly_alike_do_not_cancel(gpu_device, score, k):
     (want,) = torch.autograd.grad(p / p.sum(1, keepdim=True), zd, dw.double())
     # |c| <= 2; c, its mean, their difference, p and its factors: at most 64 roundings of values below 4 |dw/dz|
     assert (dz.double() - want).abs().max() <= 64 * U * 4
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("G,Gk", [(1, 1), (8, 2), (3, 1)])
+@pytest.mark.parametrize("renorm", [True, False])
+def test_sigmoid_of_logits_far_below_zero(gpu_device, dtype, G, Gk, renorm):
+    """scores that underflow, at -inf, the types' lowest values and below -85, beside k experts in each group that do not:
+    those are chosen, and a low one weighs its sigmoid, never NaN"""
+    from lowbit.router import route_tokens
+
+    T, E, k = 300, 96, 6
+    g = torch.Generator().manual_seed(21)
+    low = torch.cat([torch.tensor([-float("inf"), torch.finfo(torch.float32).min, torch.finfo(torch.bfloat16).min, -65504.0,
+                                   -1000.0, -200.0, -177.0]), torch.linspace(-180, -85, 401)])
+    z = torch.randn(T, E, generator=g) * 1.5
+    per = E // G
+    keep = torch.rand(T, G, per, generator=g).argsort(-1).argsort(-1) < k  # k of each group's experts
+    z = torch.where(keep.reshape(T, E), z, low[torch.randint(low.numel(), (T, E), generator=g)]).to(dtype).to(gpu_device)
+    dw = torch.randn(T, k, generator=g).to(gpu_device)
+    zl = z.clone().requires_grad_(True)
+    for bias in (None, torch.zeros(E, device=gpu_device)):
+        ids, w = route_tokens(zl, k, score="sigmoid", bias=bias, n_groups=G, topk_groups=Gk, renormalize=renorm)
+        (dz,) = torch.autograd.grad(w, zl, dw)
+        _check_ids(ids, z, k, "sigmoid", None, G, Gk)
+        _check_weights(w.detach(), dz, z, ids, "sigmoid", renorm, 1.0, dw)
+        assert dz.isfinite().all()
+
+
+@pytest.mark.parametrize("low", [-float("inf"), torch.finfo(torch.float32).min, -1e5, -200.0, -178.5])
+@pytest.mark.parametrize("biased", [False, True])
+def test_sigmoid_of_masked_experts(gpu_device, low, biased):
+    """fewer experts than top_k are left beside those masked by their logits (and by a bias of -inf): they come first,
+    then the masked ones, lowest index first and of no weight"""
+    from lowbit.router import route_tokens
+
+    z = torch.full((3, 40), low)
+    z[0, [30, 7, 12]] = torch.tensor([2.0, 1.0, 0.5])
+    z[1, 39] = -3.0
+    b = torch.zeros(40, device=gpu_device)
+    if biased:
+        b[[i for i in range(40) if i not in (7, 12, 30, 39)]] = -float("inf")
+    zl = z.to(gpu_device).requires_grad_(True)
+    for G, Gk in ((1, 1), (2, 2)):
+        ids, w = route_tokens(zl, 8, score="sigmoid", bias=b if biased else None, n_groups=G, topk_groups=Gk)
+        if biased:
+            assert ids.tolist() == [[30, 7, 12, 39, 0, 1, 2, 3], [39, 7, 12, 30, 0, 1, 2, 3], [7, 12, 30, 39, 0, 1, 2, 3]]
+        else:
+            assert ids.tolist() == [[30, 7, 12, 0, 1, 2, 3, 4], [39, 0, 1, 2, 3, 4, 5, 6], list(range(8))]
+        want = torch.zeros(3, 8, dtype=torch.float64)
+        p = torch.sigmoid(torch.tensor([2.0, 1.0, 0.5], dtype=torch.float64))
+        want[0, :3], want[1, 0] = p / p.sum(), 1.0
+        assert (w.detach().cpu().double() - want).abs().max() <= 64 * U
+        (dz,) = torch.autograd.grad(w.square().sum(), zl)
+        assert dz.isfinite().all()
+
+
+def test_sigmoid_from_minus_180_to_minus_85(gpu_device):
+    """every expert's score where exp(-z) nears and passes the largest float: to 1e-37 the sigmoid, and in its order"""
+    from lowbit.router import route_tokens
+
+    z = torch.linspace(-180, -85, 16 * 4096).reshape(16, 4096).t().contiguous().to(gpu_device)
+    ids, w = route_tokens(z, 16, score="sigmoid", renormalize=False)
+    want = torch.sigmoid(z.double()).gather(1, ids.long())
+    assert ((w.double() - want).abs() <= 64 * U * want + 1e-37).all() and (w >= 0).all()
+    assert (w[:, 1:] <= w[:, :-1]).all()
