@@ -321,7 +321,8 @@ __device__ __forceinline__ void store_bf16(uint8_t* stage, int lane, int64_t m0,
 constexpr int EPI_LSE = 0, EPI_DZ = 1, EPI_ACC = 2, EPI_STORE = 3;
 
 // The gradient that comes in: du[0] for all rows, over the number of live rows
-// if mean; or, `most` given, du[t] for row t, their common factor most[0]
+// if mean; or, `most` given, du[t] for row t, their common factor most[0], which is
+// 0 only if all are
 struct Up {
   const float* du;
   const float* most;
@@ -907,24 +908,27 @@ __global__ void __launch_bounds__(1024) total_kernel(const float* each, const in
   }
 }
 
-// the largest finite |du| of the live rows, if `most` is given, and the counters of
-// the ranges cleared, if there are any
+// the largest finite |du| of the live rows, if `most` is given (1 where the finite ones
+// are 0 but others are not finite: those have to reach dz), and the counters of the
+// ranges cleared, if there are any
 __global__ void __launch_bounds__(1024) most_kernel(const float* du, const int32_t* rows, const int32_t* live, float* most,
                                                     uint32_t* count) {
   __shared__ uint32_t red[16];
   if (count) count[threadIdx.x] = 0;
   if (!most) return;
   uint32_t m = 0;
+  int wild = 0;
   for (int i = threadIdx.x; i < live[0]; i += 1024) {
     const uint32_t a = abs_bits(du[rows[i]]);
     m = a < 0x7F800000u ? max(m, a) : m;
+    wild |= a >= 0x7F800000u;
   }
   m = wave_max_u32(m);
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
-  __syncthreads();
+  wild = __syncthreads_or(wild);
   if (threadIdx.x == 0) {
     for (int i = 1; i < 16; ++i) m = max(m, red[i]);
-    most[0] = __uint_as_float(m);
+    most[0] = m == 0 && wild ? 1.0f : __uint_as_float(m);
   }
 }
 

@@ -489,3 +489,34 @@ def test_both_directions_replay_in_a_graph(gpu_device, T, H, V, reduction):
         want = linear_cross_entropy(xl, wl, y, reduction=("none", "sum", "mean")[reduction])
         gx, gw = torch.autograd.grad(want, (xl, wl), dl if reduction == 0 else dl[0])
         assert torch.equal(loss, want.detach().reshape(-1)) and torch.equal(dx, gx) and torch.equal(dw, gw)
+
+
+@pytest.mark.parametrize("T", [1, 40, 64, 65, 300])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("others", ["zero", "bad", "one"])
+def test_incoming_gradients_that_are_no_numbers(gpu_device, T, bad, others):
+    """a position whose incoming gradient is infinite or NaN passes it on, whatever the others' are; so does none that is
+    ignored"""
+    from lowbit.loss import linear_cross_entropy
+
+    x, w, y, _ = _inputs(T, 128, 500, 31, gpu_device)
+    at = T // 2
+    dl = torch.full((T,), {"zero": 0.0, "bad": bad, "one": 1.0}[others], device=gpu_device)
+    dl[at] = bad
+    rows = dl != dl if bad != bad else dl == bad
+    for which in ("both", "hidden", "weight"):
+        xl, wl = x.clone().requires_grad_(which != "weight"), w.clone().requires_grad_(which != "hidden")
+        linear_cross_entropy(xl, wl, y, reduction="none").backward(dl)
+        if which != "weight":
+            assert not xl.grad[rows].isfinite().any() and xl.grad[~rows].isfinite().all()
+            assert others == "one" or not xl.grad[~rows].any()
+        if which != "hidden":
+            assert not wl.grad.isfinite().any()
+    y[at] = IGNORE
+    rows[at] = False
+    xl, wl = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    linear_cross_entropy(xl, wl, y, reduction="none").backward(dl)
+    assert not xl.grad[at].any()
+    if not rows.any():
+        assert xl.grad.isfinite().all() and wl.grad.isfinite().all()
+        assert others == "one" or not (xl.grad.any() or wl.grad.any())
