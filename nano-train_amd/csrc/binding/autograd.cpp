@@ -80,10 +80,13 @@ Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const Tensor& like) {
 Tensor scratch(int64_t bytes, const Tensor& like) { return fresh({bytes}, at::kByte, like); }
 
 // t as [rows, columns] with unit stride along the columns and rows one behind the
-// other (or one row repeated): a copy only where no view gives that
+// other (or one row repeated): a copy only where no view gives that.  Of a single
+// row torch's own strides may be anything, contiguous() or not.
 Tensor rows_of(const Tensor& t) {
   Tensor r = t.dim() == 2 ? t : t.reshape({t.numel() / t.size(-1), t.size(-1)});
-  if (r.stride(1) != 1 || (r.stride(0) != 0 && r.stride(0) < r.size(1))) r = r.contiguous();
+  const int64_t n = r.size(1);
+  if (r.stride(1) != 1 || (r.stride(0) != 0 && r.stride(0) < n)) r = r.contiguous();
+  if (r.size(0) == 1 && r.stride(0) < n) r = r.as_strided({1, n}, {n, 1});
   return r;
 }
 Tensor shaped(const Tensor& t, at::IntArrayRef sizes) { return t.sizes() == sizes ? t : t.reshape(sizes); }

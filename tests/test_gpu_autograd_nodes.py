@@ -107,3 +107,39 @@ def test_ids_are_not_differentiable(gpu_device):
 
     ids, w = route_tokens(torch.randn(5, 12, device=gpu_device, requires_grad=True), 3)
     assert not ids.requires_grad and w.requires_grad
+
+
+def _row(dev, n, dtype=torch.float32):
+    """[1, n] of strides (1, 1), as a column's transposition gives it"""
+    t = torch.randn(n, 1, device=dev).to(dtype).t()
+    assert t.stride() == (1, 1)
+    return t
+
+
+def test_one_row_of_any_pitch(gpu_device):
+    """a single row has no pitch, whatever its stride says: inputs and incoming gradients"""
+    from lowbit.loss import linear_cross_entropy
+    from lowbit.norm import layer_norm
+    from lowbit.router import route_tokens
+
+    def same(f, *ins, up):
+        got, want = [], []
+        for out, plain in ((got, False), (want, True)):
+            leaves = [(t.clone(memory_format=torch.contiguous_format).reshape(-1).reshape(t.shape) if plain else t)
+                      .detach().requires_grad_(True) for t in ins]
+            r = f(*leaves)
+            u = up.reshape(-1).reshape(r.shape) if plain else up
+            out += [r.detach(), *torch.autograd.grad(r, leaves, u)]
+            with torch.no_grad():
+                out.append(f(*leaves))
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+    for dtype in (torch.float32, torch.bfloat16):
+        same(lambda x: layer_norm(x), _row(gpu_device, 72, dtype), up=_row(gpu_device, 72, dtype))
+    same(lambda z: route_tokens(z, 4)[1], _row(gpu_device, 40), up=_row(gpu_device, 4))
+    y = torch.zeros(1, dtype=torch.int64, device=gpu_device)
+    w = torch.randn(90, 64, device=gpu_device).bfloat16()
+    one = torch.ones(1, device=gpu_device)
+    same(lambda x, w: linear_cross_entropy(x, w, y, reduction="none"), _row(gpu_device, 64, torch.bfloat16), w, up=one)
+    x = torch.randn(1, 64, device=gpu_device).bfloat16()
+    same(lambda x, w: linear_cross_entropy(x, w, y, reduction="none"), x, _row(gpu_device, 64, torch.bfloat16), up=one)
