@@ -93,6 +93,14 @@ Tensor shaped(const Tensor& t, at::IntArrayRef sizes) { return t.sizes() == size
 
 bool wanted(const Tensor& t) { return t.defined() && t.requires_grad(); }
 
+// No tangents are formed.  One that comes with an argument would be dropped without
+// a word: the result would count as constant along it.
+template <typename... Ts>
+void no_tangent(const char* fn, const Ts&... ts) {
+  if (((ts.defined() && ts._fw_grad(/*level=*/0).defined()) || ...))
+    C10_THROW_ERROR(NotImplementedError, std::string(fn) + " has no derivative in forward mode");
+}
+
 // The gradients are no functions of the graph: where one is being recorded, they
 // carry an error for whoever differentiates them
 variable_list once(variable_list grads) {
@@ -142,6 +150,7 @@ struct LayerNorm {
     variable_list apply(variable_list&& grads) override {
       const std::lock_guard<std::mutex> lock(mutex_);
       if (!grads[0].defined()) return variable_list(3);
+      no_tangent("the gradient of layer_norm", grads[0]);
       const Tensor xt = x.unpack(), wt = w.unpack(), bt = b.unpack();
       const c10::DeviceGuard guard(xt.device());
       const at::AutoDispatchBelowADInplaceOrView below;
@@ -225,6 +234,7 @@ struct Route {
     variable_list apply(variable_list&& grads) override {
       const std::lock_guard<std::mutex> lock(mutex_);
       if (!grads[0].defined()) return variable_list(1);
+      no_tangent("the gradient of route_tokens", grads[0]);
       const Tensor zt = z.unpack(), it = ids.unpack();
       const c10::DeviceGuard guard(zt.device());
       const at::AutoDispatchBelowADInplaceOrView below;
@@ -300,6 +310,7 @@ struct LinearXent {
     variable_list apply(variable_list&& grads) override {
       const std::lock_guard<std::mutex> lock(mutex_);
       if (!grads[0].defined()) return variable_list(2);
+      no_tangent("the gradient of linear_cross_entropy", grads[0]);
       const Tensor wt = w.unpack();
       const c10::DeviceGuard guard(wt.device());
       const at::AutoDispatchBelowADInplaceOrView below;
@@ -377,6 +388,7 @@ PyObject* py_layer_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
   Tensor y;
   {
     const NoGil nogil;
+    no_tangent("layer_norm", x, w, b);
     if (at::GradMode::is_enabled() && (wanted(x) || wanted(w) || wanted(b))) {
       y = LayerNorm::forward(x, w, b, eps);
     } else {
@@ -399,6 +411,7 @@ PyObject* py_route(PyObject*, PyObject* const* a, Py_ssize_t n) {
   std::tuple<Tensor, Tensor> r;
   {
     const NoGil nogil;
+    no_tangent("route_tokens", z);
     if (at::GradMode::is_enabled() && wanted(z)) {
       r = Route::forward(z, bias, c);
     } else {
@@ -423,6 +436,7 @@ PyObject* py_linear_xent(PyObject*, PyObject* const* a, Py_ssize_t n) {
   Tensor loss;
   {
     const NoGil nogil;
+    no_tangent("linear_cross_entropy", x, weight);
     const Tensor w = fits ? weight : LinearXent::padded(weight);
     if (at::GradMode::is_enabled() && (wanted(x) || wanted(weight))) {
       loss = LinearXent::forward(x, weight, w, y, ignore, reduction);

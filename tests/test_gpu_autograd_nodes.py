@@ -143,3 +143,24 @@ def test_one_row_of_any_pitch(gpu_device):
     same(lambda x, w: linear_cross_entropy(x, w, y, reduction="none"), _row(gpu_device, 64, torch.bfloat16), w, up=one)
     x = torch.randn(1, 64, device=gpu_device).bfloat16()
     same(lambda x, w: linear_cross_entropy(x, w, y, reduction="none"), x, _row(gpu_device, 64, torch.bfloat16), up=one)
+
+
+@ALL
+def test_forward_mode_is_refused(gpu_device, make):
+    """a tangent that comes with an input, or with the incoming gradient, is not dropped without a word"""
+    import torch.autograd.forward_ad as fwd
+
+    ins, f = make(gpu_device)
+    up = torch.randn_like(f(*ins))
+    with fwd.dual_level():
+        for i in range(len(ins)):
+            for leaf in (ins[i], ins[i].detach()):
+                dual = [fwd.make_dual(leaf, torch.ones_like(leaf)) if j == i else t for j, t in enumerate(ins)]
+                with pytest.raises(NotImplementedError, match="forward mode"):
+                    f(*dual)
+                with torch.no_grad(), pytest.raises(NotImplementedError, match="forward mode"):
+                    f(*dual)
+        out = f(*ins)
+        with pytest.raises(NotImplementedError, match="forward mode"):
+            torch.autograd.grad(out, ins, fwd.make_dual(up, torch.ones_like(up)))
+    f(*ins).backward(up)  # and outside it they run again
