@@ -146,6 +146,7 @@ struct LayerNorm {
   struct Backward : Node {
     SavedVariable x, w, b;
     Tensor mr;
+    at::DimVector sizes;  // of x, which may be kept as a copy of its rows
 
     variable_list apply(variable_list&& grads) override {
       const std::lock_guard<std::mutex> lock(mutex_);
@@ -170,7 +171,7 @@ struct LayerNorm {
             abi.norm_backward(x2.data_ptr(), dtype_of(x2), T, H, x2.stride(0), d2.data_ptr(), d2.stride(0), m, m + T,
                               ptr(wt), weight_dtype(x2, wt, bt), ptr(dx), H, ptr(dw), ptr(db), ptr(ws), need,
                               stream_of(x2)));
-      if (dx.defined()) dx = shaped(dx, xt.sizes());
+      if (dx.defined()) dx = shaped(dx, sizes);
       return once({dx, dw, db});
     }
     void release_variables() override {
@@ -197,6 +198,7 @@ struct LayerNorm {
     node->w = SavedVariable(w, false);
     node->b = SavedVariable(b, false);
     node->mr = mr;
+    node->sizes = x.sizes();
     torch::autograd::set_history(y, node);
     return y;
   }
@@ -230,6 +232,7 @@ struct Route {
   struct Backward : Node {
     SavedVariable z, ids;
     RouteConfig c;
+    at::DimVector sizes;  // of the logits, which may be kept as a copy of their rows
 
     variable_list apply(variable_list&& grads) override {
       const std::lock_guard<std::mutex> lock(mutex_);
@@ -245,7 +248,7 @@ struct Route {
             abi.route_backward(z2.data_ptr(), dtype_of(z2), T, E, z2.stride(0), c.k, (int)c.sigmoid, (int)c.renorm,
                                (float)c.scale, it.data_ptr<int32_t>(), dw.data_ptr<float>(), dz.data_ptr(), E,
                                stream_of(z2)));
-      return once({shaped(dz, zt.sizes())});
+      return once({shaped(dz, sizes)});
     }
     void release_variables() override {
       const std::lock_guard<std::mutex> lock(mutex_);
@@ -267,6 +270,7 @@ struct Route {
     node->z = kept(logits, z);
     node->ids = SavedVariable(ids, false);
     node->c = c;
+    node->sizes = logits.sizes();
     torch::autograd::set_history(w, node);
     return {ids, w};
   }
@@ -304,7 +308,7 @@ struct LinearXent {
   struct Backward : Node {
     SavedVariable w;
     Tensor state;
-    std::vector<int64_t> sizes;  // of hidden
+    at::DimVector sizes;  // of hidden
     int64_t T, reduction;
 
     variable_list apply(variable_list&& grads) override {
@@ -347,7 +351,7 @@ struct LinearXent {
     auto node = make_node<Backward>(torch::autograd::collect_next_edges(hidden, weight));
     node->w = SavedVariable(w, false);
     node->state = state;
-    node->sizes = hidden.sizes().vec();
+    node->sizes = hidden.sizes();
     node->T = hidden.numel() / hidden.size(-1);
     node->reduction = reduction;
     torch::autograd::set_history(loss, node);

@@ -164,3 +164,22 @@ def test_forward_mode_is_refused(gpu_device, make):
         with pytest.raises(NotImplementedError, match="forward mode"):
             torch.autograd.grad(out, ins, fwd.make_dual(up, torch.ones_like(up)))
     f(*ins).backward(up)  # and outside it they run again
+
+
+@ALL
+@pytest.mark.parametrize("lead", [(5, 7), (3, 4, 2)])
+def test_leading_axes_in_another_order(gpu_device, make, lead):
+    """rows that no view puts one behind the other (the sequence in front of the batch, as a transposition leaves it):
+    gradients of the input's own shape, equal to those of its copy"""
+    ins, f = make(gpu_device, lead)
+    first = ins[0].detach().transpose(0, 1).contiguous().transpose(0, 1)
+    assert not first.is_contiguous() and torch.equal(first, ins[0].detach())
+    up = torch.randn_like(f(*ins))
+    turned = up.transpose(0, 1).contiguous().transpose(0, 1)
+    want = torch.autograd.grad(f(*ins), ins, up)
+    leaves = [first.requires_grad_(True), *ins[1:]]
+    out = f(*leaves)
+    assert torch.equal(out.detach(), f(*ins).detach())
+    for u in (up, turned):
+        for a, b in zip(torch.autograd.grad(out, leaves, u, retain_graph=True), want):
+            assert a.shape == b.shape and torch.equal(a, b)
