@@ -113,9 +113,41 @@ variable_list once(variable_list grads) {
   return grads;
 }
 
+// A tensor kept for the backward.  The kernels get its address, and saved-tensor
+// hooks may hand back anything: its place, type and sizes are looked at when it
+// comes back.  Its layout may be another.
+class Kept {
+ public:
+  Kept() = default;
+  explicit Kept(const Tensor& t) : v_(t, false) {
+    if (!t.defined()) return;
+    type_ = t.scalar_type();
+    device_ = t.device();
+    sizes_ = t.sizes();
+  }
+  Tensor unpack(const char* what) const {
+    const Tensor t = v_.unpack();
+    if (device_.is_cpu()) return t;  // undefined when it was kept
+    if (!t.defined() || t.device() != device_ || t.scalar_type() != type_ || t.sizes() != at::IntArrayRef(sizes_) ||
+        (t.numel() > 0 && !t.data_ptr()))
+      C10_THROW_ERROR(Error, std::string("the ") + what + " kept for the backward did not come back as they were: " +
+                                 (t.defined() ? t.toString() + c10::str(t.sizes(), " on ", t.device()) : "nothing") +
+                                 ", not " + c10::toString(type_) + c10::str(at::IntArrayRef(sizes_), " on ", device_));
+    return t;
+  }
+  void reset() { v_.reset_data(); }
+
+ private:
+  SavedVariable v_;
+  at::ScalarType type_ = at::kFloat;
+  at::Device device_ = at::kCPU;
+  at::DimVector sizes_;
+};
+
 // What the backward is to read of t: t itself, whose changes in place are then
 // noticed, where `used` (its rows) is a view of it, else the copy
-SavedVariable kept(const Tensor& t, const Tensor& used) { return SavedVariable(used.is_alias_of(t) ? t : used, false); }
+Kept kept(const Tensor& t, const Tensor& used) { return Kept(used.is_alias_of(t) ? t : used); }
+Tensor dense(const Tensor& t) { return t.defined() ? t.contiguous() : t; }
 
 // The nodes are torch's own kind, not its custom functions, whose context of named
 // values and wrapping of results take 3 us more of a router step's 51
@@ -144,7 +176,7 @@ struct LayerNorm {
   }
 
   struct Backward : Node {
-    SavedVariable x, w, b;
+    Kept x, w, b;
     Tensor mr;
     at::DimVector sizes;  // of x, which may be kept as a copy of its rows
 
@@ -152,10 +184,10 @@ struct LayerNorm {
       const std::lock_guard<std::mutex> lock(mutex_);
       if (!grads[0].defined()) return variable_list(3);
       no_tangent("the gradient of layer_norm", grads[0]);
-      const Tensor xt = x.unpack(), wt = w.unpack(), bt = b.unpack();
+      const Tensor xt = x.unpack("rows of x"), w0 = w.unpack("values of weight"), b0 = b.unpack("values of bias");
       const c10::DeviceGuard guard(xt.device());
       const at::AutoDispatchBelowADInplaceOrView below;
-      const Tensor x2 = rows_of(xt), d2 = rows_of(grads[0]);
+      const Tensor x2 = rows_of(xt), d2 = rows_of(grads[0]), wt = dense(w0), bt = dense(b0);
       const int64_t T = x2.size(0), H = x2.size(1);
       Tensor dx, dw, db, ws;
       if (task_should_compute_output(0)) dx = fresh({T, H}, x2.scalar_type(), x2);
@@ -176,9 +208,9 @@ struct LayerNorm {
     }
     void release_variables() override {
       const std::lock_guard<std::mutex> lock(mutex_);
-      x.reset_data();
-      w.reset_data();
-      b.reset_data();
+      x.reset();
+      w.reset();
+      b.reset();
       mr.reset();
     }
     std::string name() const override { return "LayerNormBackward"; }
@@ -195,8 +227,8 @@ struct LayerNorm {
     }
     auto node = make_node<Backward>(torch::autograd::collect_next_edges(x, w, b));
     node->x = kept(x, x2);
-    node->w = SavedVariable(w, false);
-    node->b = SavedVariable(b, false);
+    node->w = Kept(w);
+    node->b = Kept(b);
     node->mr = mr;
     node->sizes = x.sizes();
     torch::autograd::set_history(y, node);
@@ -230,7 +262,7 @@ struct Route {
   }
 
   struct Backward : Node {
-    SavedVariable z, ids;
+    Kept z, ids;
     RouteConfig c;
     at::DimVector sizes;  // of the logits, which may be kept as a copy of their rows
 
@@ -238,10 +270,10 @@ struct Route {
       const std::lock_guard<std::mutex> lock(mutex_);
       if (!grads[0].defined()) return variable_list(1);
       no_tangent("the gradient of route_tokens", grads[0]);
-      const Tensor zt = z.unpack(), it = ids.unpack();
+      const Tensor zt = z.unpack("logits"), i0 = ids.unpack("expert ids");
       const c10::DeviceGuard guard(zt.device());
       const at::AutoDispatchBelowADInplaceOrView below;
-      const Tensor z2 = rows_of(zt), dw = grads[0].contiguous();
+      const Tensor z2 = rows_of(zt), it = dense(i0), dw = grads[0].contiguous();
       const int64_t T = z2.size(0), E = z2.size(1);
       Tensor dz = fresh({T, E}, z2.scalar_type(), z2);
       check("ntlb_route_topk_backward",
@@ -252,8 +284,8 @@ struct Route {
     }
     void release_variables() override {
       const std::lock_guard<std::mutex> lock(mutex_);
-      z.reset_data();
-      ids.reset_data();
+      z.reset();
+      ids.reset();
     }
     std::string name() const override { return "RouteBackward"; }
   };
@@ -268,7 +300,7 @@ struct Route {
     }
     auto node = make_node<Backward>(torch::autograd::collect_next_edges(logits));
     node->z = kept(logits, z);
-    node->ids = SavedVariable(ids, false);
+    node->ids = Kept(ids);
     node->c = c;
     node->sizes = logits.sizes();
     torch::autograd::set_history(w, node);
@@ -278,8 +310,14 @@ struct Route {
 
 // ---------------------------------------------------------------------------
 struct LinearXent {
-  // weight in rows of whole 16-byte pieces
+  // whether weight lies in rows of whole 16-byte pieces
+  static bool fits(const Tensor& weight) {
+    return weight.stride(1) == 1 && weight.stride(0) % 8 == 0 && weight.size(1) % 8 == 0 &&
+           weight.stride(0) >= weight.size(1) && (uintptr_t)weight.data_ptr() % 16 == 0;
+  }
+  // weight in such rows: a copy where they are not
   static Tensor padded(const Tensor& weight) {
+    if (fits(weight)) return weight;
     const c10::DeviceGuard guard(weight.device());
     const at::AutoDispatchBelowADInplaceOrView below;
     const Tensor w = rows_of(weight);
@@ -306,7 +344,7 @@ struct LinearXent {
   }
 
   struct Backward : Node {
-    SavedVariable w;
+    Kept w;
     Tensor state;
     at::DimVector sizes;  // of hidden
     int64_t T, reduction;
@@ -315,9 +353,10 @@ struct LinearXent {
       const std::lock_guard<std::mutex> lock(mutex_);
       if (!grads[0].defined()) return variable_list(2);
       no_tangent("the gradient of linear_cross_entropy", grads[0]);
-      const Tensor wt = w.unpack();
-      const c10::DeviceGuard guard(wt.device());
+      const Tensor w0 = w.unpack("rows of weight");
+      const c10::DeviceGuard guard(w0.device());
       const at::AutoDispatchBelowADInplaceOrView below;
+      const Tensor wt = padded(w0);
       const int64_t H = sizes.back(), V = wt.size(0);
       const Tensor dl = grads[0].reshape({-1}).contiguous();
       Tensor dx, dw;
@@ -334,7 +373,7 @@ struct LinearXent {
     }
     void release_variables() override {
       const std::lock_guard<std::mutex> lock(mutex_);
-      w.reset_data();
+      w.reset();
       state.reset();
     }
     std::string name() const override { return "LinearXentBackward"; }
@@ -349,7 +388,7 @@ struct LinearXent {
       std::tie(loss, state) = run(rows_of(hidden), w, targets, ignore, reduction);
     }
     auto node = make_node<Backward>(torch::autograd::collect_next_edges(hidden, weight));
-    node->w = SavedVariable(w, false);
+    node->w = Kept(w);
     node->state = state;
     node->sizes = hidden.sizes();
     node->T = hidden.numel() / hidden.size(-1);
@@ -430,18 +469,17 @@ PyObject* py_route(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// linear_xent(hidden, weight, whether it is in 16-byte rows, targets, ignore_index, reduction)
+// linear_xent(hidden, weight, targets, ignore_index, reduction)
 PyObject* py_linear_xent(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  count(n, 6);
-  const Tensor &x = THPVariable_Unpack(a[0]), &weight = THPVariable_Unpack(a[1]), &y = THPVariable_Unpack(a[3]);
-  const bool fits = a[2] == Py_True;
-  const int64_t ignore = integer(a[4]), reduction = integer(a[5]);
+  count(n, 5);
+  const Tensor &x = THPVariable_Unpack(a[0]), &weight = THPVariable_Unpack(a[1]), &y = THPVariable_Unpack(a[2]);
+  const int64_t ignore = integer(a[3]), reduction = integer(a[4]);
   Tensor loss;
   {
     const NoGil nogil;
     no_tangent("linear_cross_entropy", x, weight);
-    const Tensor w = fits ? weight : LinearXent::padded(weight);
+    const Tensor w = LinearXent::padded(weight);
     if (at::GradMode::is_enabled() && (wanted(x) || wanted(weight))) {
       loss = LinearXent::forward(x, weight, w, y, ignore, reduction);
     } else {

@@ -48,9 +48,7 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: to
         raise ValueError(f"targets must be {tuple(hidden.shape[:-1])}, not {tuple(targets.shape)}")
     if not (hidden.device == weight.device == targets.device):
         raise ValueError(f"hidden, weight and targets are on {hidden.device}, {weight.device} and {targets.device}")
-    fits = weight.stride(1) == 1 and weight.stride(0) % 8 == 0 and weight.shape[1] % 8 == 0 and \
-        weight.data_ptr() % 16 == 0 and weight.stride(0) >= weight.shape[1]
-    return (_lib._autograd or _lib.autograd()).linear_xent(hidden, weight, fits, targets, ignore_index,
+    return (_lib._autograd or _lib.autograd()).linear_xent(hidden, weight, targets, ignore_index,
                                                            _REDUCTIONS[reduction])
 
 

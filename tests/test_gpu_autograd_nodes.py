@@ -183,3 +183,48 @@ def test_leading_axes_in_another_order(gpu_device, make, lead):
     for u in (up, turned):
         for a, b in zip(torch.autograd.grad(out, leaves, u, retain_graph=True), want):
             assert a.shape == b.shape and torch.equal(a, b)
+
+
+@ALL
+@pytest.mark.parametrize("which", ["host", "type", "shorter", "nothing"])
+def test_other_tensors_than_those_kept_are_refused(gpu_device, make, which):
+    """the kernels take the kept tensors by address: what saved-tensor hooks hand back is looked at first"""
+    change = {"host": lambda t: t.cpu(), "type": lambda t: t.to(torch.float64), "shorter": lambda t: t[:-1],
+              "nothing": lambda t: t.new_empty(0)}[which]
+    ins, f = make(gpu_device)
+    up = torch.randn_like(f(*ins))
+    kinds = []
+
+    def pack(t):
+        kinds.append(t.dtype)
+        return t
+
+    with torch.autograd.graph.saved_tensors_hooks(pack, lambda t: t):
+        f(*ins)
+    for n in range(len(kinds)):
+        seen = []
+
+        def nth(t):
+            seen.append(t)
+            return len(seen) - 1
+
+        with torch.autograd.graph.saved_tensors_hooks(nth, lambda i: change(seen[i]) if i == n else seen[i]):
+            out = f(*ins)
+        with pytest.raises(RuntimeError, match="kept for the backward"):
+            torch.autograd.grad(out, ins, up)
+
+
+@ALL
+def test_kept_tensors_may_come_back_in_another_layout(gpu_device, make):
+    ins, f = make(gpu_device)
+    up = torch.randn_like(f(*ins))
+    want = torch.autograd.grad(f(*ins), ins, up)
+
+    def spread(t):  # every element behind an unused one
+        wide = torch.full((*t.shape, 2), 7, dtype=t.dtype, device=t.device)
+        wide[..., 1] = t
+        return wide[..., 1]
+
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, spread):
+        out = f(*ins)
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(out, ins, up), want))
