@@ -176,15 +176,15 @@ struct LayerNorm {
   }
 
   struct Backward : Node {
-    Kept x, w, b;
-    Tensor mr;
+    Kept x, w, b, mr;
     at::DimVector sizes;  // of x, which may be kept as a copy of its rows
 
     variable_list apply(variable_list&& grads) override {
       const std::lock_guard<std::mutex> lock(mutex_);
       if (!grads[0].defined()) return variable_list(3);
       no_tangent("the gradient of layer_norm", grads[0]);
-      const Tensor xt = x.unpack("rows of x"), w0 = w.unpack("values of weight"), b0 = b.unpack("values of bias");
+      const Tensor xt = x.unpack("rows of x"), w0 = w.unpack("values of weight"), b0 = b.unpack("values of bias"),
+                   r0 = mr.unpack("rows' means and deviations");
       const c10::DeviceGuard guard(xt.device());
       const at::AutoDispatchBelowADInplaceOrView below;
       const Tensor x2 = rows_of(xt), d2 = rows_of(grads[0]), wt = dense(w0), bt = dense(b0);
@@ -198,7 +198,8 @@ struct LayerNorm {
         need = abi.norm_workspace(dtype_of(x2), T, H);
         ws = scratch(need, x2);
       }
-      const float* m = mr.data_ptr<float>();
+      const Tensor stats = dense(r0);
+      const float* m = stats.data_ptr<float>();
       check("ntlb_layer_norm_backward",
             abi.norm_backward(x2.data_ptr(), dtype_of(x2), T, H, x2.stride(0), d2.data_ptr(), d2.stride(0), m, m + T,
                               ptr(wt), weight_dtype(x2, wt, bt), ptr(dx), H, ptr(dw), ptr(db), ptr(ws), need,
@@ -229,7 +230,7 @@ struct LayerNorm {
     node->x = kept(x, x2);
     node->w = Kept(w);
     node->b = Kept(b);
-    node->mr = mr;
+    node->mr = Kept(mr);
     node->sizes = x.sizes();
     torch::autograd::set_history(y, node);
     return y;
@@ -343,9 +344,14 @@ struct LinearXent {
     return {reduction ? loss.reshape({}) : shaped(T ? loss : loss.slice(0, 0, 0), targets.sizes()), state};
   }
 
+  // the forward's state as the backward takes it
+  static Tensor aligned(const Tensor& state) {
+    const Tensor s = dense(state);
+    return (uintptr_t)s.data_ptr() % 256 == 0 ? s : s.clone();
+  }
+
   struct Backward : Node {
-    Kept w;
-    Tensor state;
+    Kept w, state;
     at::DimVector sizes;  // of hidden
     int64_t T, reduction;
 
@@ -353,10 +359,10 @@ struct LinearXent {
       const std::lock_guard<std::mutex> lock(mutex_);
       if (!grads[0].defined()) return variable_list(2);
       no_tangent("the gradient of linear_cross_entropy", grads[0]);
-      const Tensor w0 = w.unpack("rows of weight");
+      const Tensor w0 = w.unpack("rows of weight"), s0 = state.unpack("live rows of hidden");
       const c10::DeviceGuard guard(w0.device());
       const at::AutoDispatchBelowADInplaceOrView below;
-      const Tensor wt = padded(w0);
+      const Tensor wt = padded(w0), st = aligned(s0);
       const int64_t H = sizes.back(), V = wt.size(0);
       const Tensor dl = grads[0].reshape({-1}).contiguous();
       Tensor dx, dw;
@@ -365,7 +371,7 @@ struct LinearXent {
       const int64_t need = abi.xent_workspace(std::max<int64_t>(T, 1), H, V, 1);
       const Tensor ws = scratch(need, wt);
       check("ntlb_linear_xent_backward",
-            abi.xent_backward(state.data_ptr(), (const uint16_t*)wt.data_ptr(), wt.stride(0), T, H, V, (int)reduction,
+            abi.xent_backward(st.data_ptr(), (const uint16_t*)wt.data_ptr(), wt.stride(0), T, H, V, (int)reduction,
                               dl.data_ptr<float>(), (uint16_t*)ptr(dx), H, (uint16_t*)ptr(dw), H, ws.data_ptr(), need,
                               stream_of(wt)));
       if (dx.defined()) dx = shaped(dx, sizes);
@@ -389,7 +395,7 @@ struct LinearXent {
     }
     auto node = make_node<Backward>(torch::autograd::collect_next_edges(hidden, weight));
     node->w = Kept(w);
-    node->state = state;
+    node->state = Kept(state);
     node->sizes = hidden.sizes();
     node->T = hidden.numel() / hidden.size(-1);
     node->reduction = reduction;

@@ -228,3 +228,40 @@ def test_kept_tensors_may_come_back_in_another_layout(gpu_device, make):
     with torch.autograd.graph.saved_tensors_hooks(lambda t: t, spread):
         out = f(*ins)
     assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(out, ins, up), want))
+
+
+@ALL
+def test_what_the_backward_reads_passes_the_hooks(gpu_device, make):
+    """saved-tensor hooks see all that a node keeps, and it may have been elsewhere in between"""
+    ins, f = make(gpu_device, (700,))
+    up = torch.randn_like(f(*ins))
+    want = torch.autograd.grad(f(*ins), ins, up)
+    kept = []
+
+    def pack(t):
+        kept.append(t.numel() * t.element_size())
+        return t.cpu()
+
+    with torch.autograd.graph.saved_tensors_hooks(pack, lambda t: t.to(gpu_device)):
+        out = f(*ins)
+    got = torch.autograd.grad(out, ins, up)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    # norm: x, weight, bias and two numbers a row; routing: logits and ids; head: weight and the live rows with their numbers
+    least = {_norm: 700 * 40 * 4 + 2 * 40 * 4 + 700 * 8, _route: 700 * 20 * 4 + 700 * 4 * 4, _xent: 90 * 40 * 2 + 700 * 64 * 2}
+    assert sum(kept) >= least[make]
+
+
+def test_a_checkpoint_keeps_no_hidden_rows(gpu_device):
+    """recomputed in the backward, the head loss holds nothing of the rows' size until then"""
+    from torch.utils.checkpoint import checkpoint
+
+    from lowbit.loss import linear_cross_entropy
+
+    x = torch.randn(4096, 1024, device=gpu_device).bfloat16().requires_grad_(True)
+    w = torch.randn(64, 1024, device=gpu_device).bfloat16().requires_grad_(True)
+    y = torch.randint(0, 64, (4096,), device=gpu_device)
+    want = torch.autograd.grad(linear_cross_entropy(x, w, y), (x, w))
+    before = torch.cuda.memory_allocated()
+    loss = checkpoint(linear_cross_entropy, x, w, y, use_reentrant=False)
+    assert torch.cuda.memory_allocated() - before < 1 << 20
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(loss, (x, w)), want))
