@@ -368,7 +368,7 @@ struct LinearXent {
       Tensor dx, dw;
       if (task_should_compute_output(0)) dx = fresh({T, H}, wt.scalar_type(), wt);
       if (task_should_compute_output(1)) dw = fresh({V, H}, wt.scalar_type(), wt);
-      const int64_t need = abi.xent_workspace(std::max<int64_t>(T, 1), H, V, 1);
+      const int64_t need = abi.xent_workspace(T, H, V, 1);
       const Tensor ws = scratch(need, wt);
       check("ntlb_linear_xent_backward",
             abi.xent_backward(st.data_ptr(), (const uint16_t*)wt.data_ptr(), wt.stride(0), T, H, V, (int)reduction,

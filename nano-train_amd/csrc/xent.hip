@@ -1184,11 +1184,14 @@ extern "C" int ntlb_pad_rows(const uint16_t* x, int64_t ldx, int64_t R, int64_t 
   return check_launch(fn);
 }
 
-extern "C" int64_t ntlb_linear_xent_state_bytes(int64_t T, int64_t H) { return T < 1 || H < 1 ? 256 : xent::state_of(T, H).bytes; }
+// An empty batch leaves the state of one row, none of it live, and its dW (zero) goes
+// through the same product
+extern "C" int64_t ntlb_linear_xent_state_bytes(int64_t T, int64_t H) { return T < 0 || H < 1 ? 0 : xent::state_of(std::max<int64_t>(T, 1), H).bytes; }
 
 extern "C" int64_t ntlb_linear_xent_workspace_bytes(int64_t T, int64_t H, int64_t V, int backward) {
-  if (T < 1 || H < 1 || V < 1) return 0;
-  return backward ? xent::plan_of(T, H, V).bytes : xent::forward_ws(T, H, V);
+  if (T < 0 || H < 1 || V < 1) return 0;
+  if (backward) return xent::plan_of(std::max<int64_t>(T, 1), H, V).bytes;
+  return T > 0 ? xent::forward_ws(T, H, V) : 0;
 }
 
 extern "C" int ntlb_linear_xent_forward(const uint16_t* x, int64_t ldx, const uint16_t* w, int64_t ldw,

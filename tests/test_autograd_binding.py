@@ -99,3 +99,17 @@ def test_entry_points_validate_without_gpu():
     need = L.ntlb_linear_xent_workspace_bytes(8, 64, 100, 1)
     assert xb(P, P, 64, 8, 64, 100, 2, P, P, 60, P, 64, P, need, None) == E
     assert xb(P, P, 64, 8, 64, 100, 2, P, P, 64, P, 64, P, need - 1, None) == E
+
+
+def test_an_empty_batch_has_the_sizes_of_one_row():
+    """the head loss's forward lays out one row of state where there is none, and its backward that row's workspace: the
+    sizes named for an empty batch hold them"""
+    from lowbit import _lib
+
+    L = _lib.lib()
+    for H in (1, 64, 72, 7168):
+        assert L.ntlb_linear_xent_state_bytes(0, H) == L.ntlb_linear_xent_state_bytes(1, H) > 256
+        for V in (1, 300, 131072):
+            assert L.ntlb_linear_xent_workspace_bytes(0, H, V, 1) == L.ntlb_linear_xent_workspace_bytes(1, H, V, 1) > 0
+            assert L.ntlb_linear_xent_workspace_bytes(0, H, V, 0) == 0
+    assert L.ntlb_linear_xent_state_bytes(-1, 64) == L.ntlb_linear_xent_workspace_bytes(-1, 64, 64, 1) == 0

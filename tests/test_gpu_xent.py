@@ -520,3 +520,23 @@ def test_incoming_gradients_that_are_no_numbers(gpu_device, T, bad, others):
     if not rows.any():
         assert xl.grad.isfinite().all() and wl.grad.isfinite().all()
         assert others == "one" or not (xl.grad.any() or wl.grad.any())
+
+
+@pytest.mark.parametrize("H", [64, 1000])
+def test_an_empty_batch_stays_inside_its_state(gpu_device, H):
+    from lowbit import _lib
+
+    V = 300
+    L = _lib.lib()
+    nb, nw = L.ntlb_linear_xent_state_bytes(0, H), L.ntlb_linear_xent_workspace_bytes(0, H, V, 1)
+    state = torch.full((nb + 65536,), 255, dtype=torch.uint8, device=gpu_device)
+    ws = torch.full((nw + 65536,), 255, dtype=torch.uint8, device=gpu_device)
+    w, dw = torch.randn(V, H, device=gpu_device).bfloat16(), torch.full((V, H), 7.0, device=gpu_device).bfloat16()
+    loss, dl = torch.ones(1, device=gpu_device), torch.ones(1, device=gpu_device)
+    s = torch.cuda.current_stream().cuda_stream
+    _lib.call("ntlb_linear_xent_forward", None, H, w.data_ptr(), H, None, 1, 0, H, V, IGNORE, 2, loss.data_ptr(),
+              state.data_ptr(), ws.data_ptr(), 0, s)
+    _lib.call("ntlb_linear_xent_backward", state.data_ptr(), w.data_ptr(), H, 0, H, V, 2, dl.data_ptr(), None, H, dw.data_ptr(), H,
+              ws.data_ptr(), nw, s)
+    assert float(loss) == 0 and not dw.any()
+    assert (state[nb:] == 255).all() and (ws[nw:] == 255).all()
