@@ -322,12 +322,15 @@ constexpr int EPI_LSE = 0, EPI_DZ = 1, EPI_ACC = 2, EPI_STORE = 3;
 
 // The gradient that comes in: du[0] for all rows, over the number of live rows
 // if mean; or, `most` given, du[t] for row t, their common factor most[0], which is
-// 0 only if all are
+// 0 only if all are.  With no live row nothing comes in: du is not read (of an empty
+// batch it may be NULL).
 struct Up {
   const float* du;
   const float* most;
   int mean;
-  __device__ float common(int live) const { return most ? most[0] : du[0] * (mean ? 1.0f / (float)max(live, 1) : 1.0f); }
+  __device__ float common(int live) const {
+    return live == 0 ? 0.f : most ? most[0] : du[0] * (mean ? 1.0f / (float)live : 1.0f);
+  }
   __device__ float rest(int row, float c) const { return !most ? 1.0f : c == 0.f ? 0.f : du[row] / c; }
 };
 

@@ -540,3 +540,36 @@ def test_an_empty_batch_stays_inside_its_state(gpu_device, H):
               ws.data_ptr(), nw, s)
     assert float(loss) == 0 and not dw.any()
     assert (state[nb:] == 255).all() and (ws[nw:] == 255).all()
+
+
+@pytest.mark.parametrize("reduction", [0, 1, 2])
+def test_an_empty_batch_reads_no_incoming_gradient(gpu_device, reduction):
+    from lowbit import _lib
+
+    H, V = 72, 300
+    L = _lib.lib()
+    new = lambda n: torch.full((n,), 255, dtype=torch.uint8, device=gpu_device)  # noqa: E731
+    w, dw = torch.randn(V, H, device=gpu_device).bfloat16(), torch.full((V, H), 7.0, device=gpu_device).bfloat16()
+    state, ws = new(L.ntlb_linear_xent_state_bytes(0, H)), new(L.ntlb_linear_xent_workspace_bytes(1, H, V, 1))
+    loss = torch.ones(1, device=gpu_device)
+    s = torch.cuda.current_stream().cuda_stream
+    _lib.call("ntlb_linear_xent_forward", None, H, w.data_ptr(), H, None, 1, 0, H, V, IGNORE, reduction, loss.data_ptr(),
+              state.data_ptr(), ws.data_ptr(), ws.numel(), s)
+    _lib.call("ntlb_linear_xent_backward", state.data_ptr(), w.data_ptr(), H, 0, H, V, reduction, None, None, H, dw.data_ptr(), H,
+              ws.data_ptr(), ws.numel(), s)
+    assert not dw.any() and (reduction == 0 or float(loss) == 0)
+
+
+@pytest.mark.parametrize("T", [3, 64, 200])
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+def test_no_live_position_passes_nothing_on(gpu_device, T, reduction):
+    """all ignored: zero gradients, whatever the incoming one"""
+    from lowbit.loss import linear_cross_entropy
+
+    x, w, y, _ = _inputs(T, 64, 300, 41, gpu_device)
+    y[:] = IGNORE
+    for up in (float("nan"), float("inf")):
+        xl, wl = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+        loss = linear_cross_entropy(xl, wl, y, reduction=reduction)
+        dx, dw = torch.autograd.grad(loss, (xl, wl), torch.full_like(loss, up))
+        assert not dx.any() and not dw.any()
