@@ -646,6 +646,16 @@ __device__ __forceinline__ void head_tile(Args g, int pid, uint8_t* la0, uint8_t
           for (int r = 0; r < 4; ++r)
             if (tn * 16 + r >= cols) acc[tm][tn][r] = 0.f;
       }
+      // rows past the live ones: zero times a word's infinity is NaN, which no factor
+      // of 0 takes out
+      const bool past = mw + tm * 16 >= g.M;
+      if (__any(past)) {
+#pragma unroll
+        for (int tn = 0; tn < 4; ++tn)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (past) acc[tm][tn][r] = 0.f;
+      }
     }
     const int64_t block = n0 / 64 + wn;
     const bool rest = D == 128 && g.half;  // (up to 64 rows always take the small tiles)

@@ -573,3 +573,22 @@ def test_no_live_position_passes_nothing_on(gpu_device, T, reduction):
         loss = linear_cross_entropy(xl, wl, y, reduction=reduction)
         dx, dw = torch.autograd.grad(loss, (xl, wl), torch.full_like(loss, up))
         assert not dx.any() and not dw.any()
+
+
+@pytest.mark.parametrize("T", [5, 40, 64, 70, 300])
+@pytest.mark.parametrize("which", ["weight", "both"])
+def test_words_without_probability_take_no_gradient(gpu_device, T, which):
+    """positive hidden rows and words of -inf: their logits are -inf and their p is 0, so their rows of dW are 0 (dX, a sum
+    with 0 times -inf, is NaN by definition), whatever fills the tiles' rows past the live ones"""
+    from lowbit.loss import linear_cross_entropy
+
+    x, w, y, _ = _inputs(T, 96, 700, 51, gpu_device, 0.2 if T > 5 else 0.0)
+    x = x.abs() + 2.0 ** -6
+    y = torch.where(y == IGNORE, y, y % 400 + 300)
+    wf = w[300:].clone()
+    w[:300] = -float("inf")
+    xl, wl = x.clone().requires_grad_(which == "both"), w.clone().requires_grad_(True)
+    loss = linear_cross_entropy(xl, wl, y)
+    loss.backward()
+    assert not wl.grad[:300].any()
+    _check(x, wf, torch.where(y == IGNORE, y, y - 300), loss.detach(), None, wl.grad[300:], "mean", torch.ones((), device=gpu_device))
