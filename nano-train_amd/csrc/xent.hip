@@ -66,7 +66,7 @@ typedef uint32_t u32x4_2 __attribute__((ext_vector_type(4), aligned(2)));
 typedef uint32_t u32x2_2 __attribute__((ext_vector_type(2), aligned(2)));
 
 constexpr int ROWB = 128, KSTEP = 64;  // bytes and values of a row's K step
-constexpr float LOG2E = 1.44269502e+00f, LN2 = 6.93147182e-01f;
+constexpr float LOG2E = 1.44269502e+00f;
 
 // LDS stages and fragments as in gemm_dq.hip: row-major [256][128 bytes] with
 // 16-byte chunks XOR-swizzled by row, or [64 contraction rows][256] as stored,
@@ -344,13 +344,13 @@ struct Args {
   uint32_t* count;      // ... of each divided tile, how many are there (0 before and after)
   int group_m;          // raster: row tiles side by side
   // LSE
-  float2* part;         // [column tiles][ldp] (ref, sum)
+  float2* part;         // [column tiles][ldp] (largest, sum)
   int64_t ldp;
   float* zl;            // [M] the label's logit
   const int32_t* y;     // labels of the live rows, < 0: none
   int64_t v0;           // first column's place in the vocabulary
   // DZ
-  const float* lse;
+  const float2* stat;   // [M] (largest logit, log2 of the sum)
   const int32_t* rows;
   Up up;
   int half;             // DZ: the row that the rest of row 0's values goes to, or 0
@@ -363,12 +363,15 @@ struct Args {
   int add;              // ACC: add to what is there
 };
 
-// A set of logits z: the largest z log2(e), ref, and the sum of 2^(z log2(e) - ref).
-// Rounded once, ref is the same number for whoever adds to the sum, so its
-// rounding costs nothing.
-__device__ __forceinline__ float2 merge(float2 a, float2 b) {
-  const float hi = fmaxf(a.x, b.x), ref = hi == -__builtin_inff() ? 0.f : hi;
-  return make_float2(hi, a.y * __builtin_amdgcn_exp2f(a.x - ref) + b.y * __builtin_amdgcn_exp2f(b.x - ref));
+// A set of logits z: the largest of them and the sum of exp(z - largest).  A row
+// keeps both to the end: one rounded logsumexp would be off by a unit of itself, and
+// with it a confident row's loss and p - 1, which are far smaller.  The largest
+// itself adds exactly 1.
+template <typename T>
+__device__ __forceinline__ void merge(float& ax, T& ay, float bx, T by) {
+  const float hi = fmaxf(ax, bx), ref = hi == -__builtin_inff() ? 0.f : hi;
+  ay = ay * (T)__builtin_amdgcn_exp2f((ax - ref) * LOG2E) + by * (T)__builtin_amdgcn_exp2f((bx - ref) * LOG2E);
+  ax = hi;
 }
 
 // Where the small tiles of z are too few for the chip, a tile's contraction is
@@ -593,13 +596,13 @@ __device__ __forceinline__ void head_tile(Args g, int pid, uint8_t* la0, uint8_t
 #pragma unroll
         for (int r = 0; r < 4; ++r) mx = fmaxf(mx, acc[tm][tn][r]);
       mx = fmaxf(mx, __shfl_xor(mx, 16));
-      mx = fmaxf(mx, __shfl_xor(mx, 32)) * LOG2E;
+      mx = fmaxf(mx, __shfl_xor(mx, 32));
       const float ref = mx == -__builtin_inff() ? 0.f : mx;
       float s = 0.f;
 #pragma unroll
       for (int tn = 0; tn < 4; ++tn)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) s += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[tm][tn][r], LOG2E, -ref));
+        for (int r = 0; r < 4; ++r) s += __builtin_amdgcn_exp2f((acc[tm][tn][r] - ref) * LOG2E);
       s += __shfl_xor(s, 16);
       s += __shfl_xor(s, 32);
       if (lane < 16) red[wn * D + wm * 16 * MT + tm * 16 + lane] = make_float2(mx, s);
@@ -608,12 +611,12 @@ __device__ __forceinline__ void head_tile(Args g, int pid, uint8_t* la0, uint8_t
     if (tid < D && m0 + tid < g.M) {
       float2 t = red[tid];
 #pragma unroll
-      for (int i = 1; i < WAVES_N; ++i) t = merge(t, red[i * D + tid]);
+      for (int i = 1; i < WAVES_N; ++i) merge(t.x, t.y, red[i * D + tid].x, red[i * D + tid].y);
       g.part[(n0 / TN) * g.ldp + m0 + tid] = t;
     }
   } else if constexpr (EPI == EPI_DZ) {
     const float c = g.up.common(live);
-    float lse[MT], u[MT];
+    float top[MT], sum[MT], u[MT];
     int lab[MT];
     // dz's rows up to the next 64 are read, zero past the live ones; so are whole
     // blocks, zero past the piece
@@ -621,7 +624,9 @@ __device__ __forceinline__ void head_tile(Args g, int pid, uint8_t* la0, uint8_t
     for (int tm = 0; tm < MT; ++tm) {
       const bool on = mw + tm * 16 < g.M;
       const int64_t m = on ? mw + tm * 16 : 0;
-      lse[tm] = on ? g.lse[m] * LOG2E : __builtin_inff();
+      const float2 st = g.stat[m];
+      top[tm] = on ? st.x : 0.f;
+      sum[tm] = on ? st.y : __builtin_inff();
       u[tm] = on ? g.up.rest(g.rows[m], c) : 0.f;
       lab[tm] = on ? (int)(g.y[m] - g.v0 - nw) : -1;
     }
@@ -631,7 +636,7 @@ __device__ __forceinline__ void head_tile(Args g, int pid, uint8_t* la0, uint8_t
       for (int tn = 0; tn < 4; ++tn)
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-          acc[tm][tn][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[tm][tn][r], LOG2E, -lse[tm]));
+          acc[tm][tn][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[tm][tn][r] - top[tm], LOG2E, -sum[tm]));
       if (__any(lab[tm] >= 0 && lab[tm] < 64)) {
 #pragma unroll
         for (int tn = 0; tn < 4; ++tn)
@@ -857,38 +862,44 @@ __global__ void __launch_bounds__(256) gather_kernel(const uint16_t* x, int64_t 
   }
 }
 
-// lse and loss of the live rows from their pairs, R rows by Q walkers; TOTAL: of
+// The live rows' pairs joined, and their losses, by R rows and Q walkers; TOTAL: of
 // all rows, in one workgroup, and then their sum or mean in a fixed order (0 where
-// none is live)
+// none is live).  Sums are 64 bits here: of a confident row's, each addition to the
+// 1 of its largest logit would otherwise round what the others add.
 template <int R, int Q, bool TOTAL>
 __global__ void __launch_bounds__(R * Q) join_kernel(const float2* part, int64_t ldp, int64_t parts, const float* zl,
-                                                     const int32_t* rows, const int32_t* live, int mean, float* lse,
+                                                     const int32_t* rows, const int32_t* live, int mean, float2* stat,
                                                      float* each, float* loss) {
   constexpr int WAVES = R * Q / 64;
-  __shared__ float2 red[WAVES][R];
+  __shared__ float red_top[WAVES][R];
+  __shared__ double red_sum[WAVES][R];
   __shared__ float losses[R];
   const int tid = threadIdx.x, r = tid % R, q = tid / R, n = live[0];
   const int64_t m = (int64_t)blockIdx.x * R + r;
   const bool on = m < n;
-  float2 p = make_float2(-__builtin_inff(), 0.f);
+  float top = -__builtin_inff();
+  double sum = 0.0;
   if (on)
 #pragma unroll 4
-    for (int64_t i = q; i < parts; i += Q) p = merge(p, part[i * ldp + m]);
+    for (int64_t i = q; i < parts; i += Q) merge<double>(top, sum, part[i * ldp + m].x, part[i * ldp + m].y);
 #pragma unroll
-  for (int d = R; d < 64; d *= 2) p = merge(p, make_float2(__shfl_xor(p.x, d), __shfl_xor(p.y, d)));
-  if ((tid & 63) < R) red[tid >> 6][r] = p;
+  for (int d = R; d < 64; d *= 2) merge<double>(top, sum, __shfl_xor(top, d), __shfl_xor(sum, d));
+  if ((tid & 63) < R) {
+    red_top[tid >> 6][r] = top;
+    red_sum[tid >> 6][r] = sum;
+  }
   __syncthreads();
   if (q == 0 && on) {
 #pragma unroll
-    for (int i = 1; i < WAVES; ++i) p = merge(p, red[i][r]);
-    const float ref = p.x == -__builtin_inff() ? 0.f : p.x;
-    const float l = (ref + __builtin_amdgcn_logf(p.y)) * LN2, z = zl[m];
-    lse[m] = z != z ? z : l;  // no such word, or its logit is NaN: so is all of the row
+    for (int i = 1; i < WAVES; ++i) merge<double>(top, sum, red_top[i][r], red_sum[i][r]);
+    const float z = zl[m], log_sum = log1pf((float)(sum - 1.0));
+    stat[m] = make_float2(top, z != z ? z : log_sum * LOG2E);  // no such word, or its logit is NaN: so is all of the row
+    const float l = log_sum + (top - z);
     if constexpr (TOTAL) {
-      losses[r] = l - z;
+      losses[r] = l;
     } else {
-      each[m] = l - z;
-      if (loss) loss[rows[m]] = l - z;
+      each[m] = l;
+      if (loss) loss[rows[m]] = l;
     }
   }
   if constexpr (TOTAL) {
@@ -986,7 +997,7 @@ static int64_t block_of(int64_t T) { return half_of(T) ? 2 * half_of(T) * 64 : c
 // what the forward leaves for the backward
 struct State {
   int64_t hk, block;  // columns of X', whole blocks; elements of one
-  int64_t xp, pos, rows, y, lse, live, bytes;
+  int64_t xp, pos, rows, y, stat, live, bytes;
 };
 static State state_of(int64_t T, int64_t H) {
   State s;
@@ -997,8 +1008,8 @@ static State state_of(int64_t T, int64_t H) {
   s.pos = up(s.hk / 64 * s.block * 2);
   s.rows = s.pos + up(T * 4);
   s.y = s.rows + up(T * 4);
-  s.lse = s.y + up(T * 4);
-  s.live = s.lse + up(T * 4);
+  s.stat = s.y + up(T * 4);
+  s.live = s.stat + up(T * 8);
   s.bytes = s.live + 256;
   return s;
 }
@@ -1224,7 +1235,7 @@ extern "C" int ntlb_linear_xent_forward(const uint16_t* x, int64_t ldx, const ui
   uint8_t* sp = (uint8_t*)state;
   const xent::Targets tg{targets, targets64, T, V, ignore_index};
   const xent::Live o{(int32_t*)(sp + s.pos), (int32_t*)(sp + s.rows), (int32_t*)(sp + s.y), (int32_t*)(sp + s.live)};
-  float* lse = (float*)(sp + s.lse);
+  float2* stat = (float2*)(sp + s.stat);
   uint16_t* xp = (uint16_t*)(sp + s.xp);
   const int64_t parts = T > 0 ? xent::forward_parts(T, V) : 0;
   float2* part = (float2*)workspace;
@@ -1251,14 +1262,14 @@ extern "C" int ntlb_linear_xent_forward(const uint16_t* x, int64_t ldx, const ui
   // up to 64 rows one workgroup does it all; many pairs of few rows: more walkers to
   // a row (16 rows of 1024 pairs: 5.6 us, by 16 walkers 27; 4096 rows of 256: 8.5 and 6.7)
   if (reduction != 0 && T <= 16)
-    xent::join_kernel<16, 64, true><<<1, 1024, 0, st>>>(part, T, parts, zl, o.rows, o.live, mean, lse, nullptr, loss);
+    xent::join_kernel<16, 64, true><<<1, 1024, 0, st>>>(part, T, parts, zl, o.rows, o.live, mean, stat, nullptr, loss);
   else if (reduction != 0 && T <= 64 && parts <= 256)
-    xent::join_kernel<64, 16, true><<<1, 1024, 0, st>>>(part, T, parts, zl, o.rows, o.live, mean, lse, nullptr, loss);
+    xent::join_kernel<64, 16, true><<<1, 1024, 0, st>>>(part, T, parts, zl, o.rows, o.live, mean, stat, nullptr, loss);
   else if (T > 0) {
     if (parts > 128 && T <= 1024)
-      xent::join_kernel<4, 256, false><<<(unsigned)cdiv(T, 4), 1024, 0, st>>>(part, T, parts, zl, o.rows, o.live, mean, lse, each, rows_loss);
+      xent::join_kernel<4, 256, false><<<(unsigned)cdiv(T, 4), 1024, 0, st>>>(part, T, parts, zl, o.rows, o.live, mean, stat, each, rows_loss);
     else
-      xent::join_kernel<16, 16, false><<<(unsigned)cdiv(T, 16), 256, 0, st>>>(part, T, parts, zl, o.rows, o.live, mean, lse, each, rows_loss);
+      xent::join_kernel<16, 16, false><<<(unsigned)cdiv(T, 16), 256, 0, st>>>(part, T, parts, zl, o.rows, o.live, mean, stat, each, rows_loss);
     if (reduction != 0) xent::total_kernel<<<1, 1024, 0, st>>>(each, o.live, mean, loss);
   }
   return check_launch(fn);
@@ -1296,7 +1307,7 @@ extern "C" int ntlb_linear_xent_backward(const void* state, const uint16_t* w, i
     g.live = live; g.group_m = 8;
     g.a = {sp + s.xp, s.block * 2, Tn, s.hk};
     g.b = {wp, ldw * 2, n, H};
-    g.M = T; g.N = n; g.y = (const int32_t*)(sp + s.y); g.v0 = v0; g.lse = (const float*)(sp + s.lse);
+    g.M = T; g.N = n; g.y = (const int32_t*)(sp + s.y); g.v0 = v0; g.stat = (const float2*)(sp + s.stat);
     g.rows = (const int32_t*)(sp + s.rows); g.up = up;
     g.out = dz; g.ldo = p.block; g.cols = np;
     // (the last piece may have fewer tiles than the others' base, or fewer past it)

@@ -592,3 +592,42 @@ def test_words_without_probability_take_no_gradient(gpu_device, T, which):
     loss.backward()
     assert not wl.grad[:300].any()
     _check(x, wf, torch.where(y == IGNORE, y, y - 300), loss.detach(), None, wl.grad[300:], "mean", torch.ones((), device=gpu_device))
+
+
+@pytest.mark.parametrize("T", [5, 40, 300])
+@pytest.mark.parametrize("V", [257, 40001])
+@pytest.mark.parametrize("top", [200.0, 24.0, -200.0])
+def test_confident_positions(gpu_device, T, V, top):
+    """x_t picks one column of the weight, whose bf16 values are the logits without a rounding; the label's is `top`, the
+    largest, and the others' exponentials add to 1e-7 ... 1 of its own.  A term exp(z - top) is off by 64 u of itself (its
+    exponent, below 50, by a rounding and log2(e)'s), and the additions that hold the 1 of the largest, at most 24 before
+    the tiles' pairs are joined, by u each; the logarithm by 4 u of itself.  So a loss is within 72 u of itself and 24 u,
+    however large the logits, and never negative.  dz, read off dW (ceil(T / 64) equal rows to a column): the same in p,
+    8 u more at p - 1, and the roundings of dz and of dW to bf16"""
+    from lowbit.loss import linear_cross_entropy
+
+    g = torch.Generator().manual_seed(V + T)
+    H = 64
+    eps = 10.0 ** -(7 * torch.rand(H, generator=g, dtype=torch.float64))
+    w = (top - torch.log(V / eps) + 0.5 * torch.randn(V, H, generator=g, dtype=torch.float64)).clamp(max=top - 1).bfloat16()
+    word = torch.randint(0, V, (H,), generator=g)
+    w[word, torch.arange(H)] = top
+    x = torch.zeros(T, H, dtype=torch.bfloat16)
+    x[torch.arange(T), torch.arange(T) % H] = 1.0
+    x, w, y = x.to(gpu_device), w.to(gpu_device), word[torch.arange(T) % H].to(gpu_device)
+    d = (w.double() - top).t()[torch.arange(T, device=gpu_device) % H]  # z - the label's
+    rest = torch.exp(d).scatter_(1, y[:, None], 0.0).sum(1)
+    want = torch.log1p(rest)
+    wl = w.clone().requires_grad_(True)
+    each = linear_cross_entropy(x, w, y, reduction="none")
+    loss = linear_cross_entropy(x, wl, y, reduction="sum")
+    bound = 72 * U * want + 24 * U
+    assert (each >= 0).all() and ((each.double() - want).abs() <= bound).all(), float(((each.double() - want).abs() / bound).max())
+    assert abs(float(loss.detach().double() - want.sum())) <= float(bound.sum() + 4 * math.sqrt(T) * U * want.sum())
+    (dw,) = torch.autograd.grad(loss, wl)
+    p = torch.exp(d) / (1 + rest)[:, None]
+    dz = p.scatter(1, y[:, None], -(rest / (1 + rest))[:, None])
+    off = (p * (72 * U * (1 + rest) + 24 * U)[:, None]).scatter_add(1, y[:, None], torch.full_like(want, 8 * U)[:, None])
+    want = dz.t() @ x.double()
+    bound = (2 * B + B * B) * want.abs() + (1 + B) * 1.01 * (off.t() @ x.double()) + 1e-37
+    assert ((dw.double() - want).abs() <= bound).all(), float(((dw.double() - want).abs() / bound).max())
