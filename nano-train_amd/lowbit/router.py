@@ -95,8 +95,13 @@ class TopKRouter(nn.Module):
 
     @torch.no_grad()
     def update_bias(self, expert_ids: torch.Tensor, rate: float = 1e-3) -> None:
-        """balance_bias += rate * sign(mean load - load) over one batch's ids."""
+        """balance_bias += rate * sign(mean load - load) over one batch's ids;
+        what is no expert's id (a dropped assignment's, say) is not counted."""
         if self.balance_bias is None:
             raise RuntimeError("the router has no balance bias")
-        load = torch.bincount(expert_ids.reshape(-1).long(), minlength=self.n_experts).float()
+        ids, E = expert_ids.reshape(-1).long(), self.n_experts
+        # bincount would ask the device for its length: the host would wait, and a graph could not hold the call
+        load = torch.zeros(E + 1, dtype=torch.int64, device=ids.device)
+        load.scatter_add_(0, torch.where((ids >= 0) & (ids < E), ids, E), torch.ones_like(ids))
+        load = load[:E].float()
         self.balance_bias += rate * torch.sign(load.mean() - load)

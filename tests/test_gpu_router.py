@@ -413,3 +413,20 @@ def test_sigmoid_from_minus_180_to_minus_85(gpu_device):
     want = torch.sigmoid(z.double()).gather(1, ids.long())
     assert ((w.double() - want).abs() <= 64 * U * want + 1e-37).all() and (w >= 0).all()
     assert (w[:, 1:] <= w[:, :-1]).all()
+
+
+def test_update_bias_does_not_wait_for_the_device(gpu_device):
+    from lowbit.router import TopKRouter
+
+    r = TopKRouter(64, 16, 2, score="sigmoid", balance_bias=True, device=gpu_device)
+    ids = torch.randint(0, 16, (500, 2), device=gpu_device, dtype=torch.int32)
+    load = torch.bincount(ids.reshape(-1).long(), minlength=16).float()
+    torch.cuda.set_sync_debug_mode("error")
+    try:
+        r.update_bias(ids, rate=0.25)
+    finally:
+        torch.cuda.set_sync_debug_mode("default")
+    want = 0.25 * torch.sign(load.mean() - load)
+    assert torch.equal(r.balance_bias, want)
+    r.update_bias(torch.cat([ids.reshape(-1), torch.tensor([-1, 16, 1 << 30], dtype=torch.int32, device=gpu_device)]), rate=0.25)
+    assert torch.equal(r.balance_bias, 2 * want)  # what is no expert's id is not counted
