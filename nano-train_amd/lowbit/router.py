@@ -74,7 +74,8 @@ class TopKRouter(nn.Module):
 
     The gate weight stays in its own dtype (fp32 by default: the recipe's
     routers are not low-bit) and the product runs in it.  balance_bias, when
-    asked for, is a buffer that update_bias() moves against the experts' load."""
+    asked for, is a buffer that update_bias() moves against the experts' load; it
+    stays fp32 when the module's type is changed."""
 
     def __init__(self, hidden_size: int, n_experts: int, top_k: int, *, score: str = "softmax",
                  balance_bias: bool = False, n_groups: int = 1, topk_groups: Optional[int] = None,
@@ -86,6 +87,14 @@ class TopKRouter(nn.Module):
         nn.init.normal_(self.weight, std=0.02)
         self.register_buffer("balance_bias",
                              torch.zeros(n_experts, dtype=torch.float32, device=device) if balance_bias else None)
+
+    def _apply(self, fn, *args, **kwargs):
+        before = self.balance_bias
+        super()._apply(fn, *args, **kwargs)
+        if before is not None and self.balance_bias.dtype != torch.float32:
+            # fewer bits would swallow its steps, and route_tokens() takes it in fp32
+            self.balance_bias = before.to(self.balance_bias.device)
+        return self
 
     def logits(self, tokens: torch.Tensor) -> torch.Tensor:
         return F.linear(tokens.to(self.weight.dtype), self.weight)

@@ -430,3 +430,17 @@ def test_update_bias_does_not_wait_for_the_device(gpu_device):
     assert torch.equal(r.balance_bias, want)
     r.update_bias(torch.cat([ids.reshape(-1), torch.tensor([-1, 16, 1 << 30], dtype=torch.int32, device=gpu_device)]), rate=0.25)
     assert torch.equal(r.balance_bias, 2 * want)  # what is no expert's id is not counted
+
+
+def test_the_balance_bias_stays_fp32(gpu_device):
+    """a module's type is changed as a whole: the bias, whose steps fewer bits would swallow, keeps its own and its values"""
+    from lowbit.router import TopKRouter
+
+    r = TopKRouter(64, 16, 2, score="sigmoid", balance_bias=True)
+    r.balance_bias += 0.1001
+    r = r.to(gpu_device).bfloat16()
+    assert r.weight.dtype == torch.bfloat16 and r.balance_bias.dtype == torch.float32 and r.balance_bias.is_cuda
+    assert torch.equal(r.balance_bias.cpu(), torch.full((16,), 0.0) + 0.1001)
+    ids, w = r(torch.randn(5, 64, device=gpu_device).bfloat16())
+    assert ids.shape == (5, 2) and w.isfinite().all()
+    assert TopKRouter(8, 4, 2).half().balance_bias is None
