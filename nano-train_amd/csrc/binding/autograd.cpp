@@ -311,10 +311,11 @@ struct Route {
 
 // ---------------------------------------------------------------------------
 struct LinearXent {
-  // whether weight lies in rows of whole 16-byte pieces
+  static constexpr int64_t MAX_PITCH = 1 << 22;  // of the products' copies
+  // whether weight lies in rows of whole 16-byte pieces, as the products take them
   static bool fits(const Tensor& weight) {
     return weight.stride(1) == 1 && weight.stride(0) % 8 == 0 && weight.size(1) % 8 == 0 &&
-           weight.stride(0) >= weight.size(1) && (uintptr_t)weight.data_ptr() % 16 == 0;
+           weight.stride(0) >= weight.size(1) && weight.stride(0) <= MAX_PITCH && (uintptr_t)weight.data_ptr() % 16 == 0;
   }
   // weight in such rows: a copy where they are not
   static Tensor padded(const Tensor& weight) {

@@ -34,7 +34,8 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: to
 
     The logits are never kept: the backward forms them again, a piece of the
     vocabulary at a time.  A weight whose rows are not whole 16-byte pieces
-    (H % 8 != 0) is copied to padded rows first.  At most 2^22 positions."""
+    (H % 8 != 0), or over 2^22 values apart, is copied to padded rows first.  At
+    most 2^22 positions."""
     ops._require_device(hidden, weight, targets)
     if reduction not in _REDUCTIONS:
         raise ValueError(f"unknown reduction {reduction!r}; expected 'none', 'sum' or 'mean'")

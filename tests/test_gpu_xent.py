@@ -631,3 +631,19 @@ def test_confident_positions(gpu_device, T, V, top):
     want = dz.t() @ x.double()
     bound = (2 * B + B * B) * want.abs() + (1 + B) * 1.01 * (off.t() @ x.double()) + 1e-37
     assert ((dw.double() - want).abs() <= bound).all(), float(((dw.double() - want).abs() / bound).max())
+
+
+@pytest.mark.parametrize("pitch", [(1 << 22) + 8, (1 << 22) + 3])
+def test_a_weight_of_very_long_rows(gpu_device, pitch):
+    """rows further apart than the products' copies reach: the weight goes through padded rows"""
+    from lowbit.loss import linear_cross_entropy
+
+    x, w, y, _ = _inputs(20, 64, 5, 61, gpu_device)
+    far = torch.zeros(5 * pitch, dtype=torch.bfloat16, device=gpu_device).as_strided((5, 64), (pitch, 1))
+    far.copy_(w)
+    got, want = [], []
+    for out, weight in ((got, far), (want, w)):
+        xl, wl = x.clone().requires_grad_(True), weight.detach().requires_grad_(True)
+        loss = linear_cross_entropy(xl, wl, y)
+        out += [loss.detach(), *torch.autograd.grad(loss, (xl, wl))]
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
