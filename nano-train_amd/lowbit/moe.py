@@ -509,7 +509,8 @@ class _LocalMoE(torch.autograd.Function):
         else:
             (pos, inv, counts, offsets, expert_ids, topk_w, xc, xs, gu, hc, hs, y, gu_codes, gu_scales, d_codes,
              d_scales) = ctx.saved_tensors
-        d_out = d_out.contiguous()
+        # one row's own stride may be anything, contiguous or not: the pitch is H
+        d_out = d_out.contiguous().view(-1).view(T, H)
         dev = d_out.device
         routing = ExpertRouting(pos, inv, counts, offsets, k)
         # combine: dY rows (y's dtype) and the routing-weight gradient

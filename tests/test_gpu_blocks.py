@@ -77,3 +77,21 @@ def test_small_model_learns(gpu_device):
     assert (right > wrong).float().mean() > 0.9
     one = model.score(words[:1], step_of[:1, None].cuda())
     assert one.shape == (1, 1)
+
+
+@pytest.mark.parametrize("rounding", ["nearest", "stochastic"])
+def test_one_token_and_a_gradient_of_any_pitch(gpu_device, rounding):
+    """the experts' single row, whose incoming gradient has strides (1, 1), as a column's transposition leaves it"""
+    from lowbit import moe
+
+    b = _block(gpu_device)
+    x, w = torch.randn(1, 256, device=gpu_device).bfloat16(), torch.rand(1, 2, device=gpu_device)
+    ids = torch.tensor([[3, 5]], dtype=torch.int32, device=gpu_device)
+    up = torch.randn(256, 1, device=gpu_device).bfloat16().t()
+    assert up.stride() == (1, 1)
+    got = []
+    for u in (up, up.reshape(-1).clone().reshape(1, 256)):
+        leaves = [x.clone().requires_grad_(True), w.clone().requires_grad_(True), b.w_gate_up, b.w_down]
+        y = moe.local_moe(leaves[0], ids, leaves[1], *leaves[2:], rounding=rounding)
+        got.append(torch.autograd.grad(y, leaves, u))
+    assert all(torch.equal(p, q) for p, q in zip(*got))
