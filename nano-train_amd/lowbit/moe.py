@@ -512,6 +512,11 @@ class _LocalMoE(torch.autograd.Function):
         # one row's own stride may be anything, contiguous or not: the pitch is H
         d_out = d_out.contiguous().view(-1).view(T, H)
         dev = d_out.device
+        if T == 0:  # nothing to multiply, and no address to give a kernel
+            zeros = lambda want, dt, *s: torch.zeros(s, dtype=dt, device=dev) if want else None  # noqa: E731
+            need = ctx.needs_input_grad
+            return (zeros(need[0], tdt, T, H), zeros(need[1], topk_w.dtype, *topk_w.shape),
+                    zeros(need[2], gudt, E, 2 * I, H), zeros(need[3], ddt, E, H, I), None, None, None, None)
         routing = ExpertRouting(pos, inv, counts, offsets, k)
         # combine: dY rows (y's dtype) and the routing-weight gradient
         ld = ops.cdiv(H, 64) * 64  # the dgrad reads whole 64-column K steps: zero pad columns

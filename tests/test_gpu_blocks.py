@@ -95,3 +95,30 @@ def test_one_token_and_a_gradient_of_any_pitch(gpu_device, rounding):
         y = moe.local_moe(leaves[0], ids, leaves[1], *leaves[2:], rounding=rounding)
         got.append(torch.autograd.grad(y, leaves, u))
     assert all(torch.equal(p, q) for p, q in zip(*got))
+
+
+@pytest.mark.parametrize("shape", [(0, 256), (2, 0, 256)])
+@pytest.mark.parametrize("rounding", ["nearest", "stochastic"])
+def test_no_tokens(gpu_device, shape, rounding):
+    """an empty batch trains: gradients of the inputs' shapes, zero for the weights"""
+    b = _block(gpu_device, rounding=rounding, score="sigmoid")
+    x = torch.randn(*shape, device=gpu_device).bfloat16().requires_grad_(True)
+    y = b(x)
+    assert y.shape == shape
+    y.sum().backward()
+    assert x.grad.shape == shape
+    for n, p in b.named_parameters():
+        assert p.grad.shape == p.shape and not p.grad.any(), n
+    with torch.no_grad():
+        assert b(x).shape == shape
+
+
+def test_small_model_without_positions(gpu_device):
+    from lowbit.blocks import MoELM
+
+    m = MoELM(50, 256, 128, 8, 2, device=gpu_device)
+    none = torch.zeros(2, 0, dtype=torch.int64, device=gpu_device)
+    loss = m(none, none)
+    loss.backward()
+    assert float(loss.detach()) == 0 and all(p.grad is None or not p.grad.any() for p in m.parameters())
+    assert m.score(none, none).shape == (2, 0)
