@@ -1024,7 +1024,8 @@ int64_t ntlb_layer_norm_workspace_bytes(int x_dtype, int64_t T, int64_t H);
  *   weights fp32 [T, top_k] = scale * p_i / (sum of the chosen p + 1e-20) if
  *     renormalize, else scale * p_i.
  * NaN orders above everything, and the ids are distinct and in range whatever
- * the logits hold; a softmax row of -infinities has p = 0.  top_k <= 16.
+ * the logits hold; a softmax row of -infinities has p = 0, and so has a sigmoid
+ * below 2^-126 (of -infinity, say).  top_k <= 16.
  */
 int ntlb_route_topk(const void* logits, int dtype, int64_t T, int64_t E, int64_t ld, int64_t top_k, int sigmoid,
                     const float* bias, int64_t n_groups, int64_t topk_groups, int renormalize, float scale,
@@ -1058,8 +1059,9 @@ int ntlb_pad_rows(const uint16_t* x, int64_t ldx, int64_t R, int64_t H, uint16_t
  * reduction 0: loss fp32 [T]; 1: loss[0] = the sum; 2: loss[0] = the mean over
  * the rows that are not ignored (0 if there are none).  A target that is
  * neither a word nor ignore_index makes its row's loss and gradients NaN.
- * Ignored rows of x are not read.  state (ntlb_linear_xent_state_bytes, 256-byte
- * aligned) holds what the backward needs: the live rows of x among it, not w.
+ * Ignored rows of x are not read.  state (ntlb_linear_xent_state_bytes(T, H),
+ * 256-byte aligned, for T = 0 too) holds what the backward needs: the live rows of x
+ * among it, not w.
  * workspace: ntlb_linear_xent_workspace_bytes(T, H, V, 0), 16-byte aligned,
  * contents free.  T <= 2^22, V <= 2^30, H <= 2^20, ldw <= 2^22, and of tiles of
  * 128 x 128 at most 2^23 in T x V and V x H, 2^19 in T x H.
@@ -1075,7 +1077,9 @@ int ntlb_linear_xent_forward(const uint16_t* x, int64_t ldx, const uint16_t* w, 
  * either NULL if not wanted.  The logits are formed again piece by piece of the
  * vocabulary; dz, without the rows' common factor, is rounded to bf16 as the
  * operand of the two products (up to 64 rows: to two bf16 values, whose sum
- * holds 16 bits).  w must be as in the forward.  workspace: ntlb_linear_xent_workspace_bytes(T, H, V, 1).
+ * holds 16 bits).  w must be as in the forward.  Without a live row dx and dw are
+ * zero and dloss is not read (for T = 0 it may be NULL).  workspace:
+ * ntlb_linear_xent_workspace_bytes(T, H, V, 1).
  */
 int ntlb_linear_xent_backward(const void* state, const uint16_t* w, int64_t ldw, int64_t T, int64_t H, int64_t V,
                               int reduction, const float* dloss, uint16_t* dx, int64_t lddx, uint16_t* dw,

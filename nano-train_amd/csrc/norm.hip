@@ -17,8 +17,8 @@
 // which a second kernel sums in a fixed order: the result does not depend on
 // how the workgroups are scheduled.
 // Measured (a large copy runs at 5.3 TB/s): 8192 x 7168 bf16 forward 38.6 us (6.1
-// TB/s), backward 70.1 (5.0) and 4.6 for dw and db's sums; 65536 x 512 fp16
-// forward 23.6 us (5.7), backward 34.9 (5.8) and 4.0; one row of 7168 3.3 us, the
+// TB/s), backward 70.0 (5.0) and 4.7 for dw and db's sums; 65536 x 512 fp16
+// forward 23.8 us (5.7), backward 34.8 (5.8) and 3.9; one row of 7168 3.2 us, the
 // launch and the latency of one pass.
 #include <hip/hip_runtime.h>
 

@@ -21,11 +21,13 @@
 // token are distinct, v_max_f64 / v_min_f64 compare and exchange choice and
 // index together, and ties go to the lowest index by themselves.
 // Measured: 65536 tokens, 256 fp32 experts in 8 groups, sigmoid and bias: forward
-// 31.6 us, the vector unit's: 1075 instructions for a wave's four tokens, of
-// which 320 sort and merge and 16 x 2 are transcendental; its 67 MB alone would
-// take 13.  Backward 15.0 us for 134 MB (part of z is still in the last cache).
-// 4096 tokens of 32 experts: 3.5 and 3.3 us, 32 tokens of 256: 4.8 us, little more
-// than an empty launch.
+// 31 to 32 us, the vector unit's: 1075 instructions for a wave's four tokens, of
+// which 320 sort and merge, 16 x 2 are transcendental, and 288 stand before the
+// loop (edges, places in LDS, which lanes hold earlier groups, scalars kept in
+// vector registers): at 16 workgroups a compute unit every wave here has one step,
+// which shares them with no other.  Its 67 MB alone would take 13.  Backward 15.5 us
+// for 134 MB (part of z is still in the last cache).  4096 tokens of 32 experts: 3.5
+// and 3.4 us, 32 tokens of 256: 4.8 us, little more than an empty launch.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>

@@ -7,8 +7,11 @@
 // fp32.
 //
 // Matrix-core bound: 2 T V H operations forward, 4 T V H for the gradients and
-// 2 T V H more to form the logits again, which costs less than it would to write
-// and read T x V values of 32 bits.  Positions that are ignored are left out
+// 2 T V H more to form the logits again.  That saves memory, T x V values of 32 bits
+// (2.1 GB at 4096 x 131072) from the forward to the backward, and costs time: at the
+// rates below a logit takes 2 H / 1.33e15 s to form, one written and read 8 / 5.3e12
+// s, which is as much at a width of 1000, half at 2048 and a seventh at 7168 (0.8 ms
+// for 5.5 at 4096 x 131072).  Positions that are ignored are left out
 // before the products: X's live rows are gathered (and padded to whole 64-column
 // steps) into X', so masked positions cost nothing, hold no part in any sum and
 // cannot pass on a NaN.  How many are live is known to the device only: tiles
@@ -16,7 +19,7 @@
 //
 // Forward: 256x256 (or 128x128) tiles of z; the epilogue reduces a tile's row to
 // its largest z and the sum of exp(z - largest) and picks the label's logit, and a
-// second kernel joins the tiles' pairs of a row.  Backward, per piece of the vocabulary (the piece's
+// second kernel joins the tiles' pairs of a row, in 64 bits.  Backward, per piece of the vocabulary (the piece's
 // dz, bf16, is the only matrix of logits' size that exists): dz from the logits
 // formed again, dX += dz W (fp32, in `slices` ranges of the piece where the tiles
 // alone would leave compute units idle), dW = dz^T X'.  dz is rounded to bf16
@@ -29,8 +32,8 @@
 // rows dz is two bf16 values, at no product's cost.
 //
 // Measured, 3891 live rows of 4096, 7168 wide, 131072 words in two pieces: logits
-// and their sums 5.41 to 5.51 ms (1.35 PFLOP/s), per piece logits and dz 2.74 to
-// 2.79 (1.33), dX and dW 5.52 (1.33; in launches of their own 2.83 and 2.74); the
+// and their sums 5.48 to 5.52 ms (1.33 PFLOP/s), per piece logits and dz 2.79 to
+// 2.80 (1.31), dX and dW 5.45 (1.34; in launches of their own 2.83 and 2.74); the
 // library's product of the forward's operands runs at 1.49.  All are held by the
 // chip's power: under such a load its clock falls from 2.4 to about 1.8 GHz.  With
 // all copies from the nearest cache (the same step again and again) the four would
@@ -389,7 +392,7 @@ __device__ __forceinline__ bool exchange(v4f (&acc)[MT][4], float4* part, uint32
 #pragma unroll
       for (int tn = 0; tn < 4; ++tn)
         part[sl * PER + (tm * 4 + tn) * THREADS] = make_float4(acc[tm][tn][0], acc[tm][tn][1], acc[tm][tn][2], acc[tm][tn][3]);
-  __syncthreads();  // the stores of all waves are in this XCD's L2; the release writes them back
+  __syncthreads();  // all waves' stores come before it, and what comes before a release it carries along
   if (tid == 0) last = __hip_atomic_fetch_add(count, 1u, __ATOMIC_RELEASE, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)(slices - 1);
   __syncthreads();
   if (!last) return false;

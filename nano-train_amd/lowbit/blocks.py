@@ -1,7 +1,8 @@
 """The MoE layer and the loss of a small language model on this package's
-kernels: what nano-train's RoutedMoE layers and head do (src/models/deepseek.py,
-src/models/moe.py) with the low-bit expert products in the middle and the
-recipe's high-precision parts around them.
+kernels: routed experts and a head as nano-train's models have them
+(src/models/deepseek.py, src/models/moe.py; the norm is LayerNorm, where
+deepseek.py has RMSNorm), with the low-bit expert products in the middle and the
+parts that stay in high precision around them.
 
   MoEBlock   x + experts(norm(x)): norm.LayerNorm, router.TopKRouter,
              moe.local_moe

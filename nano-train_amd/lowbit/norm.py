@@ -1,10 +1,11 @@
-"""Layer norm on the MI355X kernels: the norm in front of a low-bit Linear, a
-router or the expert loop, which the DeepSeek-V3 recipe keeps in high
-precision (precision.py).
+"""Layer norm on the MI355X kernels: a norm in front of a low-bit Linear, a
+router or the expert loop.  The recipe's patterns keep every norm in high
+precision (precision.py); this one is nano-train's LayerNorm
+(src/layers.py:639-781).  Its DeepSeek model has RMSNorm, another operator.
 
-layer_norm() is the operator with its gradients; LayerNorm is the module
-(src/layers.py:639-781 of nano-train).  Statistics and sums are fp32 whatever
-the input's type; outputs and gradients are rounded once.
+layer_norm() is the operator with its gradients; LayerNorm is the module.
+Statistics and sums are fp32 whatever the input's type; outputs and gradients
+are rounded once.
 """
 
 from __future__ import annotations

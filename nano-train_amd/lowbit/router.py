@@ -29,7 +29,7 @@ def route_tokens(logits: torch.Tensor, top_k: int, *, score: str = "softmax", bi
     """(expert_ids int32 [..., top_k], weights fp32 [..., top_k]) of the
     router's logits [..., E], bf16, fp16 or fp32 with rows of any pitch.
 
-    Scores are softmax(logits) or sigmoid(logits) in fp32.  The experts are
+    Scores are softmax(logits) or sigmoid(logits) in fp32 (0 below 2^-126).  The experts are
     chosen by score + bias (fp32 [E], e.g. a balance bias; it does not enter
     the weights and has no gradient), highest first, equal ones lowest index
     first.  With topk_groups < n_groups, the experts form n_groups equal runs
@@ -38,9 +38,9 @@ def route_tokens(logits: torch.Tensor, top_k: int, *, score: str = "softmax", bi
     the chosen score, renormalize dividing by the chosen scores' sum + 1e-20.
     Under autograd the weights carry the gradient of the logits.
 
-    Experts that must not be chosen take bias -inf: they are chosen only when
-    fewer than top_k others remain.  NaN logits order highest; ids are always
-    distinct and in range.  E <= 1024, top_k <= 16, n_groups <= 16."""
+    Experts that must not be chosen take bias -inf, or logits of -inf: they are
+    chosen only when fewer than top_k others remain.  NaN logits order highest;
+    ids are always distinct and in range.  E <= 1024, top_k <= 16, n_groups <= 16."""
     if not logits.is_cuda:
         ops._require_device(logits)
     if score not in _SCORES:
