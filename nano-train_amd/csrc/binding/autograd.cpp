@@ -49,13 +49,19 @@ struct Abi {
   decltype(&ntlb_linear_xent_backward) xent_backward;
   decltype(&ntlb_linear_xent_state_bytes) xent_state;
   decltype(&ntlb_linear_xent_workspace_bytes) xent_workspace;
+  PyObject* error;  // the package's exception for a failed entry point
 } abi = {};
 
 void check(const char* fn, int rc) {
   if (rc == NTLB_OK) return;
   const std::string msg = std::string(fn) + " failed (" + std::to_string(rc) + "): " + abi.last_error();
   if (rc == NTLB_EINVAL) C10_THROW_ERROR(ValueError, msg);
-  C10_THROW_ERROR(Error, msg);
+  const PyGILState_STATE gil = PyGILState_Ensure();
+  PyErr_SetString(abi.error, msg.c_str());
+  python_error err;
+  err.persist();
+  PyGILState_Release(gil);
+  throw err;
 }
 
 int dtype_of(const Tensor& t) {
@@ -499,7 +505,8 @@ PyObject* py_linear_xent(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// bind({name: address}): the C-ABI's functions
+// bind({name: address, "error": class}): the C-ABI's functions, and what is raised
+// where one of them fails for other reasons than its arguments
 template <typename F>
 void take(PyObject* table, const char* name, F& f) {
   PyObject* v = PyDict_GetItemString(table, name);  // borrowed
@@ -522,6 +529,9 @@ PyObject* py_bind(PyObject*, PyObject* table) {
   take(table, "ntlb_linear_xent_backward", a.xent_backward);
   take(table, "ntlb_linear_xent_state_bytes", a.xent_state);
   take(table, "ntlb_linear_xent_workspace_bytes", a.xent_workspace);
+  PyObject* error = PyDict_GetItemString(table, "error");  // borrowed
+  if (!error || !PyExceptionClass_Check(error)) C10_THROW_ERROR(ValueError, "no class of error");
+  a.error = Py_NewRef(error);  // for the process's life
   abi = a;
   Py_RETURN_NONE;
   END_HANDLE_TH_ERRORS

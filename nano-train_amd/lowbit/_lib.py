@@ -220,7 +220,8 @@ def autograd():
                                    f"`python nano-train_amd/build.py` ({exc})") from exc
             names = [n for n in SIGNATURES
                      if n.startswith(("ntlb_layer_norm", "ntlb_route", "ntlb_linear_xent", "ntlb_pad_rows"))]
-            mod.bind({n: ctypes.cast(getattr(L, n), ctypes.c_void_p).value for n in [*names, "ntlb_last_error"]})
+            mod.bind({"error": LowBitKernelError,
+                      **{n: ctypes.cast(getattr(L, n), ctypes.c_void_p).value for n in [*names, "ntlb_last_error"]}})
             _autograd = mod
     return _autograd
 

@@ -647,3 +647,18 @@ def test_a_weight_of_very_long_rows(gpu_device, pitch):
         loss = linear_cross_entropy(xl, wl, y)
         out += [loss.detach(), *torch.autograd.grad(loss, (xl, wl))]
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_too_large_is_refused_alike_from_python(gpu_device):
+    """the package's own error, as other entry points raise it, before a launch"""
+    from lowbit import _lib
+    from lowbit.loss import linear_cross_entropy
+
+    T = (1 << 22) + 1
+    x = torch.zeros(1, 8, dtype=torch.bfloat16, device=gpu_device).expand(T, 8)
+    w = torch.zeros(16, 8, dtype=torch.bfloat16, device=gpu_device)
+    y = torch.zeros(1, dtype=torch.int64, device=gpu_device).expand(T)
+    for wl in (w, w.clone().requires_grad_(True)):
+        with pytest.raises(_lib.LowBitKernelError, match="too large"):
+            linear_cross_entropy(x, wl, y)
+    assert float(linear_cross_entropy(x[:3], w, y[:3])) > 0  # the next call is none the worse
