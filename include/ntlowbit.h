@@ -1087,6 +1087,68 @@ int ntlb_linear_xent_backward(const void* state, const uint16_t* w, int64_t ldw,
 int64_t ntlb_linear_xent_state_bytes(int64_t T, int64_t H);
 int64_t ntlb_linear_xent_workspace_bytes(int64_t T, int64_t H, int64_t V, int backward);
 
+/*
+ * Root-mean-square norm of the rows of s = x + res [T, H] (H <= 16384), in fp32:
+ *   r = 1 / sqrt(mean(s^2) + eps), y = s r w.
+ * res (x's dtype) and s, which receives the sum rounded to x's dtype, go
+ * together; both NULL: s is x.  w (w_dtype, H entries) may be NULL (ones).  rstd,
+ * fp32 [T] or NULL, receives r.  Pitches in elements; those of inputs may be 0
+ * (one row repeated).  Rows need only the element's alignment.
+ * kept and kept_exp, both or neither: s in 8 bits for the backward.  A tile is 128
+ * columns of a row: a byte k + 127, 2^k the smallest power of two (k >= -126) with
+ * |s| <= 448 2^k for the tile's finite values, and e4m3 codes of s 2^-k (NaN for
+ * what is not finite).  kept: [T, ceil(H/128) * 128] bytes, 16-byte aligned, zero
+ * past H; kept_exp [T, ceil(H/128)].
+ */
+int ntlb_rms_norm_forward(const void* x, int x_dtype, int64_t T, int64_t H, int64_t ldx, const void* res, int64_t ldr,
+                          const void* w, int w_dtype, float eps, void* s, int64_t lds, void* y, int64_t ldy,
+                          float* rstd, uint8_t* kept, uint8_t* kept_exp, void* stream);
+
+/*
+ * The same norm with y in 8 bits: the codes (grid, round to nearest) and scales
+ * that ntlb_quant_tile_1x128 (qmax 127, NTLB_SCALE_AFTER_DIVIDE) forms of y in
+ * fp32.  codes [T, ldc], ldc = ceil(H/128) * 128, 16-byte aligned; scale (i, t)
+ * at scales[i*s_row + t*s_col]; nan_rows (int32 [T] or NULL): set to 1 where a
+ * row of y holds a NaN, else left.
+ */
+int ntlb_rms_norm_quant(const void* x, int x_dtype, int64_t T, int64_t H, int64_t ldx, const void* res, int64_t ldr,
+                        const void* w, int w_dtype, float eps, void* s, int64_t lds, int grid, uint8_t* codes,
+                        int64_t ldc, float* scales, int64_t s_row, int64_t s_col, int32_t* nan_rows, void* stream);
+
+/*
+ * Its backward, from s or (s NULL) from what was kept of it, with xh = s rstd and t = dy w:
+ *   dx = rstd (t - xh mean(t xh)) + ds   (the gradient of x and of the residual; ds NULL: 0)
+ *   dw = sum over rows of dy xh          (w_dtype; NULL: not wanted)
+ * summed in fp32 in an order that depends on the sizes only; T = 0 gives a zero
+ * dw.  workspace: ntlb_rms_norm_workspace_bytes(dtype, T, H) bytes; it need not
+ * be cleared.
+ */
+int ntlb_rms_norm_backward(const void* s, int dtype, int64_t T, int64_t H, int64_t lds, const uint8_t* kept,
+                           const uint8_t* kept_exp, const void* dy, int64_t lddy, const void* ds, int64_t ldds,
+                           const float* rstd, const void* w, int w_dtype, void* dx, int64_t lddx, void* dw,
+                           void* workspace, int64_t ws_bytes, void* stream);
+int64_t ntlb_rms_norm_workspace_bytes(int x_dtype, int64_t T, int64_t H);
+
+/*
+ * h [T, I] = silu(gate) * up of x [T, 2I], which holds both: gate in the first I
+ * columns (block 0), or gate and up in turn in blocks of `block` columns (a
+ * multiple of 128 that divides I).  fp32 inside, h rounded once to x's dtype.
+ * Pitches in elements; x's may be 0 (one row repeated).  Rows need only the
+ * element's alignment.  kept and kept_exp as for ntlb_rms_norm_forward, of gate
+ * and up apart, both in h's columns: kept [T, 2, ceil(I/128) * 128], kept_exp
+ * [T, 2, ceil(I/128)].
+ */
+int ntlb_swiglu_rows(const void* x, int dtype, int64_t T, int64_t I, int64_t ldx, int64_t block, void* h, int64_t ldh,
+                     uint8_t* kept, uint8_t* kept_exp, void* stream);
+
+/*
+ * dx [T, 2I] from dh [T, I] and x, or (x NULL) what was kept of it:
+ *   d gate = dh up sig (1 + gate (1 - sig)), d up = dh gate sig, sig = sigmoid(gate).
+ */
+int ntlb_swiglu_rows_backward(const void* x, int dtype, int64_t T, int64_t I, int64_t ldx, int64_t block,
+                              const uint8_t* kept, const uint8_t* kept_exp, const void* dh, int64_t lddh, void* dx,
+                              int64_t lddx, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,4 +1,4 @@
-// Autograd nodes of the norm, the router and the head loss: the Python module
+// Autograd nodes of the norms, the router, the head loss and the experts: the Python module
 // lowbit._autograd.
 //
 // These operators are short: at ordinary sizes a training step's kernels take
@@ -49,6 +49,12 @@ struct Abi {
   decltype(&ntlb_linear_xent_backward) xent_backward;
   decltype(&ntlb_linear_xent_state_bytes) xent_state;
   decltype(&ntlb_linear_xent_workspace_bytes) xent_workspace;
+  decltype(&ntlb_rms_norm_forward) rms_forward;
+  decltype(&ntlb_rms_norm_quant) rms_quant;
+  decltype(&ntlb_rms_norm_backward) rms_backward;
+  decltype(&ntlb_rms_norm_workspace_bytes) rms_workspace;
+  decltype(&ntlb_swiglu_rows) swiglu;
+  decltype(&ntlb_swiglu_rows_backward) swiglu_backward;
   PyObject* error;  // the package's exception for a failed entry point
 } abi = {};
 
@@ -125,14 +131,15 @@ variable_list once(variable_list grads) {
 class Kept {
  public:
   Kept() = default;
-  explicit Kept(const Tensor& t) : v_(t, false) {
+  // output: t is a result of the node that keeps it, and set_history has been called
+  explicit Kept(const Tensor& t, bool output = false) : v_(t, output) {
     if (!t.defined()) return;
     type_ = t.scalar_type();
     device_ = t.device();
     sizes_ = t.sizes();
   }
-  Tensor unpack(const char* what) const {
-    const Tensor t = v_.unpack();
+  Tensor unpack(const char* what, std::shared_ptr<Node> node = nullptr) const {
+    const Tensor t = v_.unpack(std::move(node));
     if (device_.is_cpu()) return t;  // undefined when it was kept
     if (!t.defined() || t.device() != device_ || t.scalar_type() != type_ || t.sizes() != at::IntArrayRef(sizes_) ||
         (t.numel() > 0 && !t.data_ptr()))
@@ -412,6 +419,182 @@ struct LinearXent {
 };
 
 // ---------------------------------------------------------------------------
+// What an operator keeps of its input in 8 bits: codes and their tiles' exponents
+struct Held {
+  Tensor codes, exps;
+  // of T rows of `parts` parts of n columns each
+  static Held of(int64_t T, int64_t parts, int64_t n, const Tensor& like) {
+    const int64_t tiles = (n + 127) / 128;
+    // an empty batch keeps one row that nothing writes, so that there is an address
+    const int64_t rows = std::max<int64_t>(T, 1) * parts;
+    return {fresh({rows, tiles * 128}, at::kByte, like), fresh({rows, tiles}, at::kByte, like)};
+  }
+};
+uint8_t* bytes(const Tensor& t) { return (uint8_t*)ptr(t); }
+// codes as the kernels read them
+Tensor aligned16(const Tensor& t) {
+  const Tensor s = dense(t);
+  return !s.defined() || (uintptr_t)s.data_ptr() % 16 == 0 ? s : s.clone();
+}
+
+// s = x + residual, y = its norm
+struct RmsNorm {
+  static int weight_dtype(const Tensor& x, const Tensor& w) { return dtype_of(w.defined() ? w : x); }
+
+  struct Out {
+    Tensor y, s;
+  };
+  static Out run(const Tensor& x2, const Tensor& r2, const Tensor& w, double eps, const Tensor& rstd, const Held& held) {
+    const int64_t T = x2.size(0), H = x2.size(1);
+    Out o{fresh({T, H}, x2.scalar_type(), x2), {}};
+    if (r2.defined()) o.s = fresh({T, H}, x2.scalar_type(), x2);
+    check("ntlb_rms_norm_forward",
+          abi.rms_forward(x2.data_ptr(), dtype_of(x2), T, H, x2.stride(0), ptr(r2), r2.defined() ? r2.stride(0) : 0,
+                          ptr(w), weight_dtype(x2, w), (float)eps, ptr(o.s), H, o.y.data_ptr(), H,
+                          rstd.defined() ? rstd.data_ptr<float>() : nullptr, bytes(held.codes), bytes(held.exps),
+                          stream_of(x2)));
+    return o;
+  }
+  static Tensor rows(const Tensor& t) { return t.defined() ? rows_of(t) : t; }
+
+  struct Backward : Node {
+    Kept s, codes, exps, w, rstd;
+    at::DimVector sizes;  // of x
+    at::ScalarType type;
+    bool summed;          // with a residual: s is a result, with a gradient of its own
+
+    variable_list apply(variable_list&& grads) override {
+      const std::lock_guard<std::mutex> lock(mutex_);
+      const Tensor ds0 = summed ? grads[1] : Tensor();
+      if (!grads[0].defined()) return {ds0, ds0, Tensor()};
+      no_tangent("the gradient of rms_norm", grads[0], ds0);
+      const Tensor s0 = s.unpack("rows of x", summed ? getptr() : nullptr), c0 = codes.unpack("codes of x"),
+                   e0 = exps.unpack("exponents of x"), w0 = w.unpack("values of weight"),
+                   r0 = rstd.unpack("rows' deviations");
+      const c10::DeviceGuard guard(r0.device());
+      const at::AutoDispatchBelowADInplaceOrView below;
+      const Tensor s2 = rows(s0), ct = aligned16(c0), et = dense(e0), wt = dense(w0), d2 = rows_of(grads[0]), q2 = rows(ds0);
+      const int64_t T = d2.size(0), H = d2.size(1);
+      const Tensor dx = fresh({T, H}, type, r0);
+      Tensor dw;
+      if (wt.defined() && task_should_compute_output(2)) dw = fresh({H}, wt.scalar_type(), r0);
+      const int64_t need = abi.rms_workspace(dtype_of(dx), T, H);
+      const Tensor ws = scratch(need, r0), stats = dense(r0);
+      check("ntlb_rms_norm_backward",
+            abi.rms_backward(ptr(s2), dtype_of(dx), T, H, s2.defined() ? s2.stride(0) : 0, bytes(ct), bytes(et),
+                             d2.data_ptr(), d2.stride(0), ptr(q2), q2.defined() ? q2.stride(0) : 0,
+                             stats.data_ptr<float>(), ptr(wt), weight_dtype(dx, wt), dx.data_ptr(), H, ptr(dw), ptr(ws),
+                             need, stream_of(r0)));
+      const Tensor out = shaped(dx, sizes);
+      return once({task_should_compute_output(0) ? out : Tensor(), task_should_compute_output(1) ? out : Tensor(), dw});
+    }
+    void release_variables() override {
+      const std::lock_guard<std::mutex> lock(mutex_);
+      for (Kept* k : {&s, &codes, &exps, &w, &rstd}) k->reset();
+    }
+    std::string name() const override { return "RmsNormBackward"; }
+  };
+
+  static Out forward(const Tensor& x, const Tensor& w, const Tensor& res, double eps, bool keep) {
+    const c10::DeviceGuard guard(x.device());
+    Tensor x2, rstd;
+    Held held;
+    Out o;
+    {
+      const at::AutoDispatchBelowADInplaceOrView below;
+      x2 = rows_of(x);
+      const int64_t T = x2.size(0);
+      rstd = fresh({std::max<int64_t>(1, T)}, at::kFloat, x2);
+      if (keep) held = Held::of(T, 1, x2.size(1), x2);
+      o = run(x2, rows(res), w, eps, rstd, held);
+      o.y = shaped(o.y, x.sizes());
+      if (o.s.defined()) o.s = shaped(o.s, x.sizes());
+    }
+    auto node = make_node<Backward>(torch::autograd::collect_next_edges(x, res, w));
+    node->w = Kept(w);
+    node->rstd = Kept(rstd);
+    node->sizes = x.sizes();
+    node->type = x.scalar_type();
+    node->summed = res.defined();
+    torch::autograd::set_history(o.y, node);
+    if (o.s.defined()) torch::autograd::set_history(o.s, node);
+    if (keep) {
+      node->codes = Kept(held.codes);
+      node->exps = Kept(held.exps);
+    } else {
+      node->s = node->summed ? Kept(o.s, true) : kept(x, x2);
+    }
+    return o;
+  }
+};
+
+// ---------------------------------------------------------------------------
+struct SwiGlu {
+  static Tensor run(const Tensor& x2, int64_t block, const Held& held) {
+    const int64_t T = x2.size(0), I = x2.size(1) / 2;
+    Tensor h = fresh({T, I}, x2.scalar_type(), x2);
+    check("ntlb_swiglu_rows", abi.swiglu(x2.data_ptr(), dtype_of(x2), T, I, x2.stride(0), block, h.data_ptr(), I,
+                                         bytes(held.codes), bytes(held.exps), stream_of(x2)));
+    return h;
+  }
+  static Tensor lead(const Tensor& h, const Tensor& x) {
+    at::DimVector sizes(x.sizes());
+    sizes.back() /= 2;
+    return shaped(h, sizes);
+  }
+
+  struct Backward : Node {
+    Kept x, codes, exps;
+    at::DimVector sizes;  // of x
+    int64_t block;
+
+    variable_list apply(variable_list&& grads) override {
+      const std::lock_guard<std::mutex> lock(mutex_);
+      if (!grads[0].defined()) return variable_list(1);
+      no_tangent("the gradient of swiglu", grads[0]);
+      const Tensor x0 = x.unpack("rows of x"), c0 = codes.unpack("codes of x"), e0 = exps.unpack("exponents of x");
+      const c10::DeviceGuard guard(grads[0].device());
+      const at::AutoDispatchBelowADInplaceOrView below;
+      const Tensor x2 = RmsNorm::rows(x0), ct = aligned16(c0), et = dense(e0), d2 = rows_of(grads[0]);
+      const int64_t T = d2.size(0), I = d2.size(1);
+      const Tensor dx = fresh({T, 2 * I}, d2.scalar_type(), d2);
+      check("ntlb_swiglu_rows_backward",
+            abi.swiglu_backward(ptr(x2), dtype_of(d2), T, I, x2.defined() ? x2.stride(0) : 0, block, bytes(ct), bytes(et),
+                                d2.data_ptr(), d2.stride(0), dx.data_ptr(), 2 * I, stream_of(d2)));
+      return once({shaped(dx, sizes)});
+    }
+    void release_variables() override {
+      const std::lock_guard<std::mutex> lock(mutex_);
+      for (Kept* k : {&x, &codes, &exps}) k->reset();
+    }
+    std::string name() const override { return "SwiGluBackward"; }
+  };
+
+  static Tensor forward(const Tensor& x, int64_t block, bool keep) {
+    const c10::DeviceGuard guard(x.device());
+    Tensor h, x2;
+    Held held;
+    {
+      const at::AutoDispatchBelowADInplaceOrView below;
+      x2 = rows_of(x);
+      if (keep) held = Held::of(x2.size(0), 2, x2.size(1) / 2, x2);
+      h = lead(run(x2, block, held), x);
+    }
+    auto node = make_node<Backward>(torch::autograd::collect_next_edges(x));
+    if (keep) {
+      node->codes = Kept(held.codes);
+      node->exps = Kept(held.exps);
+    } else {
+      node->x = kept(x, x2);
+    }
+    node->sizes = x.sizes();
+    node->block = block;
+    torch::autograd::set_history(h, node);
+    return h;
+  }
+};
+
+// ---------------------------------------------------------------------------
 // Python
 // ---------------------------------------------------------------------------
 Tensor maybe(PyObject* o) { return o == Py_None ? Tensor() : THPVariable_Unpack(o); }
@@ -505,6 +688,105 @@ PyObject* py_linear_xent(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+PyObject* wrap(const Tensor& t) {
+  if (!t.defined()) Py_RETURN_NONE;
+  return THPVariable_Wrap(t);
+}
+template <size_t N>
+PyObject* wrap_all(const Tensor (&ts)[N]) {
+  THPObjectPtr out(PyTuple_New(N));
+  if (!out) throw python_error();
+  for (size_t i = 0; i < N; ++i) {
+    PyObject* o = wrap(ts[i]);
+    if (!o) throw python_error();
+    PyTuple_SET_ITEM(out.get(), i, o);
+  }
+  return out.release();
+}
+
+// rms_norm(x, weight | None, residual | None, eps, keep) -> y, or (y, s) with a residual
+PyObject* py_rms_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  count(n, 5);
+  const Tensor& x = THPVariable_Unpack(a[0]);
+  const Tensor w = maybe(a[1]), res = maybe(a[2]);
+  const double eps = real(a[3]);
+  const bool keep = integer(a[4]) != 0;
+  RmsNorm::Out o;
+  {
+    const NoGil nogil;
+    no_tangent("rms_norm", x, w, res);
+    if (at::GradMode::is_enabled() && (wanted(x) || wanted(w) || wanted(res))) {
+      o = RmsNorm::forward(x, w, res, eps, keep);
+    } else {
+      const at::AutoDispatchBelowADInplaceOrView below;
+      const c10::DeviceGuard guard(x.device());
+      o = RmsNorm::run(rows_of(x), RmsNorm::rows(res), w, eps, Tensor(), Held());
+      o.y = shaped(o.y, x.sizes());
+      if (o.s.defined()) o.s = shaped(o.s, x.sizes());
+    }
+  }
+  if (!o.s.defined()) return THPVariable_Wrap(o.y);
+  return wrap_all({o.y, o.s});
+  END_HANDLE_TH_ERRORS
+}
+
+// rms_norm_quant(x, weight | None, residual | None, eps, grid, nan) ->
+// (codes, scales by tile, nan rows | None, s | None)
+PyObject* py_rms_norm_quant(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  count(n, 6);
+  const Tensor& x = THPVariable_Unpack(a[0]);
+  const Tensor w = maybe(a[1]), res = maybe(a[2]);
+  const double eps = real(a[3]);
+  const int grid = (int)integer(a[4]);
+  const bool want_nan = integer(a[5]) != 0;
+  Tensor codes, scales, nan, s;
+  {
+    const NoGil nogil;
+    no_tangent("rms_norm_quant", x, w, res);
+    const at::AutoDispatchBelowADInplaceOrView below;
+    const c10::DeviceGuard guard(x.device());
+    const Tensor x2 = rows_of(x), r2 = RmsNorm::rows(res);
+    const int64_t T = x2.size(0), H = x2.size(1), tiles = (H + 127) / 128, rp = std::max<int64_t>((T + 3) / 4 * 4, 4);
+    codes = fresh({T, tiles * 128}, at::kByte, x2);
+    scales = fresh({tiles, rp}, at::kFloat, x2);
+    if (want_nan) nan = fresh({T}, at::kInt, x2).zero_();
+    if (r2.defined()) s = fresh({T, H}, x2.scalar_type(), x2);
+    check("ntlb_rms_norm_quant",
+          abi.rms_quant(x2.data_ptr(), dtype_of(x2), T, H, x2.stride(0), ptr(r2), r2.defined() ? r2.stride(0) : 0, ptr(w),
+                        RmsNorm::weight_dtype(x2, w), (float)eps, ptr(s), H, grid, bytes(codes), tiles * 128,
+                        scales.data_ptr<float>(), 1, rp, nan.defined() ? nan.data_ptr<int32_t>() : nullptr,
+                        stream_of(x2)));
+    if (s.defined()) s = shaped(s, x.sizes());
+  }
+  return wrap_all({codes, scales, nan, s});
+  END_HANDLE_TH_ERRORS
+}
+
+// swiglu(x, block, keep) -> h
+PyObject* py_swiglu(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  count(n, 3);
+  const Tensor& x = THPVariable_Unpack(a[0]);
+  const int64_t block = integer(a[1]);
+  const bool keep = integer(a[2]) != 0;
+  Tensor h;
+  {
+    const NoGil nogil;
+    no_tangent("swiglu", x);
+    if (at::GradMode::is_enabled() && wanted(x)) {
+      h = SwiGlu::forward(x, block, keep);
+    } else {
+      const at::AutoDispatchBelowADInplaceOrView below;
+      const c10::DeviceGuard guard(x.device());
+      h = SwiGlu::lead(SwiGlu::run(rows_of(x), block, Held()), x);
+    }
+  }
+  return THPVariable_Wrap(h);
+  END_HANDLE_TH_ERRORS
+}
+
 // bind({name: address, "error": class}): the C-ABI's functions, and what is raised
 // where one of them fails for other reasons than its arguments
 template <typename F>
@@ -529,6 +811,12 @@ PyObject* py_bind(PyObject*, PyObject* table) {
   take(table, "ntlb_linear_xent_backward", a.xent_backward);
   take(table, "ntlb_linear_xent_state_bytes", a.xent_state);
   take(table, "ntlb_linear_xent_workspace_bytes", a.xent_workspace);
+  take(table, "ntlb_rms_norm_forward", a.rms_forward);
+  take(table, "ntlb_rms_norm_quant", a.rms_quant);
+  take(table, "ntlb_rms_norm_backward", a.rms_backward);
+  take(table, "ntlb_rms_norm_workspace_bytes", a.rms_workspace);
+  take(table, "ntlb_swiglu_rows", a.swiglu);
+  take(table, "ntlb_swiglu_rows_backward", a.swiglu_backward);
   PyObject* error = PyDict_GetItemString(table, "error");  // borrowed
   if (!error || !PyExceptionClass_Check(error)) C10_THROW_ERROR(ValueError, "no class of error");
   a.error = Py_NewRef(error);  // for the process's life
@@ -542,6 +830,9 @@ PyMethodDef methods[] = {
     {"layer_norm", (PyCFunction)(void (*)(void))py_layer_norm, METH_FASTCALL, nullptr},
     {"route", (PyCFunction)(void (*)(void))py_route, METH_FASTCALL, nullptr},
     {"linear_xent", (PyCFunction)(void (*)(void))py_linear_xent, METH_FASTCALL, nullptr},
+    {"rms_norm", (PyCFunction)(void (*)(void))py_rms_norm, METH_FASTCALL, nullptr},
+    {"rms_norm_quant", (PyCFunction)(void (*)(void))py_rms_norm_quant, METH_FASTCALL, nullptr},
+    {"swiglu", (PyCFunction)(void (*)(void))py_swiglu, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_autograd", nullptr, -1, methods};
 

@@ -148,6 +148,14 @@ SIGNATURES = {
     "ntlb_linear_xent_backward": [_P, _P, _I64, _I64, _I64, _I64, _I32, _P, _P, _I64, _P, _I64, _P, _I64, _P],
     "ntlb_linear_xent_state_bytes": [_I64, _I64],
     "ntlb_linear_xent_workspace_bytes": [_I64, _I64, _I64, _I32],
+    "ntlb_rms_norm_forward": [_P, _I32, _I64, _I64, _I64, _P, _I64, _P, _I32, _F32, _P, _I64, _P, _I64, _P, _P, _P, _P],
+    "ntlb_rms_norm_quant": [_P, _I32, _I64, _I64, _I64, _P, _I64, _P, _I32, _F32, _P, _I64, _I32, _P, _I64, _P, _I64,
+                            _I64, _P, _P],
+    "ntlb_rms_norm_backward": [_P, _I32, _I64, _I64, _I64, _P, _P, _P, _I64, _P, _I64, _P, _P, _I32, _P, _I64, _P, _P,
+                               _I64, _P],
+    "ntlb_rms_norm_workspace_bytes": [_I32, _I64, _I64],
+    "ntlb_swiglu_rows": [_P, _I32, _I64, _I64, _I64, _I64, _P, _I64, _P, _P, _P],
+    "ntlb_swiglu_rows_backward": [_P, _I32, _I64, _I64, _I64, _I64, _P, _P, _P, _I64, _P, _I64, _P],
 }
 
 
@@ -166,7 +174,7 @@ RESTYPES = {"ntlb_gemm_workspace_bytes": _I64, "ntlb_ep_record_bytes": _I64, "nt
             "ntlb_ep_value_record_bytes": _I64, "ntlb_persistent_quant_ws_words": _I64,
             "ntlb_gemm_lowbit_workspace_bytes": _I64, "ntlb_gemm_dq_workspace_bytes": _I64,
             "ntlb_layer_norm_workspace_bytes": _I64, "ntlb_linear_xent_state_bytes": _I64,
-            "ntlb_linear_xent_workspace_bytes": _I64}
+            "ntlb_linear_xent_workspace_bytes": _I64, "ntlb_rms_norm_workspace_bytes": _I64}
 
 _lib = None
 _lock = threading.Lock()
@@ -219,7 +227,8 @@ def autograd():
                 raise RuntimeError("the autograd module is not built or does not load; build it with "
                                    f"`python nano-train_amd/build.py` ({exc})") from exc
             names = [n for n in SIGNATURES
-                     if n.startswith(("ntlb_layer_norm", "ntlb_route", "ntlb_linear_xent", "ntlb_pad_rows"))]
+                     if n.startswith(("ntlb_layer_norm", "ntlb_route", "ntlb_linear_xent", "ntlb_pad_rows", "ntlb_rms_norm",
+                                   "ntlb_swiglu_rows"))]
             mod.bind({"error": LowBitKernelError,
                       **{n: ctypes.cast(getattr(L, n), ctypes.c_void_p).value for n in [*names, "ntlb_last_error"]}})
             _autograd = mod

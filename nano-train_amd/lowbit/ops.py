@@ -80,6 +80,15 @@ def rounding_code(mode: str) -> int:
     raise ValueError(f"unknown rounding mode {mode!r}")
 
 
+def checkpoint_code(kind: Optional[str]) -> int:
+    """Whether an operator keeps its input for the backward in 8 bits."""
+    if kind is None:
+        return 0
+    if kind == "e4m3":
+        return 1
+    raise ValueError(f"unknown checkpoint {kind!r}; expected None or 'e4m3'")
+
+
 @dataclass
 class QTensor:
     """Codes plus scales of a quantized [rows, K] matrix.
