@@ -1149,6 +1149,37 @@ int ntlb_swiglu_rows_backward(const void* x, int dtype, int64_t T, int64_t I, in
                               const uint8_t* kept, const uint8_t* kept_exp, const void* dh, int64_t lddh, void* dx,
                               int64_t lddx, void* stream);
 
+/*
+ * bf16 products grouped by expert: row r of x [R, K] belongs to the expert e with
+ * offsets[e] <= r < offsets[e+1] (int32 [E+1] on the device, offsets[0] taken as
+ * 0, not decreasing; values past R count as R), whose weight is w + e * w_stride
+ * [N, K]:
+ *   y[r] = x[r] W_e^T;   dx[r] = dy[r] W_e;   dw[e] = sum over e's rows of dy[r]^T x[r]
+ * summed in fp32, rounded once; y and dx are zero in rows at or past offsets[E],
+ * dw [E, N, K] (contiguous) for experts without rows.  Pitches in elements.  Inputs
+ * lie in 16-byte aligned rows of whole 16-byte pieces (pitch % 8 == 0, at most
+ * 2^22; w_stride % 8 == 0); where a product sums along their rows (x and w for y,
+ * dy for dx) their columns up to the next multiple of 8 are zero.  Outputs need only
+ * the element's alignment.  E <= 4096, R <= 2^30, N and K <= 2^22.
+ */
+int ntlb_grouped_matmul(const uint16_t* x, int64_t ldx, const uint16_t* w, int64_t ldw, int64_t w_stride,
+                        const int32_t* offsets, int64_t R, int64_t E, int64_t N, int64_t K, uint16_t* y, int64_t ldy,
+                        void* stream);
+int ntlb_grouped_matmul_dx(const uint16_t* dy, int64_t lddy, const uint16_t* w, int64_t ldw, int64_t w_stride,
+                           const int32_t* offsets, int64_t R, int64_t E, int64_t N, int64_t K, uint16_t* dx,
+                           int64_t lddx, void* stream);
+int ntlb_grouped_matmul_dw(const uint16_t* dy, int64_t lddy, const uint16_t* x, int64_t ldx, const int32_t* offsets,
+                           int64_t R, int64_t E, int64_t N, int64_t K, uint16_t* dw, void* stream);
+
+/*
+ * x bf16 [R, K] (rows as for the products above) in 8 bits, laid out as kept and
+ * kept_exp of ntlb_rms_norm_forward, and what they stand for as bf16 (exact) [R,
+ * ldo], ldo % 8 == 0, zero from K to the next multiple of 8.
+ */
+int ntlb_kept_rows(const uint16_t* x, int64_t ldx, int64_t R, int64_t K, uint8_t* kept, uint8_t* kept_exp, void* stream);
+int ntlb_kept_values(const uint8_t* kept, const uint8_t* kept_exp, int64_t R, int64_t K, uint16_t* out, int64_t ldo,
+                     void* stream);
+
 #ifdef __cplusplus
 }
 #endif

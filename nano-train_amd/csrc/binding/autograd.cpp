@@ -55,6 +55,11 @@ struct Abi {
   decltype(&ntlb_rms_norm_workspace_bytes) rms_workspace;
   decltype(&ntlb_swiglu_rows) swiglu;
   decltype(&ntlb_swiglu_rows_backward) swiglu_backward;
+  decltype(&ntlb_grouped_matmul) grouped;
+  decltype(&ntlb_grouped_matmul_dx) grouped_dx;
+  decltype(&ntlb_grouped_matmul_dw) grouped_dw;
+  decltype(&ntlb_kept_rows) kept_rows;
+  decltype(&ntlb_kept_values) kept_values;
   PyObject* error;  // the package's exception for a failed entry point
 } abi = {};
 
@@ -595,6 +600,118 @@ struct SwiGlu {
 };
 
 // ---------------------------------------------------------------------------
+// y = x W_e^T by rows sorted by expert
+struct Grouped {
+  static constexpr int64_t MAX_PITCH = 1 << 22;
+  static uint16_t* at(const Tensor& t) { return (uint16_t*)ptr(t); }
+  static bool pieces(const Tensor& t, int64_t pitch, int64_t cols, bool summed) {
+    return t.stride(-1) == 1 && pitch % 8 == 0 && pitch >= cols && pitch <= MAX_PITCH && (uintptr_t)t.data_ptr() % 16 == 0 &&
+           (!summed || cols % 8 == 0);
+  }
+  // [R, C] in rows of whole 16-byte pieces (summed: zero past C): t, or a copy
+  static Tensor rows(const Tensor& t, bool summed) {
+    if (t.numel() == 0) return t;
+    const Tensor r = rows_of(t);
+    if (pieces(r, r.stride(0), r.size(1), summed)) return r;
+    Tensor out = fresh({r.size(0), (r.size(1) + 7) / 8 * 8}, r.scalar_type(), r);
+    check("ntlb_pad_rows", abi.pad_rows(at(r), r.stride(0), r.size(0), r.size(1), at(out), out.size(1), stream_of(r)));
+    return out;
+  }
+  // the same of weights [E, N, K]
+  static Tensor weights(const Tensor& w) {
+    if (pieces(w, w.stride(1), w.size(2), true) && w.stride(0) >= 0 && w.stride(0) % 8 == 0) return w;
+    const int64_t E = w.size(0), N = w.size(1);
+    const Tensor r = rows(w.reshape({E * N, w.size(2)}), true);
+    return r.as_strided({E, N, r.size(1)}, {N * r.stride(0), r.stride(0), 1});
+  }
+
+  static Tensor run(const Tensor& x2, const Tensor& w3, const Tensor& offsets, int64_t N, int64_t K) {
+    const int64_t R = x2.size(0);
+    Tensor y = fresh({R, N}, x2.scalar_type(), x2);
+    check("ntlb_grouped_matmul", abi.grouped(at(x2), x2.stride(0), at(w3), w3.stride(1), w3.stride(0), offsets.data_ptr<int32_t>(),
+                                             R, w3.size(0), N, K, at(y), N, stream_of(x2)));
+    return y;
+  }
+
+  struct Backward : Node {
+    Kept x, codes, exps, w, offsets;
+    int64_t R, E, N, K;
+
+    variable_list apply(variable_list&& grads) override {
+      const std::lock_guard<std::mutex> lock(mutex_);
+      if (!grads[0].defined()) return variable_list(2);
+      no_tangent("the gradient of grouped_matmul", grads[0]);
+      const Tensor x0 = x.unpack("rows of x"), c0 = codes.unpack("codes of x"), e0 = exps.unpack("exponents of x"),
+                   w0 = w.unpack("values of weight"), o0 = offsets.unpack("offsets");
+      const c10::DeviceGuard guard(grads[0].device());
+      const at::AutoDispatchBelowADInplaceOrView below;
+      const Tensor dy = grads[0], off = dense(o0);
+      Tensor dx, dw, d2;
+      if (task_should_compute_output(0) && w0.defined()) {
+        const Tensor wt = weights(w0);
+        d2 = rows(dy, true);
+        dx = fresh({R, K}, dy.scalar_type(), dy);
+        check("ntlb_grouped_matmul_dx", abi.grouped_dx(at(d2), d2.stride(0), at(wt), wt.stride(1), wt.stride(0),
+                                                       off.data_ptr<int32_t>(), R, E, N, K, at(dx), K, stream_of(dy)));
+      }
+      if (task_should_compute_output(1) && (x0.defined() || c0.defined())) {
+        if (!d2.defined()) d2 = rows(dy, false);
+        Tensor x2;
+        if (x0.defined()) {
+          x2 = rows(x0, false);
+        } else {
+          const Tensor ct = aligned16(c0), et = dense(e0);
+          x2 = fresh({R, (K + 7) / 8 * 8}, dy.scalar_type(), dy);
+          check("ntlb_kept_values", abi.kept_values(bytes(ct), bytes(et), R, K, at(x2), x2.size(1), stream_of(dy)));
+        }
+        dw = fresh({E, N, K}, dy.scalar_type(), dy);
+        check("ntlb_grouped_matmul_dw", abi.grouped_dw(at(d2), d2.stride(0), at(x2), x2.stride(0), off.data_ptr<int32_t>(), R,
+                                                       E, N, K, at(dw), stream_of(dy)));
+      }
+      return once({dx, dw});
+    }
+    void release_variables() override {
+      const std::lock_guard<std::mutex> lock(mutex_);
+      for (Kept* k : {&x, &codes, &exps, &w, &offsets}) k->reset();
+    }
+    std::string name() const override { return "GroupedMatmulBackward"; }
+  };
+
+  static Tensor forward(const Tensor& x, const Tensor& w, const Tensor& offsets, bool keep) {
+    const c10::DeviceGuard guard(x.device());
+    const int64_t R = x.size(0), K = x.size(1), E = w.size(0), N = w.size(1);
+    Tensor y, x2, w3;
+    Held held;
+    {
+      const at::AutoDispatchBelowADInplaceOrView below;
+      x2 = rows(x, true);
+      w3 = weights(w);
+      if (keep && wanted(w)) {
+        held = Held::of(R, 1, K, x);
+        check("ntlb_kept_rows", abi.kept_rows(at(x2), x2.stride(0), R, K, bytes(held.codes), bytes(held.exps), stream_of(x)));
+      }
+      y = run(x2, w3, offsets, N, K);
+    }
+    auto node = make_node<Backward>(torch::autograd::collect_next_edges(x, w));
+    // each operand is kept for the other's gradient
+    if (held.codes.defined()) {
+      node->codes = Kept(held.codes);
+      node->exps = Kept(held.exps);
+    } else if (wanted(w)) {
+      node->x = kept(x, x2);
+    }
+    if (wanted(x)) node->w = kept(w, w3);
+    node->offsets = Kept(offsets);
+    node->R = R;
+    node->E = E;
+    node->N = N;
+    node->K = K;
+    torch::autograd::set_history(y, node);
+    return y;
+  }
+};
+
+// ---------------------------------------------------------------------------
 // Python
 // ---------------------------------------------------------------------------
 Tensor maybe(PyObject* o) { return o == Py_None ? Tensor() : THPVariable_Unpack(o); }
@@ -787,6 +904,28 @@ PyObject* py_swiglu(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// grouped_matmul(x, weight, offsets, keep) -> y
+PyObject* py_grouped_matmul(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  count(n, 4);
+  const Tensor &x = THPVariable_Unpack(a[0]), &w = THPVariable_Unpack(a[1]), &offsets = THPVariable_Unpack(a[2]);
+  const bool keep = integer(a[3]) != 0;
+  Tensor y;
+  {
+    const NoGil nogil;
+    no_tangent("grouped_matmul", x, w);
+    if (at::GradMode::is_enabled() && (wanted(x) || wanted(w))) {
+      y = Grouped::forward(x, w, offsets, keep);
+    } else {
+      const at::AutoDispatchBelowADInplaceOrView below;
+      const c10::DeviceGuard guard(x.device());
+      y = Grouped::run(Grouped::rows(x, true), Grouped::weights(w), offsets, w.size(1), w.size(2));
+    }
+  }
+  return THPVariable_Wrap(y);
+  END_HANDLE_TH_ERRORS
+}
+
 // bind({name: address, "error": class}): the C-ABI's functions, and what is raised
 // where one of them fails for other reasons than its arguments
 template <typename F>
@@ -817,6 +956,11 @@ PyObject* py_bind(PyObject*, PyObject* table) {
   take(table, "ntlb_rms_norm_workspace_bytes", a.rms_workspace);
   take(table, "ntlb_swiglu_rows", a.swiglu);
   take(table, "ntlb_swiglu_rows_backward", a.swiglu_backward);
+  take(table, "ntlb_grouped_matmul", a.grouped);
+  take(table, "ntlb_grouped_matmul_dx", a.grouped_dx);
+  take(table, "ntlb_grouped_matmul_dw", a.grouped_dw);
+  take(table, "ntlb_kept_rows", a.kept_rows);
+  take(table, "ntlb_kept_values", a.kept_values);
   PyObject* error = PyDict_GetItemString(table, "error");  // borrowed
   if (!error || !PyExceptionClass_Check(error)) C10_THROW_ERROR(ValueError, "no class of error");
   a.error = Py_NewRef(error);  // for the process's life
@@ -832,6 +976,7 @@ PyMethodDef methods[] = {
     {"linear_xent", (PyCFunction)(void (*)(void))py_linear_xent, METH_FASTCALL, nullptr},
     {"rms_norm", (PyCFunction)(void (*)(void))py_rms_norm, METH_FASTCALL, nullptr},
     {"rms_norm_quant", (PyCFunction)(void (*)(void))py_rms_norm_quant, METH_FASTCALL, nullptr},
+    {"grouped_matmul", (PyCFunction)(void (*)(void))py_grouped_matmul, METH_FASTCALL, nullptr},
     {"swiglu", (PyCFunction)(void (*)(void))py_swiglu, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_autograd", nullptr, -1, methods};

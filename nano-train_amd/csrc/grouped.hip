@@ -1,0 +1,488 @@
+// bf16 products grouped by expert: the rows of x [R, K] are sorted by expert, expert e
+// owns rows offsets[e] .. offsets[e + 1] - 1 and the weight W_e [N, K]:
+//   y = x W_e^T,  dx = dy W_e (by the row's expert),  dW_e = dy^T x over e's rows
+// Products of bf16 values are exact in fp32 and summed in fp32 on the matrix cores;
+// results are rounded once.  Rows behind the last expert's are zero in y and dx, and
+// so is dW_e of an expert without rows.  How the rows divide is known to the device
+// only: each workgroup reads the offsets (clamped to R, so that no table leads out of
+// a buffer) and finds its tile.
+//
+// Matrix-core bound where experts have a few hundred rows and more, on the tiles of
+// ntlb_bf16_tile.h; bound by the weights' way from HBM below.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+
+#include "ntlb_bf16_tile.h"
+#include "ntlb_device.h"
+#include "ntlb_host.h"
+#include "ntlb_kept.h"
+#include "ntlb_splitk.h"
+
+namespace ntlb {
+namespace grouped {
+
+using namespace tile;
+
+struct Args {
+  const uint8_t* a;  // x or dy
+  int64_t lda;       // bytes, as the others
+  const uint8_t* b;  // W, or x (dW)
+  int64_t ldb, b_expert;
+  const int32_t* offsets;
+  int64_t R;
+  int E;
+  int64_t k;  // contraction (y: K, dx: N)
+  int64_t M;  // rows of the result (dW: N)
+  int64_t N;  // columns of the result
+  uint16_t* out;
+  int64_t ldo;  // elements
+};
+
+// the rows of expert e; of e == E: those behind the last expert's
+struct Rows {
+  int lo, n;
+  __device__ __forceinline__ Rows(const int32_t* offsets, int e, int E, int R) {
+    const int from = e == 0 ? 0 : offsets[e], to = e >= E ? R : offsets[e + 1];
+    lo = min(max(from, 0), R);
+    n = min(max(to, lo), R) - lo;
+  }
+};
+
+__device__ __forceinline__ int wave_scan(int v, int lane) {  // inclusive
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const int o = __shfl_up(v, d);
+    v += lane >= d ? o : 0;
+  }
+  return v;
+}
+
+// Tile pid of those of all experts' rows (D each) by num_n column tiles; each XCD
+// walks a contiguous range of them.  t: the tile among its expert's.
+struct Found {
+  int e, lo, n, t;
+};
+template <int D>
+__device__ __forceinline__ bool find(const Args& g, int num_n, int pid, Found& f) {
+  const int lane = threadIdx.x & 63, R = (int)g.R;
+  int total = 0;
+  for (int c = 0; c <= g.E; c += 64) {
+    int m = 0;
+    if (c + lane <= g.E) m = (Rows(g.offsets, c + lane, g.E, R).n + D - 1) / D;
+    total += __builtin_amdgcn_readlane(wave_scan(m, lane), 63);
+  }
+  total *= num_n;
+  if (pid >= total) return false;
+  const int xcd = pid & 7, per = total >> 3, extra = total & 7;
+  pid = xcd * per + min(xcd, extra) + (pid >> 3);
+  int before = 0;
+  for (int c = 0; c <= g.E; c += 64) {
+    Rows r(g.offsets, min(c + lane, g.E), g.E, R);
+    const int m = c + lane <= g.E ? (r.n + D - 1) / D * num_n : 0, upto = before + wave_scan(m, lane);
+    const uint64_t b = __ballot(upto > pid);
+    if (b) {
+      const int at = __builtin_ctzll(b);
+      f.e = c + at;
+      f.lo = __builtin_amdgcn_readlane(r.lo, at);
+      f.n = __builtin_amdgcn_readlane(r.n, at);
+      f.t = pid - (__builtin_amdgcn_readlane(upto, at) - __builtin_amdgcn_readlane(m, at));
+      return true;
+    }
+    before = __builtin_amdgcn_readlane(upto, 63);
+  }
+  return false;
+}
+
+// A wave's result rows through its part of the stages
+template <int D>
+__device__ __forceinline__ void store_tile(const v4f (&acc)[D / 32][4], int wave, int wm, int wn, int lane, int64_t m0,
+                                           int64_t n0, int64_t M, int64_t N, uint16_t* out, int64_t ldo, uint8_t* la0,
+                                           uint8_t* lb0, uint8_t* la1, uint8_t* lb1) {
+  constexpr int MT = D / 32, PER = D * ROWB / 16384;
+  uint8_t* stage = (wave / PER == 0 ? la0 : wave / PER == 1 ? lb0 : wave / PER == 2 ? la1 : lb1) + (wave % PER) * 16384;
+  store_bf16<MT, true>(stage, lane, m0 + wm * 16 * MT, n0 + wn * 64, M, N, out, ldo, [&](int tm, int tn, float (&v)[4]) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) v[r] = acc[tm][tn][r];
+  });
+}
+
+#define NTLB_ZERO_ACC(D)                   \
+  v4f acc[D / 32][4];                      \
+  _Pragma("unroll") for (int i = 0; i < D / 32; ++i) _Pragma("unroll") for (int j = 0; j < 4; ++j) acc[i][j] = (v4f){0.f, 0.f, 0.f, 0.f}
+
+constexpr int GROUP_M = 4;  // row tiles of an expert that are walked side by side
+
+// y (W by rows) and dx (W transposed)
+template <int D, bool DX>
+__global__ void __launch_bounds__(2 * D, D == 256 ? 1 : 2) rows_kernel(Args g) {
+  NTLB_TILE_STAGES(D);
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  constexpr int WAVES_N = D / 64;
+  const int wm = wave / WAVES_N, wn = wave % WAVES_N;
+  const int num_n = (int)((g.N + D - 1) / D);
+  Found f;
+  if (!find<D>(g, num_n, (int)blockIdx.x, f)) return;
+  const int num_m = (f.n + D - 1) / D, group = f.t / (GROUP_M * num_n), first_m = group * GROUP_M;
+  const int gsize = min(num_m - first_m, GROUP_M), in_group = f.t - first_m * num_n;
+  const int64_t m0 = (int64_t)(first_m + in_group % gsize) * D, n0 = (int64_t)(in_group / gsize) * D;
+  NTLB_ZERO_ACC(D);
+  if (f.e < g.E) {
+    RowCopy<D> ca;
+    typename std::conditional<DX, TrCopy<D>, RowCopy<D>>::type cb;
+    ca.init(Mat{g.a + (int64_t)f.lo * g.lda, g.lda, f.n, g.k}, m0, wave, lane);
+    cb.init(Mat{g.b + (int64_t)f.e * g.b_expert, g.ldb, g.N, g.k}, n0, wave, lane);
+    multiply<D, false, DX>(ca, cb, 0, (int)((g.k + KSTEP - 1) / KSTEP), acc, wm, wn, wave, lane, la0, lb0, la1, lb1);
+  }
+  store_tile<D>(acc, wave, wm, wn, lane, m0, n0, f.n, g.N, g.out + (int64_t)f.lo * g.ldo, g.ldo, la0, lb0, la1, lb1);
+}
+
+// dW: every expert's tiles, each with the expert's rows as its contraction.  Experts
+// with many rows come first (among 64 neighbours), and each XCD takes an eighth of
+// each expert's tiles, so that long and short tiles are everywhere.
+template <int D>
+__global__ void __launch_bounds__(2 * D, D == 256 ? 1 : 2) weight_kernel(Args g) {
+  NTLB_TILE_STAGES(D);
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  constexpr int WAVES_N = D / 64;
+  const int wm = wave / WAVES_N, wn = wave % WAVES_N;
+  const int num_n = (int)((g.N + D - 1) / D), num_m = (int)((g.M + D - 1) / D), tiles = num_m * num_n, share = (tiles + 7) / 8;
+  const int pid = (int)blockIdx.x, xcd = pid & 7, at = pid >> 3, rank = at / share;
+  const int t = xcd * share + at - rank * share;
+  if (t >= tiles || rank >= g.E) return;
+  const int c = rank & ~63, here = min(g.E - c, 64);
+  const Rows r(g.offsets, min(c + lane, g.E - 1), g.E, (int)g.R);
+  int place = 0;
+  for (int j = 0; j < here; ++j) {
+    const int o = __builtin_amdgcn_readlane(r.n, j);
+    place += o > r.n || (o == r.n && j < lane);
+  }
+  const int who = __builtin_ctzll(__ballot(lane < here && place == (rank & 63)));
+  const int e = c + who, lo = __builtin_amdgcn_readlane(r.lo, who), n = __builtin_amdgcn_readlane(r.n, who);
+  const int group = t / (GROUP_M * num_n), first_m = group * GROUP_M;
+  const int gsize = min(num_m - first_m, GROUP_M), in_group = t - first_m * num_n;
+  const int64_t m0 = (int64_t)(first_m + in_group % gsize) * D, n0 = (int64_t)(in_group / gsize) * D;
+  NTLB_ZERO_ACC(D);
+  if (n > 0) {
+    TrCopy<D> ca, cb;
+    ca.init(Mat{g.a + (int64_t)lo * g.lda, g.lda, g.M, n}, m0, wave, lane);
+    cb.init(Mat{g.b + (int64_t)lo * g.ldb, g.ldb, g.N, n}, n0, wave, lane);
+    multiply<D, true, true>(ca, cb, 0, (n + KSTEP - 1) / KSTEP, acc, wm, wn, wave, lane, la0, lb0, la1, lb1);
+  }
+  store_tile<D>(acc, wave, wm, wn, lane, m0, n0, g.M, g.N, g.out + (int64_t)e * g.M * g.ldo, g.ldo, la0, lb0, la1, lb1);
+}
+
+// ---------------------------------------------------------------------------
+// y where experts have few rows: bound by the weights, read once.  A workgroup takes
+// 16 NT rows of W_e and all of e's rows (64 at a time); its four waves take
+// 64-column chunks in turn, straight from memory into fragments (a lane 32 bytes of
+// a row, 16 rows a fragment, the same columns of x and W), and their sums meet in LDS.
+// ---------------------------------------------------------------------------
+constexpr int FEW_WAVES = 4;
+
+template <int NT, int MT>
+__device__ __forceinline__ void few_rows(const Args& g, const uint8_t* wp, const uint8_t* xp, int lo, int m0, int n, int64_t n0,
+                                         int wave, int lane, float4* sums) {
+  const int r = lane & 15, gl = lane >> 4, chunks = (int)((g.k + 63) / 64);
+  const uint8_t* wr[NT];
+  const uint8_t* xr[MT];
+#pragma unroll
+  for (int i = 0; i < NT; ++i) wr[i] = wp + min<int64_t>(n0 + 16 * i + r, g.N - 1) * g.ldb + gl * 32;
+#pragma unroll
+  for (int i = 0; i < MT; ++i) xr[i] = xp + (int64_t)(lo + min(m0 + 16 * i + r, n - 1)) * g.lda + gl * 32;
+  v4f acc[MT][NT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j) acc[i][j] = (v4f){0.f, 0.f, 0.f, 0.f};
+  const int whole = (int)(g.k / 64);
+  auto load = [&](const uint8_t* p, int c) {
+    v8i v;
+    const uint4 a = *reinterpret_cast<const uint4*>(p + (int64_t)c * 128), b = *reinterpret_cast<const uint4*>(p + (int64_t)c * 128 + 16);
+    v[0] = (int)a.x; v[1] = (int)a.y; v[2] = (int)a.z; v[3] = (int)a.w;
+    v[4] = (int)b.x; v[5] = (int)b.y; v[6] = (int)b.z; v[7] = (int)b.w;
+    return v;
+  };
+  auto add = [&](const v8i (&w)[NT], const v8i (&x)[MT]) {
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        acc[i][j] = mma<0>(w[j], x[i], acc[i][j]);
+        acc[i][j] = mma<1>(w[j], x[i], acc[i][j]);
+      }
+  };
+  // a wave's chunks, U of them in flight
+  constexpr int U = MT == 4 ? 2 : 4;
+  int c = wave;
+  for (; c + (U - 1) * FEW_WAVES < whole; c += U * FEW_WAVES) {
+    v8i w[U][NT], x[U][MT];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+#pragma unroll
+      for (int j = 0; j < NT; ++j) w[u][j] = load(wr[j], c + u * FEW_WAVES);
+#pragma unroll
+      for (int i = 0; i < MT; ++i) x[u][i] = load(xr[i], c + u * FEW_WAVES);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) add(w[u], x[u]);
+  }
+  for (; c < whole; c += FEW_WAVES) {
+    v8i w[NT], x[MT];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) w[j] = load(wr[j], c);
+#pragma unroll
+    for (int i = 0; i < MT; ++i) x[i] = load(xr[i], c);
+    add(w, x);
+  }
+  if (whole < chunks && whole % FEW_WAVES == wave) {
+    // the last columns: 16-byte pieces past k are taken as zero
+    const int left = (int)(g.k - (int64_t)whole * 64) - gl * 16;
+    auto part = [&](const uint8_t* p) {
+      v8i v = {0, 0, 0, 0, 0, 0, 0, 0};
+      const uint8_t* q = p + (int64_t)whole * 128;
+      if (left > 0) {
+        const uint4 a = *reinterpret_cast<const uint4*>(q);
+        v[0] = (int)a.x; v[1] = (int)a.y; v[2] = (int)a.z; v[3] = (int)a.w;
+      }
+      if (left > 8) {
+        const uint4 a = *reinterpret_cast<const uint4*>(q + 16);
+        v[4] = (int)a.x; v[5] = (int)a.y; v[6] = (int)a.z; v[7] = (int)a.w;
+      }
+      return v;
+    };
+    v8i w[NT], x[MT];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) w[j] = part(wr[j]);
+#pragma unroll
+    for (int i = 0; i < MT; ++i) x[i] = part(xr[i]);
+    add(w, x);
+  }
+  __syncthreads();  // the sums of the rows before have been read
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+      sums[((i * NT + j) * FEW_WAVES + wave) * 64 + lane] = make_float4(acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]);
+  __syncthreads();
+  // lane: row m0 + 16 i + lane % 16, columns n0 + 16 j + 4 (lane / 16) ..
+  for (int q = wave; q < MT * NT; q += FEW_WAVES) {
+    const int i = q / NT, j = q - i * NT;
+    float4 s = sums[q * FEW_WAVES * 64 + lane];
+#pragma unroll
+    for (int w = 1; w < FEW_WAVES; ++w) {
+      const float4 o = sums[(q * FEW_WAVES + w) * 64 + lane];
+      s.x += o.x;
+      s.y += o.y;
+      s.z += o.z;
+      s.w += o.w;
+    }
+    const int m = m0 + 16 * i + r;
+    const int64_t c = n0 + 16 * j + 4 * gl;
+    if (m >= n || c >= g.N) continue;
+    uint16_t* o = g.out + (int64_t)(lo + m) * g.ldo + c;
+    const uint32_t a = pack_bf16(s.x, s.y), b = pack_bf16(s.z, s.w);
+    if (c + 4 <= g.N) {
+      *reinterpret_cast<u32x2_2*>(o) = (u32x2_2){a, b};
+    } else {
+      o[0] = (uint16_t)a;
+      if (c + 1 < g.N) o[1] = (uint16_t)(a >> 16);
+      if (c + 2 < g.N) o[2] = (uint16_t)b;
+    }
+  }
+}
+
+template <int NT>
+__global__ void __launch_bounds__(64 * FEW_WAVES) few_kernel(Args g, int blocks) {
+  __shared__ float4 sums[4 * NT * FEW_WAVES * 64];
+  const int e = (int)blockIdx.x / blocks, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t n0 = (int64_t)((int)blockIdx.x - e * blocks) * (16 * NT);
+  const Rows r(g.offsets, e, g.E, (int)g.R);
+  const int lo = __builtin_amdgcn_readfirstlane(r.lo), n = __builtin_amdgcn_readfirstlane(r.n);
+  if (e == g.E) {  // rows behind the last expert's
+    for (int i = threadIdx.x; i < n * 16 * NT; i += 64 * FEW_WAVES) {
+      const int64_t c = n0 + i % (16 * NT);
+      if (c < g.N) g.out[(int64_t)(lo + i / (16 * NT)) * g.ldo + c] = 0;
+    }
+    return;
+  }
+  const uint8_t* wp = uniform64(g.b + (int64_t)e * g.b_expert);
+  for (int m0 = 0; m0 < n; m0 += 64) {
+    const int left = n - m0;
+    if (left <= 16) few_rows<NT, 1>(g, wp, g.a, lo, m0, n, n0, wave, lane, sums);
+    else if (left <= 32) few_rows<NT, 2>(g, wp, g.a, lo, m0, n, n0, wave, lane, sums);
+    else few_rows<NT, 4>(g, wp, g.a, lo, m0, n, n0, wave, lane, sums);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// x kept in 8 bits, and back (HBM-bound): 16 lanes a tile of 128 columns
+// ---------------------------------------------------------------------------
+struct Keep {
+  const uint8_t* x;  // bf16 rows, 16-byte pieces
+  int64_t ldx;       // bytes
+  int64_t tiles;
+  int K;
+  TileRows by;
+  uint8_t* kc;
+  uint8_t* ke;
+};
+__global__ void __launch_bounds__(256) keep_kernel(Keep g) {
+  const int64_t q = ((int64_t)blockIdx.x * 256 + threadIdx.x) / 16;
+  const bool on = q < g.tiles;
+  const uint32_t t = (uint32_t)(on ? q : g.tiles - 1), row = g.by.row(t);
+  const int c = (int)(t - row * g.by.per_row) * KEPT_TILE + (threadIdx.x & 15) * 8;
+  uint4 v = make_uint4(0, 0, 0, 0);
+  if (c < g.K) v = *reinterpret_cast<const uint4*>(g.x + (int64_t)row * g.ldx + 2 * c);  // the pitch holds whole pieces
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  float f[8];
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    f[i] = c + i < g.K ? ((i & 1) ? __uint_as_float(w[i >> 1] & 0xFFFF0000u) : __uint_as_float(w[i >> 1] << 16)) : 0.f;
+    m = max(m, finite_bits(f[i]));
+  }
+  const uint32_t byte = kept_byte(tile_max<16>(m));
+  if (!on) return;
+  const float inv = kept_inverse(byte);
+  store8_nt(g.kc + (int64_t)row * (g.by.per_row * (int64_t)KEPT_TILE) + c, kept_codes4(f[0], f[1], f[2], f[3], inv),
+            kept_codes4(f[4], f[5], f[6], f[7], inv));
+  if ((threadIdx.x & 15) == 0) g.ke[t] = (uint8_t)byte;
+}
+
+__global__ void __launch_bounds__(256) values_kernel(Keep g, uint8_t* out, int64_t ldo) {
+  const int64_t q = ((int64_t)blockIdx.x * 256 + threadIdx.x) / 16;
+  if (q >= g.tiles) return;
+  const uint32_t t = (uint32_t)q, row = g.by.row(t);
+  const int c = (int)(t - row * g.by.per_row) * KEPT_TILE + (threadIdx.x & 15) * 8;
+  if (c >= g.K) return;
+  const uint2 v = *reinterpret_cast<const uint2*>(g.kc + (int64_t)row * (g.by.per_row * (int64_t)KEPT_TILE) + c);
+  const float scale = kept_scale(g.ke[t]);
+  float a[4], b[4];
+  kept_values4(v.x, scale, a);
+  kept_values4(v.y, scale, b);
+  // 4 significant bits: exact in bf16
+  *reinterpret_cast<uint4*>(out + (int64_t)row * ldo + 2 * c) =
+      make_uint4(pack_bf16(a[0], a[1]), pack_bf16(a[2], a[3]), pack_bf16(b[0], b[1]), pack_bf16(b[2], b[3]));
+}
+
+constexpr int64_t MAX_PITCH = 1 << 22, MAX_EXPERTS = 4096, MAX_GRID = ((int64_t)1 << 31) - 1;
+
+static int check(const char* fn, int64_t R, int64_t E, int64_t N, int64_t K, const int32_t* offsets) {
+  clear_error();
+  if (R < 0 || E < 1 || N < 1 || K < 1) return fail(NTLB_EINVAL, "%s: bad shape R %lld E %lld N %lld K %lld", fn, (long long)R, (long long)E, (long long)N, (long long)K);
+  if (E > MAX_EXPERTS || R > ((int64_t)1 << 30) || N > MAX_PITCH || K > MAX_PITCH) return fail(NTLB_EUNSUPPORTED, "%s: R %lld E %lld N %lld K %lld is too large", fn, (long long)R, (long long)E, (long long)N, (long long)K);
+  if (!offsets || !aligned(offsets, 4)) return fail(NTLB_EINVAL, "%s: bad offsets", fn);
+  return NTLB_OK;
+}
+// rows of whole 16-byte pieces
+static bool fits(const void* p, int64_t ld, int64_t cols) {
+  return p && aligned(p, 16) && ld % 8 == 0 && ld >= cols && ld <= MAX_PITCH;
+}
+static int bad(const char* fn, const char* what) {
+  return fail(NTLB_EINVAL, "%s: %s must lie in 16-byte aligned rows of whole 16-byte pieces, at most %lld values apart", fn, what, (long long)MAX_PITCH);
+}
+
+// The tile of y and dx: D = 256 where its tiles fill the chip
+static int tile_of(int64_t R, int64_t E, int64_t N) {
+  const int64_t live = std::min(R, E), m = cdiv(R, 256) + live / 2;
+  return m * cdiv(N, 256) >= split_device_cus() && R >= live * 128 ? 256 : 128;
+}
+template <bool DX>
+static int launch_rows(const char* fn, const Args& g, hipStream_t st) {
+  const int D = tile_of(g.R, g.E, g.N);
+  const int64_t n = (g.R / D + g.E + 1) * cdiv(g.N, D);  // every expert's last tile, and the last rows'
+  if (n > MAX_GRID) return fail(NTLB_EUNSUPPORTED, "%s: %lld tiles", fn, (long long)n);
+  if (D == 256) rows_kernel<256, DX><<<(unsigned)n, 512, 0, st>>>(g);
+  else rows_kernel<128, DX><<<(unsigned)n, 256, 0, st>>>(g);
+  return check_launch(fn);
+}
+
+}  // namespace grouped
+}  // namespace ntlb
+
+using namespace ntlb;
+
+extern "C" int ntlb_grouped_matmul(const uint16_t* x, int64_t ldx, const uint16_t* w, int64_t ldw, int64_t w_stride,
+                                   const int32_t* offsets, int64_t R, int64_t E, int64_t N, int64_t K, uint16_t* y,
+                                   int64_t ldy, void* stream) {
+  const char* fn = "ntlb_grouped_matmul";
+  if (int rc = grouped::check(fn, R, E, N, K, offsets)) return rc;
+  if (R == 0) return NTLB_OK;
+  if (!grouped::fits(x, ldx, K)) return grouped::bad(fn, "x");
+  if (!grouped::fits(w, ldw, K) || w_stride % 8 || w_stride < 0) return grouped::bad(fn, "w");
+  if (!y || ldy < N) return fail(NTLB_EINVAL, "%s: bad y", fn);
+  grouped::Args g{(const uint8_t*)x, ldx * 2, (const uint8_t*)w, ldw * 2, w_stride * 2, offsets, R, (int)E, K, 0, N, y, ldy};
+  hipStream_t st = as_stream(stream);
+  // an expert's expected rows: few ones stream the weights
+  if (R <= 32 * std::min(R, E)) {
+    const int64_t blocks = cdiv(N, 16), n = (E + 1) * blocks;
+    if (n > grouped::MAX_GRID) return fail(NTLB_EUNSUPPORTED, "%s: %lld workgroups", fn, (long long)n);
+    grouped::few_kernel<1><<<(unsigned)n, 64 * grouped::FEW_WAVES, 0, st>>>(g, (int)blocks);
+    return check_launch(fn);
+  }
+  return grouped::launch_rows<false>(fn, g, st);
+}
+
+extern "C" int ntlb_grouped_matmul_dx(const uint16_t* dy, int64_t lddy, const uint16_t* w, int64_t ldw, int64_t w_stride,
+                                      const int32_t* offsets, int64_t R, int64_t E, int64_t N, int64_t K, uint16_t* dx,
+                                      int64_t lddx, void* stream) {
+  const char* fn = "ntlb_grouped_matmul_dx";
+  if (int rc = grouped::check(fn, R, E, N, K, offsets)) return rc;
+  if (R == 0) return NTLB_OK;
+  if (!grouped::fits(dy, lddy, N)) return grouped::bad(fn, "dy");
+  if (!grouped::fits(w, ldw, K) || w_stride % 8 || w_stride < 0) return grouped::bad(fn, "w");
+  if (!dx || lddx < K) return fail(NTLB_EINVAL, "%s: bad dx", fn);
+  grouped::Args g{(const uint8_t*)dy, lddy * 2, (const uint8_t*)w, ldw * 2, w_stride * 2, offsets, R, (int)E, N, 0, K, dx, lddx};
+  return grouped::launch_rows<true>(fn, g, as_stream(stream));
+}
+
+extern "C" int ntlb_grouped_matmul_dw(const uint16_t* dy, int64_t lddy, const uint16_t* x, int64_t ldx,
+                                      const int32_t* offsets, int64_t R, int64_t E, int64_t N, int64_t K, uint16_t* dw,
+                                      void* stream) {
+  const char* fn = "ntlb_grouped_matmul_dw";
+  if (int rc = grouped::check(fn, R, E, N, K, offsets)) return rc;
+  if (!dw) return fail(NTLB_EINVAL, "%s: bad dw", fn);
+  if (R > 0 && !grouped::fits(dy, lddy, N)) return grouped::bad(fn, "dy");
+  if (R > 0 && !grouped::fits(x, ldx, K)) return grouped::bad(fn, "x");
+  grouped::Args g{(const uint8_t*)dy, lddy * 2, (const uint8_t*)x, ldx * 2, 0, offsets, R, (int)E, 0, N, K, dw, K};
+  const int D = N > 128 && K > 128 && E * cdiv(N, 256) * cdiv(K, 256) >= split_device_cus() ? 256 : 128;
+  const int64_t n = E * cdiv(cdiv(N, D) * cdiv(K, D), 8) * 8;
+  if (n > grouped::MAX_GRID) return fail(NTLB_EUNSUPPORTED, "%s: %lld tiles", fn, (long long)n);
+  hipStream_t st = as_stream(stream);
+  if (D == 256) grouped::weight_kernel<256><<<(unsigned)n, 512, 0, st>>>(g);
+  else grouped::weight_kernel<128><<<(unsigned)n, 256, 0, st>>>(g);
+  return check_launch(fn);
+}
+
+extern "C" int ntlb_kept_rows(const uint16_t* x, int64_t ldx, int64_t R, int64_t K, uint8_t* kept, uint8_t* kept_exp,
+                              void* stream) {
+  const char* fn = "ntlb_kept_rows";
+  clear_error();
+  if (R < 0 || K < 1 || K > grouped::MAX_PITCH) return fail(NTLB_EINVAL, "%s: bad shape %lld x %lld", fn, (long long)R, (long long)K);
+  if (R == 0) return NTLB_OK;
+  if (!grouped::fits(x, ldx, K)) return grouped::bad(fn, "x");
+  if (!kept || !aligned(kept, 16) || !kept_exp) return fail(NTLB_EINVAL, "%s: bad kept codes", fn);
+  const int64_t NT = cdiv(K, KEPT_TILE);
+  return row_pieces(R, NT, [&](int64_t r, int64_t n) {
+    grouped::Keep g{(const uint8_t*)(x + r * ldx), ldx * 2, n * NT, (int)K, TileRows(NT), kept + r * NT * KEPT_TILE, kept_exp + r * NT};
+    grouped::keep_kernel<<<(unsigned)cdiv(g.tiles, 16), 256, 0, as_stream(stream)>>>(g);
+    return check_launch(fn);
+  });
+}
+
+extern "C" int ntlb_kept_values(const uint8_t* kept, const uint8_t* kept_exp, int64_t R, int64_t K, uint16_t* out,
+                                int64_t ldo, void* stream) {
+  const char* fn = "ntlb_kept_values";
+  clear_error();
+  if (R < 0 || K < 1 || K > grouped::MAX_PITCH) return fail(NTLB_EINVAL, "%s: bad shape %lld x %lld", fn, (long long)R, (long long)K);
+  if (R == 0) return NTLB_OK;
+  if (!grouped::fits(out, ldo, K)) return grouped::bad(fn, "out");
+  if (!kept || !aligned(kept, 16) || !kept_exp) return fail(NTLB_EINVAL, "%s: bad kept codes", fn);
+  const int64_t NT = cdiv(K, KEPT_TILE);
+  return row_pieces(R, NT, [&](int64_t r, int64_t n) {
+    grouped::Keep g{nullptr, 0, n * NT, (int)K, TileRows(NT), const_cast<uint8_t*>(kept) + r * NT * KEPT_TILE, const_cast<uint8_t*>(kept_exp) + r * NT};
+    grouped::values_kernel<<<(unsigned)cdiv(g.tiles, 16), 256, 0, as_stream(stream)>>>(g, (uint8_t*)(out + r * ldo), ldo * 2);
+    return check_launch(fn);
+  });
+}

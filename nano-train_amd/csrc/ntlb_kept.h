@@ -11,11 +11,38 @@
 
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
+#include <cstdint>
+
 #include "ntlb_device.h"
 
 namespace ntlb {
 
 constexpr int KEPT_TILE = 128;
+
+// Tiles of rows counted in one row after another, `per_row` a row: which row a tile is of, by a
+// product (q / per_row = q mul >> (31 + l), exact for q < 2^31, where 2^l >= per_row).
+struct TileRows {
+  uint32_t per_row, mul, shift;
+  __host__ TileRows(int64_t n = 1) : per_row((uint32_t)n), mul(0), shift(0) {
+    int l = 0;
+    while (((int64_t)1 << l) < n) ++l;
+    if (n == 1) return;
+    mul = (uint32_t)(((uint64_t)1 << (31 + l)) / (uint64_t)n + 1);
+    shift = (uint32_t)(l - 1);
+  }
+  __device__ __forceinline__ uint32_t row(uint32_t tile) const { return per_row == 1 ? tile : __umulhi(tile, mul) >> shift; }
+};
+// Launches over tiles take at most this many (their threads' workgroups are counted
+// in 32 bits too): f(first row, rows) for each piece of T rows.
+constexpr int64_t MAX_TILES = (int64_t)1 << 27;
+template <typename F>
+inline int row_pieces(int64_t T, int64_t per_row, F f) {
+  const int64_t step = std::max<int64_t>(1, MAX_TILES / per_row);
+  for (int64_t t = 0; t < T; t += step)
+    if (int rc = f(t, std::min(step, T - t))) return rc;
+  return 0;
+}
 
 // The byte of a tile whose largest finite magnitude has these bits (1.75 2^8 = 448)
 __device__ __forceinline__ uint32_t kept_byte(uint32_t amax_bits) {

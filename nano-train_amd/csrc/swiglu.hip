@@ -32,7 +32,7 @@ struct Args {
   int64_t ldx;  // in bytes, as the others
   int64_t tiles;  // T NT
   int I, NT, block;
-  uint32_t mul, shift;  // division by NT
+  TileRows by;  // of NT tiles
   void* h;
   int64_t ldh;
   uint8_t* kc;
@@ -97,8 +97,7 @@ struct At {
     tile = ((int64_t)blockIdx.x * THREADS + threadIdx.x) / LANES;
     on = tile < g.tiles;
     if (!on) tile = g.tiles - 1;  // its lanes walk along and write nothing
-    const uint32_t q = (uint32_t)tile;
-    const uint32_t r = g.NT == 1 ? q : __umulhi(q, g.mul) >> g.shift;
+    const uint32_t q = (uint32_t)tile, r = g.by.row(q);
     row = r;
     c = (int)(q - r * (uint32_t)g.NT) * 128 + (int)(threadIdx.x % LANES) * N;
     n = min(max(g.I - c, 0), N);
@@ -221,32 +220,23 @@ template <int DT>
 static void launch_dt(const Args& g, bool backward, hipStream_t st) {
   g.I % El<DT>::n ? launch_of<DT, false>(g, backward, st) : launch_of<DT, true>(g, backward, st);
 }
-// tiles are counted in 32 bits and their threads' workgroups with them: rows beyond
-// that go in launches of their own
-constexpr int64_t MAX_TILES = (int64_t)1 << 27;
-static int run(const char* fn, Args g, int dt, int64_t T, bool backward, void* stream) {
-  const int64_t e = dtype_size(dt), step = std::max<int64_t>(1, MAX_TILES / g.NT);
-  int l = 0;
-  while (((int64_t)1 << l) < g.NT) ++l;
-  // q / NT = (q mul) >> (31 + l), exact for q < 2^31
-  g.mul = g.NT == 1 ? 0 : (uint32_t)(((uint64_t)1 << (31 + l)) / (uint64_t)g.NT + 1);
-  g.shift = (uint32_t)std::max(l - 1, 0);
-  g.ldx *= e; g.ldh *= e; g.lddh *= e; g.lddx *= e;
-  for (int64_t t = 0; t < T; t += step) {
-    const int64_t n = std::min(step, T - t);
+static int run(const char* fn, const Args& all, int dt, int64_t T, bool backward, void* stream) {
+  const int64_t e = dtype_size(dt);
+  return row_pieces(T, all.NT, [&](int64_t t, int64_t n) {
+    Args g = all;
+    g.ldx *= e; g.ldh *= e; g.lddh *= e; g.lddx *= e;
     g.tiles = n * g.NT;
+    if (g.x) g.x = (const uint8_t*)g.x + t * g.ldx;
+    if (g.h) g.h = (uint8_t*)g.h + t * g.ldh;
+    if (g.dh) g.dh = (const uint8_t*)g.dh + t * g.lddh;
+    if (g.dx) g.dx = (uint8_t*)g.dx + t * g.lddx;
+    if (g.kc) g.kc += t * 2 * 128 * g.NT;
+    if (g.ke) g.ke += t * 2 * g.NT;
     if (dt == NTLB_F32) launch_dt<DT_F32>(g, backward, as_stream(stream));
     else if (dt == NTLB_BF16) launch_dt<DT_BF16>(g, backward, as_stream(stream));
     else launch_dt<DT_F16>(g, backward, as_stream(stream));
-    if (int rc = check_launch(fn)) return rc;
-    if (g.x) g.x = (const uint8_t*)g.x + n * g.ldx;
-    if (g.h) g.h = (uint8_t*)g.h + n * g.ldh;
-    if (g.dh) g.dh = (const uint8_t*)g.dh + n * g.lddh;
-    if (g.dx) g.dx = (uint8_t*)g.dx + n * g.lddx;
-    if (g.kc) g.kc += n * 2 * 128 * g.NT;
-    if (g.ke) g.ke += n * 2 * g.NT;
-  }
-  return NTLB_OK;
+    return check_launch(fn);
+  });
 }
 static int begin(const char* fn, Args& g, int dt, int64_t T, int64_t I, int64_t block, const uint8_t* kept,
                  const uint8_t* kept_exp) {
@@ -258,7 +248,7 @@ static int begin(const char* fn, Args& g, int dt, int64_t T, int64_t I, int64_t 
   if ((kept == nullptr) != (kept_exp == nullptr)) return fail(NTLB_EINVAL, "%s: kept codes and their exponents go together", fn);
   if (kept && !aligned(kept, 16)) return fail(NTLB_EINVAL, "%s: kept codes must be 16-byte aligned", fn);
   g = Args{};
-  g.I = (int)I; g.NT = (int)cdiv(I, 128); g.block = (int)(block ? block : I);
+  g.I = (int)I; g.NT = (int)cdiv(I, 128); g.by = TileRows(g.NT); g.block = (int)(block ? block : I);
   g.kc = const_cast<uint8_t*>(kept); g.ke = const_cast<uint8_t*>(kept_exp);
   return NTLB_OK;
 }

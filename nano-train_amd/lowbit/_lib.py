@@ -156,6 +156,11 @@ SIGNATURES = {
     "ntlb_rms_norm_workspace_bytes": [_I32, _I64, _I64],
     "ntlb_swiglu_rows": [_P, _I32, _I64, _I64, _I64, _I64, _P, _I64, _P, _P, _P],
     "ntlb_swiglu_rows_backward": [_P, _I32, _I64, _I64, _I64, _I64, _P, _P, _P, _I64, _P, _I64, _P],
+    "ntlb_grouped_matmul": [_P, _I64, _P, _I64, _I64, _P, _I64, _I64, _I64, _I64, _P, _I64, _P],
+    "ntlb_grouped_matmul_dx": [_P, _I64, _P, _I64, _I64, _P, _I64, _I64, _I64, _I64, _P, _I64, _P],
+    "ntlb_grouped_matmul_dw": [_P, _I64, _P, _I64, _P, _I64, _I64, _I64, _I64, _P, _P],
+    "ntlb_kept_rows": [_P, _I64, _I64, _I64, _P, _P, _P],
+    "ntlb_kept_values": [_P, _P, _I64, _I64, _P, _I64, _P],
 }
 
 
@@ -228,7 +233,7 @@ def autograd():
                                    f"`python nano-train_amd/build.py` ({exc})") from exc
             names = [n for n in SIGNATURES
                      if n.startswith(("ntlb_layer_norm", "ntlb_route", "ntlb_linear_xent", "ntlb_pad_rows", "ntlb_rms_norm",
-                                   "ntlb_swiglu_rows"))]
+                                   "ntlb_swiglu_rows", "ntlb_grouped_matmul", "ntlb_kept"))]
             mod.bind({"error": LowBitKernelError,
                       **{n: ctypes.cast(getattr(L, n), ctypes.c_void_p).value for n in [*names, "ntlb_last_error"]}})
             _autograd = mod
