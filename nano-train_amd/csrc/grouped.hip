@@ -58,11 +58,35 @@ __device__ __forceinline__ int wave_scan(int v, int lane) {  // inclusive
   return v;
 }
 
-// Tile pid of those of all experts' rows (D each) by num_n column tiles; each XCD
-// walks a contiguous range of them.  t: the tile among its expert's.
+// The order of a grid's tiles.  Workgroup pid runs on XCD pid % 8, 32 of one XCD at a
+// time (its compute units): those take 32 tiles next to each other, which share
+// their operands in the XCD's L2.
+__device__ __forceinline__ int order(int pid) {
+  const int at = pid >> 3;
+  return (((pid & 7) + 8 * (at >> 5)) << 5) + (at & 31);
+}
+static int64_t ordered_grid(int64_t tiles) { return cdiv(tiles, 256) * 256; }
+
+// how many of the wave's values come before this lane's, highest first
+__device__ __forceinline__ int wave_place(int v, int lane, int lanes) {
+  int place = 0;
+  for (int j = 0; j < lanes; ++j) {
+    const int o = __builtin_amdgcn_readlane(v, j);
+    place += o > v || (o == v && j < lane);
+  }
+  return lane < lanes ? place : -1;
+}
+
+// Tile pid of all experts' rows (D each) by num_n column tiles, expert after expert,
+// then the rows behind the last expert's (e == E).  Each XCD walks a contiguous range,
+// so that few of them read one expert's weights.  m0: first row, of the expert's n; tn:
+// column tile.
 struct Found {
-  int e, lo, n, t;
+  int e, lo, n, m0, tn;
 };
+// row tiles walked side by side: of an expert for y and dx, of dW (32768 rows, 32 experts,
+// 4096 x 7168: y 1716 us with four, 1698 with eight; dx 1810, 1798; dW 1903, 1947)
+constexpr int GROUP_M = 8, GROUP_W = 4;
 template <int D>
 __device__ __forceinline__ bool find(const Args& g, int num_n, int pid, Found& f) {
   const int lane = threadIdx.x & 63, R = (int)g.R;
@@ -75,33 +99,33 @@ __device__ __forceinline__ bool find(const Args& g, int num_n, int pid, Found& f
   total *= num_n;
   if (pid >= total) return false;
   const int xcd = pid & 7, per = total >> 3, extra = total & 7;
-  pid = xcd * per + min(xcd, extra) + (pid >> 3);
-  int before = 0;
+  int q = xcd * per + min(xcd, extra) + (pid >> 3);
   for (int c = 0; c <= g.E; c += 64) {
-    Rows r(g.offsets, min(c + lane, g.E), g.E, R);
-    const int m = c + lane <= g.E ? (r.n + D - 1) / D * num_n : 0, upto = before + wave_scan(m, lane);
-    const uint64_t b = __ballot(upto > pid);
+    const Rows r(g.offsets, min(c + lane, g.E), g.E, R);
+    const int m = c + lane <= g.E ? (r.n + D - 1) / D * num_n : 0, upto = wave_scan(m, lane);
+    const uint64_t b = __ballot(upto > q);
     if (b) {
       const int at = __builtin_ctzll(b);
       f.e = c + at;
       f.lo = __builtin_amdgcn_readlane(r.lo, at);
       f.n = __builtin_amdgcn_readlane(r.n, at);
-      f.t = pid - (__builtin_amdgcn_readlane(upto, at) - __builtin_amdgcn_readlane(m, at));
+      const int t = q - (__builtin_amdgcn_readlane(upto, at) - __builtin_amdgcn_readlane(m, at));
+      const int first = t / (GROUP_M * num_n) * GROUP_M, side = min((f.n + D - 1) / D - first, GROUP_M), in = t - first * num_n;
+      f.m0 = (first + in % side) * D;
+      f.tn = in / side;
       return true;
     }
-    before = __builtin_amdgcn_readlane(upto, 63);
+    q -= __builtin_amdgcn_readlane(upto, 63);
   }
   return false;
 }
 
-// A wave's result rows through its part of the stages
+// A wave's result rows through its part of a stage
 template <int D>
 __device__ __forceinline__ void store_tile(const v4f (&acc)[D / 32][4], int wave, int wm, int wn, int lane, int64_t m0,
-                                           int64_t n0, int64_t M, int64_t N, uint16_t* out, int64_t ldo, uint8_t* la0,
-                                           uint8_t* lb0, uint8_t* la1, uint8_t* lb1) {
-  constexpr int MT = D / 32, PER = D * ROWB / 16384;
-  uint8_t* stage = (wave / PER == 0 ? la0 : wave / PER == 1 ? lb0 : wave / PER == 2 ? la1 : lb1) + (wave % PER) * 16384;
-  store_bf16<MT, true>(stage, lane, m0 + wm * 16 * MT, n0 + wn * 64, M, N, out, ldo, [&](int tm, int tn, float (&v)[4]) {
+                                           int64_t n0, int64_t M, int64_t N, uint16_t* out, int64_t ldo, uint8_t* stage) {
+  constexpr int MT = D / 32;
+  store_bf16<MT, true>(stage + wave * 4096, lane, m0 + wm * 16 * MT, n0 + wn * 64, M, N, out, ldo, [&](int tm, int tn, float (&v)[4]) {
 #pragma unroll
     for (int r = 0; r < 4; ++r) v[r] = acc[tm][tn][r];
   });
@@ -111,65 +135,110 @@ __device__ __forceinline__ void store_tile(const v4f (&acc)[D / 32][4], int wave
   v4f acc[D / 32][4];                      \
   _Pragma("unroll") for (int i = 0; i < D / 32; ++i) _Pragma("unroll") for (int j = 0; j < 4; ++j) acc[i][j] = (v4f){0.f, 0.f, 0.f, 0.f}
 
-constexpr int GROUP_M = 4;  // row tiles of an expert that are walked side by side
-
-// y (W by rows) and dx (W transposed)
-template <int D, bool DX>
+// y: W by rows.  Both operands come in the same way; A's copies two steps ahead.
+template <int D>
 __global__ void __launch_bounds__(2 * D, D == 256 ? 1 : 2) rows_kernel(Args g) {
+  NTLB_TILE_STAGES_AHEAD(D);
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  constexpr int WAVES_N = D / 64;
+  const int wm = wave / WAVES_N, wn = wave % WAVES_N;
+  Found f;
+  if (!find<D>(g, (int)((g.N + D - 1) / D), (int)blockIdx.x, f)) return;
+  const int64_t m0 = f.m0, n0 = (int64_t)f.tn * D;
+  NTLB_ZERO_ACC(D);
+  if (f.e < g.E) {
+    RowWalk<D> ca, cb;
+    ca.init(Mat{g.a + (int64_t)f.lo * g.lda, g.lda, f.n, g.k}, m0, wave, lane);
+    cb.init(Mat{g.b + (int64_t)f.e * g.b_expert, g.ldb, g.N, g.k}, n0, wave, lane);
+    prime_ahead(ca, cb, wave, stages);
+    multiply_ahead<D, false, false>(ca, cb, (int)((g.k + KSTEP - 1) / KSTEP), acc, wm, wn, wave, lane, stages);
+  }
+  store_tile<D>(acc, wave, wm, wn, own_lane(), m0, n0, f.n, g.N, g.out + (int64_t)f.lo * g.ldo, g.ldo, stage_4);
+}
+
+// dx: W transposed
+template <int D>
+__global__ void __launch_bounds__(2 * D, D == 256 ? 1 : 2) inputs_kernel(Args g) {
   NTLB_TILE_STAGES(D);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   constexpr int WAVES_N = D / 64;
   const int wm = wave / WAVES_N, wn = wave % WAVES_N;
-  const int num_n = (int)((g.N + D - 1) / D);
   Found f;
-  if (!find<D>(g, num_n, (int)blockIdx.x, f)) return;
-  const int num_m = (f.n + D - 1) / D, group = f.t / (GROUP_M * num_n), first_m = group * GROUP_M;
-  const int gsize = min(num_m - first_m, GROUP_M), in_group = f.t - first_m * num_n;
-  const int64_t m0 = (int64_t)(first_m + in_group % gsize) * D, n0 = (int64_t)(in_group / gsize) * D;
+  if (!find<D>(g, (int)((g.N + D - 1) / D), (int)blockIdx.x, f)) return;
+  const int64_t m0 = f.m0, n0 = (int64_t)f.tn * D;
   NTLB_ZERO_ACC(D);
   if (f.e < g.E) {
     RowCopy<D> ca;
-    typename std::conditional<DX, TrCopy<D>, RowCopy<D>>::type cb;
+    TrCopy<D> cb;
     ca.init(Mat{g.a + (int64_t)f.lo * g.lda, g.lda, f.n, g.k}, m0, wave, lane);
     cb.init(Mat{g.b + (int64_t)f.e * g.b_expert, g.ldb, g.N, g.k}, n0, wave, lane);
-    multiply<D, false, DX>(ca, cb, 0, (int)((g.k + KSTEP - 1) / KSTEP), acc, wm, wn, wave, lane, la0, lb0, la1, lb1);
+    multiply<D, false, true>(ca, cb, 0, (int)((g.k + KSTEP - 1) / KSTEP), acc, wm, wn, wave, lane, la0, lb0, la1, lb1);
   }
-  store_tile<D>(acc, wave, wm, wn, lane, m0, n0, f.n, g.N, g.out + (int64_t)f.lo * g.ldo, g.ldo, la0, lb0, la1, lb1);
+  store_tile<D>(acc, wave, wm, wn, lane, m0, n0, f.n, g.N, g.out + (int64_t)f.lo * g.ldo, g.ldo, la1);
 }
 
 // dW: every expert's tiles, each with the expert's rows as its contraction.  Experts
-// with many rows come first (among 64 neighbours), and each XCD takes an eighth of
-// each expert's tiles, so that long and short tiles are everywhere.
+// with many rows come first (among 64 neighbours).  A contraction of a few hundred
+// rows is 10 to 20 steps, so what stands around it counts: a workgroup stays for
+// tile after tile, and the next one's first copies are under way while this one is
+// stored.  Measured at 32 experts of 1024 rows on average, 4096 x 7168: 2.01 ms with an
+// eighth of each expert's tiles to each XCD, whose compute units then work on
+// different ones and read twice as much into L2 (3.2 GB); 32 at a time 1.81; without
+// staying 1.93.
 template <int D>
-__global__ void __launch_bounds__(2 * D, D == 256 ? 1 : 2) weight_kernel(Args g) {
+__global__ void __launch_bounds__(2 * D, D == 256 ? 1 : 2) weight_kernel(Args g, int count) {
   NTLB_TILE_STAGES(D);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   constexpr int WAVES_N = D / 64;
   const int wm = wave / WAVES_N, wn = wave % WAVES_N;
-  const int num_n = (int)((g.N + D - 1) / D), num_m = (int)((g.M + D - 1) / D), tiles = num_m * num_n, share = (tiles + 7) / 8;
-  const int pid = (int)blockIdx.x, xcd = pid & 7, at = pid >> 3, rank = at / share;
-  const int t = xcd * share + at - rank * share;
-  if (t >= tiles || rank >= g.E) return;
-  const int c = rank & ~63, here = min(g.E - c, 64);
-  const Rows r(g.offsets, min(c + lane, g.E - 1), g.E, (int)g.R);
-  int place = 0;
-  for (int j = 0; j < here; ++j) {
-    const int o = __builtin_amdgcn_readlane(r.n, j);
-    place += o > r.n || (o == r.n && j < lane);
+  const int num_n = (int)((g.N + D - 1) / D), num_m = (int)((g.M + D - 1) / D), tiles = num_m * num_n;
+  int chunk = -1, place = 0, lo = 0, n = 0;  // of 64 experts, a lane each: how many have more rows; its rows
+  struct Tile {
+    int e, lo, n, m, c;  // m, c: row and column tile
+  };
+  // the next tile from pid on, and its pid; count: none is left
+  auto next = [&](int pid, Tile& t) {
+    for (; pid < count; pid += (int)gridDim.x) {
+      const int at = order(pid), rank = at / tiles, q = at - rank * tiles;
+      if (rank >= g.E) continue;
+      const int c = rank & ~63;
+      if (c != chunk) {
+        chunk = c;
+        const Rows r(g.offsets, min(c + lane, g.E - 1), g.E, (int)g.R);
+        lo = r.lo;
+        n = r.n;
+        place = wave_place(n, lane, min(g.E - c, 64));
+      }
+      const int who = __builtin_ctzll(__ballot(place == (rank & 63)));
+      t.e = c + who;
+      t.lo = __builtin_amdgcn_readlane(lo, who);
+      t.n = __builtin_amdgcn_readlane(n, who);
+      const int first = q / (GROUP_W * num_n) * GROUP_W, side = min(num_m - first, GROUP_W), in = q - first * num_n;
+      t.m = first + in % side;
+      t.c = in / side;
+      break;
+    }
+    return pid;
+  };
+  TrCopy<D> ca, cb;
+  auto begin = [&](const Tile& t) {
+    ca.init(Mat{g.a + (int64_t)t.lo * g.lda, g.lda, g.M, t.n}, (int64_t)t.m * D, wave, lane);
+    cb.init(Mat{g.b + (int64_t)t.lo * g.ldb, g.ldb, g.N, t.n}, (int64_t)t.c * D, wave, lane);
+    prime(ca, cb, 0, wave, la0, lb0);
+  };
+  Tile t, u;
+  int pid = next((int)blockIdx.x, t);
+  if (pid >= count) return;
+  if (t.n > 0) begin(t);
+  for (;;) {
+    NTLB_ZERO_ACC(D);
+    if (t.n > 0) multiply<D, true, true, true>(ca, cb, 0, (t.n + KSTEP - 1) / KSTEP, acc, wm, wn, wave, lane, la0, lb0, la1, lb1);
+    pid = next(pid + (int)gridDim.x, u);
+    if (pid < count && u.n > 0) begin(u);
+    store_tile<D>(acc, wave, wm, wn, own_lane(), (int64_t)t.m * D, (int64_t)t.c * D, g.M, g.N, g.out + (int64_t)t.e * g.M * g.ldo, g.ldo, la1);
+    if (pid >= count) break;
+    t = u;
   }
-  const int who = __builtin_ctzll(__ballot(lane < here && place == (rank & 63)));
-  const int e = c + who, lo = __builtin_amdgcn_readlane(r.lo, who), n = __builtin_amdgcn_readlane(r.n, who);
-  const int group = t / (GROUP_M * num_n), first_m = group * GROUP_M;
-  const int gsize = min(num_m - first_m, GROUP_M), in_group = t - first_m * num_n;
-  const int64_t m0 = (int64_t)(first_m + in_group % gsize) * D, n0 = (int64_t)(in_group / gsize) * D;
-  NTLB_ZERO_ACC(D);
-  if (n > 0) {
-    TrCopy<D> ca, cb;
-    ca.init(Mat{g.a + (int64_t)lo * g.lda, g.lda, g.M, n}, m0, wave, lane);
-    cb.init(Mat{g.b + (int64_t)lo * g.ldb, g.ldb, g.N, n}, n0, wave, lane);
-    multiply<D, true, true>(ca, cb, 0, (n + KSTEP - 1) / KSTEP, acc, wm, wn, wave, lane, la0, lb0, la1, lb1);
-  }
-  store_tile<D>(acc, wave, wm, wn, lane, m0, n0, g.M, g.N, g.out + (int64_t)e * g.M * g.ldo, g.ldo, la0, lb0, la1, lb1);
 }
 
 // ---------------------------------------------------------------------------
@@ -388,15 +457,8 @@ static int tile_of(int64_t R, int64_t E, int64_t N) {
   const int64_t live = std::min(R, E), m = cdiv(R, 256) + live / 2;
   return m * cdiv(N, 256) >= split_device_cus() && R >= live * 128 ? 256 : 128;
 }
-template <bool DX>
-static int launch_rows(const char* fn, const Args& g, hipStream_t st) {
-  const int D = tile_of(g.R, g.E, g.N);
-  const int64_t n = (g.R / D + g.E + 1) * cdiv(g.N, D);  // every expert's last tile, and the last rows'
-  if (n > MAX_GRID) return fail(NTLB_EUNSUPPORTED, "%s: %lld tiles", fn, (long long)n);
-  if (D == 256) rows_kernel<256, DX><<<(unsigned)n, 512, 0, st>>>(g);
-  else rows_kernel<128, DX><<<(unsigned)n, 256, 0, st>>>(g);
-  return check_launch(fn);
-}
+// workgroups of y's and dx' tiles: every expert's last one too, and the rows' behind
+static int64_t row_tiles(const Args& g, int D) { return (g.R / D + g.E + 1) * cdiv(g.N, D); }
 
 }  // namespace grouped
 }  // namespace ntlb
@@ -421,7 +483,12 @@ extern "C" int ntlb_grouped_matmul(const uint16_t* x, int64_t ldx, const uint16_
     grouped::few_kernel<1><<<(unsigned)n, 64 * grouped::FEW_WAVES, 0, st>>>(g, (int)blocks);
     return check_launch(fn);
   }
-  return grouped::launch_rows<false>(fn, g, st);
+  const int D = grouped::tile_of(R, E, N);
+  const int64_t n = grouped::row_tiles(g, D);
+  if (n > grouped::MAX_GRID) return fail(NTLB_EUNSUPPORTED, "%s: %lld tiles", fn, (long long)n);
+  if (D == 256) grouped::rows_kernel<256><<<(unsigned)n, 512, 0, st>>>(g);
+  else grouped::rows_kernel<128><<<(unsigned)n, 256, 0, st>>>(g);
+  return check_launch(fn);
 }
 
 extern "C" int ntlb_grouped_matmul_dx(const uint16_t* dy, int64_t lddy, const uint16_t* w, int64_t ldw, int64_t w_stride,
@@ -434,7 +501,13 @@ extern "C" int ntlb_grouped_matmul_dx(const uint16_t* dy, int64_t lddy, const ui
   if (!grouped::fits(w, ldw, K) || w_stride % 8 || w_stride < 0) return grouped::bad(fn, "w");
   if (!dx || lddx < K) return fail(NTLB_EINVAL, "%s: bad dx", fn);
   grouped::Args g{(const uint8_t*)dy, lddy * 2, (const uint8_t*)w, ldw * 2, w_stride * 2, offsets, R, (int)E, N, 0, K, dx, lddx};
-  return grouped::launch_rows<true>(fn, g, as_stream(stream));
+  hipStream_t st = as_stream(stream);
+  const int D = grouped::tile_of(R, E, K);
+  const int64_t n = grouped::row_tiles(g, D);
+  if (n > grouped::MAX_GRID) return fail(NTLB_EUNSUPPORTED, "%s: %lld tiles", fn, (long long)n);
+  if (D == 256) grouped::inputs_kernel<256><<<(unsigned)n, 512, 0, st>>>(g);
+  else grouped::inputs_kernel<128><<<(unsigned)n, 256, 0, st>>>(g);
+  return check_launch(fn);
 }
 
 extern "C" int ntlb_grouped_matmul_dw(const uint16_t* dy, int64_t lddy, const uint16_t* x, int64_t ldx,
@@ -447,11 +520,12 @@ extern "C" int ntlb_grouped_matmul_dw(const uint16_t* dy, int64_t lddy, const ui
   if (R > 0 && !grouped::fits(x, ldx, K)) return grouped::bad(fn, "x");
   grouped::Args g{(const uint8_t*)dy, lddy * 2, (const uint8_t*)x, ldx * 2, 0, offsets, R, (int)E, 0, N, K, dw, K};
   const int D = N > 128 && K > 128 && E * cdiv(N, 256) * cdiv(K, 256) >= split_device_cus() ? 256 : 128;
-  const int64_t n = E * cdiv(cdiv(N, D) * cdiv(K, D), 8) * 8;
+  const int64_t n = grouped::ordered_grid(E * cdiv(N, D) * cdiv(K, D));
   if (n > grouped::MAX_GRID) return fail(NTLB_EUNSUPPORTED, "%s: %lld tiles", fn, (long long)n);
   hipStream_t st = as_stream(stream);
-  if (D == 256) grouped::weight_kernel<256><<<(unsigned)n, 512, 0, st>>>(g);
-  else grouped::weight_kernel<128><<<(unsigned)n, 256, 0, st>>>(g);
+  const unsigned wgs = (unsigned)std::min<int64_t>(n, cdiv(split_device_cus(), 8) * 8 * (D == 256 ? 1 : 2));
+  if (D == 256) grouped::weight_kernel<256><<<wgs, 512, 0, st>>>(g, (int)n);
+  else grouped::weight_kernel<128><<<wgs, 256, 0, st>>>(g, (int)n);
   return check_launch(fn);
 }
 

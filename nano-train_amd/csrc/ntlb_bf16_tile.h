@@ -57,6 +57,11 @@ struct FragAt {
   __device__ __forceinline__ void renew() {
     if constexpr (TR) asm volatile("" : "+v"(lo));
   }
+  // likewise where the stages are many: a sum for each of them would be kept
+  __device__ __forceinline__ void anew() {
+    if constexpr (TR) asm volatile("" : "+v"(lo));
+    else asm volatile("" : "+v"(lo), "+v"(hi));
+  }
 };
 // the fragment `group` groups of 16 rows on
 template <bool TR, int D>
@@ -85,6 +90,13 @@ __device__ __forceinline__ v4f mma(const v8i& p, const v8i& q, v4f acc) {
   const v4i a = {p[4 * HALF], p[4 * HALF + 1], p[4 * HALF + 2], p[4 * HALF + 3]};
   const v4i b = {q[4 * HALF], q[4 * HALF + 1], q[4 * HALF + 2], q[4 * HALF + 3]};
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), acc, 0, 0, 0);
+}
+
+// the lane, counted anew: not a value that is kept in a register from before
+__device__ __forceinline__ int own_lane() {
+  int lane = (int)__builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u));
+  asm volatile("" : "+v"(lane));
+  return lane;
 }
 
 // the workgroup's barrier alone: what must have landed is waited for before it
@@ -144,6 +156,36 @@ struct RowCopy {
   __device__ __forceinline__ void issue(uint8_t* stage, int wave, int j) const {
     __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr_t)(stage + (wave + NW * j) * 1024), 16, o,
                                              at + (uint32_t)j * (8 * NW) * pitch, 0, 0);
+  }
+};
+
+// The same for steps that are set once each, in their order: what lies past the
+// columns is taken out of the lanes' offsets for good, which saves two registers
+template <int D>
+struct RowWalk {
+  __amdgpu_buffer_rsrc_t rs;
+  uint32_t off, pitch, at;
+  int k, wave;
+  __device__ __forceinline__ void init(const Mat& m, int64_t r0, int w, int lane) {
+    RowCopy<D> c;
+    c.init(m, r0, w, lane);
+    rs = c.rs;
+    off = c.off;
+    pitch = c.pitch;
+    k = __builtin_amdgcn_readfirstlane(c.k);
+    wave = w;
+  }
+  __device__ __forceinline__ void set(int kt) {
+    at = (uint32_t)kt * ROWB;
+    const int rem = k - kt * KSTEP;
+    if (rem < KSTEP) {
+      const int lane = own_lane(), col = ((lane & 7) ^ sw_perm(wave * 8 + (lane >> 3))) * 8;
+      off = col < rem ? off : 0x80000000u;
+    }
+  }
+  __device__ __forceinline__ void issue(uint8_t* stage, int w, int j) const {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr_t)(stage + (w + RowCopy<D>::NW * j) * 1024), 16, off,
+                                             at + (uint32_t)j * (8 * RowCopy<D>::NW) * pitch, 0, 0);
   }
 };
 
@@ -232,13 +274,15 @@ struct BlockTrCopy {
   }
 };
 
-// A wave's 16 MT x 64 output rows as bf16, 32 rows at a time through its LDS
-// (rows of 64 values and 16 bytes, so that neither side's lanes share banks) to
+// A wave's 16 MT x 64 output rows as bf16, 32 rows at a time through 4 KiB of LDS
+// (16-byte chunks XOR-swizzled by row, so that neither side's lanes share banks) to
 // stores of whole 128-byte lines.  value(tm, tn, v): the lane's four of a block.
 template <int MT, bool NTS, typename F>
 __device__ __forceinline__ void store_bf16(uint8_t* stage, int lane, int64_t m0, int64_t n0, int64_t M, int64_t N,
                                            uint16_t* out, int64_t ldo, F value) {
-  constexpr int PITCH = 64 * 2 + 16;
+  constexpr int PITCH = 64 * 2;
+  // whole tiles' stores without a branch of their own: 56 of them for each compute unit take 28 us less
+  const bool full = m0 + 16 * MT <= M && n0 + 64 <= N;
 #pragma unroll
   for (int part = 0; part < MT / 2; ++part) {
 #pragma unroll
@@ -247,29 +291,48 @@ __device__ __forceinline__ void store_bf16(uint8_t* stage, int lane, int64_t m0,
       for (int tn = 0; tn < 4; ++tn) {
         float v[4];
         value(part * 2 + t, tn, v);
-        *reinterpret_cast<uint2*>(stage + (t * 16 + (lane & 15)) * PITCH + (tn * 16 + (lane >> 4) * 4) * 2) =
+        *reinterpret_cast<uint2*>(stage + (t * 16 + (lane & 15)) * PITCH + (((tn * 2 + (lane >> 5)) ^ (lane & 7)) << 4) + ((lane >> 4) & 1) * 8) =
             make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]));
       }
     __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): the wave's rows are written
     __builtin_amdgcn_wave_barrier();
+    auto at = [&](int j) {  // the place of the lane's 16 bytes in quarter j
+      const int row = (lane >> 3) + 8 * j;
+      return m0 + part * 32 + row;
+    };
+    if (full) {
+      uint4 q[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int row = (lane >> 3) + 8 * j, c = lane & 7;
-      const int64_t m = m0 + part * 32 + row, n = n0 + c * 8;
-      const uint4 q = *reinterpret_cast<const uint4*>(stage + row * PITCH + c * 16);
-      if (m >= M || n >= N) continue;
-      uint16_t* o = out + m * ldo + n;
-      if (n + 8 <= N) {
-        const u32x4_2 v = {q.x, q.y, q.z, q.w};
+      for (int j = 0; j < 4; ++j) q[j] = *reinterpret_cast<const uint4*>(stage + ((lane >> 3) + 8 * j) * PITCH + (((lane & 7) ^ (lane >> 3)) << 4));
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const u32x4_2 v = {q[j].x, q[j].y, q[j].z, q[j].w};
+        u32x4_2* o = reinterpret_cast<u32x4_2*>(out + at(j) * ldo + n0 + (lane & 7) * 8);
         if constexpr (NTS)
-          __builtin_nontemporal_store(v, reinterpret_cast<u32x4_2*>(o));
+          __builtin_nontemporal_store(v, o);
         else
-          *reinterpret_cast<u32x4_2*>(o) = v;
-      } else {
-        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+          *o = v;
+      }
+    } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (n + i < N) o[i] = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
+      for (int j = 0; j < 4; ++j) {
+        const int c = lane & 7;
+        const int64_t m = at(j), n = n0 + c * 8;
+        const uint4 q = *reinterpret_cast<const uint4*>(stage + ((lane >> 3) + 8 * j) * PITCH + ((c ^ (lane >> 3)) << 4));
+        if (m >= M || n >= N) continue;
+        uint16_t* o = out + m * ldo + n;
+        if (n + 8 <= N) {
+          const u32x4_2 v = {q.x, q.y, q.z, q.w};
+          if constexpr (NTS)
+            __builtin_nontemporal_store(v, reinterpret_cast<u32x4_2*>(o));
+          else
+            *reinterpret_cast<u32x4_2*>(o) = v;
+        } else {
+          const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (n + i < N) o[i] = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
+        }
       }
     }
     __builtin_amdgcn_s_waitcnt(0xC07F);  // read before the next rows overwrite them
@@ -277,11 +340,24 @@ __device__ __forceinline__ void store_bf16(uint8_t* stage, int lane, int64_t m0,
   }
 }
 
+// the copies of step kt into a stage
+template <typename CA, typename CB>
+__device__ __forceinline__ void prime(CA& ca, CB& cb, int kt, int wave, uint8_t* la, uint8_t* lb) {
+  ca.set(kt);
+  cb.set(kt);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    ca.issue(la, wave, j);
+    cb.issue(lb, wave, j);
+  }
+}
+
 // acc += the product of K steps kb0 .. kb1 - 1 of a tile of D x D (256: eight waves
 // of 128 x 64, one workgroup a compute unit; 128: four of 64 x 64, two workgroups),
 // wave (wm, wn) of it.  la0 ... lb1: two stages of both operands, D * ROWB bytes
-// each, which nothing reads or writes any more afterwards.
-template <int D, bool TA, bool TB, typename CA, typename CB>
+// each, which nothing reads or writes any more afterwards.  PRIMED: prime() has been
+// called for step kb0 and the first stage.
+template <int D, bool TA, bool TB, bool PRIMED = false, typename CA, typename CB>
 __device__ __forceinline__ void multiply(CA& ca, CB& cb, int kb0, int kb1, v4f (&acc)[D / 32][4], int wm, int wn, int wave,
                                          int lane, uint8_t* la0, uint8_t* lb0, uint8_t* la1, uint8_t* lb1) {
   constexpr int MT = D / 32;
@@ -308,10 +384,7 @@ __device__ __forceinline__ void multiply(CA& ca, CB& cb, int kb0, int kb1, v4f (
       asm volatile("" : "+v"(acc[tm][0]), "+v"(acc[tm][1]), "+v"(acc[tm][2]), "+v"(acc[tm][3])::"memory");
       if (TB && !TA) __builtin_amdgcn_s_setprio(0);
     };
-    ca.set(kb0);
-    cb.set(kb0);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) copy(la0, lb0, j);
+    if constexpr (!PRIMED) prime(ca, cb, kb0, wave, la0, lb0);
     v8i b0[4], b1[4], af[4];
     FragAt<TA, D> fa(wm * 16 * MT, lane);
     FragAt<TB, D> fb(wn * 64, lane);
@@ -363,6 +436,109 @@ __device__ __forceinline__ void multiply(CA& ca, CB& cb, int kb0, int kb1, v4f (
   }
 }
 
+// The same with copies two steps ahead, for operands that come from far: three stages of A
+// and two of B (5 D ROWB bytes).  B's fragments of a step are read at its beginning,
+// so a second barrier, after the products that cover those reads, frees its stage
+// for the step after next; of A the stage of the step before is free by then.  At
+// a step's end a wave waits for its copies of the next step only.
+// prime_ahead() has been called; nk >= 1.  Afterwards nothing reads or writes the stages.
+struct Stages {
+  uint8_t *a0, *a1, *a2, *b0, *b1;
+  template <int I>
+  __device__ __forceinline__ uint8_t* a() const { return I == 0 ? a0 : I == 1 ? a1 : a2; }
+  template <int I>
+  __device__ __forceinline__ uint8_t* b() const { return I == 0 ? b0 : b1; }
+};
+template <typename CA, typename CB>
+__device__ __forceinline__ void prime_ahead(CA& ca, CB& cb, int wave, const Stages& st) {
+  prime(ca, cb, 0, wave, st.a0, st.b0);
+  ca.set(1);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) ca.issue(st.a1, wave, j);
+}
+template <int D, bool TA, bool TB, typename CA, typename CB>
+__device__ __forceinline__ void multiply_ahead(CA& ca, CB& cb, int nk, v4f (&acc)[D / 32][4], int wm, int wn, int wave, int lane,
+                                               const Stages& st) {
+  constexpr int MT = D / 32;
+  constexpr int NONE = 0x0070, EIGHT = 0x0074;  // s_waitcnt: lgkmcnt(0) with vmcnt(0), vmcnt(8)
+  auto rows = [&](int tm, const v8i (&bf)[4], const v8i& a) {
+    if (TB && !TA) __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+    for (int tn = 0; tn < 4; ++tn) acc[tm][tn] = mma<0>(bf[tn], a, acc[tm][tn]);
+#pragma unroll
+    for (int tn = 0; tn < 4; ++tn) acc[tm][tn] = mma<1>(bf[tn], a, acc[tm][tn]);
+    asm volatile("" : "+v"(acc[tm][0]), "+v"(acc[tm][1]), "+v"(acc[tm][2]), "+v"(acc[tm][3])::"memory");
+    if (TB && !TA) __builtin_amdgcn_s_setprio(0);
+  };
+  v8i b0[4], b1[4], af[4];
+  FragAt<TA, D> fa(wm * 16 * MT, lane);
+  FragAt<TB, D> fb(wn * 64, lane);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) b1[i] = af[i] = (v8i){0, 0, 0, 0, 0, 0, 0, 0};
+  __builtin_amdgcn_s_waitcnt(EIGHT);
+  barrier();
+  // step kt, from stages ta and tb, the step after next's A to na; bo: B's fragments of the step before.
+  // Copies of steps past the last one fetch nothing (all of them is out of their
+  // resources' bounds), so that no step has a branch.
+  auto step = [&](uint8_t* ta, uint8_t* tb, uint8_t* na, uint8_t* nb, int kt, const v8i (&bo)[4], v8i (&bf)[4]) __attribute__((always_inline)) {
+    ca.set(kt + 2);
+    cb.set(kt + 1);
+#pragma unroll
+    for (int tn = 0; tn < 4; ++tn) {
+      fb.anew();
+      bf[tn] = frag(tb, fb, tn);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      fa.anew();
+      af[i] = frag(ta, fa, i);
+      cb.issue(nb, wave, 2 * i);
+      cb.issue(nb, wave, 2 * i + 1);
+      rows(MT - 2 + i, bo, af[2 + i]);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) ca.issue(na, wave, j);
+#pragma unroll
+    for (int tm = 0; tm < MT - 2; ++tm) {
+      fa.anew();
+      af[(tm + 2) & 3] = frag(ta, fa, tm + 2);
+      rows(tm, bf, af[tm & 3]);
+    }
+    __builtin_amdgcn_s_waitcnt(EIGHT);
+    barrier();
+  };
+#define NTLB_STEP(I, BO, BF) step(st.a<(I) % 3>(), st.b<(I) % 2>(), st.a<((I) + 2) % 3>(), st.b<((I) + 1) % 2>(), kt + I, BO, BF)
+  int kt = 0;
+  for (; kt + 6 <= nk; kt += 6) {
+    NTLB_STEP(0, b1, b0);
+    NTLB_STEP(1, b0, b1);
+    NTLB_STEP(2, b1, b0);
+    NTLB_STEP(3, b0, b1);
+    NTLB_STEP(4, b1, b0);
+    NTLB_STEP(5, b0, b1);
+  }
+  // Up to five more, their stages found at run time: the compiler then waits for every
+  // copy before it reads one, and unrolled as above they take more registers than
+  // there are.
+  uint8_t *p0 = st.a0, *p1 = st.a1, *p2 = st.a2, *q0 = st.b0, *q1 = st.b1;
+  for (; kt < nk; ++kt) {
+    step(p0, q0, p2, q1, kt, b1, b0);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) b1[j] = b0[j];
+    uint8_t *p = p0, *q = q0;
+    p0 = p1;
+    p1 = p2;
+    p2 = p;
+    q0 = q1;
+    q1 = q;
+  }
+  rows(MT - 2, b1, af[2]);
+  rows(MT - 1, b1, af[3]);
+#undef NTLB_STEP
+  __builtin_amdgcn_s_waitcnt(NONE);
+  barrier();  // nothing is on its way into a stage any more
+}
+
 }  // namespace tile
 }  // namespace ntlb
 
@@ -372,3 +548,12 @@ __device__ __forceinline__ void multiply(CA& ca, CB& cb, int kb0, int kb1, v4f (
   __shared__ __attribute__((aligned(16))) uint8_t lb0[D * ROWB]; \
   __shared__ __attribute__((aligned(16))) uint8_t la1[D * ROWB]; \
   __shared__ __attribute__((aligned(16))) uint8_t lb1[D * ROWB]
+// three of A, two of B.  B's come first (they lie by name): its fragments' offsets then fit into the reads,
+// which saves registers where it is transposed.
+#define NTLB_TILE_STAGES_AHEAD(D)                                   \
+  __shared__ __attribute__((aligned(16))) uint8_t stage_0[D * ROWB]; \
+  __shared__ __attribute__((aligned(16))) uint8_t stage_1[D * ROWB]; \
+  __shared__ __attribute__((aligned(16))) uint8_t stage_2[D * ROWB]; \
+  __shared__ __attribute__((aligned(16))) uint8_t stage_3[D * ROWB]; \
+  __shared__ __attribute__((aligned(16))) uint8_t stage_4[D * ROWB]; \
+  const Stages stages{stage_2, stage_3, stage_4, stage_0, stage_1}
