@@ -5,6 +5,7 @@ grouped_matmul() is one Linear per expert over rows sorted by expert
 (src/models/moe.py:888-962, :1062-1097) in bf16, with its gradients; swiglu() is
 silu(gate) * up of a product's output that holds both (ExpertMLP.forward,
 moe.py:190-193).  Both can keep what their backward reads in 8 bits.
+local_moe_bf16() is the routed expert loop of them, moe.local_moe() without codes.
 """
 
 from __future__ import annotations
@@ -14,6 +15,7 @@ from typing import Optional
 import torch
 
 from . import _lib
+from . import moe
 from . import ops
 
 
@@ -72,3 +74,82 @@ def grouped_matmul(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor,
     if offsets.stride(0) != 1:
         offsets = offsets.contiguous()
     return (_lib._autograd or _lib.autograd()).grouped_matmul(x, weight, offsets, ops.checkpoint_code(checkpoint))
+
+
+class _Dispatch(torch.autograd.Function):
+    """tokens[token_indices] of every expert (moe.py:1086, :488): the rows of the
+    routing's order.  Rows past the kept ones hold any token; nothing reads them."""
+
+    @staticmethod
+    def forward(ctx, tokens, routing, expert_ids):
+        T, k = tokens.shape[0], routing.top_k
+        ctx.routing, ctx.shape = routing, tokens.shape
+        ctx.save_for_backward(routing.pos, expert_ids)
+        return tokens.index_select(0, routing.inv.clamp(0, max(T * k - 1, 0)) // k)
+
+    @staticmethod
+    def backward(ctx, d_rows):
+        pos, expert_ids = ctx.saved_tensors
+        T, H = ctx.shape
+        d_rows = d_rows.contiguous().view(-1).view(-1, H)
+        out = torch.empty((T, H), dtype=d_rows.dtype, device=d_rows.device)
+        if T:
+            ids = expert_ids.contiguous()
+            _lib.call("ntlb_moe_token_grad", d_rows.data_ptr(), H, ops._dtype_code(d_rows.dtype), pos.data_ptr(),
+                      ids.data_ptr(), 1 if ids.dtype == torch.int64 else 0, T, ctx.routing.top_k, H, out.data_ptr(), H,
+                      ops._stream())
+        return out, None, None
+
+
+class _Combine(torch.autograd.Function):
+    """output[token_indices] += expert_out * weights (moe.py:1087-1088, :489-490)"""
+
+    @staticmethod
+    def forward(ctx, rows, topk_w, routing, expert_ids):
+        ctx.routing = routing
+        ctx.save_for_backward(rows, topk_w, routing.pos)
+        return moe.combine_rows(rows, routing, expert_ids, topk_w, expert_ids.shape[0])
+
+    @staticmethod
+    def backward(ctx, d_out):
+        rows, topk_w, pos = ctx.saved_tensors
+        T, k, H = topk_w.shape[0], ctx.routing.top_k, rows.shape[1]
+        w = topk_w.contiguous()
+        d_rows = torch.empty((rows.shape[0], H), dtype=rows.dtype, device=rows.device)
+        d_w = torch.empty(w.shape, dtype=w.dtype, device=w.device)
+        if T:
+            d_out = d_out.contiguous().view(-1).view(T, H)
+            _lib.call("ntlb_moe_combine_backward", d_out.data_ptr(), H, rows.data_ptr(), rows.stride(0),
+                      ops._dtype_code(rows.dtype), pos.data_ptr(), w.data_ptr(), ops._dtype_code(w.dtype), T, k, H,
+                      d_rows.data_ptr(), H, d_w.data_ptr(), ops._stream())
+        return d_rows, d_w, None, None
+
+
+def local_moe_bf16(tokens: torch.Tensor, expert_ids: torch.Tensor, topk_w: torch.Tensor, w_gate_up: torch.Tensor,
+                   w_down: torch.Tensor, *, capacity: int = 0, checkpoint: Optional[str] = None) -> torch.Tensor:
+    """The single-rank routed expert loop with its products in bf16 (moe.py:1062-1093,
+    LocalRoutedMoE.forward :476-491, ExpertMLP.forward :190-193): moe.local_moe()'s
+    arguments, shapes and capacity, without codes in its products, and the gradients of
+    tokens, routing weights and expert weights under autograd.  grouped_matmul(),
+    swiglu(block=128), grouped_matmul() and the weighted sum of each token's rows.
+
+    checkpoint "e4m3" keeps the rows of both products and the projections between
+    them in 8 bits for the backward, 1/2 of what the bf16 loop keeps beside the
+    down projection's output."""
+    ops._require_device(tokens, expert_ids, topk_w, w_gate_up, w_down)
+    if tokens.dim() != 2 or expert_ids.dim() != 2 or topk_w.shape != expert_ids.shape or expert_ids.shape[0] != tokens.shape[0]:
+        raise ValueError("tokens must be [T, H], expert_ids and topk_w [T, k]")
+    if tokens.dtype != torch.bfloat16 or w_gate_up.dtype != torch.bfloat16 or w_down.dtype != torch.bfloat16:
+        raise TypeError("local_moe_bf16 takes bf16 tokens and bf16 expert weights")
+    if w_gate_up.dim() != 3 or w_gate_up.shape[1] % 256 or w_gate_up.shape[2] != tokens.shape[1] \
+            or w_down.shape != (w_gate_up.shape[0], tokens.shape[1], w_gate_up.shape[1] // 2):
+        raise ValueError(f"weights must be w_gate_up [E, 2I, H] (2I % 256 == 0) and w_down [E, H, I]; got "
+                         f"{tuple(w_gate_up.shape)}, {tuple(w_down.shape)}")
+    if expert_ids.shape[1] > 8:
+        raise ValueError("local_moe_bf16 supports top_k <= 8")
+    ops.checkpoint_code(checkpoint)
+    routing = moe.route_by_expert(expert_ids, w_gate_up.shape[0], capacity=int(capacity), topk_w=topk_w)
+    rows = _Dispatch.apply(tokens, routing, expert_ids)
+    gate_up = grouped_matmul(rows, w_gate_up, routing.offsets, checkpoint=checkpoint)
+    h = swiglu(gate_up, block=128, checkpoint=checkpoint)
+    return _Combine.apply(grouped_matmul(h, w_down, routing.offsets, checkpoint=checkpoint), topk_w, routing, expert_ids)
