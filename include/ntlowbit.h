@@ -1105,9 +1105,11 @@ int ntlb_rms_norm_forward(const void* x, int x_dtype, int64_t T, int64_t H, int6
                           float* rstd, uint8_t* kept, uint8_t* kept_exp, void* stream);
 
 /*
- * The same norm with y in 8 bits: the codes (grid, round to nearest) and scales
- * that ntlb_quant_tile_1x128 (qmax 127, NTLB_SCALE_AFTER_DIVIDE) forms of y in
- * fp32.  codes [T, ldc], ldc = ceil(H/128) * 128, 16-byte aligned; scale (i, t)
+ * The same norm with y in 8 bits: codes (grid, round to nearest) and scales as
+ * ntlb_quant_tile_1x128 (qmax 127, NTLB_SCALE_AFTER_DIVIDE) has them, of y's own
+ * value: a code is s w qmax / max|s w| over its 128 columns, rounded to fp32 and
+ * then to the grid, a scale rstd max|s w| / qmax.  Tiles of zeros, of values that are
+ * not finite or of magnitudes past 2^100 take y in fp32 first.  codes [T, ldc], ldc = ceil(H/128) * 128, 16-byte aligned; scale (i, t)
  * at scales[i*s_row + t*s_col]; nan_rows (int32 [T] or NULL): set to 1 where a
  * row of y holds a NaN, else left.
  */

@@ -1,9 +1,12 @@
 // Root-mean-square norm of rows of s = x + residual [T, H], forward:
 //   s = x + res (rounded to x's type; x itself without a residual)
 //   r = 1 / sqrt(mean(s^2) + eps),  y = s r w
-// y in x's type, or in 8 bits with a scale for each 128 columns: the codes that
-// quant_tile_1x128 forms, here of the fp32 y (rounded once, where a norm and a
-// quantizer one after the other round twice).  Optionally s is kept in 8 bits for
+// y in x's type, or in 8 bits with a scale for each 128 columns, amax / 448 (int grid
+// 127) as quant_tile_1x128 has it.  A code is y over its scale, in which r is no part:
+// it is s w 448 / max|s w|, one division rounded once.  Values of 16 bits meet ties
+// often (a value in 10,000 lies in the middle of two codes), and those are then
+// decided as by exact arithmetic; with y rounded first they fell to either side.
+// Optionally s is kept in 8 bits for
 // the backward (ntlb_kept.h), which then needs no s.  The norm is that of the s
 // that is stored.
 //
@@ -96,6 +99,10 @@ __global__ void __launch_bounds__(block_threads<RT>()) forward_kernel(Forward g)
     row_sum<RT, 1>(q, red[buf]);
     const float r = 1.0f / sqrtf(q[0] * inv + g.eps);
     if (OUT != OUT_CODES && g.rstd && t == 0) g.rstd[row] = r;
+    // r = r1 r2, r2 a power of two
+    const uint32_t rbits = __float_as_uint(r);
+    const bool usual = rbits >= 0x00800000u && rbits < 0x7F800000u;
+    const float r2 = __uint_as_float(rbits & 0x7F800000u), r1 = __uint_as_float((rbits & 0x007FFFFFu) | 0x3F800000u);
 #pragma unroll
     for (int v = 0; v < VPT; ++v) {
       const int c0 = (t + v * RT) * N;
@@ -118,30 +125,44 @@ __global__ void __launch_bounds__(block_threads<RT>()) forward_kernel(Forward g)
         store_codes<N, MODE>(g.kc + row * g.ldk, c0, (int)g.ldk, sp.first, lo, hi);
         if (t % LANES == 0 && c0 < H) g.ke[row * (g.ldk / KEPT_TILE) + c0 / KEPT_TILE] = (uint8_t)byte;
       }
-#pragma unroll
-      for (int i = 0; i < N; ++i) f[i] = f[i] * r * w[v][i];
       if constexpr (OUT != OUT_CODES) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) f[i] = f[i] * r * w[v][i];
         store_vec((uint8_t*)g.y + row * g.ldy, sp, f);
       } else {
+        // of p = s w 2^e, exact but for the weight's factor; r itself enters the scale only
+        float p[N];
         uint32_t m = 0;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-          f[i] = sp.own(i) ? f[i] : 0.f;
-          m = max(m, abs_bits(f[i]));
+          p[i] = sp.own(i) ? f[i] * r2 * w[v][i] : 0.f;
+          m = max(m, abs_bits(p[i]));
         }
         m = tile_max<LANES>(m);
-        const float scale = scale_from_amax_bits(m, g.qmax, SCALE_AFTER_DIVIDE);
-        const float rs = fast_div_ok<false>(m) ? 1.0f / scale : 1.0f;
+        float div = __uint_as_float(m), scale = div * r1 / g.qmax;
+        if (usual && m >= 0x1A000000u && m <= 0x71800000u) {  // 2^-75 .. 2^100
+#pragma unroll
+          for (int i = 0; i < N; ++i) p[i] *= g.qmax;
+        } else {  // zeros, what is not finite, magnitudes that products might not hold: y and its scale as they are
+          m = 0;
+#pragma unroll
+          for (int i = 0; i < N; ++i) {
+            p[i] = sp.own(i) ? f[i] * r * w[v][i] : 0.f;
+            m = max(m, abs_bits(p[i]));
+          }
+          m = tile_max<LANES>(m);
+          div = scale = scale_from_amax_bits(m, g.qmax, SCALE_AFTER_DIVIDE);
+        }
+        const float rs = fast_div_ok<false>(m) ? 1.0f / div : 1.0f;
         uint32_t rb[N] = {}, lo, hi;
         float qv[N];
-        bool nan;
         if (g.grid == GRID_E4M3)
-          nan = quant8_tile_rs<GRID_E4M3, false, false, N>(f, m, scale, rs, g.qmax, rb, lo, hi, qv);
+          quant8_tile_rs<GRID_E4M3, false, false, N>(p, m, div, rs, g.qmax, rb, lo, hi, qv);
         else
-          nan = quant8_tile_rs<GRID_INT, false, false, N>(f, m, scale, rs, g.qmax, rb, lo, hi, qv);
+          quant8_tile_rs<GRID_INT, false, false, N>(p, m, div, rs, g.qmax, rb, lo, hi, qv);
         store_codes<N, MODE>((uint8_t*)g.y + row * g.ldy, c0, (int)g.ldy, sp.first, lo, hi);
         if (t % LANES == 0 && c0 < H) g.scales[row * g.s_row + (int64_t)(c0 / 128) * g.s_col] = scale;
-        if (m > 0x7F800000u && nan && g.nan_rows) g.nan_rows[row] = 1;
+        if (m > 0x7F800000u && g.nan_rows) g.nan_rows[row] = 1;
       }
     }
   }

@@ -101,8 +101,9 @@ def rms_norm_quant(x: torch.Tensor, weight: Optional[torch.Tensor] = None, *, re
     a scale for each 128 columns of a row, tile-major), or (QTensor, s) with a
     residual.  ops.gemm_blockscaled and moe.expert_mlp take it as it is.
 
-    The codes are those of ops.quant_tile_1x128 (fmt "e4m3" or "int_grid", 8 bits,
-    round to nearest) of y in fp32: rounded once.  They have no gradient: where one
+    Codes and scales are laid out as those of ops.quant_tile_1x128 (fmt "e4m3" or
+    "int_grid", 8 bits, round to nearest) and are of y's own value, rounded once: where y
+    lies in the middle of two codes, the even one.  They have no gradient: where one
     is being recorded for x, weight or residual, the call is refused.  want_nan_rows
     as for ops.quant_tile_1x128 (the int grid needs it to carry a NaN on)."""
     weight = _check_rms("rms_norm_quant", x, weight, residual, eps)

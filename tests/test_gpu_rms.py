@@ -246,28 +246,81 @@ def test_gradients_against_differences(gpu_device):
     assert abs(float((4 * d1 - d2) / 3 - want)) <= abs(float(d1 - d2)) + 8 * U * scale / h
 
 
+def _exact_codes(s, w, fmt):
+    """the code values of s w over its tiles' scales in 64 bits, and how near each lies to the middle of two (0: a tie)"""
+    from _kept import round_e4m3
+
+    p, qmax = s.double() * w.double(), 448.0 if fmt == "e4m3" else 127.0
+    v = torch.cat([t * qmax / t.abs().amax(1, keepdim=True).clamp(min=1e-300) for t in p.split(128, 1)], 1)
+    if fmt == "e4m3":
+        q = round_e4m3(v)
+        a, b = round_e4m3(v * (1 - 4 * U)), round_e4m3(v * (1 + 4 * U))
+    else:
+        q, a, b = v.round(), (v * (1 - 4 * U)).round(), (v * (1 + 4 * U)).round()
+    return q, a, b
+
+
+def _code_values(q, H):
+    if q.grid == 1:
+        return q.codes[:, :H].view(torch.float8_e4m3fn).double()
+    return q.codes[:, :H].view(torch.int8).double()
+
+
 @pytest.mark.parametrize("fmt", ["e4m3", "int_grid"])
 @pytest.mark.parametrize("T,H", [(1, 7168), (3, 5), (37, 129), (130, 1541), (2, 16384), (300, 1000), (64, 128), (9, 2)])
-def test_codes_are_the_quantizers(gpu_device, fmt, T, H):
-    """of an fp32 input the codes, scales and NaN rows are quant_tile_1x128's of rms_norm's y, bit for bit"""
+@pytest.mark.parametrize("dtype,wdtype", TYPES)
+def test_codes_are_the_nearest(gpu_device, fmt, T, H, dtype, wdtype):
+    """of bf16 values and weights, whose products and their multiples by 448 or 127 have 24 bits, every code is the exact
+    quotient's, ties included (no other quotient of such numbers is nearer to a tie than 2^-23 of itself); of others it is where
+    the quotient is not within 4 u of the middle of two codes"""
+    from lowbit.norm import rms_norm_quant
+
+    x, res, w, _, _ = _inputs(T, H, dtype, wdtype, T + H, gpu_device)
+    total = (x.float() + res.float()).to(dtype)
+    for residual, at in ((None, x), (res, total)):
+        q = rms_norm_quant(x, w, residual=residual, fmt=fmt, want_nan_rows=True)
+        q = q if residual is None else q[0]
+        got, (want, low, high) = _code_values(q, H), _exact_codes(at, w, fmt)
+        if dtype == wdtype == torch.bfloat16:
+            assert torch.equal(got, want)
+        else:
+            assert ((got == want) | (got == low) | (got == high)).all()
+        top = torch.stack([p.abs().amax(1) for p in (at.double() * w.double()).split(128, 1)]) * _r(at, 1e-6)[:, 0]
+        want = top / (448.0 if fmt == "e4m3" else 127.0)
+        assert ((q.scales[:, :T].double() - want).abs() <= 80 * U * want).all()
+        assert not q.codes[:, H:].any() and not q.nan_rows.any()
+        assert (q.rows, q.K, q.s_row, q.s_col, q.shift) == (T, H, 1, q.scales.shape[1], 0)
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int_grid"])
+def test_codes_of_special_rows_are_the_quantizers(gpu_device, fmt):
+    """zeros, NaN, infinities, magnitudes at fp32's ends: codes, scales and NaN rows are quant_tile_1x128's of y"""
     from lowbit import ops
     from lowbit.norm import rms_norm, rms_norm_quant
 
-    x, res, w, _, _ = _inputs(T, H, torch.float32, torch.float32, T + H, gpu_device)
-    if T > 5:
-        x[1], res[1] = 0, 0
-        x[2, H // 2], x[3, 0], res[4, H - 1] = float("nan"), float("inf"), float("-inf")
-        x[5] *= 1e-30
-    for residual in (None, res):
-        y = rms_norm(x, w, residual=residual, eps=0.0 if T <= 5 else 1e-6)
-        q = rms_norm_quant(x, w, residual=residual, eps=0.0 if T <= 5 else 1e-6, fmt=fmt, want_nan_rows=True)
-        if residual is not None:
-            (y, s), (q, sq) = y, q
-            assert torch.equal(s.view(torch.int32), sq.view(torch.int32))
+    x, res, w, _, _ = _inputs(12, 300, torch.float32, torch.float32, 5, gpu_device)
+    x[1], res[1] = 0, 0
+    x[2, 150], x[3, 0], res[4, 299] = float("nan"), float("inf"), float("-inf")
+    x[5], res[5] = x[5] * 1e-30, 0
+    x[6, :128], res[6] = 0, 0
+    x[7] *= 1e30
+    x[8, 3] = 1e18
+    w = w.clone()
+    w[200] = 0
+    for eps in (0.0, 1e-6):
+        y, s = rms_norm(x, w, residual=res, eps=eps)
+        q, s2 = rms_norm_quant(x, w, residual=res, eps=eps, fmt=fmt, want_nan_rows=True)
+        assert torch.equal(s.view(torch.int32), s2.view(torch.int32))
         want = ops.quant_tile_1x128(y, fmt=fmt, want_nan_rows=True)
-        assert torch.equal(q.codes, want.codes) and torch.equal(q.nan_rows, want.nan_rows)
-        assert torch.equal(q.scales[:, :T], want.scales[:, :T])
-        assert (q.rows, q.K, q.s_row, q.s_col, q.shift, q.grid) == (want.rows, want.K, want.s_row, want.s_col, want.shift, want.grid)
+        assert torch.equal(q.nan_rows, want.nan_rows)
+        odd = torch.tensor([1, 2, 3, 4, 7], device=gpu_device)  # row 7: its squares pass fp32, so that y is 0
+        assert torch.equal(q.codes[odd], want.codes[odd]) and torch.equal(q.scales[:, odd], want.scales[:, odd])
+        rest = torch.tensor([5, 6, 8, 9, 10, 11], device=gpu_device)
+        a, b = q.scales[:, rest].double(), want.scales[:, rest].double()
+        assert ((a - b).abs() <= 4 * U * b).all()
+        if eps:
+            got, ref = _code_values(q, 300)[rest], _exact_codes(s[rest], w, fmt)
+            assert ((got == ref[0]) | (got == ref[1]) | (got == ref[2])).all()
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
