@@ -59,8 +59,8 @@ __global__ void __launch_bounds__(block_threads<RT>()) forward_kernel(Forward g)
 #pragma unroll
     for (int v = 0; v < VPT; ++v) {
       const Span<DT, MODE> sp(t + v * RT, H);
-      nx[v] = load_vec(p, sp);
-      if constexpr (RES) nr[v] = load_vec(q, sp);
+      nx[v] = load_vec<true>(p, sp);
+      if constexpr (RES) nr[v] = load_vec<true>(q, sp);
     }
   };
   if (row < g.T) fetch(row);

@@ -67,7 +67,7 @@ __device__ __forceinline__ void load_part(const uint8_t* p, int n, float (&f)[El
   constexpr int N = El<DT>::n;
   if (WHOLE_ || n >= N) {
     Span<DT, WHOLE> s(0, N);
-    unpack<DT>(load_vec(p, s), f);
+    unpack<DT>(load_vec<true>(p, s), f);
   } else {
 #pragma unroll
     for (int i = 0; i < N; ++i) f[i] = i < n ? load_elem(p, DT, i) : 0.f;
@@ -158,9 +158,10 @@ template <int N>
 __device__ __forceinline__ void load_codes(const uint8_t* p, float scale, float (&f)[N]) {
   uint32_t w[2];
   if constexpr (N == 8) {
-    const uint2 v = *reinterpret_cast<const uint2*>(p);
-    w[0] = v.x;
-    w[1] = v.y;
+    typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+    const u32x2 v = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(p));
+    w[0] = v[0];
+    w[1] = v[1];
   } else {
     w[0] = *reinterpret_cast<const uint32_t*>(p);
   }
