@@ -1162,14 +1162,17 @@ int ntlb_swiglu_rows_backward(const void* x, int dtype, int64_t T, int64_t I, in
  * lie in 16-byte aligned rows of whole 16-byte pieces (pitch % 8 == 0, at most
  * 2^22; w_stride % 8 == 0); where a product sums along their rows (x and w for y,
  * dy for dx) their columns up to the next multiple of 8 are zero.  Outputs need only
- * the element's alignment.  E <= 4096, R <= 2^30, N and K <= 2^22.
+ * the element's alignment.  E <= 4096, R <= 2^30, N and K <= 2^22.  workspace: of y and dx
+ * ntlb_grouped_matmul_workspace_bytes(R, E, N, K, 0 and 1) bytes, 16-byte aligned,
+ * contents free.
  */
 int ntlb_grouped_matmul(const uint16_t* x, int64_t ldx, const uint16_t* w, int64_t ldw, int64_t w_stride,
                         const int32_t* offsets, int64_t R, int64_t E, int64_t N, int64_t K, uint16_t* y, int64_t ldy,
-                        void* stream);
+                        void* workspace, int64_t ws_bytes, void* stream);
 int ntlb_grouped_matmul_dx(const uint16_t* dy, int64_t lddy, const uint16_t* w, int64_t ldw, int64_t w_stride,
                            const int32_t* offsets, int64_t R, int64_t E, int64_t N, int64_t K, uint16_t* dx,
-                           int64_t lddx, void* stream);
+                           int64_t lddx, void* workspace, int64_t ws_bytes, void* stream);
+int64_t ntlb_grouped_matmul_workspace_bytes(int64_t R, int64_t E, int64_t N, int64_t K, int dx);
 int ntlb_grouped_matmul_dw(const uint16_t* dy, int64_t lddy, const uint16_t* x, int64_t ldx, const int32_t* offsets,
                            int64_t R, int64_t E, int64_t N, int64_t K, uint16_t* dw, void* stream);
 

@@ -58,6 +58,7 @@ struct Abi {
   decltype(&ntlb_grouped_matmul) grouped;
   decltype(&ntlb_grouped_matmul_dx) grouped_dx;
   decltype(&ntlb_grouped_matmul_dw) grouped_dw;
+  decltype(&ntlb_grouped_matmul_workspace_bytes) grouped_workspace;
   decltype(&ntlb_kept_rows) kept_rows;
   decltype(&ntlb_kept_values) kept_values;
   PyObject* error;  // the package's exception for a failed entry point
@@ -627,9 +628,11 @@ struct Grouped {
 
   static Tensor run(const Tensor& x2, const Tensor& w3, const Tensor& offsets, int64_t N, int64_t K) {
     const int64_t R = x2.size(0);
-    Tensor y = fresh({R, N}, x2.scalar_type(), x2);
+    Tensor y = fresh({R, N}, x2.scalar_type(), x2), ws;
+    const int64_t E = w3.size(0), need = abi.grouped_workspace(R, E, N, K, 0);
+    if (need) ws = scratch(need, x2);
     check("ntlb_grouped_matmul", abi.grouped(at(x2), x2.stride(0), at(w3), w3.stride(1), w3.stride(0), offsets.data_ptr<int32_t>(),
-                                             R, w3.size(0), N, K, at(y), N, stream_of(x2)));
+                                             R, E, N, K, at(y), N, ptr(ws), need, stream_of(x2)));
     return y;
   }
 
@@ -651,8 +654,12 @@ struct Grouped {
         const Tensor wt = weights(w0);
         d2 = rows(dy, true);
         dx = fresh({R, K}, dy.scalar_type(), dy);
-        check("ntlb_grouped_matmul_dx", abi.grouped_dx(at(d2), d2.stride(0), at(wt), wt.stride(1), wt.stride(0),
-                                                       off.data_ptr<int32_t>(), R, E, N, K, at(dx), K, stream_of(dy)));
+        Tensor ws;
+        const int64_t need = abi.grouped_workspace(R, E, N, K, 1);
+        if (need) ws = scratch(need, dy);
+        check("ntlb_grouped_matmul_dx",
+              abi.grouped_dx(at(d2), d2.stride(0), at(wt), wt.stride(1), wt.stride(0), off.data_ptr<int32_t>(), R, E, N, K,
+                             at(dx), K, ptr(ws), need, stream_of(dy)));
       }
       if (task_should_compute_output(1) && (x0.defined() || c0.defined())) {
         if (!d2.defined()) d2 = rows(dy, false);
@@ -959,6 +966,7 @@ PyObject* py_bind(PyObject*, PyObject* table) {
   take(table, "ntlb_grouped_matmul", a.grouped);
   take(table, "ntlb_grouped_matmul_dx", a.grouped_dx);
   take(table, "ntlb_grouped_matmul_dw", a.grouped_dw);
+  take(table, "ntlb_grouped_matmul_workspace_bytes", a.grouped_workspace);
   take(table, "ntlb_kept_rows", a.kept_rows);
   take(table, "ntlb_kept_values", a.kept_values);
   PyObject* error = PyDict_GetItemString(table, "error");  // borrowed

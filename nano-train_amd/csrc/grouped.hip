@@ -37,6 +37,9 @@ struct Args {
   int64_t N;  // columns of the result
   uint16_t* out;
   int64_t ldo;  // elements
+  int parts;    // y, dx by tiles of 128: ranges of the contraction, each to a matrix of its own in `sums`
+  float* sums;  // [parts][R][lds]
+  int64_t lds;
 };
 
 // the rows of expert e; of e == E: those behind the last expert's
@@ -78,11 +81,12 @@ __device__ __forceinline__ int wave_place(int v, int lane, int lanes) {
 }
 
 // Tile pid of all experts' rows (D each) by num_n column tiles, expert after expert,
-// then the rows behind the last expert's (e == E).  Each XCD walks a contiguous range,
-// so that few of them read one expert's weights.  m0: first row, of the expert's n; tn:
+// then the rows behind the last expert's (e == E), each as often as the contraction
+// has ranges.  Each XCD walks a contiguous range, so that few of them read one
+// expert's weights.  m0: first row, of the expert's n; tn:
 // column tile.
 struct Found {
-  int e, lo, n, m0, tn;
+  int e, lo, n, m0, tn, part;
 };
 // row tiles walked side by side: of an expert for y and dx, of dW (32768 rows, 32 experts,
 // 4096 x 7168: y 1716 us with four, 1698 with eight; dx 1810, 1798; dW 1903, 1947)
@@ -96,10 +100,12 @@ __device__ __forceinline__ bool find(const Args& g, int num_n, int pid, Found& f
     if (c + lane <= g.E) m = (Rows(g.offsets, c + lane, g.E, R).n + D - 1) / D;
     total += __builtin_amdgcn_readlane(wave_scan(m, lane), 63);
   }
-  total *= num_n;
+  total *= num_n * g.parts;
   if (pid >= total) return false;
   const int xcd = pid & 7, per = total >> 3, extra = total & 7;
   int q = xcd * per + min(xcd, extra) + (pid >> 3);
+  f.part = D == 128 ? q % g.parts : 0;  // a tile's ranges on one XCD
+  if (D == 128) q /= g.parts;
   for (int c = 0; c <= g.E; c += 64) {
     const Rows r(g.offsets, min(c + lane, g.E), g.E, R);
     const int m = c + lane <= g.E ? (r.n + D - 1) / D * num_n : 0, upto = wave_scan(m, lane);
@@ -120,6 +126,14 @@ __device__ __forceinline__ bool find(const Args& g, int num_n, int pid, Found& f
   return false;
 }
 
+// the steps of a tile's range
+template <int D>
+__device__ __forceinline__ void steps_of(const Args& g, const Found& f, int& k0, int& k1) {
+  const int nk = (int)((g.k + KSTEP - 1) / KSTEP);
+  k0 = D == 128 ? f.part * nk / g.parts : 0;
+  k1 = D == 128 ? (f.part + 1) * nk / g.parts : nk;
+}
+
 // A wave's result rows through its part of a stage
 template <int D>
 __device__ __forceinline__ void store_tile(const v4f (&acc)[D / 32][4], int wave, int wm, int wn, int lane, int64_t m0,
@@ -129,6 +143,43 @@ __device__ __forceinline__ void store_tile(const v4f (&acc)[D / 32][4], int wave
 #pragma unroll
     for (int r = 0; r < 4; ++r) v[r] = acc[tm][tn][r];
   });
+}
+
+// the same of one range's sums, fp32
+template <int D>
+__device__ __forceinline__ void store_sums(const v4f (&acc)[D / 32][4], int wm, int wn, int lane, int64_t m0, int64_t n0,
+                                           int64_t M, float* out, int64_t ldo) {
+  constexpr int MT = D / 32;
+#pragma unroll
+  for (int tm = 0; tm < MT; ++tm) {
+    const int64_t m = m0 + wm * 16 * MT + tm * 16 + (lane & 15);
+    if (m >= M) continue;
+#pragma unroll
+    for (int tn = 0; tn < 4; ++tn) {
+      const int64_t n = n0 + wn * 64 + tn * 16 + (lane >> 4) * 4;
+      if (n < ldo) *reinterpret_cast<v4f*>(out + m * ldo + n) = acc[tm][tn];  // the pitch is a multiple of four
+    }
+  }
+}
+
+// the ranges' sums added in their order
+__global__ void __launch_bounds__(256) join_kernel(Args g) {
+  const int64_t quads = g.lds / 4, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= g.R * quads) return;
+  const int64_t m = i / quads, n = (i - m * quads) * 4;
+  const float* p = g.sums + m * g.lds + n;
+  v4f v = *reinterpret_cast<const v4f*>(p);
+#pragma unroll 4
+  for (int k = 1; k < g.parts; ++k) v += *reinterpret_cast<const v4f*>(p + k * (g.R * g.lds));
+  uint16_t* o = g.out + m * g.ldo + n;
+  const uint32_t a = pack_bf16(v[0], v[1]), b = pack_bf16(v[2], v[3]);
+  if (n + 4 <= g.N) {
+    *reinterpret_cast<u32x2_2*>(o) = (u32x2_2){a, b};
+  } else {
+    o[0] = (uint16_t)a;
+    if (n + 1 < g.N) o[1] = (uint16_t)(a >> 16);
+    if (n + 2 < g.N) o[2] = (uint16_t)b;
+  }
 }
 
 #define NTLB_ZERO_ACC(D)                   \
@@ -150,10 +201,15 @@ __global__ void __launch_bounds__(2 * D, D == 256 ? 1 : 2) rows_kernel(Args g) {
     RowWalk<D> ca, cb;
     ca.init(Mat{g.a + (int64_t)f.lo * g.lda, g.lda, f.n, g.k}, m0, wave, lane);
     cb.init(Mat{g.b + (int64_t)f.e * g.b_expert, g.ldb, g.N, g.k}, n0, wave, lane);
-    prime_ahead(ca, cb, wave, stages);
-    multiply_ahead<D, false, false>(ca, cb, (int)((g.k + KSTEP - 1) / KSTEP), acc, wm, wn, wave, lane, stages);
+    int k0, k1;
+    steps_of<D>(g, f, k0, k1);
+    prime_ahead(ca, cb, k0, wave, stages);
+    multiply_ahead<D, false, false>(ca, cb, k0, k1, acc, wm, wn, wave, lane, stages);
   }
-  store_tile<D>(acc, wave, wm, wn, own_lane(), m0, n0, f.n, g.N, g.out + (int64_t)f.lo * g.ldo, g.ldo, stage_4);
+  if (D == 128 && g.parts > 1)
+    store_sums<D>(acc, wm, wn, own_lane(), m0, n0, f.n, g.sums + (f.part * g.R + f.lo) * g.lds, g.lds);
+  else
+    store_tile<D>(acc, wave, wm, wn, own_lane(), m0, n0, f.n, g.N, g.out + (int64_t)f.lo * g.ldo, g.ldo, stage_4);
 }
 
 // dx: W transposed
@@ -172,9 +228,14 @@ __global__ void __launch_bounds__(2 * D, D == 256 ? 1 : 2) inputs_kernel(Args g)
     TrCopy<D> cb;
     ca.init(Mat{g.a + (int64_t)f.lo * g.lda, g.lda, f.n, g.k}, m0, wave, lane);
     cb.init(Mat{g.b + (int64_t)f.e * g.b_expert, g.ldb, g.N, g.k}, n0, wave, lane);
-    multiply<D, false, true>(ca, cb, 0, (int)((g.k + KSTEP - 1) / KSTEP), acc, wm, wn, wave, lane, la0, lb0, la1, lb1);
+    int k0, k1;
+    steps_of<D>(g, f, k0, k1);
+    multiply<D, false, true>(ca, cb, k0, k1, acc, wm, wn, wave, lane, la0, lb0, la1, lb1);
   }
-  store_tile<D>(acc, wave, wm, wn, lane, m0, n0, f.n, g.N, g.out + (int64_t)f.lo * g.ldo, g.ldo, la1);
+  if (D == 128 && g.parts > 1)
+    store_sums<D>(acc, wm, wn, lane, m0, n0, f.n, g.sums + (f.part * g.R + f.lo) * g.lds, g.lds);
+  else
+    store_tile<D>(acc, wave, wm, wn, lane, m0, n0, f.n, g.N, g.out + (int64_t)f.lo * g.ldo, g.ldo, la1);
 }
 
 // dW: every expert's tiles, each with the expert's rows as its contraction.  Experts
@@ -452,62 +513,107 @@ static int bad(const char* fn, const char* what) {
   return fail(NTLB_EINVAL, "%s: %s must lie in 16-byte aligned rows of whole 16-byte pieces, at most %lld values apart", fn, what, (long long)MAX_PITCH);
 }
 
-// The tile of y and dx: D = 256 where its tiles fill the chip
-static int tile_of(int64_t R, int64_t E, int64_t N) {
-  const int64_t live = std::min(R, E), m = cdiv(R, 256) + live / 2;
-  return m * cdiv(N, 256) >= split_device_cus() && R >= live * 128 ? 256 : 128;
+// How y and dx are formed for N columns over K: by streaming the weights past few rows
+// (FEW, y only), or by tiles of D, their contraction in `parts` ranges.
+//
+// How many rows an expert has is known to the device only; R rows over the experts
+// that can have some is what the host goes by.  256 tiles where they fill the chip and
+// experts have half a tile's rows at least.  Few rows stream: 32 experts, 4096 x 7168,
+// 128 rows 349 us and by tiles 337, 256 rows 429 and 333; 64 rows 331 and 339.  Where the
+// tiles are few too, up to 32 rows an expert: 8 experts, 2048 x 4096, 128 rows 41 and 67
+// us, 256 rows 58 and 51; 768 x 1024, 256 rows 14.5 and 22.  Tiles that leave compute units idle
+// divide the contraction: one expert, 4096 x 4096, 64 rows 46 us whole and 24 in 16
+// ranges, their sum included; 1003 rows of 4 experts, 345 x 1000, 19.5 and 15.9.
+struct Plan {
+  bool few;
+  int D, parts;
+};
+static Plan plan_of(int64_t R, int64_t E, int64_t N, int64_t K, bool y) {
+  const int64_t live = std::min(R, E), cus = split_device_cus();
+  Plan p{false, 128, 1};
+  if ((cdiv(R, 256) + live / 2) * cdiv(N, 256) >= cus && R >= live * 128) {
+    p.D = 256;
+    return p;
+  }
+  const int64_t tiles = (R / 128 + cdiv(live, 2)) * cdiv(N, 128), nk = cdiv(K, KSTEP);
+  p.few = y && R <= (live * cdiv(N, 128) >= 2 * cus ? 6 : 32) * live;
+  // ranges of four steps at least, and sums of 64 MB at most
+  if (!p.few && tiles < cus)
+    p.parts = (int)std::max<int64_t>(1, std::min({2 * cus / tiles, nk / 4, (int64_t)16, ((int64_t)64 << 20) / (R * cdiv(N, 4) * 16)}));
+  return p;
 }
-// workgroups of y's and dx' tiles: every expert's last one too, and the rows' behind
-static int64_t row_tiles(const Args& g, int D) { return (g.R / D + g.E + 1) * cdiv(g.N, D); }
+static int64_t sums_bytes(const Plan& p, int64_t R, int64_t N) { return p.parts > 1 ? p.parts * R * cdiv(N, 4) * 16 : 0; }
+// workgroups of the tiles: every expert's last one too, and the rows' behind
+static int64_t row_tiles(const Args& g, const Plan& p) { return (g.R / p.D + g.E + 1) * cdiv(g.N, p.D) * p.parts; }
+
+// y's or dx' tiles, and their ranges' sum
+template <bool Y>
+static int launch(const char* fn, Args g, const Plan& p, void* ws, int64_t ws_bytes, hipStream_t st) {
+  const int64_t need = sums_bytes(p, g.R, g.N), n = row_tiles(g, p);
+  if (ws_bytes < need || (need && (!ws || !aligned(ws, 16)))) return fail(NTLB_EINVAL, "%s: workspace of %lld bytes, %lld needed", fn, (long long)ws_bytes, (long long)need);
+  if (n > MAX_GRID) return fail(NTLB_EUNSUPPORTED, "%s: %lld tiles", fn, (long long)n);
+  g.parts = p.parts;
+  g.sums = (float*)ws;
+  g.lds = cdiv(g.N, 4) * 4;
+  const dim3 grd((unsigned)n);
+  if constexpr (Y) {
+    if (p.D == 256) rows_kernel<256><<<grd, 512, 0, st>>>(g);
+    else rows_kernel<128><<<grd, 256, 0, st>>>(g);
+  } else {
+    if (p.D == 256) inputs_kernel<256><<<grd, 512, 0, st>>>(g);
+    else inputs_kernel<128><<<grd, 256, 0, st>>>(g);
+  }
+  if (int rc = check_launch(fn)) return rc;
+  if (p.parts == 1) return NTLB_OK;
+  join_kernel<<<(unsigned)cdiv(g.R * (g.lds / 4), 256), 256, 0, st>>>(g);
+  return check_launch(fn);
+}
 
 }  // namespace grouped
 }  // namespace ntlb
 
 using namespace ntlb;
 
+extern "C" int64_t ntlb_grouped_matmul_workspace_bytes(int64_t R, int64_t E, int64_t N, int64_t K, int dx) {
+  if (R < 1 || E < 1 || N < 1 || K < 1) return 0;
+  return dx ? grouped::sums_bytes(grouped::plan_of(R, E, K, N, false), R, K)
+            : grouped::sums_bytes(grouped::plan_of(R, E, N, K, true), R, N);
+}
+
 extern "C" int ntlb_grouped_matmul(const uint16_t* x, int64_t ldx, const uint16_t* w, int64_t ldw, int64_t w_stride,
                                    const int32_t* offsets, int64_t R, int64_t E, int64_t N, int64_t K, uint16_t* y,
-                                   int64_t ldy, void* stream) {
+                                   int64_t ldy, void* workspace, int64_t ws_bytes, void* stream) {
   const char* fn = "ntlb_grouped_matmul";
   if (int rc = grouped::check(fn, R, E, N, K, offsets)) return rc;
   if (R == 0) return NTLB_OK;
   if (!grouped::fits(x, ldx, K)) return grouped::bad(fn, "x");
   if (!grouped::fits(w, ldw, K) || w_stride % 8 || w_stride < 0) return grouped::bad(fn, "w");
   if (!y || ldy < N) return fail(NTLB_EINVAL, "%s: bad y", fn);
-  grouped::Args g{(const uint8_t*)x, ldx * 2, (const uint8_t*)w, ldw * 2, w_stride * 2, offsets, R, (int)E, K, 0, N, y, ldy};
+  grouped::Args g{};
+  g.a = (const uint8_t*)x; g.lda = ldx * 2; g.b = (const uint8_t*)w; g.ldb = ldw * 2; g.b_expert = w_stride * 2;
+  g.offsets = offsets; g.R = R; g.E = (int)E; g.k = K; g.N = N; g.out = y; g.ldo = ldy;
   hipStream_t st = as_stream(stream);
-  // an expert's expected rows: few ones stream the weights
-  if (R <= 32 * std::min(R, E)) {
-    const int64_t blocks = cdiv(N, 16), n = (E + 1) * blocks;
-    if (n > grouped::MAX_GRID) return fail(NTLB_EUNSUPPORTED, "%s: %lld workgroups", fn, (long long)n);
-    grouped::few_kernel<1><<<(unsigned)n, 64 * grouped::FEW_WAVES, 0, st>>>(g, (int)blocks);
-    return check_launch(fn);
-  }
-  const int D = grouped::tile_of(R, E, N);
-  const int64_t n = grouped::row_tiles(g, D);
-  if (n > grouped::MAX_GRID) return fail(NTLB_EUNSUPPORTED, "%s: %lld tiles", fn, (long long)n);
-  if (D == 256) grouped::rows_kernel<256><<<(unsigned)n, 512, 0, st>>>(g);
-  else grouped::rows_kernel<128><<<(unsigned)n, 256, 0, st>>>(g);
+  const grouped::Plan p = grouped::plan_of(R, E, N, K, true);
+  if (!p.few) return grouped::launch<true>(fn, g, p, workspace, ws_bytes, st);
+  const int64_t blocks = cdiv(N, 16), n = (E + 1) * blocks;
+  if (n > grouped::MAX_GRID) return fail(NTLB_EUNSUPPORTED, "%s: %lld workgroups", fn, (long long)n);
+  grouped::few_kernel<1><<<(unsigned)n, 64 * grouped::FEW_WAVES, 0, st>>>(g, (int)blocks);
   return check_launch(fn);
 }
 
 extern "C" int ntlb_grouped_matmul_dx(const uint16_t* dy, int64_t lddy, const uint16_t* w, int64_t ldw, int64_t w_stride,
                                       const int32_t* offsets, int64_t R, int64_t E, int64_t N, int64_t K, uint16_t* dx,
-                                      int64_t lddx, void* stream) {
+                                      int64_t lddx, void* workspace, int64_t ws_bytes, void* stream) {
   const char* fn = "ntlb_grouped_matmul_dx";
   if (int rc = grouped::check(fn, R, E, N, K, offsets)) return rc;
   if (R == 0) return NTLB_OK;
   if (!grouped::fits(dy, lddy, N)) return grouped::bad(fn, "dy");
   if (!grouped::fits(w, ldw, K) || w_stride % 8 || w_stride < 0) return grouped::bad(fn, "w");
   if (!dx || lddx < K) return fail(NTLB_EINVAL, "%s: bad dx", fn);
-  grouped::Args g{(const uint8_t*)dy, lddy * 2, (const uint8_t*)w, ldw * 2, w_stride * 2, offsets, R, (int)E, N, 0, K, dx, lddx};
-  hipStream_t st = as_stream(stream);
-  const int D = grouped::tile_of(R, E, K);
-  const int64_t n = grouped::row_tiles(g, D);
-  if (n > grouped::MAX_GRID) return fail(NTLB_EUNSUPPORTED, "%s: %lld tiles", fn, (long long)n);
-  if (D == 256) grouped::inputs_kernel<256><<<(unsigned)n, 512, 0, st>>>(g);
-  else grouped::inputs_kernel<128><<<(unsigned)n, 256, 0, st>>>(g);
-  return check_launch(fn);
+  grouped::Args g{};
+  g.a = (const uint8_t*)dy; g.lda = lddy * 2; g.b = (const uint8_t*)w; g.ldb = ldw * 2; g.b_expert = w_stride * 2;
+  g.offsets = offsets; g.R = R; g.E = (int)E; g.k = N; g.N = K; g.out = dx; g.ldo = lddx;
+  return grouped::launch<false>(fn, g, grouped::plan_of(R, E, K, N, false), workspace, ws_bytes, as_stream(stream));
 }
 
 extern "C" int ntlb_grouped_matmul_dw(const uint16_t* dy, int64_t lddy, const uint16_t* x, int64_t ldx,
@@ -518,7 +624,9 @@ extern "C" int ntlb_grouped_matmul_dw(const uint16_t* dy, int64_t lddy, const ui
   if (!dw) return fail(NTLB_EINVAL, "%s: bad dw", fn);
   if (R > 0 && !grouped::fits(dy, lddy, N)) return grouped::bad(fn, "dy");
   if (R > 0 && !grouped::fits(x, ldx, K)) return grouped::bad(fn, "x");
-  grouped::Args g{(const uint8_t*)dy, lddy * 2, (const uint8_t*)x, ldx * 2, 0, offsets, R, (int)E, 0, N, K, dw, K};
+  grouped::Args g{};
+  g.a = (const uint8_t*)dy; g.lda = lddy * 2; g.b = (const uint8_t*)x; g.ldb = ldx * 2;
+  g.offsets = offsets; g.R = R; g.E = (int)E; g.M = N; g.N = K; g.out = dw; g.ldo = K;
   const int D = N > 128 && K > 128 && E * cdiv(N, 256) * cdiv(K, 256) >= split_device_cus() ? 256 : 128;
   const int64_t n = grouped::ordered_grid(E * cdiv(N, D) * cdiv(K, D));
   if (n > grouped::MAX_GRID) return fail(NTLB_EUNSUPPORTED, "%s: %lld tiles", fn, (long long)n);

@@ -436,12 +436,13 @@ __device__ __forceinline__ void multiply(CA& ca, CB& cb, int kb0, int kb1, v4f (
   }
 }
 
-// The same with copies two steps ahead, for operands that come from far: three stages of A
-// and two of B (5 D ROWB bytes).  B's fragments of a step are read at its beginning,
-// so a second barrier, after the products that cover those reads, frees its stage
-// for the step after next; of A the stage of the step before is free by then.  At
-// a step's end a wave waits for its copies of the next step only.
-// prime_ahead() has been called; nk >= 1.  Afterwards nothing reads or writes the stages.
+// The same with A's copies two steps ahead, for operands that come from far: three
+// stages of A, two of B (5 D ROWB bytes).  A step's copies of B are issued before
+// its copies of A, so that at its end a wave waits for those of the next step only.
+// (32768 x 7168 by 4096 rows: 1507 us with both one step ahead, 1404 so; with B's two
+// ahead too, its stage freed by a second barrier after its fragments are read, 1501.)
+// prime_ahead() has been called for step k0; k0 < k1.  Afterwards nothing reads or
+// writes the stages.
 struct Stages {
   uint8_t *a0, *a1, *a2, *b0, *b1;
   template <int I>
@@ -450,17 +451,17 @@ struct Stages {
   __device__ __forceinline__ uint8_t* b() const { return I == 0 ? b0 : b1; }
 };
 template <typename CA, typename CB>
-__device__ __forceinline__ void prime_ahead(CA& ca, CB& cb, int wave, const Stages& st) {
-  prime(ca, cb, 0, wave, st.a0, st.b0);
-  ca.set(1);
+__device__ __forceinline__ void prime_ahead(CA& ca, CB& cb, int k0, int wave, const Stages& st) {
+  prime(ca, cb, k0, wave, st.a0, st.b0);
+  ca.set(k0 + 1);
 #pragma unroll
   for (int j = 0; j < 4; ++j) ca.issue(st.a1, wave, j);
 }
 template <int D, bool TA, bool TB, typename CA, typename CB>
-__device__ __forceinline__ void multiply_ahead(CA& ca, CB& cb, int nk, v4f (&acc)[D / 32][4], int wm, int wn, int wave, int lane,
+__device__ __forceinline__ void multiply_ahead(CA& ca, CB& cb, int k0, int k1, v4f (&acc)[D / 32][4], int wm, int wn, int wave, int lane,
                                                const Stages& st) {
   constexpr int MT = D / 32;
-  constexpr int NONE = 0x0070, EIGHT = 0x0074;  // s_waitcnt: lgkmcnt(0) with vmcnt(0), vmcnt(8)
+  constexpr int NONE = 0x0070, FOUR = 0x0074;  // s_waitcnt: lgkmcnt(0) with vmcnt(0), vmcnt(4)
   auto rows = [&](int tm, const v8i (&bf)[4], const v8i& a) {
     if (TB && !TA) __builtin_amdgcn_s_setprio(1);
 #pragma unroll
@@ -475,12 +476,12 @@ __device__ __forceinline__ void multiply_ahead(CA& ca, CB& cb, int nk, v4f (&acc
   FragAt<TB, D> fb(wn * 64, lane);
 #pragma unroll
   for (int i = 0; i < 4; ++i) b1[i] = af[i] = (v8i){0, 0, 0, 0, 0, 0, 0, 0};
-  __builtin_amdgcn_s_waitcnt(EIGHT);
+  __builtin_amdgcn_s_waitcnt(FOUR);
   barrier();
   // step kt, from stages ta and tb, the step after next's A to na; bo: B's fragments of the step before.
-  // Copies of steps past the last one fetch nothing (all of them is out of their
-  // resources' bounds), so that no step has a branch.
-  auto step = [&](uint8_t* ta, uint8_t* tb, uint8_t* na, uint8_t* nb, int kt, const v8i (&bo)[4], v8i (&bf)[4]) __attribute__((always_inline)) {
+  // Copies of steps past k1 are made all the same, so that no step has a branch: past the
+  // contraction they fetch nothing (all of them is out of their resources' bounds).
+  auto step = [&](uint8_t* ta, uint8_t* tb, uint8_t* na, uint8_t* nb, int kt, const v8i (&bo)[4], v8i (&bf)[4]) {
     ca.set(kt + 2);
     cb.set(kt + 1);
 #pragma unroll
@@ -504,12 +505,12 @@ __device__ __forceinline__ void multiply_ahead(CA& ca, CB& cb, int nk, v4f (&acc
       af[(tm + 2) & 3] = frag(ta, fa, tm + 2);
       rows(tm, bf, af[tm & 3]);
     }
-    __builtin_amdgcn_s_waitcnt(EIGHT);
+    __builtin_amdgcn_s_waitcnt(FOUR);
     barrier();
   };
 #define NTLB_STEP(I, BO, BF) step(st.a<(I) % 3>(), st.b<(I) % 2>(), st.a<((I) + 2) % 3>(), st.b<((I) + 1) % 2>(), kt + I, BO, BF)
-  int kt = 0;
-  for (; kt + 6 <= nk; kt += 6) {
+  int kt = k0;
+  for (; kt + 6 <= k1; kt += 6) {
     NTLB_STEP(0, b1, b0);
     NTLB_STEP(1, b0, b1);
     NTLB_STEP(2, b1, b0);
@@ -521,7 +522,7 @@ __device__ __forceinline__ void multiply_ahead(CA& ca, CB& cb, int nk, v4f (&acc
   // copy before it reads one, and unrolled as above they take more registers than
   // there are.
   uint8_t *p0 = st.a0, *p1 = st.a1, *p2 = st.a2, *q0 = st.b0, *q1 = st.b1;
-  for (; kt < nk; ++kt) {
+  for (; kt < k1; ++kt) {
     step(p0, q0, p2, q1, kt, b1, b0);
 #pragma unroll
     for (int j = 0; j < 4; ++j) b1[j] = b0[j];

@@ -868,7 +868,8 @@ extern "C" int ntlb_pad_rows(const uint16_t* x, int64_t ldx, int64_t R, int64_t 
   if (ldo > (1 << 22) || R > ((int64_t)1 << 31) - 1) return fail(NTLB_EUNSUPPORTED, "%s: R %lld ldo %lld is too large", fn, (long long)R, (long long)ldo);
   if (R == 0) return NTLB_OK;
   if (!x || !out || !aligned(out, 16)) return fail(NTLB_EINVAL, "%s: bad pointer", fn);
-  const int per = (int)std::max<int64_t>(1, 2048 / (ldo / 8));
+  // few rows: one each to a thousand workgroups (1003 x 345: 9.2 us by 46 rows a workgroup)
+  const int per = (int)std::max<int64_t>(1, std::min(2048 / (ldo / 8), R / 1024));
   xent::pad_kernel<<<(unsigned)cdiv(R, per), 256, 0, as_stream(stream)>>>(x, ldx, R, H, out, ldo, per);
   return check_launch(fn);
 }

@@ -156,8 +156,9 @@ SIGNATURES = {
     "ntlb_rms_norm_workspace_bytes": [_I32, _I64, _I64],
     "ntlb_swiglu_rows": [_P, _I32, _I64, _I64, _I64, _I64, _P, _I64, _P, _P, _P],
     "ntlb_swiglu_rows_backward": [_P, _I32, _I64, _I64, _I64, _I64, _P, _P, _P, _I64, _P, _I64, _P],
-    "ntlb_grouped_matmul": [_P, _I64, _P, _I64, _I64, _P, _I64, _I64, _I64, _I64, _P, _I64, _P],
-    "ntlb_grouped_matmul_dx": [_P, _I64, _P, _I64, _I64, _P, _I64, _I64, _I64, _I64, _P, _I64, _P],
+    "ntlb_grouped_matmul": [_P, _I64, _P, _I64, _I64, _P, _I64, _I64, _I64, _I64, _P, _I64, _P, _I64, _P],
+    "ntlb_grouped_matmul_dx": [_P, _I64, _P, _I64, _I64, _P, _I64, _I64, _I64, _I64, _P, _I64, _P, _I64, _P],
+    "ntlb_grouped_matmul_workspace_bytes": [_I64, _I64, _I64, _I64, _I32],
     "ntlb_grouped_matmul_dw": [_P, _I64, _P, _I64, _P, _I64, _I64, _I64, _I64, _P, _P],
     "ntlb_kept_rows": [_P, _I64, _I64, _I64, _P, _P, _P],
     "ntlb_kept_values": [_P, _P, _I64, _I64, _P, _I64, _P],
@@ -179,7 +180,8 @@ RESTYPES = {"ntlb_gemm_workspace_bytes": _I64, "ntlb_ep_record_bytes": _I64, "nt
             "ntlb_ep_value_record_bytes": _I64, "ntlb_persistent_quant_ws_words": _I64,
             "ntlb_gemm_lowbit_workspace_bytes": _I64, "ntlb_gemm_dq_workspace_bytes": _I64,
             "ntlb_layer_norm_workspace_bytes": _I64, "ntlb_linear_xent_state_bytes": _I64,
-            "ntlb_linear_xent_workspace_bytes": _I64, "ntlb_rms_norm_workspace_bytes": _I64}
+            "ntlb_linear_xent_workspace_bytes": _I64, "ntlb_rms_norm_workspace_bytes": _I64,
+            "ntlb_grouped_matmul_workspace_bytes": _I64}
 
 _lib = None
 _lock = threading.Lock()

@@ -61,6 +61,8 @@ CASES = [  # rows of each expert, K, N, spare rows
     ([0, 0], 72, 40, 9), ([16, 17, 33, 65, 1], 264, 264, 0), ([300, 7, 0, 129], 520, 384, 30), ([1003, 1], 129, 257, 0),
     ([128, 256, 384], 256, 512, 0), ([700, 513, 255, 257], 1024, 768, 1), ([2, 1] * 50, 96, 72, 3), ([90] * 70, 64, 136, 0),
     ([2500, 2600], 320, 2304, 0), ([1] * 8, 7168, 512, 0), ([40, 3, 64, 100], 2049, 100, 0), ([1, 1], 1, 1, 1),
+    # the contraction in ranges: of y, of dx, of both; rows behind, no rows, a last quad cut
+    ([160], 4096, 128, 0), ([0, 90, 0, 133], 1111, 77, 9), ([200], 72, 4096, 40), ([257, 40], 1025, 1027, 0), ([70, 0], 7168, 1, 3),
 ]
 
 
@@ -214,12 +216,12 @@ def test_gradients_against_differences(gpu_device):
         assert abs(float(a.sum() - b.sum())) <= 1.1 * V * float(a.abs().sum() + b.abs().sum())
 
 
-@pytest.mark.parametrize("counts", [[3, 0, 9], [600, 200, 0, 300]])
-def test_other_stream_and_graph(gpu_device, counts):
+@pytest.mark.parametrize("counts,K,N", [([3, 0, 9], 264, 136), ([600, 200, 0, 300], 264, 136), ([100, 0, 150], 1032, 520)])
+def test_other_stream_and_graph(gpu_device, counts, K, N):
     """both directions on another stream and replayed from a graph, over new rows, new offsets among them"""
     from lowbit.experts import grouped_matmul
 
-    x, w, dy, offsets = _inputs(counts, 264, 136, 4, gpu_device)
+    x, w, dy, offsets = _inputs(counts, K, N, 4, gpu_device)
     lx, lw = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
 
     def step():
@@ -238,7 +240,7 @@ def test_other_stream_and_graph(gpu_device, counts):
         out = step()
     n = len(counts)
     for k in range(4):
-        other = _inputs([c for c in counts[k % n:] + counts[:k % n]], 264, 136, 40 + k, gpu_device)
+        other = _inputs([c for c in counts[k % n:] + counts[:k % n]], K, N, 40 + k, gpu_device)
         with torch.no_grad():
             lx.copy_(other[0])
             offsets.copy_(other[3])
