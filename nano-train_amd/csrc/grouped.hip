@@ -516,30 +516,40 @@ static int bad(const char* fn, const char* what) {
 // How y and dx are formed for N columns over K: by streaming the weights past few rows
 // (FEW, y only), or by tiles of D, their contraction in `parts` ranges.
 //
-// How many rows an expert has is known to the device only; R rows over the experts
-// that can have some is what the host goes by.  256 tiles where they fill the chip and
-// experts have half a tile's rows at least.  Few rows stream: 32 experts, 4096 x 7168,
-// 128 rows 349 us and by tiles 337, 256 rows 429 and 333; 64 rows 331 and 339.  Where the
-// tiles are few too, up to 32 rows an expert: 8 experts, 2048 x 4096, 128 rows 41 and 67
-// us, 256 rows 58 and 51; 768 x 1024, 256 rows 14.5 and 22.  Tiles that leave compute units idle
-// divide the contraction: one expert, 4096 x 4096, 64 rows 46 us whole and 24 in 16
-// ranges, their sum included; 1003 rows of 4 experts, 345 x 1000, 19.5 and 15.9.
+// How many rows an expert has is known to the device only; the host goes by R rows over
+// the experts that can have some.
+//
+// Few rows stream: past the weights goes x once for 16 of their rows, tiles of some
+// rows take a tile's time.  Up to 2 to 32 rows an expert, by the weights' size: 768 x 1024
+// of 8 experts 11 us at 32 rows and 12 by tiles, at 64 rows 18 and 14; 2048 x 4096 of 8
+// 26 us at 4 and 27, at 16 37 and 28; 4096 x 7168 of 32 331 us at 2 and 339, at 4 361 and 316.
+//
+// Tiles by the rounds that they take, one workgroup of 256 tiles a compute unit or two of
+// 128, a round of the latter 2/3 of the former's time: 4096 x 7168, 32 experts of 256
+// rows, y 612 us by 256 tiles and 727, dx 643 and 720, of 64 rows 531 and 445, 423 and 394;
+// 768 x 1024, 64 experts of 256 rows, 55 and 42; 2048 x 4096, 8 experts of 512, 84 and 99.
+//
+// Tiles that leave compute units idle divide the contraction: one expert, 4096 x 4096,
+// 64 rows 46 us whole and 24 in 15 ranges, their sum included; 2048 x 4096, 8 experts of 64
+// rows 47 and 33 in 3 (in 4, more workgroups than places, 44); 1003 rows of 4 experts, 345 x 1000,
+// 19.5 and 15.9.
 struct Plan {
   bool few;
   int D, parts;
 };
 static Plan plan_of(int64_t R, int64_t E, int64_t N, int64_t K, bool y) {
-  const int64_t live = std::min(R, E), cus = split_device_cus();
-  Plan p{false, 128, 1};
-  if ((cdiv(R, 256) + live / 2) * cdiv(N, 256) >= cus && R >= live * 128) {
+  const int64_t live = std::min(R, E), cus = split_device_cus(), nk = cdiv(K, KSTEP);
+  Plan p{y && R <= live * std::clamp<int64_t>(400000000 / (live * N * K), 2, 32), 128, 1};
+  if (p.few) return p;
+  auto tiles = [&](int64_t D) {  // a last one of every expert's is half empty
+    return (live == 1 ? cdiv(R, D) : std::max(live, R / D + cdiv(live, 2))) * cdiv(N, D);
+  };
+  const int64_t t = tiles(128);
+  if (3 * cdiv(tiles(256), cus) <= 2 * cdiv(t, 2 * cus)) {
     p.D = 256;
-    return p;
+  } else if (t < cus) {  // ranges of four steps at least, and sums of 64 MB at most
+    p.parts = (int)std::max<int64_t>(1, std::min({(2 * cus - cus / 8) / t, nk / 4, (int64_t)16, ((int64_t)64 << 20) / (R * cdiv(N, 4) * 16)}));
   }
-  const int64_t tiles = (R / 128 + cdiv(live, 2)) * cdiv(N, 128), nk = cdiv(K, KSTEP);
-  p.few = y && R <= (live * cdiv(N, 128) >= 2 * cus ? 6 : 32) * live;
-  // ranges of four steps at least, and sums of 64 MB at most
-  if (!p.few && tiles < cus)
-    p.parts = (int)std::max<int64_t>(1, std::min({2 * cus / tiles, nk / 4, (int64_t)16, ((int64_t)64 << 20) / (R * cdiv(N, 4) * 16)}));
   return p;
 }
 static int64_t sums_bytes(const Plan& p, int64_t R, int64_t N) { return p.parts > 1 ? p.parts * R * cdiv(N, 4) * 16 : 0; }
