@@ -13,6 +13,7 @@ from __future__ import annotations
 from typing import Optional
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 from . import moe
@@ -88,6 +89,7 @@ class _Dispatch(torch.autograd.Function):
         return tokens.index_select(0, routing.inv.clamp(0, max(T * k - 1, 0)) // k)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, d_rows):
         pos, expert_ids = ctx.saved_tensors
         T, H = ctx.shape
@@ -111,6 +113,7 @@ class _Combine(torch.autograd.Function):
         return moe.combine_rows(rows, routing, expert_ids, topk_w, expert_ids.shape[0])
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, d_out):
         rows, topk_w, pos = ctx.saved_tensors
         T, k, H = topk_w.shape[0], ctx.routing.top_k, rows.shape[1]

@@ -121,6 +121,37 @@ def test_a_row_of_any_pitch_and_no_tokens(gpu_device):
     assert [t.grad.shape for t in leaves] == [t.shape for t in leaves] and not leaves[2].grad.any()
 
 
+def test_an_expert_named_twice_and_long_ids(gpu_device):
+    """a token's slots count one by one, also where they name the same expert; ids of 64 bits are the same ids"""
+    from lowbit.experts import local_moe_bf16
+
+    x, _, w, gu, down, dy = _inputs(30, 4, 2, 256, 128, gpu_device, 3)
+    ids = (torch.arange(60, device=gpu_device, dtype=torch.int32).view(30, 2) // 2) % 4  # both slots alike
+    leaves = [t.clone().requires_grad_(True) for t in (x, w, gu, down)]
+    y = local_moe_bf16(leaves[0], ids, *leaves[1:])
+    got = torch.autograd.grad(y, leaves, dy)
+    wide = [t.double().requires_grad_(True) for t in (x, w, gu, down)]
+    want_y = _reference(wide[0], ids, *wide[1:], _pairs(ids, w, 4, 0))
+    want = torch.autograd.grad(want_y, wide, dy.double())
+    assert _far(y.detach(), want_y.detach()) < 6 * V
+    assert all(_far(a, b) < 6 * V for a, b in zip(got, want))
+    again = local_moe_bf16(leaves[0], ids.long(), *leaves[1:])
+    assert torch.equal(again, y)
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(again, leaves, dy), got))
+
+
+def test_second_gradient_is_refused(gpu_device):
+    from lowbit.experts import local_moe_bf16
+
+    x, ids, w, gu, down, _ = _inputs(16, 4, 2, 256, 128, gpu_device)
+    for which in range(4):
+        leaves = [t.clone().requires_grad_(i == which) for i, t in enumerate((x, w, gu, down))]
+        y = local_moe_bf16(leaves[0], ids, *leaves[1:])
+        (d,) = torch.autograd.grad(y.square().sum(), leaves[which], create_graph=True)
+        with pytest.raises(RuntimeError):
+            d.square().sum().backward()
+
+
 def test_refusals(gpu_device):
     from lowbit.blocks import MoEBlock
     from lowbit.experts import local_moe_bf16

@@ -423,6 +423,22 @@ def test_results_may_be_changed_only_where_nothing_reads_them(gpu_device):
         torch.autograd.grad(y, leaves, dy)
 
 
+def test_x_is_its_own_residual(gpu_device):
+    """s = 2 x, and x has the gradients of both places"""
+    from lowbit.norm import rms_norm
+
+    g = torch.Generator().manual_seed(2)
+    x, dy, ds = (torch.randn(9, 200, generator=g).to(gpu_device) for _ in range(3))
+    a, b, c = (x.clone().requires_grad_(True) for _ in range(3))
+    one, two = rms_norm(a, residual=a), rms_norm(b, residual=c)
+    assert torch.equal(one[1], 2 * x) and torch.equal(one[0], two[0])
+    (da,) = torch.autograd.grad(one, a, (dy, ds))
+    db, dc = torch.autograd.grad(two, (b, c), (dy, ds))
+    assert torch.equal(db, dc) and torch.equal(da, 2 * db)
+    torch.autograd.backward(rms_norm(b, residual=c), (dy, ds))
+    assert torch.equal(b.grad, db) and torch.equal(c.grad, db) and b.grad.data_ptr() != c.grad.data_ptr()
+
+
 def test_module(gpu_device):
     from lowbit.norm import RMSNorm
 
