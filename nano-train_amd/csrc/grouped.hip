@@ -529,10 +529,11 @@ static int bad(const char* fn, const char* what) {
 // rows, y 612 us by 256 tiles and 727, dx 643 and 720, of 64 rows 531 and 445, 423 and 394;
 // 768 x 1024, 64 experts of 256 rows, 55 and 42; 2048 x 4096, 8 experts of 512, 84 and 99.
 //
-// Tiles that leave compute units idle divide the contraction: one expert, 4096 x 4096,
-// 64 rows 46 us whole and 24 in 15 ranges, their sum included; 2048 x 4096, 8 experts of 64
-// rows 47 and 33 in 3 (in 4, more workgroups than places, 44); 1003 rows of 4 experts, 345 x 1000,
-// 19.5 and 15.9.
+// Tiles that leave compute units idle divide the contraction where that pays: a step of
+// 64 is half a us, the ranges' join 4, and their sums go out and in at 4 TB/s.  One expert,
+// 4096 x 4096, 64 rows 46 us whole and 17 in 8 ranges; 2048 x 4096, 8 experts of 64 rows 47 and
+// 33 in 3 ranges (in 4, more workgroups than places, 44); 768 x 1024, 8 experts of 250
+// rows 13 whole and 20 in 2.
 struct Plan {
   bool few;
   int D, parts;
@@ -548,7 +549,15 @@ static Plan plan_of(int64_t R, int64_t E, int64_t N, int64_t K, bool y) {
   if (3 * cdiv(tiles(256), cus) <= 2 * cdiv(t, 2 * cus)) {
     p.D = 256;
   } else if (t < cus) {  // ranges of four steps at least, and sums of 64 MB at most
-    p.parts = (int)std::max<int64_t>(1, std::min({(2 * cus - cus / 8) / t, nk / 4, (int64_t)16, ((int64_t)64 << 20) / (R * cdiv(N, 4) * 16)}));
+    const int64_t sums = R * cdiv(N, 4) * 16, most = std::min({(2 * cus - cus / 8) / t, nk / 4, (int64_t)16, ((int64_t)64 << 20) / sums});
+    double best = 0;
+    for (int n = 2; n <= most; ++n) {
+      const double gain = 0.5 * (double)nk * (n - 1) / n - 4 - (double)(n * sums) * 5e-7;
+      if (gain > best) {
+        best = gain;
+        p.parts = n;
+      }
+    }
   }
   return p;
 }

@@ -144,14 +144,16 @@ __device__ __forceinline__ void store_vec(void* row, const Span<DT, MODE>& s, co
   store_raw<DT, MODE>(row, s, pack<DT>(f));
 }
 
-// sum over the 64 lanes, in every lane
+// sum over each L lanes, in every lane
+template <int L = 64>
 __device__ __forceinline__ float wave_sum(float v) {
+  static_assert(L == 16 || L == 32 || L == 64, "lanes of a row");
   v += __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), 0xB1, 0xF, 0xF, false));
   v += __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), 0x4E, 0xF, 0xF, false));
   v += __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), 0x141, 0xF, 0xF, false));
   v += __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), 0x140, 0xF, 0xF, false));
-  v += __shfl_xor(v, 16);
-  v += __shfl_xor(v, 32);
+  if constexpr (L >= 32) v += __shfl_xor(v, 16);
+  if constexpr (L == 64) v += __shfl_xor(v, 32);
   return v;
 }
 
@@ -160,7 +162,7 @@ __device__ __forceinline__ float wave_sum(float v) {
 template <int RT, int N>
 __device__ __forceinline__ void row_sum(float (&v)[N], float* slot) {
 #pragma unroll
-  for (int i = 0; i < N; ++i) v[i] = wave_sum(v[i]);
+  for (int i = 0; i < N; ++i) v[i] = wave_sum<(RT < 64 ? RT : 64)>(v[i]);
   if constexpr (RT > 64) {
     constexpr int NW = RT / 64;
     if ((threadIdx.x & 63) == 0) {
@@ -224,7 +226,13 @@ __device__ __forceinline__ void load_weights(const void* w, int dt, int t, int H
 }
 
 template <int RT>
-constexpr int block_threads() { return RT == 64 ? 256 : RT; }  // one-wave rows share no barrier
+constexpr int block_threads() { return RT <= 64 ? 256 : RT; }  // rows of one wave or less share no barrier
+// which of a workgroup's rows a thread has, uniform in the wave where it is
+template <int RT>
+__device__ __forceinline__ int row_of_block() {
+  const int r = threadIdx.x / RT;
+  return RT >= 64 ? __builtin_amdgcn_readfirstlane(r) : r;
+}
 
 // dw / db (blockIdx.y) of 32 columns, two a thread, so that a partial row's piece
 // is a whole line: 64 walkers down the P partial rows, their sums added in a fixed

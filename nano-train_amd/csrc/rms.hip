@@ -45,10 +45,11 @@ __device__ __forceinline__ void store_codes(uint8_t* row, int c0, int cols, int 
 template <int DT, int RT, int VPT, int MODE, bool RES, int OUT>
 __global__ void __launch_bounds__(block_threads<RT>()) forward_kernel(Forward g) {
   constexpr int N = El<DT>::n, ROWS = block_threads<RT>() / RT, LANES = 128 / N;
-  __shared__ float red[2][RT / 64];
+  static_assert(RT >= LANES, "a tile of 128 columns is one row's");
+  __shared__ float red[2][RT > 64 ? RT / 64 : 1];
   const int t = threadIdx.x % RT, H = g.H;
   const int64_t stride = (int64_t)gridDim.x * ROWS;
-  int64_t row = (int64_t)blockIdx.x * ROWS + __builtin_amdgcn_readfirstlane(threadIdx.x / RT);
+  int64_t row = (int64_t)blockIdx.x * ROWS + row_of_block<RT>();
   const float inv = 1.0f / (float)H;
   float w[VPT][N];
   load_weights<DT, RT, VPT, MODE>(g.w, g.w_dtype, t, H, 1.0f, w);
@@ -106,6 +107,9 @@ __global__ void __launch_bounds__(block_threads<RT>()) forward_kernel(Forward g)
 #pragma unroll
     for (int v = 0; v < VPT; ++v) {
       const int c0 = (t + v * RT) * N;
+      // a wave past the row's last tile has no codes (8192 x 5120 bf16: 57 us with their
+      // arithmetic, 41 without)
+      if (OUT != OUT_VALUES && VPT > 1 && __builtin_amdgcn_readfirstlane(c0) >= (OUT == OUT_KEEP ? (int)g.ldk : (int)g.ldy)) continue;
       const Span<DT, MODE> sp(t + v * RT, H);
       float f[N];
       renew(x[v], r);
@@ -168,11 +172,14 @@ __global__ void __launch_bounds__(block_threads<RT>()) forward_kernel(Forward g)
   }
 }
 
-// Threads and vectors a row, and workgroups a compute unit, as layer norm's forward
+// Threads and vectors a row, and workgroups a compute unit, as layer norm's forward; rows of up
+// to 16 or 32 vectors share a wave (262144 x 64 bf16 16 us, by a wave a row 55; codes 27, 167)
 struct Shape {
   int rt, vpt, per_cu;
 };
-static Shape shape_of(int64_t nv) {
+static Shape shape_of(int dt, int64_t nv) {
+  if (nv <= 16 && dt != NTLB_F32) return {16, 1, 8};
+  if (nv <= 32) return {32, 1, 8};
   if (nv <= 64) return {64, 1, 4};
   if (nv <= 128) return {64, 2, 4};
   if (nv <= 256) return {64, 4, 4};
@@ -187,9 +194,9 @@ static bool launch(const Shape& s, const Forward& g, int64_t n, hipStream_t st) 
 #define NTLB_CASE(RT, VPT)                                                                                            \
   if (s.rt == RT && s.vpt == VPT)                                                                                     \
     return forward_kernel<DT, RT, VPT, MODE, RES, OUT><<<(unsigned)n, block_threads<RT>(), 0, st>>>(g), true;
-  if constexpr (MODE == TINY) {
-    NTLB_CASE(64, 1)
-  } else {
+  if constexpr (DT != DT_F32) NTLB_CASE(16, 1)
+  if constexpr (DT == DT_F32 || MODE != TINY) NTLB_CASE(32, 1)
+  if constexpr (MODE != TINY) {
     NTLB_CASE(64, 1) NTLB_CASE(64, 2) NTLB_CASE(64, 4) NTLB_CASE(128, 4) NTLB_CASE(256, 4) NTLB_CASE(512, 4)
     if constexpr (DT == DT_F32) NTLB_CASE(512, 8)
   }
@@ -214,8 +221,8 @@ static bool pick_mode(const Shape& s, const Forward& g, int64_t n, int out, hipS
 }
 static int run(const char* fn, int dt, const Forward& g, int out, void* stream) {
   const int64_t nv = cdiv((int64_t)g.H * dtype_size(dt), 16);
-  const Shape s = shape_of(nv);
-  const int64_t n = std::max<int64_t>(1, std::min(cdiv(g.T, s.rt == 64 ? 4 : 1), (int64_t)split_device_cus() * s.per_cu));
+  const Shape s = shape_of(dt, nv);
+  const int64_t n = std::max<int64_t>(1, std::min(cdiv(g.T, s.rt <= 64 ? 256 / s.rt : 1), (int64_t)split_device_cus() * s.per_cu));
   hipStream_t st = as_stream(stream);
   const bool ok = dt == NTLB_F32 ? pick_mode<DT_F32>(s, g, n, out, st)
                   : dt == NTLB_BF16 ? pick_mode<DT_BF16>(s, g, n, out, st)

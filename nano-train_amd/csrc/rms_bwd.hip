@@ -95,10 +95,10 @@ struct Held {
 template <int DT, int RT, int VPT, int MODE, bool DS, bool KEEP>
 __global__ void __launch_bounds__(block_threads<RT>()) backward_kernel(Backward g) {
   constexpr int N = El<DT>::n, BT = block_threads<RT>(), ROWS = BT / RT;
-  __shared__ float red[2][RT / 64];
+  __shared__ float red[2][RT > 64 ? RT / 64 : 1];
   const int t = threadIdx.x % RT, H = g.H;
   const int64_t stride = (int64_t)gridDim.x * ROWS;
-  int64_t row = (int64_t)blockIdx.x * ROWS + __builtin_amdgcn_readfirstlane(threadIdx.x / RT);
+  int64_t row = (int64_t)blockIdx.x * ROWS + row_of_block<RT>();
   const float inv = 1.0f / (float)H;
   float w[VPT][N], aw[VPT][N];
   load_weights<DT, RT, VPT, MODE>(g.w, g.w_dtype, t, H, 1.0f, w);
@@ -207,11 +207,15 @@ __global__ void __launch_bounds__(block_threads<RT>()) backward_kernel(Backward 
 
 // Threads and vectors a row, and workgroups a compute unit, as layer norm's backward but for
 // rows of 513 to 1024 vectors (8192 x 7168 bf16 with a residual, s kept: 512 x 2 75 us, 256 x
-// 4 79, 1024 x 1 81)
+// 4 79, 1024 x 1 81) and of up to 32, which share a wave (262144 x 64 bf16 29 us, by a wave a
+// row 110)
 struct Shape {
   int rt, vpt, per_cu;
 };
-static Shape shape_of(int64_t nv) {
+static Shape shape_of(int dt, int64_t H) {
+  const int64_t nv = cdiv(H * dtype_size(dt), 16);
+  if (nv <= 16 && dt != NTLB_F32) return {16, 1, 4};
+  if (nv <= 32) return {32, 1, 4};
   if (nv <= 64) return {64, 1, 2};
   if (nv <= 128) return {128, 1, 4};
   if (nv <= 256) return {256, 1, 2};
@@ -220,9 +224,8 @@ static Shape shape_of(int64_t nv) {
   if (nv <= 2048) return {512, 4, 1};
   return {512, 8, 1};
 }
-static Shape shape_of(int dt, int64_t H) { return shape_of(cdiv(H * dtype_size(dt), 16)); }
 static int64_t groups(const Shape& s, int64_t T) {
-  return std::max<int64_t>(1, std::min(cdiv(T, s.rt == 64 ? 4 : 1), (int64_t)split_device_cus() * s.per_cu));
+  return std::max<int64_t>(1, std::min(cdiv(T, s.rt <= 64 ? 256 / s.rt : 1), (int64_t)split_device_cus() * s.per_cu));
 }
 
 template <int DT, int MODE, bool DS, bool KEEP>
@@ -230,9 +233,9 @@ static bool launch(const Shape& s, const Backward& g, int64_t n, hipStream_t st)
 #define NTLB_CASE(RT, VPT)                                                                                            \
   if (s.rt == RT && s.vpt == VPT)                                                                                     \
     return backward_kernel<DT, RT, VPT, MODE, DS, KEEP><<<(unsigned)n, block_threads<RT>(), 0, st>>>(g), true;
-  if constexpr (MODE == TINY) {
-    NTLB_CASE(64, 1)
-  } else {
+  if constexpr (DT != DT_F32) NTLB_CASE(16, 1)
+  if constexpr (DT == DT_F32 || MODE != TINY) NTLB_CASE(32, 1)
+  if constexpr (MODE != TINY) {
     NTLB_CASE(64, 1) NTLB_CASE(128, 1) NTLB_CASE(256, 1) NTLB_CASE(512, 1) NTLB_CASE(512, 2) NTLB_CASE(512, 4)
     if constexpr (DT == DT_F32) NTLB_CASE(512, 8)
   }
