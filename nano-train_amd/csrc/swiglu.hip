@@ -10,7 +10,10 @@
 // With t = exp(-|g|) sigmoid and its complement are 1 / (1 + t) and t / (1 + t), the
 // former at g's own side: neither overflows nor cancels.
 //
-// HBM-bound.  16 lanes (fp32: 32) take a tile, a lane 16 bytes of gate and of up.
+// HBM-bound.  16 lanes (fp32: 32) take a tile, a lane 16 bytes of gate and of up, so
+// that a tile's scale is a reduction within the wave and nothing is read twice.  32768 x
+// 2048 bf16: 66 us (6.1 TB/s), keeping codes 93 (5.8), backward 106 (6.3), from codes
+// 86 (6.2).  Codes as 16-byte stores, two lanes' exchanged: slower.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
