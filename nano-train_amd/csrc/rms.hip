@@ -12,7 +12,8 @@
 //
 // HBM-bound: a row is read once, stays in registers (ntlb_rows.h) and is written
 // once (8192 x 7168 bf16 with a residual: 85 us, 5.5 TB/s; with codes kept 99; to codes 80).  To
-// codes without a residual the arithmetic takes as long (49 us, 3.6 TB/s).  Statistics are fp32.  A tile of 128 columns lies in 16 (fp32: 32) lanes
+// codes without a residual the arithmetic takes as long (49 us, 3.6 TB/s).  Statistics
+// are fp32.  A tile of 128 columns lies in 16 (fp32: 32) lanes
 // next to each other, so its largest magnitude is a reduction within the wave.
 #include <hip/hip_runtime.h>
 
