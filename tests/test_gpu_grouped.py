@@ -84,6 +84,49 @@ def test_values_and_gradients(gpu_device, counts, K, N, spare, checkpoint):
     assert torch.equal(again[0], dx) and torch.equal(again[1], dw)
 
 
+@pytest.mark.parametrize("counts,K,N", [([1] * 4095 + [3], 16, 8), ([2], 1 << 22, 3), ([3, 0], 8, 1 << 22), ([1 << 20, 5], 8, 8),
+                                        ([0] * 64 + [70] + [0] * 70 + [9], 320, 128)])
+def test_the_largest_of_each_size(gpu_device, counts, K, N):
+    from lowbit.experts import grouped_matmul
+
+    g = torch.Generator(gpu_device).manual_seed(K + N)
+    R, E = sum(counts), len(counts)
+    x, w, dy = (torch.randn(*size, generator=g, device=gpu_device).bfloat16() for size in ((R, K), (E, N, K), (R, N)))
+    offsets = torch.tensor([0] + counts).cumsum(0).int().to(gpu_device)
+    lx, lw = x.requires_grad_(True), w.requires_grad_(True)
+    y = grouped_matmul(lx, lw, offsets)
+    dx, dw = torch.autograd.grad(y, (lx, lw), dy)
+    ends = offsets.tolist()
+    for e in [0, E // 2, E - 1]:
+        part = slice(ends[e], ends[e + 1])
+        n = ends[e + 1] - ends[e]
+        if n == 0:
+            assert not dw[e].any()
+            continue
+        xe, we, de = x.detach()[part].double(), w.detach()[e].double(), dy[part].double()
+        _check(y.detach()[part], xe @ we.t(), K, xe.abs() @ we.t().abs(), ("y", e))
+        _check(dx[part], de @ we, N, de.abs() @ we.abs(), ("dx", e))
+        _check(dw[e], de.t() @ xe, n, de.t().abs() @ xe.abs(), ("dw", e))
+
+
+def test_calls_side_by_side(gpu_device):
+    """two streams at once, each with ranges of a contraction: every call has sums of its own"""
+    from lowbit.experts import grouped_matmul
+
+    sets = [_inputs([60, 0, 77], 2048, 264, seed, gpu_device) for seed in (1, 2)]
+    with torch.no_grad():
+        want = [grouped_matmul(x, w, o) for x, w, _, o in sets]
+        streams = [torch.cuda.Stream() for _ in sets]
+        torch.cuda.synchronize()
+        got = [[], []]
+        for _ in range(20):
+            for i, (x, w, _, o) in enumerate(sets):
+                with torch.cuda.stream(streams[i]):
+                    got[i].append(grouped_matmul(x, w, o))
+        torch.cuda.synchronize()
+    assert all(torch.equal(t, want[i]) for i in range(2) for t in got[i])
+
+
 @pytest.mark.parametrize("which", ["pitch", "offset", "transposed", "weights_t", "weights_shared", "weights_slice", "dy_pitch",
                                    "dy_repeated", "x_repeated"])
 def test_strides(gpu_device, which):
