@@ -187,7 +187,9 @@ __global__ void __launch_bounds__(256) join_kernel(Args g) {
   v4f acc[D / 32][4];                      \
   _Pragma("unroll") for (int i = 0; i < D / 32; ++i) _Pragma("unroll") for (int j = 0; j < 4; ++j) acc[i][j] = (v4f){0.f, 0.f, 0.f, 0.f}
 
-// y: W by rows.  Both operands come in the same way; A's copies two steps ahead.
+// y: W by rows.  Both operands come in the same way.  By 256 tiles x's copies run two
+// steps ahead, by 128 those of W, which then is the larger and read once (64 experts of
+// 16 rows, 2048 x 4096: 243 us, so 233; 32 of 40, 4096 x 7168: 430, 418).
 template <int D>
 __global__ void __launch_bounds__(2 * D, D == 256 ? 1 : 2) rows_kernel(Args g) {
   NTLB_TILE_STAGES_AHEAD(D);
@@ -204,8 +206,8 @@ __global__ void __launch_bounds__(2 * D, D == 256 ? 1 : 2) rows_kernel(Args g) {
     cb.init(Mat{g.b + (int64_t)f.e * g.b_expert, g.ldb, g.N, g.k}, n0, wave, lane);
     int k0, k1;
     steps_of<D>(g, f, k0, k1);
-    prime_ahead(ca, cb, k0, wave, stages);
-    multiply_ahead<D, false, false>(ca, cb, k0, k1, acc, wm, wn, wave, lane, stages);
+    prime_ahead<D == 128>(ca, cb, k0, wave, stages);
+    multiply_ahead<D, false, false, D == 128>(ca, cb, k0, k1, acc, wm, wn, wave, lane, stages);
   }
   if (D == 128 && g.parts > 1)
     store_sums<D>(acc, wm, wn, own_lane(), m0, n0, f.n, g.sums + (f.part * g.R + f.lo) * g.lds, g.lds);

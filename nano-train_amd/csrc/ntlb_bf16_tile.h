@@ -436,28 +436,32 @@ __device__ __forceinline__ void multiply(CA& ca, CB& cb, int kb0, int kb1, v4f (
   }
 }
 
-// The same with A's copies two steps ahead, for operands that come from far: three
-// stages of A, two of B (5 D ROWB bytes).  A step's copies of B are issued before
-// its copies of A, so that at its end a wave waits for those of the next step only.
+// The same with the copies of A (FAR_B: of B) two steps ahead, for operands that come
+// from far: three stages of it, two of the other (5 D ROWB bytes).  A step's copies of
+// the near one are issued first, so that at its end a wave waits for those of the next step only.
 // (32768 x 7168 by 4096 rows: 1507 us with both one step ahead, 1404 so; with B's two
 // ahead too, its stage freed by a second barrier after its fragments are read, 1501.)
 // prime_ahead() has been called for step k0; k0 < k1.  Afterwards nothing reads or
 // writes the stages.
 struct Stages {
-  uint8_t *a0, *a1, *a2, *b0, *b1;
+  uint8_t *far0, *far1, *far2, *near0, *near1;  // of the operand two steps ahead, of the other
   template <int I>
-  __device__ __forceinline__ uint8_t* a() const { return I == 0 ? a0 : I == 1 ? a1 : a2; }
+  __device__ __forceinline__ uint8_t* far() const { return I == 0 ? far0 : I == 1 ? far1 : far2; }
   template <int I>
-  __device__ __forceinline__ uint8_t* b() const { return I == 0 ? b0 : b1; }
+  __device__ __forceinline__ uint8_t* near() const { return I == 0 ? near0 : near1; }
 };
-template <typename CA, typename CB>
+template <bool FAR_B = false, typename CA, typename CB>
 __device__ __forceinline__ void prime_ahead(CA& ca, CB& cb, int k0, int wave, const Stages& st) {
-  prime(ca, cb, k0, wave, st.a0, st.b0);
-  ca.set(k0 + 1);
+  prime(ca, cb, k0, wave, FAR_B ? st.near0 : st.far0, FAR_B ? st.far0 : st.near0);
+  if constexpr (FAR_B) cb.set(k0 + 1);
+  else ca.set(k0 + 1);
 #pragma unroll
-  for (int j = 0; j < 4; ++j) ca.issue(st.a1, wave, j);
+  for (int j = 0; j < 4; ++j) {
+    if constexpr (FAR_B) cb.issue(st.far1, wave, j);
+    else ca.issue(st.far1, wave, j);
+  }
 }
-template <int D, bool TA, bool TB, typename CA, typename CB>
+template <int D, bool TA, bool TB, bool FAR_B = false, typename CA, typename CB>
 __device__ __forceinline__ void multiply_ahead(CA& ca, CB& cb, int k0, int k1, v4f (&acc)[D / 32][4], int wm, int wn, int wave, int lane,
                                                const Stages& st) {
   constexpr int MT = D / 32;
@@ -478,27 +482,35 @@ __device__ __forceinline__ void multiply_ahead(CA& ca, CB& cb, int k0, int k1, v
   for (int i = 0; i < 4; ++i) b1[i] = af[i] = (v8i){0, 0, 0, 0, 0, 0, 0, 0};
   __builtin_amdgcn_s_waitcnt(FOUR);
   barrier();
-  // step kt, from stages ta and tb, the step after next's A to na; bo: B's fragments of the step before.
+  // step kt, from stages tf and tn, the step after next's copies to nf, the next one's to nn; bo: B's fragments
+  // of the step before.
   // Copies of steps past k1 are made all the same, so that no step has a branch: past the
   // contraction they fetch nothing (all of them is out of their resources' bounds).
-  auto step = [&](uint8_t* ta, uint8_t* tb, uint8_t* na, uint8_t* nb, int kt, const v8i (&bo)[4], v8i (&bf)[4]) {
-    ca.set(kt + 2);
-    cb.set(kt + 1);
+  auto step = [&](uint8_t* tf, uint8_t* tn, uint8_t* nf, uint8_t* nn, int kt, const v8i (&bo)[4], v8i (&bf)[4]) {
+    uint8_t *ta = FAR_B ? tn : tf, *tb = FAR_B ? tf : tn;
+    ca.set(kt + (FAR_B ? 1 : 2));
+    cb.set(kt + (FAR_B ? 2 : 1));
 #pragma unroll
-    for (int tn = 0; tn < 4; ++tn) {
+    for (int i = 0; i < 4; ++i) {
       fb.anew();
-      bf[tn] = frag(tb, fb, tn);
+      bf[i] = frag(tb, fb, i);
     }
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       fa.anew();
       af[i] = frag(ta, fa, i);
-      cb.issue(nb, wave, 2 * i);
-      cb.issue(nb, wave, 2 * i + 1);
+#pragma unroll
+      for (int j = 2 * i; j < 2 * i + 2; ++j) {
+        if constexpr (FAR_B) ca.issue(nn, wave, j);
+        else cb.issue(nn, wave, j);
+      }
       rows(MT - 2 + i, bo, af[2 + i]);
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) ca.issue(na, wave, j);
+    for (int j = 0; j < 4; ++j) {
+      if constexpr (FAR_B) cb.issue(nf, wave, j);
+      else ca.issue(nf, wave, j);
+    }
 #pragma unroll
     for (int tm = 0; tm < MT - 2; ++tm) {
       fa.anew();
@@ -508,7 +520,7 @@ __device__ __forceinline__ void multiply_ahead(CA& ca, CB& cb, int k0, int k1, v
     __builtin_amdgcn_s_waitcnt(FOUR);
     barrier();
   };
-#define NTLB_STEP(I, BO, BF) step(st.a<(I) % 3>(), st.b<(I) % 2>(), st.a<((I) + 2) % 3>(), st.b<((I) + 1) % 2>(), kt + I, BO, BF)
+#define NTLB_STEP(I, BO, BF) step(st.far<(I) % 3>(), st.near<(I) % 2>(), st.far<((I) + 2) % 3>(), st.near<((I) + 1) % 2>(), kt + I, BO, BF)
   int kt = k0;
   for (; kt + 6 <= k1; kt += 6) {
     NTLB_STEP(0, b1, b0);
@@ -521,7 +533,7 @@ __device__ __forceinline__ void multiply_ahead(CA& ca, CB& cb, int k0, int k1, v
   // Up to five more, their stages found at run time: the compiler then waits for every
   // copy before it reads one, and unrolled as above they take more registers than
   // there are.
-  uint8_t *p0 = st.a0, *p1 = st.a1, *p2 = st.a2, *q0 = st.b0, *q1 = st.b1;
+  uint8_t *p0 = st.far0, *p1 = st.far1, *p2 = st.far2, *q0 = st.near0, *q1 = st.near1;
   for (; kt < k1; ++kt) {
     step(p0, q0, p2, q1, kt, b1, b0);
 #pragma unroll
@@ -549,8 +561,9 @@ __device__ __forceinline__ void multiply_ahead(CA& ca, CB& cb, int k0, int k1, v
   __shared__ __attribute__((aligned(16))) uint8_t lb0[D * ROWB]; \
   __shared__ __attribute__((aligned(16))) uint8_t la1[D * ROWB]; \
   __shared__ __attribute__((aligned(16))) uint8_t lb1[D * ROWB]
-// three of A, two of B.  B's come first (they lie by name): its fragments' offsets then fit into the reads,
-// which saves registers where it is transposed.
+// three of the far operand, two of the near one, which come first (they lie by name):
+// its fragments' offsets then fit into the reads, which saves registers where it is
+// transposed.
 #define NTLB_TILE_STAGES_AHEAD(D)                                   \
   __shared__ __attribute__((aligned(16))) uint8_t stage_0[D * ROWB]; \
   __shared__ __attribute__((aligned(16))) uint8_t stage_1[D * ROWB]; \
