@@ -9,7 +9,7 @@
 //
 // Matrix-core bound where experts have a few hundred rows and more, on the tiles of
 // ntlb_bf16_tile.h (32768 rows of 32 experts, 4096 x 7168: y 1.69 ms, 1.14 PFLOP/s; dx 1.73;
-// dW 1.89); bound by the weights' way from HBM below (256 rows of them: y 334 us, 5.6 TB/s).
+// dW 1.89); bound by the weights' way from HBM below (256 rows of them: y 327 us, 5.8 TB/s).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
