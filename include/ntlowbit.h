@@ -1157,8 +1157,9 @@ int ntlb_swiglu_rows_backward(const void* x, int dtype, int64_t T, int64_t I, in
  * 0, not decreasing; values past R count as R), whose weight is w + e * w_stride
  * [N, K]:
  *   y[r] = x[r] W_e^T;   dx[r] = dy[r] W_e;   dw[e] = sum over e's rows of dy[r]^T x[r]
- * summed in fp32, rounded once; y and dx are zero in rows at or past offsets[E],
- * dw [E, N, K] (contiguous) for experts without rows.  Pitches in elements.  Inputs
+ * summed in fp32 in an order that R, E, N and K alone decide, rounded once; y and dx
+ * are zero in rows at or past offsets[E], dw [E, N, K] (contiguous) for experts
+ * without rows.  Pitches in elements.  Inputs
  * lie in 16-byte aligned rows of whole 16-byte pieces (pitch % 8 == 0, at most
  * 2^22; w_stride % 8 == 0); where a product sums along their rows (x and w for y,
  * dy for dx) their columns up to the next multiple of 8 are zero.  Outputs need only

@@ -55,9 +55,10 @@ def grouped_matmul(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor,
     [E + 1], not decreasing, on x's device: expert e has the rows offsets[e] ..
     offsets[e + 1] - 1, any number of them, offsets[0] being 0.  Rows at or past offsets[E]
     (a capacity's spare rows) are not read; y and the gradient of x are zero there.  The
-    gradient of an expert without rows is zero.  Sums are fp32, results rounded once.
-    x and weight of any strides: what is not in rows of whole 16-byte pieces (K % 8,
-    for the backward N % 8) is copied to padded rows first.  E <= 4096.
+    gradient of an expert without rows is zero.  Sums are fp32, in an order that R, E,
+    N and K alone decide, results rounded once.  x and weight of any strides: what is
+    not in rows of whole 16-byte pieces (K % 8, for the backward N % 8) is copied to
+    padded rows first.  E <= 4096.
 
     checkpoint None keeps x for the weight's gradient; "e4m3" keeps it in 8 bits (a
     power of two for each 128 columns, values rounded by at most 2^-4 of
