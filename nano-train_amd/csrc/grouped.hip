@@ -8,7 +8,7 @@
 // a buffer) and finds its tile.
 //
 // Matrix-core bound where experts have a few hundred rows and more, on the tiles of
-// ntlb_bf16_tile.h (32768 rows of 32 experts, 4096 x 7168: y 1.69 ms, 1.14 PFLOP/s; dx 1.73;
+// ntlb_bf16_tile.h (32768 rows of 32 experts, 4096 x 7168: y 1.66 ms, 1.16 PFLOP/s; dx 1.76;
 // dW 1.89); bound by the weights' way from HBM below (256 rows of them: y 327 us, 5.8 TB/s).
 #include <hip/hip_runtime.h>
 
@@ -207,7 +207,7 @@ __global__ void __launch_bounds__(2 * D, D == 256 ? 1 : 2) rows_kernel(Args g) {
     int k0, k1;
     steps_of<D>(g, f, k0, k1);
     prime_ahead<D == 128>(ca, cb, k0, wave, stages);
-    multiply_ahead<D, false, false, D == 128>(ca, cb, k0, k1, acc, wm, wn, wave, lane, stages);
+    multiply_ahead<D, D == 128>(ca, cb, k0, k1, acc, wm, wn, wave, lane, stages);
   }
   if (D == 128 && g.parts > 1)
     store_sums<D>(acc, wm, wn, own_lane(), m0, n0, f.n, g.sums + (f.part * g.R + f.lo) * g.lds, g.lds);

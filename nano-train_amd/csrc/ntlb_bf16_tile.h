@@ -436,9 +436,10 @@ __device__ __forceinline__ void multiply(CA& ca, CB& cb, int kb0, int kb1, v4f (
   }
 }
 
-// The same with the copies of A (FAR_B: of B) two steps ahead, for operands that come
-// from far: three stages of it, two of the other (5 D ROWB bytes).  A step's copies of
-// the near one are issued first, so that at its end a wave waits for those of the next step only.
+// The same of two operands by rows with the copies of A (FAR_B: of B) two steps ahead,
+// for what comes from far: three stages of it, two of the other (5 D ROWB bytes).  A
+// step's copies of the near one are issued first, so that at its end a wave waits for
+// those of the next step only.
 // (32768 x 7168 by 4096 rows: 1507 us with both one step ahead, 1404 so; with B's two
 // ahead too, its stage freed by a second barrier after its fragments are read, 1501.)
 // prime_ahead() has been called for step k0; k0 < k1.  Afterwards nothing reads or
@@ -461,23 +462,21 @@ __device__ __forceinline__ void prime_ahead(CA& ca, CB& cb, int k0, int wave, co
     else ca.issue(st.far1, wave, j);
   }
 }
-template <int D, bool TA, bool TB, bool FAR_B = false, typename CA, typename CB>
+template <int D, bool FAR_B = false, typename CA, typename CB>
 __device__ __forceinline__ void multiply_ahead(CA& ca, CB& cb, int k0, int k1, v4f (&acc)[D / 32][4], int wm, int wn, int wave, int lane,
                                                const Stages& st) {
   constexpr int MT = D / 32;
   constexpr int NONE = 0x0070, FOUR = 0x0074;  // s_waitcnt: lgkmcnt(0) with vmcnt(0), vmcnt(4)
   auto rows = [&](int tm, const v8i (&bf)[4], const v8i& a) {
-    if (TB && !TA) __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int tn = 0; tn < 4; ++tn) acc[tm][tn] = mma<0>(bf[tn], a, acc[tm][tn]);
 #pragma unroll
     for (int tn = 0; tn < 4; ++tn) acc[tm][tn] = mma<1>(bf[tn], a, acc[tm][tn]);
     asm volatile("" : "+v"(acc[tm][0]), "+v"(acc[tm][1]), "+v"(acc[tm][2]), "+v"(acc[tm][3])::"memory");
-    if (TB && !TA) __builtin_amdgcn_s_setprio(0);
   };
   v8i b0[4], b1[4], af[4];
-  FragAt<TA, D> fa(wm * 16 * MT, lane);
-  FragAt<TB, D> fb(wn * 64, lane);
+  FragAt<false, D> fa(wm * 16 * MT, lane);
+  FragAt<false, D> fb(wn * 64, lane);
 #pragma unroll
   for (int i = 0; i < 4; ++i) b1[i] = af[i] = (v8i){0, 0, 0, 0, 0, 0, 0, 0};
   __builtin_amdgcn_s_waitcnt(FOUR);
@@ -521,29 +520,28 @@ __device__ __forceinline__ void multiply_ahead(CA& ca, CB& cb, int k0, int k1, v
     barrier();
   };
 #define NTLB_STEP(I, BO, BF) step(st.far<(I) % 3>(), st.near<(I) % 2>(), st.far<((I) + 2) % 3>(), st.near<((I) + 1) % 2>(), kt + I, BO, BF)
-  int kt = k0;
-  for (; kt + 6 <= k1; kt += 6) {
+  // A contraction may end behind each of the six steps.  (Up to five steps in a loop of
+  // their own, stages found at run time: the compiler then waits for every copy before
+  // it reads one, 32768 x 7168 by 32 matrices of 4096 rows 1700 us and so 1657.  Of
+  // transposed operands the exits cost more registers than there are.)
+  for (int kt = k0;; kt += 6) {
     NTLB_STEP(0, b1, b0);
+    if (kt + 1 >= k1) goto even;
     NTLB_STEP(1, b0, b1);
+    if (kt + 2 >= k1) break;
     NTLB_STEP(2, b1, b0);
+    if (kt + 3 >= k1) goto even;
     NTLB_STEP(3, b0, b1);
+    if (kt + 4 >= k1) break;
     NTLB_STEP(4, b1, b0);
+    if (kt + 5 >= k1) goto even;
     NTLB_STEP(5, b0, b1);
+    if (kt + 6 >= k1) break;
   }
-  // Up to five more, their stages found at run time: the compiler then waits for every
-  // copy before it reads one, and unrolled as above they take more registers than
-  // there are.
-  uint8_t *p0 = st.far0, *p1 = st.far1, *p2 = st.far2, *q0 = st.near0, *q1 = st.near1;
-  for (; kt < k1; ++kt) {
-    step(p0, q0, p2, q1, kt, b1, b0);
+  if (false) {
+  even:
 #pragma unroll
-    for (int j = 0; j < 4; ++j) b1[j] = b0[j];
-    uint8_t *p = p0, *q = q0;
-    p0 = p1;
-    p1 = p2;
-    p2 = p;
-    q0 = q1;
-    q1 = q;
+    for (int i = 0; i < 4; ++i) b1[i] = b0[i];
   }
   rows(MT - 2, b1, af[2]);
   rows(MT - 1, b1, af[3]);
@@ -561,9 +559,7 @@ __device__ __forceinline__ void multiply_ahead(CA& ca, CB& cb, int k0, int k1, v
   __shared__ __attribute__((aligned(16))) uint8_t lb0[D * ROWB]; \
   __shared__ __attribute__((aligned(16))) uint8_t la1[D * ROWB]; \
   __shared__ __attribute__((aligned(16))) uint8_t lb1[D * ROWB]
-// three of the far operand, two of the near one, which come first (they lie by name):
-// its fragments' offsets then fit into the reads, which saves registers where it is
-// transposed.
+// three of the far operand, two of the near one
 #define NTLB_TILE_STAGES_AHEAD(D)                                   \
   __shared__ __attribute__((aligned(16))) uint8_t stage_0[D * ROWB]; \
   __shared__ __attribute__((aligned(16))) uint8_t stage_1[D * ROWB]; \
