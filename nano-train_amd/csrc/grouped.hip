@@ -188,8 +188,9 @@ __global__ void __launch_bounds__(256) join_kernel(Args g) {
   _Pragma("unroll") for (int i = 0; i < D / 32; ++i) _Pragma("unroll") for (int j = 0; j < 4; ++j) acc[i][j] = (v4f){0.f, 0.f, 0.f, 0.f}
 
 // y: W by rows.  Both operands come in the same way.  By 256 tiles x's copies run two
-// steps ahead, by 128 those of W, which then is the larger and read once (64 experts of
-// 16 rows, 2048 x 4096: 243 us, so 233; 32 of 40, 4096 x 7168: 430, 418).
+// steps ahead (32768 rows of 32 experts, 4096 x 7168: 1640 us, W's instead 1733), by 128
+// those of W, which then is the larger and read once (64 experts of 16 rows, 2048 x
+// 4096: x's 243 us, W's 233; 32 of 40, 4096 x 7168: 430, 418).
 template <int D>
 __global__ void __launch_bounds__(2 * D, D == 256 ? 1 : 2) rows_kernel(Args g) {
   NTLB_TILE_STAGES_AHEAD(D);
