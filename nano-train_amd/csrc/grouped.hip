@@ -9,7 +9,7 @@
 //
 // Matrix-core bound where experts have a few hundred rows and more, on the tiles of
 // ntlb_bf16_tile.h (32768 rows of 32 experts, 4096 x 7168: y 1.66 ms, 1.16 PFLOP/s; dx 1.76;
-// dW 1.89); bound by the weights' way from HBM below (256 rows of them: y 327 us, 5.8 TB/s).
+// dW 1.89); bound by the weights' way from HBM below (256 rows of them: y 315 us, 6.0 TB/s).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -200,6 +200,7 @@ __global__ void __launch_bounds__(2 * D, D == 256 ? 1 : 2) rows_kernel(Args g) {
   Found f;
   if (!find<D>(g, (int)((g.N + D - 1) / D), (int)blockIdx.x, f)) return;
   const int64_t m0 = f.m0, n0 = (int64_t)f.tn * D;
+  const bool idle = __builtin_amdgcn_readfirstlane(f.m0 + wm * (D / 2) >= f.n);
   NTLB_ZERO_ACC(D);
   if (f.e < g.E) {
     RowWalk<D> ca, cb;
@@ -208,7 +209,7 @@ __global__ void __launch_bounds__(2 * D, D == 256 ? 1 : 2) rows_kernel(Args g) {
     int k0, k1;
     steps_of<D>(g, f, k0, k1);
     prime_ahead<D == 128>(ca, cb, k0, wave, stages);
-    multiply_ahead<D, D == 128>(ca, cb, k0, k1, acc, wm, wn, wave, lane, stages);
+    multiply_ahead<D, D == 128>(ca, cb, k0, k1, acc, wm, wn, wave, lane, stages, idle);
   }
   if (D == 128 && g.parts > 1)
     store_sums<D>(acc, wm, wn, own_lane(), m0, n0, f.n, g.sums + (f.part * g.R + f.lo) * g.lds, g.lds);
@@ -226,6 +227,7 @@ __global__ void __launch_bounds__(2 * D, D == 256 ? 1 : 2) inputs_kernel(Args g)
   Found f;
   if (!find<D>(g, (int)((g.N + D - 1) / D), (int)blockIdx.x, f)) return;
   const int64_t m0 = f.m0, n0 = (int64_t)f.tn * D;
+  const bool idle = __builtin_amdgcn_readfirstlane(f.m0 + wm * (D / 2) >= f.n);
   NTLB_ZERO_ACC(D);
   if (f.e < g.E) {
     RowCopy<D> ca;
@@ -234,7 +236,7 @@ __global__ void __launch_bounds__(2 * D, D == 256 ? 1 : 2) inputs_kernel(Args g)
     cb.init(Mat{g.b + (int64_t)f.e * g.b_expert, g.ldb, g.N, g.k}, n0, wave, lane);
     int k0, k1;
     steps_of<D>(g, f, k0, k1);
-    multiply<D, false, true>(ca, cb, k0, k1, acc, wm, wn, wave, lane, la0, lb0, la1, lb1);
+    multiply<D, false, true>(ca, cb, k0, k1, acc, wm, wn, wave, lane, la0, lb0, la1, lb1, idle);
   }
   if (D == 128 && g.parts > 1)
     store_sums<D>(acc, wm, wn, lane, m0, n0, f.n, g.sums + (f.part * g.R + f.lo) * g.lds, g.lds);

@@ -356,11 +356,35 @@ __device__ __forceinline__ void prime(CA& ca, CB& cb, int kt, int wave, uint8_t*
 // of 128 x 64, one workgroup a compute unit; 128: four of 64 x 64, two workgroups),
 // wave (wm, wn) of it.  la0 ... lb1: two stages of both operands, D * ROWB bytes
 // each, which nothing reads or writes any more afterwards.  PRIMED: prime() has been
-// called for step kb0 and the first stage.
+// called for step kb0 and the first stage.  idle: the wave's rows lie behind the
+// operand's last one; it copies its share and multiplies nothing, which leaves the matrix
+// cores and their power to the others (256 rows of 32 experts, 4096 x 7168: 325 us and so 315;
+// 4096 rows 568 and 542; dx of 32768 1773 and 1748).
 template <int D, bool TA, bool TB, bool PRIMED = false, typename CA, typename CB>
 __device__ __forceinline__ void multiply(CA& ca, CB& cb, int kb0, int kb1, v4f (&acc)[D / 32][4], int wm, int wn, int wave,
-                                         int lane, uint8_t* la0, uint8_t* lb0, uint8_t* la1, uint8_t* lb1) {
+                                         int lane, uint8_t* la0, uint8_t* lb0, uint8_t* la1, uint8_t* lb1,
+                                         bool idle = false) {
   constexpr int MT = D / 32;
+  if (idle && kb0 < kb1) {  // the copies and barriers of the loop below
+    if constexpr (!PRIMED) prime(ca, cb, kb0, wave, la0, lb0);
+    __builtin_amdgcn_s_waitcnt(0);
+    barrier();
+#pragma unroll 1
+    for (int kt = kb0; kt < kb1; ++kt) {
+      const bool odd = (kt - kb0) & 1;
+      const int kn = min(kt + 1, kb1 - 1);
+      ca.set(kn);
+      cb.set(kn);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        ca.issue(odd ? la0 : la1, wave, j);
+        cb.issue(odd ? lb0 : lb1, wave, j);
+      }
+      __builtin_amdgcn_s_waitcnt(0);
+      barrier();
+    }
+    return;
+  }
   // K loop.  A step's fragments stream through registers, A's two row groups
   // ahead.  The one barrier of a step stands after its last LDS read, before the
   // products of its last two row groups: those cover the first reads of the next
@@ -443,7 +467,7 @@ __device__ __forceinline__ void multiply(CA& ca, CB& cb, int kb0, int kb1, v4f (
 // (32768 x 7168 by 4096 rows: 1507 us with both one step ahead, 1404 so; with B's two
 // ahead too, its stage freed by a second barrier after its fragments are read, 1501.)
 // prime_ahead() has been called for step k0; k0 < k1.  Afterwards nothing reads or
-// writes the stages.
+// writes the stages.  idle: as above.
 struct Stages {
   uint8_t *far0, *far1, *far2, *near0, *near1;  // of the operand two steps ahead, of the other
   template <int I>
@@ -464,9 +488,40 @@ __device__ __forceinline__ void prime_ahead(CA& ca, CB& cb, int k0, int wave, co
 }
 template <int D, bool FAR_B = false, typename CA, typename CB>
 __device__ __forceinline__ void multiply_ahead(CA& ca, CB& cb, int k0, int k1, v4f (&acc)[D / 32][4], int wm, int wn, int wave, int lane,
-                                               const Stages& st) {
+                                               const Stages& st, bool idle) {
   constexpr int MT = D / 32;
   constexpr int NONE = 0x0070, FOUR = 0x0074;  // s_waitcnt: lgkmcnt(0) with vmcnt(0), vmcnt(4)
+  if (idle) {  // the copies and barriers of the loop below
+    __builtin_amdgcn_s_waitcnt(FOUR);
+    barrier();
+    uint8_t *f0 = st.far2, *f1 = st.far0, *f2 = st.far1, *n0 = st.near1, *n1 = st.near0;
+#pragma unroll 1
+    for (int kt = k0; kt < k1; ++kt) {
+      ca.set(kt + (FAR_B ? 1 : 2));
+      cb.set(kt + (FAR_B ? 2 : 1));
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (FAR_B) ca.issue(n0, wave, j);
+        else cb.issue(n0, wave, j);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (FAR_B) cb.issue(f0, wave, j);
+        else ca.issue(f0, wave, j);
+      }
+      uint8_t *f = f0, *n = n0;
+      f0 = f1;
+      f1 = f2;
+      f2 = f;
+      n0 = n1;
+      n1 = n;
+      __builtin_amdgcn_s_waitcnt(FOUR);
+      barrier();
+    }
+    __builtin_amdgcn_s_waitcnt(NONE);
+    barrier();
+    return;
+  }
   auto rows = [&](int tm, const v8i (&bf)[4], const v8i& a) {
 #pragma unroll
     for (int tn = 0; tn < 4; ++tn) acc[tm][tn] = mma<0>(bf[tn], a, acc[tm][tn]);
