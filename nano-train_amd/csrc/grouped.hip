@@ -8,7 +8,7 @@
 // a buffer) and finds its tile.
 //
 // Matrix-core bound where experts have a few hundred rows and more, on the tiles of
-// ntlb_bf16_tile.h (32768 rows of 32 experts, 4096 x 7168: y 1.66 ms, 1.16 PFLOP/s; dx 1.76;
+// ntlb_bf16_tile.h (32768 rows of 32 experts, 4096 x 7168: y 1.66 ms, 1.16 PFLOP/s; dx 1.75;
 // dW 1.89); bound by the weights' way from HBM below (256 rows of them: y 315 us, 6.0 TB/s).
 #include <hip/hip_runtime.h>
 
