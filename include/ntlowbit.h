@@ -1134,7 +1134,8 @@ int64_t ntlb_rms_norm_workspace_bytes(int x_dtype, int64_t T, int64_t H);
 /*
  * h [T, I] = silu(gate) * up of x [T, 2I], which holds both: gate in the first I
  * columns (block 0), or gate and up in turn in blocks of `block` columns (a
- * multiple of 128 that divides I).  fp32 inside, h rounded once to x's dtype.
+ * multiple of 128 that divides I).  fp32 inside, h rounded once to x's dtype; a
+ * gate below -174 gives 0.
  * Pitches in elements; x's may be 0 (one row repeated).  Rows need only the
  * element's alignment.  kept and kept_exp as for ntlb_rms_norm_forward, of gate
  * and up apart, both in h's columns: kept [T, 2, ceil(I/128) * 128], kept_exp

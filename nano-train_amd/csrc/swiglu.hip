@@ -8,7 +8,11 @@
 // [T][gate, up][NT].
 //
 // With t = exp(-|g|) sigmoid and its complement are 1 / (1 + t) and t / (1 + t), the
-// former at g's own side: neither overflows nor cancels.
+// former at g's own side: neither overflows nor cancels.  Of a gate below -87.3 t is
+// under the normal numbers of fp32 (and of the exponential's unit, which gives 0), while its
+// product with g, u and dh may be any number: t is the square of exp(-|g| / 2), and a
+// sigmoid below 1/2 is held as two factors, the second multiplied last.  So results are
+// right down to g = -174, where the root ends too; below it they are 0.
 //
 // HBM-bound.  16 lanes (fp32: 32) take a tile, a lane 16 bytes of gate and of up, so
 // that a tile's scale is a reduction within the wave and nothing is read twice.  32768 x
@@ -46,22 +50,24 @@ struct Args {
   int64_t lddx;
 };
 
+// sig(g) = near far, far being 1 or t's root; rest = 1 - sig(g).
 // For 16-bit results the exponential's argument is rounded once (|g| 2^-24 of the
 // result) and the reciprocal is the unit's own (2^-23); fp32 takes the exact ones.
+struct Sigmoid {
+  float near, far, rest;
+};
 template <int DT>
-__device__ __forceinline__ void sigmoids(float g, float& sig, float& rest) {
-  float t, a;
+__device__ __forceinline__ Sigmoid sigmoid(float g) {
+  float root, a;
   if constexpr (DT == DT_F32) {
-    t = expf(-__builtin_fabsf(g));
-    a = 1.0f / (1.0f + t);
+    root = expf(-0.5f * __builtin_fabsf(g));
+    a = 1.0f / (1.0f + root * root);
   } else {
-    t = __builtin_amdgcn_exp2f(-__builtin_fabsf(g) * 1.44269502e+00f);
-    a = __builtin_amdgcn_rcpf(1.0f + t);
+    root = __builtin_amdgcn_exp2f(-__builtin_fabsf(g) * 7.21347511e-01f);
+    a = __builtin_amdgcn_rcpf(1.0f + root * root);
   }
-  const float b = t * a;
-  sig = g >= 0.f ? a : b;
-  rest = g >= 0.f ? b : a;
-  if (g != g) sig = rest = g;
+  const float b = root * a;
+  return g >= 0.f ? Sigmoid{a, 1.0f, root * b} : Sigmoid{b, root, a};  // NaN: all three
 }
 
 // N values from column c of a row, those past the I of its part zero
@@ -123,9 +129,8 @@ __global__ void __launch_bounds__(THREADS) forward_kernel(Args g) {
     float f[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      float sig, rest;
-      sigmoids<DT>(a[i], sig, rest);
-      f[i] = a[i] * sig * u[i];
+      const Sigmoid s = sigmoid<DT>(a[i]);
+      f[i] = a[i] * s.near * u[i] * s.far;
     }
     store_part<DT, W>((uint8_t*)g.h + at.row * g.ldh + (int64_t)at.c * E, n, f);
   }
@@ -199,10 +204,9 @@ __global__ void __launch_bounds__(THREADS) backward_kernel(Args g) {
   float da[N], du[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    float sig, rest;
-    sigmoids<DT>(a[i], sig, rest);
-    da[i] = d[i] * u[i] * sig * (1.0f + a[i] * rest);
-    du[i] = d[i] * a[i] * sig;
+    const Sigmoid s = sigmoid<DT>(a[i]);
+    da[i] = d[i] * u[i] * (s.near * (1.0f + a[i] * s.rest)) * s.far;
+    du[i] = d[i] * (a[i] * s.near) * s.far;
   }
   uint8_t* o = (uint8_t*)g.dx + at.row * g.lddx + (int64_t)at.col * E;
   store_part<DT, W>(o, n, da);

@@ -27,7 +27,7 @@ def swiglu(x: torch.Tensor, *, block: int = 0, checkpoint: Optional[str] = None)
     block 0: gate is the first half of the columns; a multiple of 128 that divides
     I: gate and up alternate in blocks of that many columns (128: the row order of
     moe.stack_gate_up).  x bf16, fp16 or fp32 with rows of any pitch; fp32 inside,
-    rounded once.
+    rounded once.  A gate below -174 (of which sigmoid is 3e-76) gives 0.
 
     checkpoint None keeps x for the backward; "e4m3" keeps gate and up in 8 bits (a
     power of two for each 128 columns, values rounded by at most 2^-4 of

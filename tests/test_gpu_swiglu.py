@@ -230,3 +230,26 @@ def test_refusals(gpu_device):
             swiglu(x, block=block)
     with pytest.raises(ValueError, match="checkpoint"):
         swiglu(x, checkpoint="int8")
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("checkpoint", [None, "e4m3"])
+def test_far_gates_keep_what_the_type_holds(gpu_device, dtype, checkpoint):
+    """the sigmoid of a gate below -87.3 lies under the normal numbers of fp32 and of bf16, its product with the gate, up
+    and the incoming gradient need not: each comes out within the bounds, up to gates of -174"""
+    from lowbit.experts import swiglu
+
+    gates = torch.tensor([-60.0, -80.0, -87.0, -87.5, -88.0, -90.0, -92.0, -96.0, -103.0, -104.0, -120.0, -144.0, -160.0,
+                          60.0, 88.0, 104.0, 160.0] + [-168.0, -174.0] * (checkpoint is None))
+    ups = torch.tensor([1.0, -3.0, 1e10, -1e20, 1e30, 2.5e38])
+    incoming = torch.tensor([1.0, -1e5, 1e25])
+    rows = torch.cartesian_prod(gates, ups, incoming)
+    # neither dh up nor h past the largest number
+    rows = rows[(rows[:, 1:].prod(1).abs() < 3e38) & ((rows[:, 0] < 0) | (rows[:, 1:].prod(1).abs() < 1e36))]
+    # one value a row: a kept tile is its own
+    x = rows[:, :2].to(dtype).to(gpu_device)
+    dh = rows[:, 2:].to(dtype).to(gpu_device)
+    leaf = x.clone().requires_grad_(True)
+    h = swiglu(leaf, checkpoint=checkpoint)
+    (dx,) = torch.autograd.grad(h, leaf, dh)
+    _check_all(h.detach(), dx, x, dh, 0, checkpoint)
