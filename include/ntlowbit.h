@@ -1155,7 +1155,8 @@ int ntlb_swiglu_rows_backward(const void* x, int dtype, int64_t T, int64_t I, in
 /*
  * bf16 products grouped by expert: row r of x [R, K] belongs to the expert e with
  * offsets[e] <= r < offsets[e+1] (int32 [E+1] on the device, offsets[0] taken as
- * 0, not decreasing; values past R count as R), whose weight is w + e * w_stride
+ * 0, not decreasing; values past R count as R, one below 0 or below one before it as
+ * that), whose weight is w + e * w_stride
  * [N, K]:
  *   y[r] = x[r] W_e^T;   dx[r] = dy[r] W_e;   dw[e] = sum over e's rows of dy[r]^T x[r]
  * summed in fp32 in an order that R, E, N and K alone decide, rounded once; y and dx

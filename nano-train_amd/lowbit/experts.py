@@ -53,7 +53,8 @@ def grouped_matmul(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor,
 
     x bf16 [R, K], its rows sorted by expert; weight bf16 [E, N, K]; offsets int32
     [E + 1], not decreasing, on x's device: expert e has the rows offsets[e] ..
-    offsets[e + 1] - 1, any number of them, offsets[0] being 0.  Rows at or past offsets[E]
+    offsets[e + 1] - 1, any number of them, offsets[0] being 0.  (One below 0 or below one
+    before it counts as that, one past R as R.)  Rows at or past offsets[E]
     (a capacity's spare rows) are not read; y and the gradient of x are zero there.  The
     gradient of an expert without rows is zero.  Sums are fp32, in an order that R, E,
     N and K alone decide, results rounded once.  x and weight of any strides: what is

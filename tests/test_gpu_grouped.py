@@ -339,3 +339,26 @@ def test_refusals(gpu_device):
     many = w[:1, :1, :1].expand(4097, 1, 64)
     with pytest.raises(RuntimeError, match="too large"):
         grouped_matmul(x, many, torch.zeros(4098, dtype=torch.int32, device=gpu_device))
+
+
+@pytest.mark.parametrize("table,R,K,N", [
+    ([0, 4096, 0, 4096], 4096, 64, 136),  # more row tiles, were the experts apart, than rows have
+    ([0, 300, 100, 700, 650, 900], 1000, 72, 40), ([0, -5, 600, -9, 2 ** 31 - 1, 0], 700, 64, 264),
+    ([0, 3, 1, 5, 4, 4, 12, 2, 9], 14, 200, 130),  # few rows
+    ([0, 160, 0], 170, 4096, 128),  # the contraction in ranges
+    ([0] + [(37 * e) % 1001 for e in range(200)], 1100, 64, 136),  # experts past the first 64
+    ([0] + [(5 * e) % 131 for e in range(200)], 140, 64, 24),
+])
+def test_offsets_that_decrease(gpu_device, table, R, K, N):
+    """an offset below one before it counts as that one: every row has one expert or none, and its result"""
+    from lowbit.experts import grouped_matmul
+
+    E = len(table) - 1
+    x, w, dy, _ = _inputs([R] + [0] * (E - 1), K, N, R + E, gpu_device)
+    offsets = torch.tensor(table, dtype=torch.int32, device=gpu_device)
+    lx, lw = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    unwritten = [torch.full((R, n), float("nan"), dtype=torch.bfloat16, device=gpu_device) for n in (N, K)]
+    del unwritten  # the memory that the results take next
+    y = grouped_matmul(lx, lw, offsets)
+    dx, dw = torch.autograd.grad(y, (lx, lw), dy)
+    _check_all(y.detach(), dx, dw, x, w, dy, offsets.cummax(0).values.clamp(0, R))
