@@ -1165,7 +1165,8 @@ int ntlb_swiglu_rows_backward(const void* x, int dtype, int64_t T, int64_t I, in
  * lie in 16-byte aligned rows of whole 16-byte pieces (pitch % 8 == 0, at most
  * 2^22; w_stride % 8 == 0); where a product sums along their rows (x and w for y,
  * dy for dx) their columns up to the next multiple of 8 are zero.  Outputs need only
- * the element's alignment.  E <= 4096, R <= 2^30, N and K <= 2^22.  workspace: of y and dx
+ * the element's alignment.  E <= 4096, R <= 2^30, N and K <= 2^22, and of y and dx at
+ * most 2^23 in (R / 128 + min(R, E + 1)) ceil(columns / 128).  workspace: of y and dx
  * ntlb_grouped_matmul_workspace_bytes(R, E, N, K, 0 and 1) bytes, 16-byte aligned,
  * contents free.
  */

@@ -522,7 +522,8 @@ __global__ void __launch_bounds__(256) values_kernel(Keep g, uint8_t* out, int64
       make_uint4(pack_bf16(a[0], a[1]), pack_bf16(a[2], a[3]), pack_bf16(b[0], b[1]), pack_bf16(b[2], b[3]));
 }
 
-constexpr int64_t MAX_PITCH = 1 << 22, MAX_EXPERTS = 4096, MAX_GRID = ((int64_t)1 << 31) - 1;
+constexpr int64_t MAX_PITCH = 1 << 22, MAX_EXPERTS = 4096;
+constexpr int64_t MAX_THREADS = ((int64_t)1 << 32) - 1;  // of a launch
 
 static int check(const char* fn, int64_t R, int64_t E, int64_t N, int64_t K, const int32_t* offsets) {
   clear_error();
@@ -539,13 +540,16 @@ static int bad(const char* fn, const char* what) {
   return fail(NTLB_EINVAL, "%s: %s must lie in 16-byte aligned rows of whole 16-byte pieces, at most %lld values apart", fn, what, (long long)MAX_PITCH);
 }
 
+// workgroups that stream: 16 rows of each expert's weights, and of the columns of the rows behind
+static int64_t few_blocks(int64_t E, int64_t N) { return (E + 1) * cdiv(N, 16); }
+
 // How y and dx are formed for N columns over K: by streaming the weights past few rows
 // (FEW, y only), or by tiles of D, their contraction in `parts` ranges.
 //
 // How many rows an expert has is known to the device only; the host goes by R rows over
 // the experts that can have some.
 //
-// Few rows stream: past the weights goes x once for 16 of their rows, tiles of some
+// Few rows stream, where their grid fits a launch: past the weights goes x once for 16 of their rows, tiles of some
 // rows take a tile's time.  Up to 2 to 32 rows an expert, by the weights' size: 768 x 1024
 // of 8 experts 11 us at 32 rows and 12 by tiles, at 64 rows 18 and 14; 2048 x 4096 of 8
 // 26 us at 4 and 27, at 16 37 and 28; 4096 x 7168 of 32 331 us at 2 and 339, at 4 361 and 316.
@@ -566,7 +570,8 @@ struct Plan {
 };
 static Plan plan_of(int64_t R, int64_t E, int64_t N, int64_t K, bool y) {
   const int64_t live = std::min(R, E), cus = split_device_cus(), nk = cdiv(K, KSTEP);
-  Plan p{y && R <= live * std::clamp<int64_t>(400000000 / (live * N * K), 2, 32), 128, 1};
+  const bool fits = few_blocks(E, N) * 64 * FEW_WAVES <= MAX_THREADS;
+  Plan p{y && fits && R <= live * std::clamp<int64_t>(400000000 / (live * N * K), 2, 32), 128, 1};
   if (p.few) return p;
   auto tiles = [&](int64_t D) {  // a last one of every expert's is half empty
     return (live == 1 ? cdiv(R, D) : std::max(live, R / D + cdiv(live, 2))) * cdiv(N, D);
@@ -588,15 +593,15 @@ static Plan plan_of(int64_t R, int64_t E, int64_t N, int64_t K, bool y) {
   return p;
 }
 static int64_t sums_bytes(const Plan& p, int64_t R, int64_t N) { return p.parts > 1 ? p.parts * R * cdiv(N, 4) * 16 : 0; }
-// workgroups of the tiles: every expert's last one too, and the rows' behind
-static int64_t row_tiles(const Args& g, const Plan& p) { return (g.R / p.D + g.E + 1) * cdiv(g.N, p.D) * p.parts; }
+// workgroups of the tiles: the last one of each expert that can have rows, and of the rows behind, too
+static int64_t row_tiles(const Args& g, const Plan& p) { return (g.R / p.D + std::min<int64_t>(g.R, g.E + 1)) * cdiv(g.N, p.D) * p.parts; }
 
 // y's or dx' tiles, and their ranges' sum
 template <bool Y>
 static int launch(const char* fn, Args g, const Plan& p, void* ws, int64_t ws_bytes, hipStream_t st) {
   const int64_t need = sums_bytes(p, g.R, g.N), n = row_tiles(g, p);
   if (ws_bytes < need || (need && (!ws || !aligned(ws, 16)))) return fail(NTLB_EINVAL, "%s: workspace of %lld bytes, %lld needed", fn, (long long)ws_bytes, (long long)need);
-  if (n > MAX_GRID) return fail(NTLB_EUNSUPPORTED, "%s: %lld tiles", fn, (long long)n);
+  if (n * 2 * p.D > MAX_THREADS) return fail(NTLB_EUNSUPPORTED, "%s: %lld tiles are too many", fn, (long long)n);
   g.parts = p.parts;
   g.sums = (float*)ws;
   g.lds = cdiv(g.N, 4) * 4;
@@ -640,9 +645,7 @@ extern "C" int ntlb_grouped_matmul(const uint16_t* x, int64_t ldx, const uint16_
   hipStream_t st = as_stream(stream);
   const grouped::Plan p = grouped::plan_of(R, E, N, K, true);
   if (!p.few) return grouped::launch<true>(fn, g, p, workspace, ws_bytes, st);
-  const int64_t blocks = cdiv(N, 16), n = (E + 1) * blocks;
-  if (n > grouped::MAX_GRID) return fail(NTLB_EUNSUPPORTED, "%s: %lld workgroups", fn, (long long)n);
-  grouped::few_kernel<1><<<(unsigned)n, 64 * grouped::FEW_WAVES, 0, st>>>(g, (int)blocks);
+  grouped::few_kernel<1><<<(unsigned)grouped::few_blocks(E, N), 64 * grouped::FEW_WAVES, 0, st>>>(g, (int)cdiv(N, 16));
   return check_launch(fn);
 }
 
@@ -674,7 +677,7 @@ extern "C" int ntlb_grouped_matmul_dw(const uint16_t* dy, int64_t lddy, const ui
   g.offsets = offsets; g.R = R; g.E = (int)E; g.M = N; g.N = K; g.out = dw; g.ldo = K;
   const int D = N > 128 && K > 128 && E * cdiv(N, 256) * cdiv(K, 256) >= split_device_cus() ? 256 : 128;
   const int64_t n = grouped::ordered_grid(E * cdiv(N, D) * cdiv(K, D));
-  if (n > grouped::MAX_GRID) return fail(NTLB_EUNSUPPORTED, "%s: %lld tiles", fn, (long long)n);
+  if (n > ((int64_t)1 << 30)) return fail(NTLB_EUNSUPPORTED, "%s: %lld tiles are too many", fn, (long long)n);  // counted in 32 bits
   hipStream_t st = as_stream(stream);
   const unsigned wgs = (unsigned)std::min<int64_t>(n, cdiv(split_device_cus(), 8) * 8 * (D == 256 ? 1 : 2));
   if (D == 256) grouped::weight_kernel<256><<<wgs, 512, 0, st>>>(g, (int)n);

@@ -362,3 +362,18 @@ def test_offsets_that_decrease(gpu_device, table, R, K, N):
     y = grouped_matmul(lx, lw, offsets)
     dx, dw = torch.autograd.grad(y, (lx, lw), dy)
     _check_all(y.detach(), dx, dw, x, w, dy, offsets.cummax(0).values.clamp(0, R))
+
+
+def test_a_row_of_many_experts_and_columns(gpu_device):
+    """few rows whose weights, by 16 columns of every expert a workgroup, would take more threads than a launch has"""
+    from lowbit.experts import grouped_matmul
+
+    E, N, K, R = 4096, 65536, 8, 10
+    x, w, _, _ = _inputs([R], K, N, 5, gpu_device)
+    counts = torch.zeros(E, dtype=torch.int32, device=gpu_device)
+    counts[torch.randperm(E, generator=torch.Generator().manual_seed(1))[:R - 2].to(gpu_device)] = 1
+    counts[E - 1] += 2
+    offsets = torch.cat([counts.new_zeros(1), counts.cumsum(0).int()])
+    with torch.no_grad():
+        y = grouped_matmul(x, w.expand(E, N, K), offsets)
+    _check(y, x.double() @ w[0].double().t(), K, x.double().abs() @ w[0].double().t().abs(), "y")

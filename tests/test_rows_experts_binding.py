@@ -149,6 +149,20 @@ def test_grouped_products_validate_without_gpu():
     assert L.ntlb_grouped_matmul_workspace_bytes(0, 1, 64, 64, 0) == L.ntlb_grouped_matmul_workspace_bytes(4, 0, 64, 64, 1) == 0
 
 
+def test_grouped_products_of_too_many_tiles_are_refused():
+    """a launch counts its threads in 32 bits: more tiles than that are refused before one"""
+    from lowbit import _lib
+
+    L = _lib.lib()
+    U = _lib.NTLB_EUNSUPPORTED
+    for R, E in ((5000, 4096), (1 << 30, 1)):
+        wide = 1 << 22
+        assert L.ntlb_grouped_matmul(P, 8, P, 8, 0, P, R, E, wide, 8, P, wide, None, 0, None) == U
+        assert b"tiles" in L.ntlb_last_error()
+        assert L.ntlb_grouped_matmul_dx(P, 8, P, wide, 0, P, R, E, 8, wide, P, wide, None, 0, None) == U
+        assert b"tiles" in L.ntlb_last_error()
+
+
 def test_kept_rows_validate_without_gpu():
     from lowbit import _lib
 
