@@ -33,9 +33,9 @@ struct TileRows {
   }
   __device__ __forceinline__ uint32_t row(uint32_t tile) const { return per_row == 1 ? tile : __umulhi(tile, mul) >> shift; }
 };
-// Launches over tiles take at most this many (their threads' workgroups are counted
-// in 32 bits too): f(first row, rows) for each piece of T rows.
-constexpr int64_t MAX_TILES = (int64_t)1 << 27;
+// Launches over tiles take at most this many: a tile has up to 32 threads, and a launch's
+// are counted in 32 bits, 2^32 of them no longer.  f(first row, rows) for each piece of T rows.
+constexpr int64_t MAX_TILES = (int64_t)1 << 26;
 template <typename F>
 inline int row_pieces(int64_t T, int64_t per_row, F f) {
   const int64_t step = std::max<int64_t>(1, MAX_TILES / per_row);

@@ -253,3 +253,19 @@ def test_far_gates_keep_what_the_type_holds(gpu_device, dtype, checkpoint):
     h = swiglu(leaf, checkpoint=checkpoint)
     (dx,) = torch.autograd.grad(h, leaf, dh)
     _check_all(h.detach(), dx, x, dh, 0, checkpoint)
+
+
+@pytest.mark.parametrize("checkpoint", [None, "e4m3"])
+def test_more_rows_than_a_launch_has_tiles(gpu_device, checkpoint):
+    """fp32 rows of one tile each, whose threads in one launch would be 2^32"""
+    from lowbit.experts import swiglu
+
+    T = (1 << 27) + 3
+    x = torch.randn(T, 2, generator=torch.Generator(gpu_device).manual_seed(1), device=gpu_device).requires_grad_(True)
+    h = swiglu(x, checkpoint=checkpoint)
+    (dx,) = torch.autograd.grad(h, x, torch.ones_like(h))
+    for part in (slice(0, 5000), slice((1 << 26) - 5000, (1 << 26) + 5000), slice(T - 5000, T)):
+        _check_all(h.detach()[part], dx[part], x.detach()[part], torch.ones_like(h[part]).detach(), 0, checkpoint)
+    with torch.no_grad():  # no row left out: fp32's own formula, both sides off by less than 32 u
+        want = x[:, :1] / (1 + torch.exp(-x[:, :1])) * x[:, 1:]
+        assert ((h - want).abs() <= 64 * U * want.abs() + 2.0 ** -126).all()
