@@ -377,3 +377,57 @@ def test_a_row_of_many_experts_and_columns(gpu_device):
     with torch.no_grad():
         y = grouped_matmul(x, w.expand(E, N, K), offsets)
     _check(y, x.double() @ w[0].double().t(), K, x.double().abs() @ w[0].double().t().abs(), "y")
+
+
+def _long(n, rows, cols, seed, dev):
+    """a [rows, n] and b [cols, n] of -1, 0 and 1 in bf16 with a b^T exact in fp32 and in bf16, whatever the order: of each
+    64 columns one is not zero in a.  Those columns' products cancel in pairs that lie anywhere, but for 66 of them: the
+    sums stay below 128, and without any one of the columns each sum is another."""
+    g = torch.Generator().manual_seed(seed)
+    steps = n // 64
+    at = torch.arange(steps) * 64 + torch.randint(0, 64, (steps,), generator=g)
+    sa, sb = (torch.randint(0, 2, (m, steps), generator=g) * 2 - 1 for m in (rows, cols))
+    order = torch.randperm(steps, generator=g)
+    half = (steps - 66) // 2
+    sa[:, order[half:2 * half]] = -sa[:, order[:half]]
+    sb[:, order[half:2 * half]] = sb[:, order[:half]]
+    a = torch.zeros(rows, n)
+    a[:, at] = sa.float()
+    b = torch.randint(0, 2, (cols, n), generator=g) * 2.0 - 1
+    b[:, at] = sb.float()
+    want = (sa.double() @ sb.double().t()).float()
+    assert want.any() and want.abs().max() < 128
+    for lost in (slice(0, 1), slice(steps - 1, steps), slice(0, steps // 16), slice(steps // 2, steps), slice(0, steps)):
+        short = want - (sa[:, lost].double() @ sb[:, lost].double().t()).float()
+        assert not torch.equal(short, want), lost  # a sum that leaves columns out is told
+    return a.bfloat16().to(dev), b.bfloat16().to(dev), want.to(dev)
+
+
+@pytest.mark.parametrize("n,rows", [(1 << 22, 2), (1 << 18, 40), (1 << 16, 300)])
+def test_long_contractions_are_whole(gpu_device, n, rows):
+    """sums over the largest K, N and number of rows, exact: by streaming, by ranges, by one tile"""
+    from lowbit.experts import grouped_matmul
+
+    offsets = torch.tensor([0, rows, rows], dtype=torch.int32, device=gpu_device)
+    x, w, want = _long(n, rows, 5, 1, gpu_device)
+    with torch.no_grad():
+        y = grouped_matmul(x, w.expand(2, 5, n), offsets)
+    assert torch.equal(y.float(), want)
+    dy, w, want = _long(n, rows, 16, 2, gpu_device)  # dx = dy W
+    lx = torch.zeros(rows, 16, dtype=torch.bfloat16, device=gpu_device, requires_grad=True)
+    (dx,) = torch.autograd.grad(grouped_matmul(lx, w.t().contiguous().expand(2, n, 16), offsets), lx, dy)
+    assert torch.equal(dx.float(), want)
+
+
+@pytest.mark.parametrize("checkpoint", [None, "e4m3"])
+def test_an_expert_of_many_rows_is_whole(gpu_device, checkpoint):
+    """dW over 2^20 rows, exact"""
+    from lowbit.experts import grouped_matmul
+
+    n = 1 << 20
+    dy, x, want = _long(n, 24, 40, 3, gpu_device)
+    x, dy = (torch.cat([t.t(), torch.ones_like(t[:, :5]).t()]) for t in (x, dy))  # and an expert of five rows
+    offsets = torch.tensor([0, n, n + 5], dtype=torch.int32, device=gpu_device)
+    lw = torch.zeros(2, 24, 40, dtype=torch.bfloat16, device=gpu_device, requires_grad=True)
+    (dw,) = torch.autograd.grad(grouped_matmul(x, lw, offsets, checkpoint=checkpoint), lw, dy)
+    assert torch.equal(dw[0].float(), want) and (dw[1] == 5).all()
