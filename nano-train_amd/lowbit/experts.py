@@ -135,13 +135,16 @@ def local_moe_bf16(tokens: torch.Tensor, expert_ids: torch.Tensor, topk_w: torch
     """The single-rank routed expert loop with its products in bf16 (moe.py:1062-1093,
     LocalRoutedMoE.forward :476-491, ExpertMLP.forward :190-193): moe.local_moe()'s
     arguments, shapes and capacity, without codes in its products, and the gradients of
-    tokens, routing weights and expert weights under autograd.  grouped_matmul(),
-    swiglu(block=128), grouped_matmul() and the weighted sum of each token's rows.
+    tokens, routing weights and expert weights under autograd, all of them on one
+    device, which need not be the current one.  grouped_matmul(), swiglu(block=128), grouped_matmul() and the weighted sum of each token's rows.
 
     checkpoint "e4m3" keeps the rows of both products and the projections between
     them in 8 bits for the backward, 1/2 of what the bf16 loop keeps beside the
     down projection's output."""
     ops._require_device(tokens, expert_ids, topk_w, w_gate_up, w_down)
+    if any(t.device != tokens.device for t in (expert_ids, topk_w, w_gate_up, w_down)):
+        raise ValueError(f"tokens are on {tokens.device}, expert_ids, topk_w, w_gate_up and w_down on {expert_ids.device}, "
+                         f"{topk_w.device}, {w_gate_up.device} and {w_down.device}")
     if tokens.dim() != 2 or expert_ids.dim() != 2 or topk_w.shape != expert_ids.shape or expert_ids.shape[0] != tokens.shape[0]:
         raise ValueError("tokens must be [T, H], expert_ids and topk_w [T, k]")
     if tokens.dtype != torch.bfloat16 or w_gate_up.dtype != torch.bfloat16 or w_down.dtype != torch.bfloat16:
@@ -153,8 +156,10 @@ def local_moe_bf16(tokens: torch.Tensor, expert_ids: torch.Tensor, topk_w: torch
     if expert_ids.shape[1] > 8:
         raise ValueError("local_moe_bf16 supports top_k <= 8")
     ops.checkpoint_code(checkpoint)
-    routing = moe.route_by_expert(expert_ids, w_gate_up.shape[0], capacity=int(capacity), topk_w=topk_w)
-    rows = _Dispatch.apply(tokens, routing, expert_ids)
-    gate_up = grouped_matmul(rows, w_gate_up, routing.offsets, checkpoint=checkpoint)
-    h = swiglu(gate_up, block=128, checkpoint=checkpoint)
-    return _Combine.apply(grouped_matmul(h, w_down, routing.offsets, checkpoint=checkpoint), topk_w, routing, expert_ids)
+    with torch.cuda.device(tokens.device):  # the gather and the sum launch on the current device's stream
+        routing = moe.route_by_expert(expert_ids, w_gate_up.shape[0], capacity=int(capacity), topk_w=topk_w)
+        rows = _Dispatch.apply(tokens, routing, expert_ids)
+        gate_up = grouped_matmul(rows, w_gate_up, routing.offsets, checkpoint=checkpoint)
+        h = swiglu(gate_up, block=128, checkpoint=checkpoint)
+        return _Combine.apply(grouped_matmul(h, w_down, routing.offsets, checkpoint=checkpoint), topk_w, routing,
+                              expert_ids)

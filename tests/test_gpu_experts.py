@@ -227,3 +227,23 @@ def test_example_runs(gpu_device, options):
     for n, p in model.named_parameters():
         assert p.grad is not None and p.grad.isfinite().all() and p.grad.any(), n
     assert model.score(torch.tensor([[7]], device=gpu_device), step_of[7].reshape(1, 1).cuda()).isfinite().all()
+
+
+@pytest.mark.parametrize("capacity", [0, 20])
+def test_generation_replays_in_a_graph(gpu_device, capacity):
+    """the loop without gradients, captured: every replay is the eager result of the tokens, ids and weights then there"""
+    from lowbit.experts import local_moe_bf16
+
+    x, ids, w, gu, down, _ = _inputs(60, 6, 2, 256, 128, gpu_device)
+    with torch.no_grad():
+        local_moe_bf16(x, ids, w, gu, down, capacity=capacity)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = local_moe_bf16(x, ids, w, gu, down, capacity=capacity)
+        for seed in range(1, 5):
+            for t, new in zip((x, ids, w), _inputs(60, 6, 2, 256, 128, gpu_device, seed)):
+                t.copy_(new)
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(y, local_moe_bf16(x, ids, w, gu, down, capacity=capacity)), seed

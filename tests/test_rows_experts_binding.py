@@ -33,6 +33,41 @@ def test_operators_refuse_cpu_tensors():
             call()
 
 
+def test_expert_loop_runs_on_its_tensors_device(monkeypatch):
+    """operands of two devices are refused, and every launch is made with theirs as the current one"""
+    from lowbit import experts
+
+    class Reached(Exception):
+        pass
+
+    current = []
+
+    class Device:
+        def __init__(self, device):
+            self.device = device
+
+        def __enter__(self):
+            current.append(self.device)
+
+        def __exit__(self, *exc):
+            current.pop()
+
+    def route(*a, **kw):
+        raise Reached(list(current))
+
+    monkeypatch.setattr(experts.ops, "_require_device", lambda *t: None)
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(experts.moe, "route_by_expert", route)
+    ok = [torch.zeros(2, 8).bfloat16(), torch.zeros(2, 1, dtype=torch.int32), torch.ones(2, 1),
+          torch.zeros(1, 256, 8).bfloat16(), torch.zeros(1, 8, 128).bfloat16()]
+    for i in range(5):
+        with pytest.raises(ValueError, match="are on"):
+            experts.local_moe_bf16(*(t.to("meta") if j == i else t for j, t in enumerate(ok)))
+    with pytest.raises(Reached) as seen:
+        experts.local_moe_bf16(*ok)
+    assert seen.value.args[0] == [ok[0].device] and not current
+
+
 def test_checkpoint_names():
     from lowbit import ops
     from lowbit.norm import RMSNorm
