@@ -324,7 +324,7 @@ __global__ void __launch_bounds__(2 * D, D == 256 ? 1 : 2) weight_kernel(Args g,
 
 // ---------------------------------------------------------------------------
 // y where experts have few rows: bound by the weights, read once.  A workgroup takes
-// 16 NT rows of W_e and all of e's rows (64 at a time); its four waves take
+// 16 rows of W_e and all of e's rows (64 at a time); its four waves take
 // 64-column chunks in turn, straight from memory into fragments (a lane 32 bytes of
 // a row, 16 rows a fragment, the same columns of x and W), and their sums meet in LDS.
 // 8 rows of as many experts, 4096 x 7168: 80 us, 5.9 TB/s; with W's loads hinted as read once
@@ -332,21 +332,17 @@ __global__ void __launch_bounds__(2 * D, D == 256 ? 1 : 2) weight_kernel(Args g,
 // ---------------------------------------------------------------------------
 constexpr int FEW_WAVES = 4;
 
-template <int NT, int MT>
+template <int MT>
 __device__ __forceinline__ void few_rows(const Args& g, const uint8_t* wp, const uint8_t* xp, int lo, int m0, int n, int64_t n0,
                                          int wave, int lane, float4* sums) {
   const int r = lane & 15, gl = lane >> 4, chunks = (int)((g.k + 63) / 64);
-  const uint8_t* wr[NT];
+  const uint8_t* wr = wp + min<int64_t>(n0 + r, g.N - 1) * g.ldb + gl * 32;
   const uint8_t* xr[MT];
 #pragma unroll
-  for (int i = 0; i < NT; ++i) wr[i] = wp + min<int64_t>(n0 + 16 * i + r, g.N - 1) * g.ldb + gl * 32;
-#pragma unroll
   for (int i = 0; i < MT; ++i) xr[i] = xp + (int64_t)(lo + min(m0 + 16 * i + r, n - 1)) * g.lda + gl * 32;
-  v4f acc[MT][NT];
+  v4f acc[MT];
 #pragma unroll
-  for (int i = 0; i < MT; ++i)
-#pragma unroll
-    for (int j = 0; j < NT; ++j) acc[i][j] = (v4f){0.f, 0.f, 0.f, 0.f};
+  for (int i = 0; i < MT; ++i) acc[i] = (v4f){0.f, 0.f, 0.f, 0.f};
   const int whole = (int)(g.k / 64);
   auto load = [&](const uint8_t* p, int c) {
     v8i v;
@@ -355,24 +351,21 @@ __device__ __forceinline__ void few_rows(const Args& g, const uint8_t* wp, const
     v[4] = (int)b.x; v[5] = (int)b.y; v[6] = (int)b.z; v[7] = (int)b.w;
     return v;
   };
-  auto add = [&](const v8i (&w)[NT], const v8i (&x)[MT]) {
+  auto add = [&](const v8i& w, const v8i (&x)[MT]) {
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
-#pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        acc[i][j] = mma<0>(w[j], x[i], acc[i][j]);
-        acc[i][j] = mma<1>(w[j], x[i], acc[i][j]);
-      }
+    for (int i = 0; i < MT; ++i) {
+      acc[i] = mma<0>(w, x[i], acc[i]);
+      acc[i] = mma<1>(w, x[i], acc[i]);
+    }
   };
   // a wave's chunks, U of them in flight
   constexpr int U = MT == 4 ? 2 : 4;
   int c = wave;
   for (; c + (U - 1) * FEW_WAVES < whole; c += U * FEW_WAVES) {
-    v8i w[U][NT], x[U][MT];
+    v8i w[U], x[U][MT];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-#pragma unroll
-      for (int j = 0; j < NT; ++j) w[u][j] = load(wr[j], c + u * FEW_WAVES);
+      w[u] = load(wr, c + u * FEW_WAVES);
 #pragma unroll
       for (int i = 0; i < MT; ++i) x[u][i] = load(xr[i], c + u * FEW_WAVES);
     }
@@ -380,9 +373,8 @@ __device__ __forceinline__ void few_rows(const Args& g, const uint8_t* wp, const
     for (int u = 0; u < U; ++u) add(w[u], x[u]);
   }
   for (; c < whole; c += FEW_WAVES) {
-    v8i w[NT], x[MT];
-#pragma unroll
-    for (int j = 0; j < NT; ++j) w[j] = load(wr[j], c);
+    const v8i w = load(wr, c);
+    v8i x[MT];
 #pragma unroll
     for (int i = 0; i < MT; ++i) x[i] = load(xr[i], c);
     add(w, x);
@@ -403,34 +395,29 @@ __device__ __forceinline__ void few_rows(const Args& g, const uint8_t* wp, const
       }
       return v;
     };
-    v8i w[NT], x[MT];
-#pragma unroll
-    for (int j = 0; j < NT; ++j) w[j] = part(wr[j]);
+    const v8i w = part(wr);
+    v8i x[MT];
 #pragma unroll
     for (int i = 0; i < MT; ++i) x[i] = part(xr[i]);
     add(w, x);
   }
   __syncthreads();  // the sums of the rows before have been read
 #pragma unroll
-  for (int i = 0; i < MT; ++i)
-#pragma unroll
-    for (int j = 0; j < NT; ++j)
-      sums[((i * NT + j) * FEW_WAVES + wave) * 64 + lane] = make_float4(acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]);
+  for (int i = 0; i < MT; ++i) sums[(i * FEW_WAVES + wave) * 64 + lane] = make_float4(acc[i][0], acc[i][1], acc[i][2], acc[i][3]);
   __syncthreads();
-  // lane: row m0 + 16 i + lane % 16, columns n0 + 16 j + 4 (lane / 16) ..
-  for (int q = wave; q < MT * NT; q += FEW_WAVES) {
-    const int i = q / NT, j = q - i * NT;
-    float4 s = sums[q * FEW_WAVES * 64 + lane];
+  // lane: row m0 + 16 i + lane % 16, columns n0 + 4 (lane / 16) ..
+  for (int i = wave; i < MT; i += FEW_WAVES) {
+    float4 s = sums[i * FEW_WAVES * 64 + lane];
 #pragma unroll
     for (int w = 1; w < FEW_WAVES; ++w) {
-      const float4 o = sums[(q * FEW_WAVES + w) * 64 + lane];
+      const float4 o = sums[(i * FEW_WAVES + w) * 64 + lane];
       s.x += o.x;
       s.y += o.y;
       s.z += o.z;
       s.w += o.w;
     }
     const int m = m0 + 16 * i + r;
-    const int64_t c = n0 + 16 * j + 4 * gl;
+    const int64_t c = n0 + 4 * gl;
     if (m >= n || c >= g.N) continue;
     uint16_t* o = g.out + (int64_t)(lo + m) * g.ldo + c;
     const uint32_t a = pack_bf16(s.x, s.y), b = pack_bf16(s.z, s.w);
@@ -444,29 +431,28 @@ __device__ __forceinline__ void few_rows(const Args& g, const uint8_t* wp, const
   }
 }
 
-template <int NT>
 __global__ void __launch_bounds__(64 * FEW_WAVES) few_kernel(Args g, int blocks) {
-  __shared__ float4 sums[4 * NT * FEW_WAVES * 64];
+  __shared__ float4 sums[4 * FEW_WAVES * 64];
   const int e = (int)blockIdx.x / blocks, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t n0 = (int64_t)((int)blockIdx.x - e * blocks) * (16 * NT);
+  const int64_t n0 = (int64_t)((int)blockIdx.x - e * blocks) * 16;
   const int to = e < g.E ? min(g.offsets[e + 1], (int)g.R) : (int)g.R;
   if (to <= (e ? g.offsets[e] : 0)) return;  // no rows, whatever came before (8 rows of 32 experts: 83 us without, 80 with)
   int lo = 0;
   for (int c = 0; c < e; c += 64) Rows(g, c, min(lane, e - 1 - c), lo);
   const int n = to - lo;
   if (e == g.E) {  // rows behind the last expert's
-    for (int i = threadIdx.x; i < n * 16 * NT; i += 64 * FEW_WAVES) {
-      const int64_t c = n0 + i % (16 * NT);
-      if (c < g.N) g.out[(int64_t)(lo + i / (16 * NT)) * g.ldo + c] = 0;
+    for (int i = threadIdx.x; i < n * 16; i += 64 * FEW_WAVES) {
+      const int64_t c = n0 + i % 16;
+      if (c < g.N) g.out[(int64_t)(lo + i / 16) * g.ldo + c] = 0;
     }
     return;
   }
   const uint8_t* wp = uniform64(g.b + (int64_t)e * g.b_expert);
   for (int m0 = 0; m0 < n; m0 += 64) {
     const int left = n - m0;
-    if (left <= 16) few_rows<NT, 1>(g, wp, g.a, lo, m0, n, n0, wave, lane, sums);
-    else if (left <= 32) few_rows<NT, 2>(g, wp, g.a, lo, m0, n, n0, wave, lane, sums);
-    else few_rows<NT, 4>(g, wp, g.a, lo, m0, n, n0, wave, lane, sums);
+    if (left <= 16) few_rows<1>(g, wp, g.a, lo, m0, n, n0, wave, lane, sums);
+    else if (left <= 32) few_rows<2>(g, wp, g.a, lo, m0, n, n0, wave, lane, sums);
+    else few_rows<4>(g, wp, g.a, lo, m0, n, n0, wave, lane, sums);
   }
 }
 
@@ -645,7 +631,7 @@ extern "C" int ntlb_grouped_matmul(const uint16_t* x, int64_t ldx, const uint16_
   hipStream_t st = as_stream(stream);
   const grouped::Plan p = grouped::plan_of(R, E, N, K, true);
   if (!p.few) return grouped::launch<true>(fn, g, p, workspace, ws_bytes, st);
-  grouped::few_kernel<1><<<(unsigned)grouped::few_blocks(E, N), 64 * grouped::FEW_WAVES, 0, st>>>(g, (int)cdiv(N, 16));
+  grouped::few_kernel<<<(unsigned)grouped::few_blocks(E, N), 64 * grouped::FEW_WAVES, 0, st>>>(g, (int)cdiv(N, 16));
   return check_launch(fn);
 }
 
