@@ -1107,9 +1107,11 @@ int ntlb_rms_norm_forward(const void* x, int x_dtype, int64_t T, int64_t H, int6
 /*
  * The same norm with y in 8 bits: codes (grid, round to nearest) and scales as
  * ntlb_quant_tile_1x128 (qmax 127, NTLB_SCALE_AFTER_DIVIDE) has them, of y's own
- * value: a code is s w qmax / max|s w| over its 128 columns, rounded to fp32 and
- * then to the grid, a scale rstd max|s w| / qmax.  Tiles of zeros, of values that are
- * not finite or of magnitudes past 2^100 take y in fp32 first.  codes [T, ldc], ldc = ceil(H/128) * 128, 16-byte aligned; scale (i, t)
+ * value: a code is s w qmax / max|s w| over its 128 columns (products in fp32, exact
+ * for values of 16 bits), rounded to fp32 and then to the grid, a scale rstd max|s w| /
+ * qmax.  With 2^e <= rstd < 2^(e+1), tiles whose max|s w| 2^e is 0, not finite, below
+ * 2^-75 or above 2^100, and rows whose rstd is no normal number, take y in fp32 first
+ * and its codes and scales from that.  codes [T, ldc], ldc = ceil(H/128) * 128, 16-byte aligned; scale (i, t)
  * at scales[i*s_row + t*s_col]; nan_rows (int32 [T] or NULL): set to 1 where a
  * row of y holds a NaN, else left.
  */
@@ -1182,8 +1184,8 @@ int ntlb_grouped_matmul_dw(const uint16_t* dy, int64_t lddy, const uint16_t* x, 
 
 /*
  * x bf16 [R, K] (rows as for the products above) in 8 bits, laid out as kept and
- * kept_exp of ntlb_rms_norm_forward, and what they stand for as bf16 (exact) [R,
- * ldo], ldo % 8 == 0, zero from K to the next multiple of 8.
+ * kept_exp of ntlb_rms_norm_forward, and what they stand for as bf16 (exact, but for
+ * multiples of less than 2^-133) [R, ldo], ldo % 8 == 0, zero from K to the next multiple of 8.
  */
 int ntlb_kept_rows(const uint16_t* x, int64_t ldx, int64_t R, int64_t K, uint8_t* kept, uint8_t* kept_exp, void* stream);
 int ntlb_kept_values(const uint8_t* kept, const uint8_t* kept_exp, int64_t R, int64_t K, uint16_t* out, int64_t ldo,

@@ -9,7 +9,7 @@
 //
 // Matrix-core bound where experts have a few hundred rows and more, on the tiles of
 // ntlb_bf16_tile.h (32768 rows of 32 experts, 4096 x 7168: y 1.66 ms, 1.16 PFLOP/s; dx 1.75;
-// dW 1.89); bound by the weights' way from HBM below (256 rows of them: y 315 us, 6.0 TB/s).
+// dW 1.89); bound by the weights' way from HBM below (256 rows of them: y 307 to 316 us, 6 TB/s).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -503,7 +503,7 @@ __global__ void __launch_bounds__(256) values_kernel(Keep g, uint8_t* out, int64
   float a[4], b[4];
   kept_values4(v.x, scale, a);
   kept_values4(v.y, scale, b);
-  // 4 significant bits: exact in bf16
+  // 4 significant bits: exact in bf16, down to its least step of 2^-133
   *reinterpret_cast<uint4*>(out + (int64_t)row * ldo + 2 * c) =
       make_uint4(pack_bf16(a[0], a[1]), pack_bf16(a[2], a[3]), pack_bf16(b[0], b[1]), pack_bf16(b[2], b[3]));
 }
@@ -535,21 +535,28 @@ static int64_t few_blocks(int64_t E, int64_t N) { return (E + 1) * cdiv(N, 16); 
 // How many rows an expert has is known to the device only; the host goes by R rows over
 // the experts that can have some.
 //
+// In the figures rows are averages over experts of which the most popular has five to eight times
+// as many; in brackets, as many rows for each.
+//
 // Few rows stream, where their grid fits a launch: past the weights goes x once for 16 of their rows, tiles of some
 // rows take a tile's time.  Up to 2 to 32 rows an expert, by the weights' size: 768 x 1024
-// of 8 experts 11 us at 32 rows and 12 by tiles, at 64 rows 18 and 14; 2048 x 4096 of 8
-// 26 us at 4 and 27, at 16 37 and 28; 4096 x 7168 of 32 331 us at 2 and 339, at 4 361 and 316.
+// of 8 experts 12 us at 32 rows and 11 by tiles [8 and 10], at 64 rows 21 and 11 [12 and 10]; 2048 x 4096
+// of 8 25 us at 4 and 39 by whole tiles [24 and 39], at 16 38 and 26 by ranges [31 and 25]; 4096 x 7168 of 32
+// 309 us at 2 and 306 [307 and 306], at 4 326 and 307 [322 and 307].
 //
 // Tiles by the rounds that they take, one workgroup of 256 tiles a compute unit or two of
 // 128, a round of the latter 2/3 of the former's time: 4096 x 7168, 32 experts of 256
-// rows, y 612 us by 256 tiles and 727, dx 643 and 720, of 64 rows 531 and 445, 423 and 394;
-// 768 x 1024, 64 experts of 256 rows, 55 and 42; 2048 x 4096, 8 experts of 512, 84 and 99.
+// rows, y 586 us by 256 tiles and 658 [455 and 582], dx 636 and 683 [498 and 619], of 64 rows y 474 and 412
+// [359 and 321], dx 401 and 377 [392 and 369]; 768 x 1024, 64 experts of 256 rows, y 49 and 36 [30 and 34].
+// Where the two are near each other, how the rows divide decides, which the rule cannot see: 2048 x
+// 4096, 8 experts of 512, y 76 and 97 [80 and 58], dx 95 and 85 [56 and 68]; 4096 x 7168, 32 of
+// 128, y 511 and 463 [374 and 367], dx 437 and 513 [416 and 413].
 //
 // Tiles that leave compute units idle divide the contraction where that pays: a step of
 // 64 is half a us, the ranges' join 4, and their sums go out and in at 4 TB/s.  One expert,
-// 4096 x 4096, 64 rows 46 us whole and 17 in 8 ranges; 2048 x 4096, 8 experts of 64 rows 47 and
-// 33 in 3 ranges (in 4, more workgroups than places, 44); 768 x 1024, 8 experts of 250
-// rows 13 whole and 20 in 2.
+// 4096 x 4096, 64 rows 38 us whole and 14 in 8 ranges; 2048 x 4096, 8 experts of 64 rows 43 and
+// 33 in 3 ranges [39 and 29] (in 4, more workgroups than places, 42 [30]); 768 x 1024, 8 experts of 250
+// rows 12 whole and 18 in 2.
 struct Plan {
   bool few;
   int D, parts;
