@@ -1111,9 +1111,9 @@ int ntlb_rms_norm_forward(const void* x, int x_dtype, int64_t T, int64_t H, int6
  * for values of 16 bits), rounded to fp32 and then to the grid, a scale rstd max|s w| /
  * qmax.  With 2^e <= rstd < 2^(e+1), tiles whose max|s w| 2^e is 0, not finite, below
  * 2^-75 or above 2^100, and rows whose rstd is no normal number, take y in fp32 first
- * and its codes and scales from that.  codes [T, ldc], ldc = ceil(H/128) * 128, 16-byte aligned; scale (i, t)
- * at scales[i*s_row + t*s_col]; nan_rows (int32 [T] or NULL): set to 1 where a
- * row of y holds a NaN, else left.
+ * and its codes and scales from that.  codes [T, ldc], ldc = ceil(H/128) * 128, 16-byte
+ * aligned; scale (i, t) at scales[i*s_row + t*s_col]; nan_rows (int32 [T] or NULL): set
+ * to 1 where a row of y holds a NaN, else left.
  */
 int ntlb_rms_norm_quant(const void* x, int x_dtype, int64_t T, int64_t H, int64_t ldx, const void* res, int64_t ldr,
                         const void* w, int w_dtype, float eps, void* s, int64_t lds, int grid, uint8_t* codes,

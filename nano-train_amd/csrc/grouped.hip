@@ -535,7 +535,7 @@ static int64_t few_blocks(int64_t E, int64_t N) { return (E + 1) * cdiv(N, 16); 
 // How many rows an expert has is known to the device only; the host goes by R rows over
 // the experts that can have some.
 //
-// In the figures rows are averages over experts of which the most popular has five to eight times
+// In the figures rows are averages over experts of which the most popular has two to nine times
 // as many; in brackets, as many rows for each.
 //
 // Few rows stream, where their grid fits a launch: past the weights goes x once for 16 of their rows, tiles of some

@@ -136,7 +136,8 @@ def local_moe_bf16(tokens: torch.Tensor, expert_ids: torch.Tensor, topk_w: torch
     LocalRoutedMoE.forward :476-491, ExpertMLP.forward :190-193): moe.local_moe()'s
     arguments, shapes and capacity, without codes in its products, and the gradients of
     tokens, routing weights and expert weights under autograd, all of them on one
-    device, which need not be the current one.  grouped_matmul(), swiglu(block=128), grouped_matmul() and the weighted sum of each token's rows.
+    device, which need not be the current one.  grouped_matmul(), swiglu(block=128),
+    grouped_matmul() and the weighted sum of each token's rows.
 
     checkpoint "e4m3" keeps the rows of both products and the projections between
     them in 8 bits for the backward, 1/2 of what the bf16 loop keeps beside the
